@@ -387,6 +387,145 @@ typedef struct ormi_reduce_map_desc {
 int ormi_hip_reduce_map_workspace_size(const ormi_reduce_map_desc* desc, size_t* bytes);
 int ormi_hip_reduce_map(const ormi_reduce_map_desc* desc);
 
+/* -------------------------------------------------------------- rotary --
+ * Rotary positions. No counterpart in the reference. x is (batch, length,
+ * heads, dim), any strided view; the first `part` features (even) of each row
+ * are turned in pairs by the angle whose cosine and sine stand in the tables'
+ * row of the token's position, the others are copied:
+ *   a' = a cos - b sin,  b' = b cos + a sin    (inverse: sin negated)
+ * Pair p is (p, p + part / 2), or (2 p, 2 p + 1) when interleaved. cos and sin
+ * are (table_rows, part / 2), contiguous fp32. The position of token l is
+ * positions[b * positions_strides[0] + l * positions_strides[1]], or offset + l
+ * when positions is NULL; a position outside the tables turns its row's pairs
+ * into NaN and reads nothing. out is contiguous. Arithmetic is fp32, rounded
+ * once to out_dtype. dtypes: F32, BF16, F16, in any combination. */
+typedef struct ormi_rotary_desc {
+    int            dtype, out_dtype;
+    int            batch, length, heads, dim, part;
+    int            interleaved, inverse;
+    const void*    x;
+    int64_t        x_strides[4];           /* elements */
+    void*          out;
+    const float*   cos;
+    const float*   sin;
+    int            table_rows;
+    const int32_t* positions;              /* or NULL */
+    int64_t        positions_strides[2];
+    int            offset;
+} ormi_rotary_desc;
+int ormi_hip_rotary(const ormi_rotary_desc* desc);
+
+/* ----------------------------------------------------------- attention --
+ * Softmax attention whose mask is given by rules, and its gradient. No
+ * counterpart in the reference, whose graphs compose it from products, maps
+ * and sums over stored scores. q and out are (batch, queries, heads, dim), k
+ * and v (batch, keys, kv_heads, dim), heads a multiple of kv_heads: query head
+ * h reads key head h / (heads / kv_heads). Query i stands at position
+ * pos = length - queries + i of its sequence (the queries are its last ones),
+ * length = lengths[b], clamped to [0, keys], or keys when lengths is NULL.
+ *   t = scale q.k;   t = cap tanh(t / cap) when cap > 0
+ *   t -= slopes[h] |pos - j|                       when slopes is not NULL
+ *   query i sees key j when j < length,
+ *     and j <= pos or j < prefix[b]                when causal (prefix may be NULL)
+ *     and documents[pos] == documents[j] >= 0      when documents is not NULL
+ *   out = sum_j p_ij v_j, p the softmax of t over the keys i sees.
+ * A query that sees no key gives zeros, and so do its gradients. Keys at or
+ * past the length are never read, and neither k nor v need hold numbers there.
+ * q, k, v are strided views; out is contiguous. dtype is F32, BF16 or F16;
+ * scores, sums and the softmax are fp32, out is rounded once. 16-bit
+ * probabilities are rounded to 16 bits for their product with v.
+ * lse (or NULL) receives log2 of each row's sum of exponentials, (batch,
+ * kv_heads, queries, heads / kv_heads), +inf where nothing is seen: the
+ * gradient needs it.
+ * workspace: device memory of *_workspace_size() bytes, 256-byte aligned (NULL
+ * where that is 0).
+ * Sums have a fixed order: the same call gives the same bits. */
+#define ORMI_ATTENTION_MAX_DIM 256
+typedef struct ormi_attention_desc {
+    int            dtype;
+    int            batch, queries, keys, heads, kv_heads, dim;
+    const void*    q;
+    const void*    k;
+    const void*    v;
+    int64_t        q_strides[4], k_strides[4], v_strides[4];  /* elements */
+    float          scale, cap;
+    int            causal;
+    const float*   slopes;                                    /* (heads), or NULL */
+    const int32_t* documents;                                 /* (batch, keys), or NULL */
+    int64_t        documents_batch_stride;                    /* elements; the keys are contiguous */
+    const int32_t* prefix;                                    /* (batch), or NULL */
+    const int32_t* lengths;                                   /* (batch), or NULL */
+    void*          out;
+    float*         lse;
+    void*          workspace;
+    size_t         workspace_bytes;
+} ormi_attention_desc;
+int ormi_hip_attention_workspace_size(const ormi_attention_desc* desc, size_t* bytes);
+int ormi_hip_attention(const ormi_attention_desc* desc);
+
+/* The gradient of ormi_hip_attention with respect to q, k and v. forward
+ * describes the call that was made, with its out and lse; its workspace fields
+ * hold this call's workspace. dout is a view like q, of the same dtype; dq, dk
+ * and dv are contiguous, laid out like q, k and v's extents, of the same dtype
+ * (NULL: not wanted). Shared key heads' gradients add up over their query
+ * heads. float16 score gradients are held times a power of two taken from the
+ * largest rows of dout and v, so that a small loss does not lose them. */
+typedef struct ormi_attention_grad_desc {
+    ormi_attention_desc forward;
+    const void*         dout;
+    int64_t             dout_strides[4];
+    void*               dq;
+    void*               dk;
+    void*               dv;
+} ormi_attention_grad_desc;
+int ormi_hip_attention_grad_workspace_size(const ormi_attention_grad_desc* desc, size_t* bytes);
+int ormi_hip_attention_grad(const ormi_attention_grad_desc* desc);
+
+/* --------------------------------------------------------------- AdamW --
+ * One AdamW step over a list of tensors (no counterpart in the reference,
+ * whose programs write out an SGD update per weight):
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g g
+ *   out = p - lr ((m / c1) / (sqrt(v / c2) + eps) + weight_decay p)
+ * with c = 1 - beta^step, in fp32, each operation rounded on its own. All
+ * tensors go through as few launches as their number allows. p, g and out may
+ * be F32, BF16 or F16 (out has p's dtype) and are contiguous; out may be p.
+ * state_bits 32: m, v, m_out, v_out are fp32 and may be the same buffers.
+ * state_bits 8: they are codes of 8 bits in blocks of 256 consecutive elements
+ * (padded to whole blocks), each with a scale in m_scale, v_scale, the block's
+ * largest magnitude:
+ *   m = sign(c) (|c| / 127)^2 scale, c in -127..127
+ *   v = (c / 255)^4 scale, c in 0..255, never 0 for a v above 0
+ * the new values' codes being rint(127 sqrt(|m| / scale)) and
+ * rint(255 (v / scale)^(1/4)). A block with a value that is not finite gets a
+ * scale that is not finite either: its values are NaN from then on. */
+#define ORMI_ADAMW_BLOCK 256
+typedef struct ormi_adamw_tensor {
+    const void* p;
+    const void* g;
+    void*       out;
+    const void* m;
+    const void* v;
+    void*       m_out;
+    void*       v_out;
+    const float* m_scale;
+    const float* v_scale;
+    float*      m_scale_out;
+    float*      v_scale_out;
+    int64_t     count;
+    int         p_dtype, g_dtype;
+} ormi_adamw_tensor;
+typedef struct ormi_adamw_desc {
+    int                      num_tensors;
+    const ormi_adamw_tensor* tensors;
+    int                      state_bits;                 /* 32 or 8 */
+    int64_t                  step;                       /* 1 at the first */
+    double                   lr, beta1, beta2, eps, weight_decay;
+} ormi_adamw_desc;
+int ormi_hip_adamw(const ormi_adamw_desc* desc);
+/* The fp32 values of m and v that one tensor's 8-bit codes stand for. */
+int ormi_hip_adamw_values(float* m, float* v, const void* m_codes, const float* m_scale, const void* v_codes,
+                          const float* v_scale, int64_t count);
+
 /* ---------------------------------------------------------------- timing --
  * HIP events on the library's stream, for measuring kernel time from
  * outside (benchmarks). */

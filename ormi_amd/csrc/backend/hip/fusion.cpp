@@ -25,7 +25,7 @@ namespace ormi::hip {
     // walks ask for every node they visit. unordered_map elements keep their
     // addresses across inserts, so the pointers stay valid.
     constexpr size_t kOpSlots = 64;
-    static_assert((size_t)OpEnum::CAST < kOpSlots, "op table too small");
+    static_assert((size_t)OpEnum::ATTENTION_GRAD < kOpSlots, "op table too small");
     static const LoweringFunc* lowering_slots[kOpSlots] = {};
 
     void HIPLoweringRegistry::register_func(OpEnum op, LoweringFunc f) {

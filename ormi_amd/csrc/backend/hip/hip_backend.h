@@ -81,6 +81,26 @@ namespace ormi::hip {
     // Realize several nodes together: element-wise roots of the same shape share
     // one multi-output kernel (each input read once); the rest realize in order.
     void realize_group(const std::vector<NodePtr>& roots);
+    // ------------------------------------------ transformer (transformer.cpp) --
+    // The parent of n that is a gradient it may read through gradient_operand
+    // (-1: none), and the type it reads it as.
+    int gradient_parent(const Node& n);
+    DType gradient_dtype(const Node& n);
+    const NodePtr& gradient_operand(const NodePtr& n, DType want);
+
+    // One AdamW step: the new parameters and states, new buffers throughout.
+    // state: per parameter (m, v) in float32, or with bits 8 (m codes, m scales,
+    // v codes, v scales), codes as int32 words of four bytes.
+    struct AdamWOptions {
+        long long step = 1;
+        double lr = 1e-3, beta1 = 0.9, beta2 = 0.999, eps = 1e-8, weight_decay = 0.01;
+        int bits = 32;
+    };
+    void adamw(const std::vector<NodePtr>& params, const std::vector<NodePtr>& grads, const std::vector<std::vector<NodePtr>>& states,
+               const AdamWOptions& options, std::vector<NodePtr>* new_params, std::vector<std::vector<NodePtr>>* new_states);
+    // The float32 moments that 8-bit states stand for, of the given shape.
+    std::pair<NodePtr, NodePtr> adamw_values(const std::vector<NodePtr>& state, const std::vector<int>& shape);
+
     // Element-wise nodes run as a GEMM epilogue so far (ormi_hip_gemm_ex), and
     // the switch for that matching (on unless ORMI_GEMM_EPILOGUE=0).
     uint64_t gemm_epilogue_count();

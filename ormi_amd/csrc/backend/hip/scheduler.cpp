@@ -172,6 +172,22 @@ namespace ormi::hip {
         return n;
     }
 
+    // The same for the gradient that a rotation's or an attention's adjoint reads
+    // as `want`: x where n, or what n casts, is an unrealized 1 * x with x of that
+    // type (a product by one and a cast back are exact), of any strides.
+    const NodePtr& gradient_operand(const NodePtr& n, DType want) {
+        const NodePtr& m = !n->is_realized() && n->op == OpEnum::CAST && n->dtype == want ? n->parents[0] : n;
+        if (m->is_realized() || m->op != OpEnum::MUL || m->device.type != DeviceEnum::HIP) return n;
+        for (int k = 0; k < 2; ++k) {
+            const NodePtr* u = &m->parents[k];
+            const NodePtr& x = m->parents[1 - k];
+            while (!(*u)->is_realized() && is_view_op((*u)->op)) u = &(*u)->parents[0];
+            if (!(*u)->is_realized() || !(*u)->data->one || !x->is_realized()) continue;
+            if (x->data->dtype == want && x->device.type == DeviceEnum::HIP && x->view.shape == m->view.shape) return x;
+        }
+        return n;
+    }
+
     // Operand of a GEMM in the form ormi_hip_gemm takes: dtype f32/bf16/f16,
     // realized. Other dtypes (and mixed pairs) are converted to f32 by a fused
     // cast kernel.
@@ -741,7 +757,10 @@ namespace ormi::hip {
             return {x};
         }
         if (n->op == OpEnum::MATMUL) return {product_operand(n->parents[0]), product_operand(n->parents[1])};
-        return n->parents;
+        std::vector<NodePtr> deps = n->parents;
+        const int g = gradient_parent(*n);
+        if (g >= 0) deps[g] = gradient_operand(deps[g], gradient_dtype(*n));
+        return deps;
     }
 
     // One node whose dependencies are realized; rows: they are a row program's

@@ -270,7 +270,7 @@ PYBIND11_MODULE(ormi_backend, m) {
 
     {
         auto e = py::enum_<ops::OpEnum>(m, "OpEnum");
-        for (int i = (int)ops::OpEnum::LEAF; i <= (int)ops::OpEnum::CAST; ++i) {
+        for (int i = (int)ops::OpEnum::LEAF; i <= (int)ops::OpEnum::ATTENTION_GRAD; ++i) {
             auto op = (ops::OpEnum)i;
             e.value(ops::op_name(op), op);
         }
@@ -358,6 +358,31 @@ PYBIND11_MODULE(ormi_backend, m) {
     m.def("expand", &ops::expand);
     m.def("reshape", &ops::reshape);
     m.def("cast", [](std::shared_ptr<Node> x, const std::string& dt) { return ops::cast(x, dtype_from_name(dt)); });
+
+    m.def("rotary", [](std::shared_ptr<Node> x, std::shared_ptr<Node> cos, std::shared_ptr<Node> sin, std::shared_ptr<Node> positions,
+                       int offset, bool interleaved, const std::string& dt) {
+        return ops::rotary(x, cos, sin, positions, offset, interleaved, dtype_from_name(dt));
+    }, py::arg("x"), py::arg("cos"), py::arg("sin"), py::arg("positions").none(true), py::arg("offset"), py::arg("interleaved"), py::arg("dtype"));
+    m.def("attention", &ops::attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("cap"), py::arg("causal"),
+          py::arg("slopes").none(true), py::arg("documents").none(true), py::arg("prefix").none(true), py::arg("lengths").none(true));
+    m.def("adamw", [](const std::vector<std::shared_ptr<Node>>& params, const std::vector<std::shared_ptr<Node>>& grads,
+                      const std::vector<std::vector<std::shared_ptr<Node>>>& states, int bits, long long step, double lr, double beta1,
+                      double beta2, double eps, double weight_decay) {
+        hip::AdamWOptions o;
+        o.bits = bits;
+        o.step = step;
+        o.lr = lr;
+        o.beta1 = beta1;
+        o.beta2 = beta2;
+        o.eps = eps;
+        o.weight_decay = weight_decay;
+        std::vector<std::shared_ptr<Node>> p;
+        std::vector<std::vector<std::shared_ptr<Node>>> s;
+        hip::adamw(params, grads, states, o, &p, &s);
+        return py::make_tuple(p, s);
+    }, py::arg("params"), py::arg("grads"), py::arg("states"), py::arg("bits"), py::arg("step"), py::arg("lr"), py::arg("beta1"),
+       py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"));
+    m.def("adamw_values", &hip::adamw_values);
 
     m.def("execute_graph", &execute_graph);
     // Run the device's element-wise JIT on root with whatever tape reaches it

@@ -18,6 +18,9 @@ namespace ormi {
             case ops::OpEnum::TRANSPOSE: case ops::OpEnum::RESHAPE: case ops::OpEnum::EXPAND:
                 return parents.empty() ? DType::Float32 : parents[0]->dtype;
             case ops::OpEnum::CAST: return std::get<CastAttrs>(attrs).dtype;
+            case ops::OpEnum::ROTARY: return std::get<RotaryAttrs>(attrs).dtype;
+            case ops::OpEnum::ATTENTION: return parents[0]->dtype;
+            case ops::OpEnum::ATTENTION_GRAD: return parents[2 + std::get<AttentionAttrs>(attrs).which]->dtype;
             case ops::OpEnum::ARGMAX: return DType::Int64;
             default: return DType::Float32;
         }

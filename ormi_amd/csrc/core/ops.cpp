@@ -17,6 +17,8 @@ namespace ormi::ops {
             case OpEnum::GELU: return "GELU"; case OpEnum::GELU_GRAD: return "GELU_GRAD";
             case OpEnum::MAX: return "MAX"; case OpEnum::ARGMAX: return "ARGMAX";
             case OpEnum::EQ: return "EQ"; case OpEnum::CAST: return "CAST";
+            case OpEnum::ROTARY: return "ROTARY"; case OpEnum::ATTENTION: return "ATTENTION";
+            case OpEnum::ATTENTION_GRAD: return "ATTENTION_GRAD";
         }
         return "?";
     }

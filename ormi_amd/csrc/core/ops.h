@@ -5,7 +5,8 @@ namespace ormi::ops {
     // order (csrc/core/ops.h:4-10). The rest are the ops the benchmark configs
     // need and the reference lacks: activations with their derivative ops
     // (adjoints build these instead of allocating constants), MAX/ARGMAX
-    // reductions, an equality mask for the MAX adjoint, and a dtype CAST.
+    // reductions, an equality mask for the MAX adjoint, a dtype CAST, and a
+    // transformer block's rotary positions and attention with its gradient.
     enum class OpEnum {
         LEAF, CONST,
         NEG, EXP, LOG, SIN, COS,
@@ -13,7 +14,8 @@ namespace ormi::ops {
         SUM, TRANSPOSE, RESHAPE, EXPAND,
         FRAC_DERIV,
         RELU, STEP, TANH, TANH_GRAD, SIGMOID, SIGMOID_GRAD, GELU, GELU_GRAD,
-        MAX, ARGMAX, EQ, CAST
+        MAX, ARGMAX, EQ, CAST,
+        ROTARY, ATTENTION, ATTENTION_GRAD
     };
 
     const char* op_name(OpEnum op);

@@ -38,4 +38,16 @@ namespace ormi::ops {
     NodePtr reshape(NodePtr x, const std::vector<int>& shape);
     NodePtr expand(NodePtr x, const std::vector<int>& shape);
     NodePtr cast(NodePtr x, DType dtype);
+
+    // x (batch, length, heads, features), its first 2 * pairs features turned by
+    // the angles whose cosines and sines the tables (positions, pairs) hold;
+    // positions (length) or (batch, length) int32, or null: offset, offset + 1, ...
+    NodePtr rotary(NodePtr x, NodePtr cos, NodePtr sin, NodePtr positions, int offset, bool interleaved, DType dtype);
+
+    // Softmax attention of q (batch, queries, heads, features) over k and v
+    // (batch, keys, kv heads, features); the mask rules' tensors may be null:
+    // slopes (heads) float32, documents (batch, keys), prefix (batch) and
+    // lengths (batch) int32. The queries are the last of their sequence.
+    NodePtr attention(NodePtr q, NodePtr k, NodePtr v, float scale, float cap, bool causal, NodePtr slopes, NodePtr documents,
+                      NodePtr prefix, NodePtr lengths);
 }

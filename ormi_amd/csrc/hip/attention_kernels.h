@@ -1,0 +1,1124 @@
+// Attention kernels (attention_bf16.hip, attention_f16.hip and attention_f32.hip
+// each instantiate them for one element type; attention.hip holds the C entry).
+//
+// For query row i and key j of one head
+//   t_ij = scale q_i.k_j;  t = cap tanh(t / cap);  t -= slope |pos_i - j|
+//   p_ij = 2^(t log2 e - lse_i) over the visible keys, o_i = sum_j p_ij v_j
+// with a running maximum and sum, so that no score leaves the registers.
+//
+// Rows. The query heads that share a key/value head are folded into the rows:
+// row r is query r / group of head kv * group + r % group, so shared keys and
+// values are read once for all of them and their gradients add up in order in
+// one work-group's registers, without atomics.
+//
+// Masks. Row i sees key j when j < lim_i and (with documents) both belong to the
+// same one: causal, prefix and length rules all bound j from above, and one
+// integer per row, lim = min(length, max(pos + 1, prefix)), holds them.
+//
+// Tiles. The product of a tile of keys (rows of the first MFMA operand, from
+// LDS) and a wave's 32 query rows (second operand, in registers) puts one query
+// in each lane's column: a row's maximum and sum are reductions over the lane's
+// own registers and one exchange of the wave's halves. The accumulator's
+// register order (keys 8 b + 4 half + 0..3) is taken as the order of the second
+// product's depth, so p goes from the first product's accumulators into the
+// second product's operand without leaving its lane; the values follow that
+// order through transposing LDS reads (16-bit) or plain ones (32-bit).
+// Keys and values come straight from memory into two LDS stages, one 16-byte
+// chunk per lane, their chunks exchanged by row (swz) so that neither the row
+// reads nor the transposing reads meet in a bank.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cstdint>
+
+#include "attention.h"
+#include "device/ormi_device.h"
+#include "gemm_mfma.h"
+
+namespace ormi_hip {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) float lds_float;
+typedef __attribute__((address_space(3))) int lds_int;
+
+constexpr float kInf = __builtin_huge_valf();
+
+// ---------------------------------------------------------------- helpers --
+__device__ __forceinline__ unsigned pack2(TrBF16, float a, float b) {
+    const f32x2_t f = {a, b};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f, bf16x2_t));
+}
+__device__ __forceinline__ unsigned pack2(TrF16, float a, float b) {
+    const f32x2_t f = {a, b};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f, f16x2_t));
+}
+// NaN when any is: a row with a NaN score is NaN whatever its maximum.
+__device__ __forceinline__ float max3(float a, float b, float c) { return ormi_maximum(ormi_maximum(a, b), c); }
+// Both halves of the wave hold the result for lane % 32.
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return ormi_maximum(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ const char* uniform_ptr(const char* p) {
+    const unsigned long long t = (unsigned long long)(uintptr_t)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)t);
+    const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)(t >> 32));
+    return (const char*)(((unsigned long long)hi << 32) | lo);
+}
+// tanh for scores: 1 - 2 / (1 + e^2|y|) is exact to about 1e-7 of the cap, far
+// below the rounding of 16-bit operands; 32-bit scores take the full form.
+__device__ __forceinline__ float tanh_score(TrF32, float y) { return ormi_tanh(y); }
+template <class Tr>
+__device__ __forceinline__ float tanh_score(Tr, float y) {
+    const float e = __builtin_amdgcn_exp2f(y * 2.88539004f);
+    return __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f, 1.0f);
+}
+
+// The wait states between a matrix instruction and a vector instruction that
+// reads its result (its passes and two more), spelled out: across the branches
+// that masks bring, the compiler (ROCm 7.2) has left too few of them, and rows
+// came out wrong now and then. tests/test_mfma_waits.py checks the assembly.
+template <class Tr>
+__device__ __forceinline__ void settle(f32x16_t& a) {
+    if constexpr (Tr::ESIZE == 4) asm("s_nop 15\n\ts_nop 1" : "+v"(a));
+    else asm("s_nop 9" : "+v"(a));
+}
+
+// 16-bit probabilities are held 2^kShift above their value (of at most 1, or
+// 2^8 before a row's maximum is brought up to date), so that those of long rows
+// stay in float16's normal range; the sums they go into undo it.
+template <class Tr> struct Shift { static constexpr float fwd = 0.0f, bwd = 0.0f; };
+template <> struct Shift<TrF16> { static constexpr float fwd = 7.0f, bwd = 12.0f; };
+
+// ------------------------------------------------------------------ tiles --
+// A tile of rows of DP features in LDS, 16-byte chunks exchanged by row.
+template <class Tr, int DP>
+struct Tile {
+    static constexpr int ES = Tr::ESIZE, VE = Tr::VE, ROWB = DP * ES, CPR = ROWB / 16;
+    static constexpr int NF = DP / (2 * VE);  // operand fragments along the features
+    static constexpr int DT = DP / 32;        // accumulator tiles along the features
+
+    // Sixteen rows in a row meet in no bank (row reads), and neither do four
+    // rows' 64-byte pieces (transposing reads).
+    __device__ __forceinline__ static int swz(int row) {
+        return CPR == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+    }
+    // Rows [row0, row0 + 32), fragment f: lane l holds the chunk 2 f + l / 32 of row l % 32.
+    __device__ __forceinline__ static u32x4_t frag(const lds_char* t, int row0, int f) {
+        const int lane = threadIdx.x & 63, row = lane & 31, c = 2 * f + (lane >> 5);
+        return *(const __attribute__((address_space(3))) u32x4_t*)(t + row0 * ROWB + row * ROWB + ((c ^ swz(row)) << 4));
+    }
+    // 16-bit: features [32 dt, 32 dt + 32) as rows, the depth the tile rows
+    // row0 + 16 step + {4 half + 0..3, 8 + 4 half + 0..3}, accumulator order.
+    __device__ __forceinline__ static u32x4_t turned(const lds_char* t, int row0, int step, int dt) {
+        const int lane = threadIdx.x & 63, i = lane & 15;
+        const int col = dt * 32 + ((lane >> 4) & 1) * 16 + 4 * (i & 3);
+        u32x4_t out;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = 8 * h + 4 * (lane >> 5) + (i >> 2);  // row % 16
+            const lds_char* p = t + (row0 + 16 * step) * ROWB + k * ROWB + (((col >> 3) ^ swz(k)) << 4) + ((col & 4) << 1);
+            const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p);
+            const uint2 w = __builtin_bit_cast(uint2, v);
+            out[2 * h] = w.x;
+            out[2 * h + 1] = w.y;
+        }
+        return out;
+    }
+    // 32-bit: feature 32 dt + l % 32 of the tile row that accumulator register r of the lane's half stands for.
+    __device__ __forceinline__ static float turned1(const lds_char* t, int row0, int r, int dt) {
+        const int lane = threadIdx.x & 63, row = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        const int d = dt * 32 + (lane & 31);
+        return *(const lds_float*)(t + row0 * ROWB + row * ROWB + (((d >> 2) ^ swz(row)) << 4) + (d & 3) * 4);
+    }
+    // acc[dt] += (the tile's rows row0.. turned) x (accumulator `a` as 16- or 32-bit operand)
+    __device__ __forceinline__ static void second(const lds_char* t, int row0, const f32x16_t& a, f32x16_t (&acc)[DT]) {
+        if constexpr (ES == 2) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                u32x4_t b;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) b[e] = pack2(Tr{}, a[8 * s + 2 * e], a[8 * s + 2 * e + 1]);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) Tr::mma(turned(t, row0, s, dt), b, acc[dt]);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(turned1(t, row0, r, dt), a[r], acc[dt], 0, 0, 0);
+        }
+    }
+    // A row's fragments from memory: lane l holds row `row`'s chunks 2 f + l / 32 (zero past the row's end).
+    __device__ __forceinline__ static void row_frags(const char* row, int chunks, u32x4_t (&out)[NF]) {
+        const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int c = 2 * f + half;
+            out[f] = c < chunks ? *(const u32x4_t*)(row + c * 16) : u32x4_t{0, 0, 0, 0};
+        }
+    }
+};
+
+// Direct loads of a tile's 16-byte chunks into LDS: 1 KB per instruction, whose
+// lanes' chunks land one after the other; the exchange of chunks is made on the
+// source side. Inline assembly, as in the GEMMs: the compiler would make every
+// LDS read of the current stage wait for the next stage's loads. The kernels
+// wait themselves before the barrier that publishes a stage.
+// Chunks past the row's end re-read chunk 0: what meets them is zero in the
+// first product and is not stored in the second.
+template <class Tr, int DP, int ROWS, int NW>
+struct Loader {
+    using T = Tile<Tr, DP>;
+    static constexpr int SEGS = ROWS * T::CPR / 64, PER = SEGS / NW;
+    static_assert(SEGS % NW == 0 && T::CPR <= 64, "whole segments per wave");
+
+    __device__ __forceinline__ static int seg_row(int s) {  // this lane's tile row in segment s
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        return (wave * PER + s) * (64 / T::CPR) + lane / T::CPR;
+    }
+    __device__ __forceinline__ static unsigned seg_chunk(int row, int chunks) {  // bytes within the row
+        const int lane = threadIdx.x & 63;
+        const int c = (lane % T::CPR) ^ T::swz(row);
+        return c < chunks ? (unsigned)c * 16u : 0u;
+    }
+    // All of the wave's segments from base + off[s], up to four per asm block. The
+    // assembler's text is not checked for hazards, so the waits are written out:
+    // five cycles before a memory instruction reads a scalar register that a
+    // vector instruction (a lane read that restores a spilled one, say) may have
+    // written, one between a write of m0 and a load to LDS.
+    __device__ __forceinline__ static void load(lds_char* dst, const char* base, const unsigned (&off)[PER]) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const unsigned d = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(dst + wave * PER * 1024));
+        constexpr int N = PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1;
+#pragma unroll
+        for (int s = 0; s < PER; s += N) {
+            if constexpr (N == 4)
+                asm volatile(
+                    "s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
+                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
+                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5" ::"s"(d + s * 1024),
+                    "v"(off[s]), "v"(off[s + 1]), "v"(off[s + 2]), "v"(off[s + 3]), "s"(base)
+                    : "memory", "m0", "scc");
+            else if constexpr (N == 2)
+                asm volatile(
+                    "s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(d + s * 1024),
+                    "v"(off[s]), "v"(off[s + 1]), "s"(base)
+                    : "memory", "m0", "scc");
+            else
+                asm volatile("s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(d + s * 1024),
+                             "v"(off[s]), "s"(base)
+                             : "memory", "m0");
+        }
+    }
+    // Rows base + row * row_bytes, rows past `last` re-reading it.
+    __device__ __forceinline__ static void rows(lds_char* dst, const char* base, unsigned row_bytes, int last, int chunks) {
+        unsigned off[PER];
+#pragma unroll
+        for (int s = 0; s < PER; ++s) {
+            const int row = seg_row(s);
+            off[s] = (unsigned)min(row, last) * row_bytes + seg_chunk(row, chunks);
+        }
+        load(dst, uniform_ptr(base), off);
+    }
+};
+
+// Waits for this wave's direct loads and LDS reads, then for the other waves.
+__device__ __forceinline__ void publish() {
+    wait_vmcnt_lds<0>();
+    lds_barrier();
+}
+
+// Work item of a work-group. Consecutive work-groups go to different XCDs, each
+// with an L2 of its own; every XCD takes one run of items, so work-groups that
+// share keys and values share an L2.
+__device__ __forceinline__ int xcd_item(int total) {
+    const int per = (total + 7) / 8;
+    return (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+}
+
+// ------------------------------------------------------------------ masks --
+// Per batch: keys that exist, position of query 0, prefix.
+struct Span {
+    int end, off, prefix;
+    __device__ __forceinline__ Span(const AttnParams& p, int b) {
+        end = p.lengths ? min(max(p.lengths[b], 0), p.keys) : p.keys;
+        off = end - p.queries;
+        prefix = p.prefix ? min(max(p.prefix[b], 0), end) : 0;
+    }
+    __device__ __forceinline__ int limit(const AttnParams& p, int pos) const {
+        return p.causal ? min(end, max(max(pos + 1, prefix), 0)) : end;
+    }
+};
+__device__ __forceinline__ int doc_at(const AttnParams& p, int b, int pos) {
+    return pos >= 0 && pos < p.keys ? p.docs[b * p.docs_sb + pos] : -1;
+}
+// Documents of a set of tokens as a range; a token without one makes the range
+// wider than a single document, so that the set never counts as uniform.
+__device__ __forceinline__ int2 widen(int lo, int hi, bool none) {
+    if (lo > hi || !none || lo != hi) return make_int2(lo, hi);
+    return hi < 0x7fffffff ? make_int2(lo, hi + 1) : make_int2(lo - 1, hi);
+}
+
+// Bits of tiles base + lane: those that share a document with `mine`.
+__device__ __forceinline__ unsigned long long tiles_meeting(const int2* ranges, int base, int tiles, int2 mine) {
+    const int t = base + (int)(threadIdx.x & 63);
+    const int2 r = t < tiles ? ranges[t] : make_int2(0x7fffffff, -1);
+    return __ballot(t < tiles && r.x <= mine.y && mine.x <= r.y);
+}
+
+// A score in powers of two; its derivative with respect to scale q.k in slope (kCap).
+template <class Tr, int FORM>
+__device__ __forceinline__ float score2(const AttnParams& p, float s, float slope2, float away, float& slope) {
+    float t;
+    if constexpr (FORM == kCap) {
+        const float u = tanh_score(Tr{}, s * p.scale_over_cap);
+        t = u * p.cap2;
+        slope = __builtin_fmaf(-u, u, 1.0f);
+    } else {
+        t = s * p.scale2;
+    }
+    return __builtin_fmaf(-slope2, __builtin_fabsf(away), t);
+}
+
+// ---------------------------------------------------------------- outputs --
+// Accumulators acc[dt][r], feature 32 dt + 8 (r / 4) + 4 half + r % 4 of the
+// lane's row, times f, rounded once to the output's type.
+template <class Tr, int DT>
+__device__ __forceinline__ void store_row(char* row, int dim, const f32x16_t (&acc)[DT], float f) {
+    const int half = (threadIdx.x & 63) >> 5;
+    const bool vec = dim % 4 == 0;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = dt * 32 + 8 * q + 4 * half;
+            if (d >= dim) continue;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * q + e] * f;
+            if constexpr (Tr::ESIZE == 4) {
+                float* o = (float*)row + d;
+                if (vec) *(float4*)o = make_float4(v[0], v[1], v[2], v[3]);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < dim) o[e] = v[e];
+            } else {
+                const uint2 w = make_uint2(pack2(Tr{}, v[0], v[1]), pack2(Tr{}, v[2], v[3]));
+                unsigned short* o = (unsigned short*)row + d;
+                if (vec) *(uint2*)o = w;
+                else {
+                    o[0] = (unsigned short)w.x;
+                    if (d + 1 < dim) o[1] = (unsigned short)(w.x >> 16);
+                    if (d + 2 < dim) o[2] = (unsigned short)w.y;
+                    if (d + 3 < dim) o[3] = (unsigned short)(w.y >> 16);
+                }
+            }
+        }
+}
+// The same as fp32 partial values, DT * 32 a row.
+template <int DT>
+__device__ __forceinline__ void store_part(float* row, const f32x16_t (&acc)[DT]) {
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *(float4*)(row + dt * 32 + 8 * q + 4 * half) =
+                make_float4(acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]);
+}
+
+// ---------------------------------------------------------------- forward --
+// NW waves of 32 rows; BN keys per tile.
+template <class Tr, int DP, int NW, int BN, int FORM>
+__global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
+    using T = Tile<Tr, DP>;
+    constexpr int MT = BN / 32, TILEB = BN * T::ROWB;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
+    __shared__ int shared_i[3 * NW];
+    lds_char* lds = (lds_char*)smem;
+
+    const int item = xcd_item(p.row_blocks * p.splits * p.batch * p.kv_heads);
+    if (item >= p.row_blocks * p.splits * p.batch * p.kv_heads) return;
+    const int split = item % p.splits, rest = item / p.splits;
+    const int rb = p.row_blocks - 1 - rest % p.row_blocks, bh = rest / p.row_blocks;  // the longest causal rows first
+    const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+
+    // This lane's row.
+    const Span span(p, b);
+    const int r = (rb * NW + wave) * 32 + (lane & 31);
+    const int rc = min(r, p.rows - 1), i = rc / p.group, head = kvh * p.group + rc % p.group;
+    const int pos = i + span.off;
+    int lim = span.limit(p, pos), doc = 0;
+    if (p.docs) {
+        doc = doc_at(p, b, pos);
+        if (doc < 0) lim = 0;
+    }
+    const float slope2 = FORM != kPlain && p.slopes ? p.slopes[head] * 1.44269504f : 0.0f;
+    u32x4_t qf[T::NF];
+    T::row_frags(p.q + (b * p.q_sb + (long long)i * p.q_sl + head * p.q_sh) * T::ES, p.chunks, qf);
+
+    // What the wave and the work-group see.
+    const int lim_min = wave_min_i(lim), lim_max = wave_max_i(lim);
+    int2 docs_wave = make_int2(0, 0), docs_group = make_int2(0, 0);
+    int lim_group = lim_max;
+    if (NW > 1 || p.docs) {
+        if (p.docs) {
+            const int lo = wave_min_i(lim > 0 ? doc : 0x7fffffff), hi = wave_max_i(lim > 0 ? doc : -1);
+            docs_wave = widen(lo, hi, __any(lim <= 0));
+            docs_group = docs_wave;
+        }
+        if (NW > 1) {
+            if (lane == 0) {
+                shared_i[wave] = lim_max;
+                shared_i[NW + wave] = docs_wave.x;
+                shared_i[2 * NW + wave] = docs_wave.y;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                lim_group = max(lim_group, shared_i[w]);
+                docs_group.x = min(docs_group.x, shared_i[NW + w]);
+                docs_group.y = max(docs_group.y, shared_i[2 * NW + w]);
+            }
+            lim_group = __builtin_amdgcn_readfirstlane(lim_group);
+        }
+    }
+    const int tiles = (lim_group + BN - 1) / BN;
+    const int per = (tiles + p.splits - 1) / p.splits;
+    const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
+
+    const int2* ranges = p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr;
+    constexpr int RT = kDocTile / BN;  // tiles per range
+    unsigned long long meet = 0;
+    int meet_base = -1;
+    // The next tile from t on that shares a document with the rows, or t1.
+    auto next = [&](int t) {
+        if (!p.docs) return t;
+        while (t < t1) {
+            const int rt = t / RT;
+            if (meet_base < 0 || rt >= meet_base + 64) {
+                meet_base = rt;
+                meet = tiles_meeting(ranges, rt, p.range_tiles, docs_group);
+            }
+            const unsigned long long left = meet >> (rt - meet_base);
+            if (left & 1) return t;
+            t = left ? (rt + __builtin_ctzll(left)) * RT : (meet_base + 64) * RT;
+        }
+        return t1;
+    };
+    const char* kb = p.k + (b * p.k_sb + kvh * p.k_sh) * T::ES;
+    const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh) * T::ES;
+    using L = Loader<Tr, DP, BN, NW>;
+    auto issue = [&](int t, int stage) {
+        const int last = span.end - 1 - t * BN;
+        L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks);
+        L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks);
+    };
+
+    f32x16_t acc[T::DT];
+#pragma unroll
+    for (int dt = 0; dt < T::DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
+    // m: the row's maximum in powers of two (of the unscaled products' sizes when
+    // kPlain), which may lag by up to 2^8 (the sums then grow by as much).
+    float m = -kInf, l = 0.0f;
+    const float unit = FORM != kPlain ? 1.0f : p.scale2;
+
+    int t = next(t0), stage = 0;
+    if (t < t1) issue(t, 0);
+    while (t < t1) {
+        publish();
+        const int tn = next(t + 1);
+        if (tn < t1) issue(tn, stage ^ 1);
+        const int j0 = t * BN;
+        if (j0 < lim_max) {
+            const lds_char* kt = lds + stage * 2 * TILEB;
+            const lds_char* vt = kt + TILEB;
+            bool same = true;
+            if (p.docs) {
+                const int2 kr = ranges[t / RT];
+                same = kr.x == kr.y && docs_wave.x == docs_wave.y && kr.x == docs_wave.x;
+            }
+            f32x16_t s[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[mt][e] = 0.0f;
+#pragma unroll
+                for (int f = 0; f < T::NF; ++f) Tr::mma(T::frag(kt, mt * 32, f), qf[f], s[mt]);
+                settle<Tr>(s[mt]);
+                if constexpr (FORM != kPlain) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+                        float slope;
+                        s[mt][e] = score2<Tr, FORM>(p, s[mt][e], slope2, (float)(pos - j), slope);
+                    }
+                }
+            }
+            if (j0 + BN > lim_min || !same) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+                        bool seen = j < lim;
+                        if (!same) seen = seen && doc_at(p, b, j) == doc;
+                        s[mt][e] = seen ? s[mt][e] : -kInf;
+                    }
+            }
+            float top = -kInf;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) top = max3(top, s[mt][e], s[mt][e + 1]);
+            top = halves_max(top);
+            if (__any((top - m) * unit > 8.0f)) {
+                const float mn = fmaxf(m, top);
+                const float a = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * unit);
+                l *= a;
+#pragma unroll
+                for (int dt = 0; dt < T::DT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[dt][e] *= a;
+                m = mn;
+            }
+            const float base = m == -kInf ? 0.0f : Shift<Tr>::fwd - m * unit;
+            float part[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[mt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][e], unit, base));
+                    part[e & 1] += s[mt][e];
+                }
+            l += part[0] + part[1];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) T::second(vt, mt * 32, s[mt], acc);
+        }
+        t = tn;
+        stage ^= 1;
+    }
+
+#pragma unroll
+    for (int dt = 0; dt < T::DT; ++dt) settle<Tr>(acc[dt]);
+    l = halves_sum(l);
+    if (r >= p.rows) return;
+    if (p.splits > 1) {
+        const long long at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows + r;
+        store_part(p.part + at * DP, acc);
+        if (half == 0) p.part_ml[at] = make_float2(m == -kInf ? -kInf : m * unit - Shift<Tr>::fwd, l);
+        return;
+    }
+    store_row<Tr, T::DT>(p.out + (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES, p.dim, acc, l == 0.0f ? 0.0f : 1.0f / l);
+    if (p.lse && half == 0) p.lse[(long long)bh * p.rows + r] = l == 0.0f ? kInf : m * unit - Shift<Tr>::fwd + __builtin_log2f(l);
+}
+
+// Joins the splits of a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
+// in split order. One wave per row, lanes along the features.
+template <class Tr, int DP>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
+    const long long total = (long long)p.batch * p.kv_heads * p.rows;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= total) return;
+    float top = -kInf;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[s * total + row].x);
+    float l = 0.0f, o[DP / 64];
+#pragma unroll
+    for (int e = 0; e < DP / 64; ++e) o[e] = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 ml = p.part_ml[s * total + row];
+        const float a = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
+        if (ml.y == 0.0f) continue;  // saw no key; its values are zero
+        l += a * ml.y;
+#pragma unroll
+        for (int e = 0; e < DP / 64; ++e) o[e] += a * p.part[(s * total + row) * DP + e * 64 + lane];
+    }
+    const int bh = (int)(row / p.rows), r = (int)(row % p.rows), b = bh / p.kv_heads;
+    const int i = r / p.group, head = (bh % p.kv_heads) * p.group + r % p.group;
+    const long long at = (((long long)b * p.queries + i) * p.heads + head) * p.dim;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < DP / 64; ++e) {
+        const int d = e * 64 + lane;
+        if (d < p.dim) {
+            const float v = o[e] * inv;
+            if constexpr (Tr::ESIZE == 4) ((float*)p.out)[at + d] = v;
+            else ((unsigned short*)p.out)[at + d] = (unsigned short)pack2(Tr{}, v, v);
+        }
+    }
+    if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? kInf : top + __builtin_log2f(l);
+}
+
+template <class Tr, int DP, int FORM>
+void launch_attention_fwd_form(const AttnParams& p) {
+    const int items = p.row_blocks * p.splits * p.batch * p.kv_heads;
+    const unsigned grid = (unsigned)((items + 7) / 8 * 8);
+    if (p.wide) attention_fwd_kernel<Tr, DP, 4, fwd_tile(DP, Tr::ESIZE, false), FORM><<<grid, 256>>>(p);
+    else attention_fwd_kernel<Tr, DP, 1, fwd_tile(DP, Tr::ESIZE, true), FORM><<<grid, 64>>>(p);
+}
+
+template <class Tr, int DP>
+int launch_attention_fwd_dp(const AttnParams& p) {
+    if (p.form == kPlain) launch_attention_fwd_form<Tr, DP, kPlain>(p);
+    else if (p.form == kBias) launch_attention_fwd_form<Tr, DP, kBias>(p);
+    else launch_attention_fwd_form<Tr, DP, kCap>(p);
+    if (p.splits > 1) {
+        const long long rows = (long long)p.batch * p.kv_heads * p.rows;
+        attention_join_kernel<Tr, DP><<<(unsigned)((rows + 3) / 4), 256>>>(p);
+    }
+    return (int)hipGetLastError();
+}
+
+// --------------------------------------------------------------- gradient --
+// delta = sum of out * dout of a row; 16 lanes per row. float16 also collects
+// the largest squared norms of a dout row and of a value row: |score gradient|
+// <= p (|dp| + |delta|) <= 2 |dout| |v|, and held times the power of two that
+// takes that bound to 2^15 the score gradients keep to float16's normal range
+// whatever the scale of the loss. A maximum does not depend on its order.
+template <class Tr>
+__device__ __forceinline__ float load1(const char* row, int d) {
+    if constexpr (Tr::ESIZE == 4) return ((const float*)row)[d];
+    const unsigned short h = ((const unsigned short*)row)[d];
+    if constexpr (sizeof(Shift<Tr>) && Shift<Tr>::bwd != 0.0f) return ormi_f16_to_f32(h);
+    return ormi_bf16_to_f32(h);
+}
+template <class Tr>
+__device__ __forceinline__ void load_chunk(const char* at, float (&v)[Tr::VE]) {
+    const u32x4_t w = *(const u32x4_t*)at;
+#pragma unroll
+    for (int e = 0; e < Tr::VE; ++e) {
+        if constexpr (Tr::ESIZE == 4) v[e] = __uint_as_float(w[e]);
+        else {
+            const unsigned short h = (unsigned short)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
+            v[e] = Shift<Tr>::bwd != 0.0f ? ormi_f16_to_f32(h) : ormi_bf16_to_f32(h);
+        }
+    }
+}
+template <class Tr>
+__global__ __launch_bounds__(256) void attention_delta_kernel(AttnParams p, float* delta, unsigned* bounds, unsigned row_groups) {
+    const int sub = threadIdx.x & 15;
+    float dot = 0.0f, norm = 0.0f;
+    if (blockIdx.x < row_groups) {
+        const long long n = (long long)p.batch * p.queries * p.heads;
+        const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+        const bool live = at < n;
+        const long long row = live ? at : n - 1;
+        const int head = (int)(row % p.heads);
+        const long long bi = row / p.heads;
+        const int b = (int)(bi / p.queries), i = (int)(bi % p.queries);
+        const char* o = p.out + row * p.dim * Tr::ESIZE;
+        const char* g = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * Tr::ESIZE;
+        if (p.dim % Tr::VE == 0) {
+            for (int c = sub; c < p.dim / Tr::VE; c += 16) {
+                float x[Tr::VE], y[Tr::VE];
+                load_chunk<Tr>(o + c * 16, x);
+                load_chunk<Tr>(g + c * 16, y);
+#pragma unroll
+                for (int e = 0; e < Tr::VE; ++e) {
+                    dot = __builtin_fmaf(x[e], y[e], dot);
+                    norm = __builtin_fmaf(y[e], y[e], norm);
+                }
+            }
+        } else {
+            for (int d = sub; d < p.dim; d += 16) {
+                const float y = load1<Tr>(g, d);
+                dot = __builtin_fmaf(load1<Tr>(o, d), y, dot);
+                norm = __builtin_fmaf(y, y, norm);
+            }
+        }
+        dot = ormi_lanes_sum<16>(dot);
+        const int kvh = head / p.group;
+        if (live && sub == 0) delta[((long long)b * p.kv_heads + kvh) * p.rows + (long long)i * p.group + head % p.group] = dot;
+    } else {
+        const long long n = (long long)p.batch * p.keys * p.kv_heads;
+        const long long at = (long long)(blockIdx.x - row_groups) * 16 + (threadIdx.x >> 4);
+        const long long row = at < n ? at : n - 1;
+        const int kvh = (int)(row % p.kv_heads);
+        const long long bj = row / p.kv_heads;
+        const int b = (int)(bj / p.keys), j = (int)(bj % p.keys);
+        if (j < Span(p, b).end) {
+            const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + kvh * p.v_sh) * Tr::ESIZE;
+            for (int c = sub; c < p.chunks; c += 16) {
+                float y[Tr::VE];
+                load_chunk<Tr>(v + c * 16, y);
+#pragma unroll
+                for (int e = 0; e < Tr::VE; ++e) norm = __builtin_fmaf(y[e], y[e], norm);
+            }
+        }
+    }
+    if (!bounds) return;
+    norm = ormi_lanes_sum<16>(norm);
+    norm = fmaxf(norm, __shfl_xor(norm, 16, 64));
+    norm = fmaxf(norm, __shfl_xor(norm, 32, 64));
+    __shared__ float most[4];
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = norm;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        atomicMax(bounds + (blockIdx.x < row_groups ? 0 : 1),
+                  __float_as_uint(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))));
+}
+// The power of two that the score gradients are held times.
+template <class Tr>
+__device__ __forceinline__ float grad_hold(const AttnParams& p) {
+    if (Shift<Tr>::bwd == 0.0f) return 1.0f;
+    const float bound = 2.0f * __builtin_sqrtf(p.grad_scale[0] * p.grad_scale[1]);
+    if (!(bound > 0.0f && bound < 1e30f)) return 1.0f;
+    return __builtin_amdgcn_ldexpf(1.0f, min(100, max(-100, 15 - __builtin_amdgcn_frexp_expf(bound))));
+}
+
+// dq. Rows, tiles and masks as in the forward kernel, with both products of a
+// tile's keys and values against the row's q and dout; the score gradients then
+// meet the keys again, turned.
+template <class Tr, int DP, int BN, int FORM>
+__global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
+    using T = Tile<Tr, DP>;
+    constexpr int NW = 4, MT = BN / 32, TILEB = BN * T::ROWB;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
+    __shared__ int shared_i[3 * NW];
+    lds_char* lds = (lds_char*)smem;
+
+    const int total = p.row_blocks * p.batch * p.kv_heads, item = xcd_item(total);
+    if (item >= total) return;
+    const int rb = p.row_blocks - 1 - item % p.row_blocks, bh = item / p.row_blocks;
+    const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+
+    const Span span(p, b);
+    const int r = (rb * NW + wave) * 32 + (lane & 31);
+    const int rc = min(r, p.rows - 1), i = rc / p.group, head = kvh * p.group + rc % p.group;
+    const int pos = i + span.off;
+    int lim = r < p.rows ? span.limit(p, pos) : 0, doc = 0;
+    if (p.docs) {
+        doc = doc_at(p, b, pos);
+        if (doc < 0) lim = 0;
+    }
+    const float slope2 = FORM != kPlain && p.slopes ? p.slopes[head] * 1.44269504f : 0.0f;
+    const float lse = p.lse[(long long)bh * p.rows + rc], delta = p.delta[(long long)bh * p.rows + rc];
+    const float hold = grad_hold<Tr>(p);
+    u32x4_t qf[T::NF], gf[T::NF];
+    T::row_frags(p.q + (b * p.q_sb + (long long)i * p.q_sl + head * p.q_sh) * T::ES, p.chunks, qf);
+    T::row_frags(p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * T::ES, p.chunks, gf);
+
+    const int lim_min = wave_min_i(lim), lim_max = wave_max_i(lim);
+    int2 docs_wave = make_int2(0, 0), docs_group;
+    if (p.docs) docs_wave = widen(wave_min_i(lim > 0 ? doc : 0x7fffffff), wave_max_i(lim > 0 ? doc : -1), __any(lim <= 0));
+    docs_group = docs_wave;
+    int lim_group = lim_max;
+    if (lane == 0) {
+        shared_i[wave] = lim_max;
+        shared_i[NW + wave] = docs_wave.x;
+        shared_i[2 * NW + wave] = docs_wave.y;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        lim_group = max(lim_group, shared_i[w]);
+        docs_group.x = min(docs_group.x, shared_i[NW + w]);
+        docs_group.y = max(docs_group.y, shared_i[2 * NW + w]);
+    }
+    lim_group = __builtin_amdgcn_readfirstlane(lim_group);
+    const int t1 = (lim_group + BN - 1) / BN;
+
+    const int2* ranges = p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr;
+    constexpr int RT = kDocTile / BN;
+    unsigned long long meet = 0;
+    int meet_base = -1;
+    auto next = [&](int t) {
+        if (!p.docs) return t;
+        while (t < t1) {
+            const int rt = t / RT;
+            if (meet_base < 0 || rt >= meet_base + 64) {
+                meet_base = rt;
+                meet = tiles_meeting(ranges, rt, p.range_tiles, docs_group);
+            }
+            const unsigned long long left = meet >> (rt - meet_base);
+            if (left & 1) return t;
+            t = left ? (rt + __builtin_ctzll(left)) * RT : (meet_base + 64) * RT;
+        }
+        return t1;
+    };
+    const char* kb = p.k + (b * p.k_sb + kvh * p.k_sh) * T::ES;
+    const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh) * T::ES;
+    using L = Loader<Tr, DP, BN, NW>;
+    auto issue = [&](int t, int stage) {
+        const int last = span.end - 1 - t * BN;
+        L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks);
+        L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks);
+    };
+
+    f32x16_t acc[T::DT];
+#pragma unroll
+    for (int dt = 0; dt < T::DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
+    const float unit = FORM != kPlain ? 1.0f : p.scale2;
+
+    int t = next(0), stage = 0;
+    if (t < t1) issue(t, 0);
+    while (t < t1) {
+        publish();
+        const int tn = next(t + 1);
+        if (tn < t1) issue(tn, stage ^ 1);
+        const int j0 = t * BN;
+        if (j0 < lim_max) {
+            const lds_char* kt = lds + stage * 2 * TILEB;
+            const lds_char* vt = kt + TILEB;
+            bool same = true;
+            if (p.docs) {
+                const int2 kr = ranges[t / RT];
+                same = kr.x == kr.y && docs_wave.x == docs_wave.y && kr.x == docs_wave.x;
+            }
+            const bool masked = j0 + BN > lim_min || !same;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                f32x16_t s, g;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = g[e] = 0.0f;
+#pragma unroll
+                for (int f = 0; f < T::NF; ++f) {
+                    Tr::mma(T::frag(kt, mt * 32, f), qf[f], s);
+                    Tr::mma(T::frag(vt, mt * 32, f), gf[f], g);
+                }
+                settle<Tr>(s);
+                settle<Tr>(g);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+                    float slope = 1.0f, t2 = s[e];
+                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, slope2, (float)(pos - j), slope);
+                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, -lse));
+                    float ds = pr * (g[e] - delta);
+                    if (FORM == kCap) ds *= slope;
+                    if (Shift<Tr>::bwd != 0.0f) ds *= hold;
+                    s[e] = ds;
+                }
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+                        bool seen = j < lim;
+                        if (!same) seen = seen && doc_at(p, b, j) == doc;
+                        s[e] = seen ? s[e] : 0.0f;
+                    }
+                }
+                T::second(kt, mt * 32, s, acc);
+            }
+        }
+        t = tn;
+        stage ^= 1;
+    }
+#pragma unroll
+    for (int dt = 0; dt < T::DT; ++dt) settle<Tr>(acc[dt]);
+    if (r >= p.rows) return;
+    store_row<Tr, T::DT>(p.dq + (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES, p.dim, acc, p.scale / hold);
+}
+
+// dk and dv. A wave owns 32 keys, one per lane's column: their k and v stay in
+// registers as second operands, and tiles of BM rows of q and dout pass through
+// LDS. Here the accumulators of the first products hold rows in their registers
+// and a key per lane, so what belongs to a row (its sum, delta, limit, position)
+// comes from LDS, four rows at a time. DV, DK: which gradients this launch makes
+// (32-bit rows of 256 features hold the registers of one at a time).
+template <class Tr, int DP, int FORM, bool DK, bool DV>
+__global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
+    using T = Tile<Tr, DP>;
+    constexpr int NW = 4, BM = 32, TILEB = BM * T::ROWB;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
+    __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM], row_slope[2][BM];
+    __shared__ __attribute__((aligned(16))) int row_lim[2][BM], row_pos[2][BM], row_doc[2][BM];
+    lds_char* lds = (lds_char*)smem;
+
+    const int total = p.key_blocks * p.key_splits * p.batch * p.kv_heads, item = xcd_item(total);
+    if (item >= total) return;
+    const int split = item % p.key_splits, rest = item / p.key_splits;
+    const int kblock = rest % p.key_blocks, bh = rest / p.key_blocks;  // the first keys have the most causal rows
+    const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+
+    const Span span(p, b);
+    const int k0 = kblock * NW * 32, kw = k0 + wave * 32;  // first key of the group, of the wave
+    const int key = kw + (lane & 31), keyc = min(key, max(span.end - 1, 0));
+    const int doc = p.docs && key < span.end ? doc_at(p, b, key) : -1;
+    const int first_doc = p.docs ? __builtin_amdgcn_readfirstlane(doc) : 0;
+    const bool one_doc = p.docs && __all(doc == first_doc) && first_doc >= 0;
+    const float hold = grad_hold<Tr>(p), shift = Shift<Tr>::bwd;
+    const float hold_p = Shift<Tr>::bwd != 0.0f ? hold * __builtin_amdgcn_exp2f(-shift) : 1.0f;
+    u32x4_t kf[T::NF], vf[T::NF];
+    T::row_frags(p.k + (b * p.k_sb + (long long)keyc * p.k_sl + kvh * p.k_sh) * T::ES, p.chunks, kf);
+    if (DK) T::row_frags(p.v + (b * p.v_sb + (long long)keyc * p.v_sl + kvh * p.v_sh) * T::ES, p.chunks, vf);
+
+    // Tiles of rows that can see the group's keys.
+    const int tiles = (p.rows + BM - 1) / BM;
+    int lo = 0, hi = tiles;
+    if (k0 >= span.end) hi = 0;
+    else if (p.causal && span.prefix <= k0) lo = min(tiles, (int)((long long)max(0, k0 - span.off) * p.group / BM));
+    const int per = (max(hi - lo, 0) + p.key_splits - 1) / p.key_splits;
+    const int t0 = min(lo + split * per, hi), t1 = min(t0 + per, hi);
+
+    // With documents, tiles whose positions share none with the group's keys are passed over.
+    const int2* ranges = p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr;
+    int2 mine = make_int2(0x7fffffff, -1);
+    if (p.docs)
+        for (int c = k0 / kDocTile; c < min(p.range_tiles, (k0 + NW * 32 + kDocTile - 1) / kDocTile); ++c) {
+            const int2 q = ranges[c];
+            mine.x = min(mine.x, q.x);
+            mine.y = max(mine.y, q.y);
+        }
+    unsigned long long meet = 0;
+    int meet_base = -1;
+    auto next = [&](int t) {
+        if (!p.docs) return t;
+        while (t < t1) {
+            if (meet_base < 0 || t >= meet_base + 64) {
+                meet_base = t;
+                const int at = t + lane;
+                bool yes = false;
+                if (at < t1) {
+                    const int a = max(at * BM / p.group + span.off, 0);
+                    const int z = min((min(at * BM + BM, p.rows) - 1) / p.group + span.off, p.keys - 1);
+                    for (int c = a / kDocTile; z >= 0 && c <= z / kDocTile; ++c)
+                        yes = yes || (ranges[c].x <= mine.y && mine.x <= ranges[c].y);
+                }
+                meet = __ballot(yes);
+            }
+            const unsigned long long left = meet >> (t - meet_base);
+            if (left & 1) return t;
+            t = left ? t + __builtin_ctzll(left) : meet_base + 64;
+        }
+        return t1;
+    };
+    const char* qb = p.q + (b * p.q_sb + (long long)kvh * p.group * p.q_sh) * T::ES;
+    const char* gb = p.dout + (b * p.do_sb + (long long)kvh * p.group * p.do_sh) * T::ES;
+    using L = Loader<Tr, DP, BM, NW>;
+    auto issue = [&](int t, int stage) {
+        const int r0 = t * BM, i0 = r0 / p.group;
+        const char* qt = uniform_ptr(qb + (long long)i0 * p.q_sl * T::ES);
+        const char* gt = uniform_ptr(gb + (long long)i0 * p.do_sl * T::ES);
+        unsigned qo[L::PER], go[L::PER];
+#pragma unroll
+        for (int s = 0; s < L::PER; ++s) {
+            const int row = L::seg_row(s), rr = min(r0 + row, p.rows - 1);
+            const int i = (int)ormi_fdiv((unsigned)rr, p.group_m, p.group_s), g = rr - i * p.group;
+            const unsigned c = L::seg_chunk(row, p.chunks);
+            qo[s] = ((unsigned)(i - i0) * (unsigned)p.q_sl + (unsigned)g * (unsigned)p.q_sh) * T::ES + c;
+            go[s] = ((unsigned)(i - i0) * (unsigned)p.do_sl + (unsigned)g * (unsigned)p.do_sh) * T::ES + c;
+        }
+        L::load(lds + stage * 2 * TILEB, qt, qo);
+        L::load(lds + stage * 2 * TILEB + TILEB, gt, go);
+    };
+    // What belongs to the rows of a tile, one row per lane of the first wave:
+    // fetched before the tile's own loads, written behind the previous tile's work.
+    struct Row { float lse, delta, slope; int lim, pos, doc; };
+    auto fetch = [&](int t) {
+        Row m = {kInf, 0.0f, 0.0f, 0, 0, -1};
+        const int rr = t * BM + (int)threadIdx.x;
+        if (threadIdx.x < BM && rr < p.rows) {
+            const int i = (int)ormi_fdiv((unsigned)rr, p.group_m, p.group_s);
+            m.lse = p.lse[(long long)bh * p.rows + rr] - shift;
+            m.delta = p.delta[(long long)bh * p.rows + rr];
+            m.pos = i + span.off;
+            m.lim = span.limit(p, m.pos);
+            if (p.docs) {
+                m.doc = doc_at(p, b, m.pos);
+                if (m.doc < 0) m.lim = 0;
+            }
+            if (FORM != kPlain && p.slopes) m.slope = p.slopes[kvh * p.group + rr - i * p.group] * 1.44269504f;
+        }
+        return m;
+    };
+    auto put = [&](const Row& m, int stage) {
+        if (threadIdx.x < BM) {
+            row_lse[stage][threadIdx.x] = m.lse;
+            row_delta[stage][threadIdx.x] = m.delta;
+            row_lim[stage][threadIdx.x] = m.lim;
+            if (FORM != kPlain) {
+                row_slope[stage][threadIdx.x] = m.slope;
+                row_pos[stage][threadIdx.x] = m.pos;
+            }
+            if (p.docs) row_doc[stage][threadIdx.x] = m.doc;
+        }
+    };
+
+    f32x16_t acc_k[T::DT], acc_v[T::DT];
+#pragma unroll
+    for (int dt = 0; dt < T::DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc_k[dt][e] = acc_v[dt][e] = 0.0f;
+    const float unit = FORM != kPlain ? 1.0f : p.scale2;
+
+    int t = next(t0), stage = 0;
+    if (t < t1) {
+        put(fetch(t), 0);
+        issue(t, 0);
+    }
+    while (t < t1) {
+        publish();
+        const int tn = next(t + 1);
+        Row ahead;
+        if (tn < t1) {
+            ahead = fetch(tn);
+            issue(tn, stage ^ 1);
+        }
+        const int lim_lane = row_lim[stage][lane & 31];
+        if (__any(lim_lane > kw)) {
+            const lds_char* qt = lds + stage * 2 * TILEB;
+            const lds_char* gt = qt + TILEB;
+            bool same = true;
+            if (p.docs) same = one_doc && __all(row_doc[stage][lane & 31] == first_doc);
+            const bool masked = !__all(lim_lane >= kw + 32) || !same;
+            f32x16_t s, g;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = g[e] = 0.0f;
+#pragma unroll
+            for (int f = 0; f < T::NF; ++f) {
+                Tr::mma(T::frag(qt, 0, f), kf[f], s);
+                if (DK) Tr::mma(T::frag(gt, 0, f), vf[f], g);
+            }
+            settle<Tr>(s);
+            if (DK) settle<Tr>(g);
+            f32x16_t slope;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const int row = 8 * q4 + 4 * half;
+                const float4 ls = *(const float4*)&row_lse[stage][row];
+                const float* lsv = (const float*)&ls;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = 4 * q4 + e;
+                    float t2 = s[x], sl = 1.0f;
+                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, row_slope[stage][row + e], (float)(row_pos[stage][row + e] - key), sl);
+                    if (FORM == kCap) slope[x] = sl;
+                    s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, -lsv[e]));
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const int row = 8 * (x >> 2) + 4 * half + (x & 3);
+                    bool seen = key < row_lim[stage][row];
+                    if (!same) seen = seen && row_doc[stage][row] == doc;
+                    s[x] = seen ? s[x] : 0.0f;
+                    if (DK) g[x] = seen ? g[x] : 0.0f;
+                }
+            }
+            if (DV) T::second(gt, 0, s, acc_v);
+            if (DK) {
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const float4 de = *(const float4*)&row_delta[stage][8 * q4 + 4 * half];
+                    const float* dev = (const float*)&de;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int x = 4 * q4 + e;
+                        float ds = s[x] * (g[x] - dev[e]);
+                        if (FORM == kCap) ds *= slope[x];
+                        if (Shift<Tr>::bwd != 0.0f) ds *= hold_p;
+                        s[x] = ds;
+                    }
+                }
+                T::second(qt, 0, s, acc_k);
+            }
+        }
+        if (tn < t1) put(ahead, stage ^ 1);
+        t = tn;
+        stage ^= 1;
+    }
+#pragma unroll
+    for (int dt = 0; dt < T::DT; ++dt) {
+        if (DK) settle<Tr>(acc_k[dt]);
+        if (DV) settle<Tr>(acc_v[dt]);
+    }
+    if (key >= p.keys) return;
+    if (p.key_splits > 1) {
+        const long long n = (long long)p.batch * p.kv_heads * p.keys, at = (long long)bh * p.keys + key;
+        if (DK) store_part(p.part + (split * n + at) * DP, acc_k);
+        if (DV) store_part(p.part + ((p.key_splits + split) * n + at) * DP, acc_v);
+        return;
+    }
+    const long long at = (((long long)b * p.keys + key) * p.kv_heads + kvh) * p.dim * T::ES;
+    if (DK && p.dk) store_row<Tr, T::DT>(p.dk + at, p.dim, acc_k, p.scale / hold);
+    if (DV && p.dv) store_row<Tr, T::DT>(p.dv + at, p.dim, acc_v, __builtin_amdgcn_exp2f(-shift));
+}
+
+// Adds the splits' partial dk and dv in split order. One wave per key.
+template <class Tr, int DP>
+__global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttnParams p) {
+    const long long n = (long long)p.batch * p.kv_heads * p.keys;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= n) return;
+    const int bh = (int)(row / p.keys), j = (int)(row % p.keys), b = bh / p.kv_heads, kvh = bh % p.kv_heads;
+    const long long at = (((long long)b * p.keys + j) * p.kv_heads + kvh) * p.dim;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        char* out = which == 0 ? p.dk : p.dv;
+        if (!out) continue;
+        const float f = which == 0 ? p.scale / grad_hold<Tr>(p) : __builtin_amdgcn_exp2f(-Shift<Tr>::bwd);
+#pragma unroll
+        for (int e = 0; e < DP / 64; ++e) {
+            const int d = e * 64 + lane;
+            float v = 0.0f;
+            for (int s = 0; s < p.key_splits; ++s) v += p.part[((which * p.key_splits + s) * n + row) * DP + d];
+            v *= f;
+            if (d >= p.dim) continue;
+            if constexpr (Tr::ESIZE == 4) ((float*)out)[at + d] = v;
+            else ((unsigned short*)out)[at + d] = (unsigned short)pack2(Tr{}, v, v);
+        }
+    }
+}
+
+template <class Tr, int DP, int FORM>
+void launch_attention_grad_form(const AttnParams& p) {
+    if (p.dq) {
+        const unsigned items = (unsigned)(p.row_blocks * p.batch * p.kv_heads);
+        attention_dq_kernel<Tr, DP, fwd_tile(DP, Tr::ESIZE, false), FORM><<<(items + 7) / 8 * 8, 256>>>(p);
+    }
+    if (p.dk || p.dv) {
+        const unsigned items = (unsigned)(p.key_blocks * p.key_splits * p.batch * p.kv_heads), grid = (items + 7) / 8 * 8;
+        if constexpr (DP * Tr::ESIZE > 512) {
+            if (p.dk) attention_dkv_kernel<Tr, DP, FORM, true, false><<<grid, 256>>>(p);
+            if (p.dv) attention_dkv_kernel<Tr, DP, FORM, false, true><<<grid, 256>>>(p);
+        } else {
+            attention_dkv_kernel<Tr, DP, FORM, true, true><<<grid, 256>>>(p);
+        }
+    }
+}
+
+template <class Tr, int DP>
+int launch_attention_grad_dp(const AttnParams& p, float* delta, unsigned* bounds) {
+    const long long rows = (long long)p.batch * p.queries * p.heads, values = (long long)p.batch * p.keys * p.kv_heads;
+    const unsigned row_groups = (unsigned)((rows + 15) / 16), value_groups = bounds ? (unsigned)((values + 15) / 16) : 0;
+    attention_delta_kernel<Tr><<<row_groups + value_groups, 256>>>(p, delta, bounds, row_groups);
+    if (p.form == kPlain) launch_attention_grad_form<Tr, DP, kPlain>(p);
+    else if (p.form == kBias) launch_attention_grad_form<Tr, DP, kBias>(p);
+    else launch_attention_grad_form<Tr, DP, kCap>(p);
+    if ((p.dk || p.dv) && p.key_splits > 1) attention_dkv_join_kernel<Tr, DP><<<(unsigned)((values + 3) / 4), 256>>>(p);
+    return (int)hipGetLastError();
+}
+
+}  // namespace ormi_hip
