@@ -434,6 +434,8 @@ int ormi_hip_rotary(const ormi_rotary_desc* desc);
  * q, k, v are strided views; out is contiguous. dtype is F32, BF16 or F16;
  * scores, sums and the softmax are fp32, out is rounded once. 16-bit
  * probabilities are rounded to 16 bits for their product with v.
+ * rest (or NULL; not read or written for F32) receives what out's rounding to
+ * 16 bits left, itself rounded to them: the gradient is more exact with it.
  * lse (or NULL) receives log2 of each row's sum of exponentials, (batch,
  * kv_heads, queries, heads / kv_heads), +inf where nothing is seen: the
  * gradient needs it.
@@ -456,6 +458,7 @@ typedef struct ormi_attention_desc {
     const int32_t* prefix;                                    /* (batch), or NULL */
     const int32_t* lengths;                                   /* (batch), or NULL */
     void*          out;
+    void*          rest;                                      /* laid out like out, or NULL */
     float*         lse;
     void*          workspace;
     size_t         workspace_bytes;
@@ -464,7 +467,7 @@ int ormi_hip_attention_workspace_size(const ormi_attention_desc* desc, size_t* b
 int ormi_hip_attention(const ormi_attention_desc* desc);
 
 /* The gradient of ormi_hip_attention with respect to q, k and v. forward
- * describes the call that was made, with its out and lse; its workspace fields
+ * describes the call that was made, with its out, rest and lse; its workspace fields
  * hold this call's workspace. dout is a view like q, of the same dtype; dq, dk
  * and dv are contiguous, laid out like q, k and v's extents, of the same dtype
  * (NULL: not wanted). Shared key heads' gradients add up over their query

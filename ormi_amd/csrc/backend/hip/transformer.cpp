@@ -129,9 +129,11 @@ namespace ormi::hip {
         std::vector<NodePtr> hold;
         ormi_attention_desc d = attention_desc(a, n->parents.data(), hold);
         auto out = empty(n->view.shape, DeviceEnum::HIP, n->dtype);
-        std::shared_ptr<Buffer> lse;
+        std::shared_ptr<Buffer> lse, rest;
+        if (n->requires_grad && n->dtype != DType::Float32) rest = empty(n->view.shape, DeviceEnum::HIP, n->dtype);
         if (n->requires_grad) lse = empty({d.batch, d.kv_heads, d.queries, d.heads / d.kv_heads}, DeviceEnum::HIP);
         d.out = out->ptr;
+        d.rest = rest ? rest->ptr : nullptr;
         d.lse = lse ? (float*)lse->ptr : nullptr;
         size_t bytes = 0;
         ORMI_HIP_CHECK(ormi_hip_attention_workspace_size(&d, &bytes));
@@ -139,6 +141,7 @@ namespace ormi::hip {
         if (ws) d.workspace = ws->ptr, d.workspace_bytes = ws->bytes;
         ORMI_HIP_CHECK(ormi_hip_attention(&d));
         a.saved->lse = lse;
+        a.saved->rest = rest;
         n->data = out;
         n->view.strides = calc_contiguous_strides(n->view.shape);
     }
@@ -155,6 +158,7 @@ namespace ormi::hip {
             ormi_attention_grad_desc d{};
             d.forward = attention_desc(a, n->parents.data() + 2, hold);
             d.forward.out = out->data->ptr;
+            d.forward.rest = a.saved->rest ? a.saved->rest->ptr : nullptr;
             d.forward.lse = (float*)a.saved->lse->ptr;
             d.dout = g->data->ptr;
             strides4(*g, d.dout_strides);

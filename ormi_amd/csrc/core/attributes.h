@@ -37,8 +37,9 @@ namespace ormi {
         float scale = 1.0f, cap = 0.0f;
         bool causal = false;
         bool slopes = false, documents = false, prefix = false, lengths = false;
-        // What realizing the node leaves for its gradient: each row's log-sum.
-        struct Saved { std::shared_ptr<Buffer> lse; };
+        // What realizing the node leaves for its gradient: each row's log-sum, and
+        // what rounding a 16-bit result left.
+        struct Saved { std::shared_ptr<Buffer> lse, rest; };
         std::shared_ptr<Saved> saved;
         // The gradients of one backward pass are computed together by the first
         // of them that is realized; the others take theirs from here.

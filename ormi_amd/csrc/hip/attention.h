@@ -20,6 +20,7 @@ constexpr int fwd_tile(int dp, int es, bool few) { return few || es == 4 || dp >
 struct AttnParams {
     const char *q, *k, *v;
     char* out;
+    char* rest;  // 16-bit: what out's rounding left, rounded in turn, laid out like out
     float* lse;  // base-2 logarithm of a row's sum, (batch, kv head, row); +inf: the row sees no key
     long long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;  // strides in elements
     int batch, queries, keys, heads, kv_heads, group, dim;

@@ -134,6 +134,7 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
     p.lengths = d->lengths;
     p.out = (char*)d->out;
     p.lse = d->lse;
+    p.rest = d->dtype == ORMI_DTYPE_F32 ? nullptr : (char*)d->rest;
     p.form = d->cap > 0.0f ? kCap : d->slopes || !(p.scale2 > 0.0f) ? kBias : kPlain;
     const int es = pl.es = d->dtype == ORMI_DTYPE_F32 ? 4 : 2, ve = 16 / es;
     pl.padded = (d->dim + ve - 1) / ve * ve;
@@ -262,6 +263,7 @@ int ormi_hip_attention(const ormi_attention_desc* desc) {
         const float none = __builtin_huge_valf();
         const size_t rows = (size_t)desc->batch * desc->queries * desc->heads;
         if ((rc = zeros(desc->out, rows * desc->dim, pl.es)) != ORMI_HIP_OK) return rc;
+        if ((rc = zeros(pl.p.rest, rows * desc->dim, pl.es)) != ORMI_HIP_OK) return rc;
         return desc->lse ? ormi_hip_fill(desc->lse, &none, 4, rows) : ORMI_HIP_OK;
     }
     settle(pl, (char*)desc->workspace, desc, nullptr);

@@ -54,6 +54,12 @@ __device__ __forceinline__ unsigned pack2(TrF16, float a, float b) {
     const f32x2_t f = {a, b};
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f, f16x2_t));
 }
+template <class Tr> struct IsF16 { static constexpr bool value = false; };
+template <> struct IsF16<TrF16> { static constexpr bool value = true; };
+template <class Tr>
+__device__ __forceinline__ float unpack(unsigned low16) {
+    return IsF16<Tr>::value ? ormi_f16_to_f32((unsigned short)low16) : ormi_bf16_to_f32((unsigned short)low16);
+}
 // NaN when any is: a row with a NaN score is NaN whatever its maximum.
 __device__ __forceinline__ float max3(float a, float b, float c) { return ormi_maximum(ormi_maximum(a, b), c); }
 // Both halves of the wave hold the result for lane % 32.
@@ -302,9 +308,10 @@ __device__ __forceinline__ float score2(const AttnParams& p, float s, float slop
 
 // ---------------------------------------------------------------- outputs --
 // Accumulators acc[dt][r], feature 32 dt + 8 (r / 4) + 4 half + r % 4 of the
-// lane's row, times f, rounded once to the output's type.
+// lane's row, times f, rounded once to the output's type; what that left goes to
+// `rest` (or null), rounded in turn.
 template <class Tr, int DT>
-__device__ __forceinline__ void store_row(char* row, int dim, const f32x16_t (&acc)[DT], float f) {
+__device__ __forceinline__ void store_row(char* row, int dim, const f32x16_t (&acc)[DT], float f, char* rest = nullptr) {
     const int half = (threadIdx.x & 63) >> 5;
     const bool vec = dim % 4 == 0;
 #pragma unroll
@@ -324,14 +331,22 @@ __device__ __forceinline__ void store_row(char* row, int dim, const f32x16_t (&a
                     for (int e = 0; e < 4; ++e)
                         if (d + e < dim) o[e] = v[e];
             } else {
-                const uint2 w = make_uint2(pack2(Tr{}, v[0], v[1]), pack2(Tr{}, v[2], v[3]));
-                unsigned short* o = (unsigned short*)row + d;
-                if (vec) *(uint2*)o = w;
-                else {
-                    o[0] = (unsigned short)w.x;
-                    if (d + 1 < dim) o[1] = (unsigned short)(w.x >> 16);
-                    if (d + 2 < dim) o[2] = (unsigned short)w.y;
-                    if (d + 3 < dim) o[3] = (unsigned short)(w.y >> 16);
+                uint2 w = make_uint2(pack2(Tr{}, v[0], v[1]), pack2(Tr{}, v[2], v[3]));
+                auto put = [&](char* to) {
+                    unsigned short* o = (unsigned short*)to + d;
+                    if (vec) *(uint2*)o = w;
+                    else {
+                        o[0] = (unsigned short)w.x;
+                        if (d + 1 < dim) o[1] = (unsigned short)(w.x >> 16);
+                        if (d + 2 < dim) o[2] = (unsigned short)w.y;
+                        if (d + 3 < dim) o[3] = (unsigned short)(w.y >> 16);
+                    }
+                };
+                put(row);
+                if (rest) {
+                    w = make_uint2(pack2(Tr{}, v[0] - unpack<Tr>(w.x), v[1] - unpack<Tr>(w.x >> 16)),
+                                   pack2(Tr{}, v[2] - unpack<Tr>(w.y), v[3] - unpack<Tr>(w.y >> 16)));
+                    put(rest);
                 }
             }
         }
@@ -533,7 +548,8 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
         if (half == 0) p.part_ml[at] = make_float2(m == -kInf ? -kInf : m * unit - Shift<Tr>::fwd, l);
         return;
     }
-    store_row<Tr, T::DT>(p.out + (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES, p.dim, acc, l == 0.0f ? 0.0f : 1.0f / l);
+    const long long to = (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES;
+    store_row<Tr, T::DT>(p.out + to, p.dim, acc, l == 0.0f ? 0.0f : 1.0f / l, p.rest ? p.rest + to : nullptr);
     if (p.lse && half == 0) p.lse[(long long)bh * p.rows + r] = l == 0.0f ? kInf : m * unit - Shift<Tr>::fwd + __builtin_log2f(l);
 }
 
@@ -568,7 +584,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
         if (d < p.dim) {
             const float v = o[e] * inv;
             if constexpr (Tr::ESIZE == 4) ((float*)p.out)[at + d] = v;
-            else ((unsigned short*)p.out)[at + d] = (unsigned short)pack2(Tr{}, v, v);
+            else {
+                const unsigned w = pack2(Tr{}, v, v);
+                ((unsigned short*)p.out)[at + d] = (unsigned short)w;
+                if (p.rest) {
+                    const float left = v - unpack<Tr>(w);
+                    ((unsigned short*)p.rest)[at + d] = (unsigned short)pack2(Tr{}, left, left);
+                }
+            }
         }
     }
     if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? kInf : top + __builtin_log2f(l);
@@ -595,7 +618,9 @@ int launch_attention_fwd_dp(const AttnParams& p) {
 }
 
 // --------------------------------------------------------------- gradient --
-// delta = sum of out * dout of a row; 16 lanes per row. float16 also collects
+// delta = sum of out * dout of a row; 16 lanes per row. out comes with what its
+// rounding left: an error of delta is common to a row's score gradients, and in
+// short rows it would be as large as their own rounding. float16 also collects
 // the largest squared norms of a dout row and of a value row: |score gradient|
 // <= p (|dp| + |delta|) <= 2 |dout| |v|, and held times the power of two that
 // takes that bound to 2^15 the score gradients keep to float16's normal range
@@ -603,9 +628,7 @@ int launch_attention_fwd_dp(const AttnParams& p) {
 template <class Tr>
 __device__ __forceinline__ float load1(const char* row, int d) {
     if constexpr (Tr::ESIZE == 4) return ((const float*)row)[d];
-    const unsigned short h = ((const unsigned short*)row)[d];
-    if constexpr (sizeof(Shift<Tr>) && Shift<Tr>::bwd != 0.0f) return ormi_f16_to_f32(h);
-    return ormi_bf16_to_f32(h);
+    else return unpack<Tr>(((const unsigned short*)row)[d]);
 }
 template <class Tr>
 __device__ __forceinline__ void load_chunk(const char* at, float (&v)[Tr::VE]) {
@@ -613,10 +636,7 @@ __device__ __forceinline__ void load_chunk(const char* at, float (&v)[Tr::VE]) {
 #pragma unroll
     for (int e = 0; e < Tr::VE; ++e) {
         if constexpr (Tr::ESIZE == 4) v[e] = __uint_as_float(w[e]);
-        else {
-            const unsigned short h = (unsigned short)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
-            v[e] = Shift<Tr>::bwd != 0.0f ? ormi_f16_to_f32(h) : ormi_bf16_to_f32(h);
-        }
+        else v[e] = unpack<Tr>(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
     }
 }
 template <class Tr>
@@ -632,12 +652,19 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(AttnParams p, floa
         const long long bi = row / p.heads;
         const int b = (int)(bi / p.queries), i = (int)(bi % p.queries);
         const char* o = p.out + row * p.dim * Tr::ESIZE;
+        const char* rest = p.rest ? p.rest + row * p.dim * Tr::ESIZE : nullptr;
         const char* g = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * Tr::ESIZE;
         if (p.dim % Tr::VE == 0) {
             for (int c = sub; c < p.dim / Tr::VE; c += 16) {
                 float x[Tr::VE], y[Tr::VE];
                 load_chunk<Tr>(o + c * 16, x);
                 load_chunk<Tr>(g + c * 16, y);
+                if (rest) {
+                    float z[Tr::VE];
+                    load_chunk<Tr>(rest + c * 16, z);
+#pragma unroll
+                    for (int e = 0; e < Tr::VE; ++e) x[e] += z[e];
+                }
 #pragma unroll
                 for (int e = 0; e < Tr::VE; ++e) {
                     dot = __builtin_fmaf(x[e], y[e], dot);
@@ -647,7 +674,7 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(AttnParams p, floa
         } else {
             for (int d = sub; d < p.dim; d += 16) {
                 const float y = load1<Tr>(g, d);
-                dot = __builtin_fmaf(load1<Tr>(o, d), y, dot);
+                dot = __builtin_fmaf(load1<Tr>(o, d) + (rest ? load1<Tr>(rest, d) : 0.0f), y, dot);
                 norm = __builtin_fmaf(y, y, norm);
             }
         }

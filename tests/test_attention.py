@@ -247,7 +247,7 @@ def test_offsets_past_32_bits(hip, cabi):
                     ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_strides", ctypes.c_int64 * 4), ("k_strides", ctypes.c_int64 * 4),
                     ("v_strides", ctypes.c_int64 * 4), ("scale", ctypes.c_float), ("cap", ctypes.c_float), ("causal", ctypes.c_int),
                     ("slopes", ctypes.c_void_p), ("documents", ctypes.c_void_p), ("documents_batch_stride", ctypes.c_int64),
-                    ("prefix", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                    ("prefix", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("out", ctypes.c_void_p), ("rest", ctypes.c_void_p), ("lse", ctypes.c_void_p),
                     ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
     cabi.ormi_hip_attention.argtypes = [ctypes.POINTER(Desc)]
@@ -279,7 +279,7 @@ def test_offsets_past_32_bits(hip, cabi):
                     assert cabi.ormi_hip_memcpy_h2d(ctypes.c_void_p(at), row.ctypes.data, row.nbytes) == 0
         strides = (ctypes.c_int64 * 4)(batch_stride, token_stride, 64, 1)
         d = Desc(0, 2, 1, 3, 2, 1, 64, small[0], big, vbig, (ctypes.c_int64 * 4)(128, 128, 64, 1), strides, strides, 1 / 8, 0.0, 0, None, None, 0,
-                 None, None, small[1], None, None, 0)
+                 None, None, small[1], None, None, None, 0)
         n = ctypes.c_size_t()
         assert cabi.ormi_hip_attention_workspace_size(ctypes.byref(d), ctypes.byref(n)) == 0
         ws = malloc(max(n.value, 1))
