@@ -66,7 +66,7 @@ struct Plan {
     Operand q, k, v, g;
     int es = 0, padded = 0;
     bool empty = false;
-    size_t ranges = 0, part = 0, part_ml = 0, delta = 0, bounds = 0, bytes = 0;
+    size_t ranges = 0, part = 0, part_q = 0, part_ml = 0, delta = 0, bounds = 0, bytes = 0;
     bool hold = false;  // float16 gradients
 };
 
@@ -183,6 +183,10 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
         const int tiles = (p.rows + 31) / 32;
         p.key_splits = items > 0 ? (int)std::max<long long>(1, std::min<long long>({slots / items, tiles / 8, 16})) : 1;
         if (p.key_splits > 1 && (g->dk || g->dv)) pl.part = take(pl.bytes, 2 * sizeof(float) * (size_t)p.key_splits * heads * d->keys * dp);
+        const long long row_items = heads * p.row_blocks;
+        const int key_tiles = (d->keys + 31) / 32;
+        p.splits = row_items > 0 && row_items * 2 <= cus * 2 ? (int)std::max<long long>(1, std::min<long long>({cus * 2 / row_items, key_tiles / 4, 16})) : 1;
+        if (p.splits > 1 && g->dq) pl.part_q = take(pl.bytes, sizeof(float) * (size_t)p.splits * heads * p.rows * dp);
         if (items * p.key_splits >= (1ll << 30) || heads * p.row_blocks >= (1ll << 30)) return bad("too many work-groups");
         pl.delta = take(pl.bytes, sizeof(float) * (size_t)heads * p.rows);
         pl.hold = d->dtype == ORMI_DTYPE_F16;
@@ -223,6 +227,7 @@ void settle(Plan& pl, char* ws, const ormi_attention_desc* d, const ormi_attenti
         p.ranges = r;
     }
     p.part = (float*)(ws + pl.part);
+    p.part_q = (float*)(ws + pl.part_q);
     p.part_ml = (float2*)(ws + pl.part_ml);
 }
 

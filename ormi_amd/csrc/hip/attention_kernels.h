@@ -28,6 +28,7 @@
 // reads nor the transposing reads meet in a bank.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cstdint>
 
 #include "attention.h"
@@ -285,12 +286,36 @@ __device__ __forceinline__ int2 widen(int lo, int hi, bool none) {
     return hi < 0x7fffffff ? make_int2(lo, hi + 1) : make_int2(lo - 1, hi);
 }
 
-// Bits of tiles base + lane: those that share a document with `mine`.
-__device__ __forceinline__ unsigned long long tiles_meeting(const int2* ranges, int base, int tiles, int2 mine) {
-    const int t = base + (int)(threadIdx.x & 63);
-    const int2 r = t < tiles ? ranges[t] : make_int2(0x7fffffff, -1);
-    return __ballot(t < tiles && r.x <= mine.y && mine.x <= r.y);
-}
+// Walks the tiles of BN keys that share a document with a work-group's rows: 64
+// ranges at a time become two masks, of those that share one with the group and
+// of those whose keys and the wave's rows all have one and the same (no mask).
+template <int BN>
+struct DocTiles {
+    static constexpr int RT = kDocTile / BN;  // tiles per range
+    const int2* ranges;
+    int count, base = -1;
+    int2 group, wave;
+    unsigned long long meet = 0, one = 0;
+    // The next tile from t on, or end.
+    __device__ __forceinline__ int next(int t, int end) {
+        while (t < end) {
+            const int rt = t / RT;
+            if (base < 0 || rt >= base + 64) {
+                base = rt;
+                const int at = rt + (int)(threadIdx.x & 63);
+                const int2 r = at < count ? ranges[at] : make_int2(0x7fffffff, -1);
+                meet = __ballot(r.x <= group.y && group.x <= r.y);
+                one = __ballot(r.x == r.y && wave.x == wave.y && r.x == wave.x);
+            }
+            const unsigned long long left = meet >> (rt - base);
+            if (left & 1) return t;
+            t = left ? (rt + __builtin_ctzll(left)) * RT : (base + 64) * RT;
+        }
+        return end;
+    }
+    // Whether tile t, the last that next gave, needs no document mask.
+    __device__ __forceinline__ bool same(int t) const { return one >> (t / RT - base) & 1; }
+};
 
 // A score in powers of two; its derivative with respect to scale q.k in slope (kCap).
 template <class Tr, int FORM>
@@ -371,6 +396,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
     constexpr int MT = BN / 32, TILEB = BN * T::ROWB;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
     __shared__ int shared_i[3 * NW];
+    __shared__ __attribute__((aligned(16))) int key_doc[2][BN];  // of a stage's keys
     lds_char* lds = (lds_char*)smem;
 
     const int item = xcd_item(p.row_blocks * p.splits * p.batch * p.kv_heads);
@@ -424,25 +450,8 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
     const int per = (tiles + p.splits - 1) / p.splits;
     const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
 
-    const int2* ranges = p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr;
-    constexpr int RT = kDocTile / BN;  // tiles per range
-    unsigned long long meet = 0;
-    int meet_base = -1;
-    // The next tile from t on that shares a document with the rows, or t1.
-    auto next = [&](int t) {
-        if (!p.docs) return t;
-        while (t < t1) {
-            const int rt = t / RT;
-            if (meet_base < 0 || rt >= meet_base + 64) {
-                meet_base = rt;
-                meet = tiles_meeting(ranges, rt, p.range_tiles, docs_group);
-            }
-            const unsigned long long left = meet >> (rt - meet_base);
-            if (left & 1) return t;
-            t = left ? (rt + __builtin_ctzll(left)) * RT : (meet_base + 64) * RT;
-        }
-        return t1;
-    };
+    DocTiles<BN> walk{p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr, p.range_tiles, -1, docs_group, docs_wave};
+    auto next = [&](int t) { return p.docs ? walk.next(t, t1) : t; };
     const char* kb = p.k + (b * p.k_sb + kvh * p.k_sh) * T::ES;
     const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh) * T::ES;
     using L = Loader<Tr, DP, BN, NW>;
@@ -462,21 +471,33 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
     float m = -kInf, l = 0.0f;
     const float unit = FORM != kPlain ? 1.0f : p.scale2;
 
+    // The documents of a tile's keys, one per thread: fetched before the tile's own
+    // loads, written behind the previous tile's work.
+    auto fetch_docs = [&](int t) { return p.docs && threadIdx.x < BN ? doc_at(p, b, t * BN + (int)threadIdx.x) : -1; };
+    auto put_docs = [&](int doc, int stage) {
+        if (p.docs && threadIdx.x < BN) key_doc[stage][threadIdx.x] = doc;
+    };
+
     int t = next(t0), stage = 0;
-    if (t < t1) issue(t, 0);
+    bool same = !p.docs || (t < t1 && walk.same(t));
+    if (t < t1) {
+        put_docs(fetch_docs(t), 0);
+        issue(t, 0);
+    }
     while (t < t1) {
         publish();
         const int tn = next(t + 1);
-        if (tn < t1) issue(tn, stage ^ 1);
+        bool same_next = !p.docs;
+        int docs_next = -1;
+        if (tn < t1) {
+            if (p.docs) same_next = walk.same(tn);
+            docs_next = fetch_docs(tn);
+            issue(tn, stage ^ 1);
+        }
         const int j0 = t * BN;
         if (j0 < lim_max) {
             const lds_char* kt = lds + stage * 2 * TILEB;
             const lds_char* vt = kt + TILEB;
-            bool same = true;
-            if (p.docs) {
-                const int2 kr = ranges[t / RT];
-                same = kr.x == kr.y && docs_wave.x == docs_wave.y && kr.x == docs_wave.x;
-            }
             f32x16_t s[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -500,10 +521,20 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-                        bool seen = j < lim;
-                        if (!same) seen = seen && doc_at(p, b, j) == doc;
-                        s[mt][e] = seen ? s[mt][e] : -kInf;
+                        s[mt][e] = j < lim ? s[mt][e] : -kInf;
                     }
+                if (!same) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int4 kd = *(const int4*)&key_doc[stage][mt * 32 + 8 * q + 4 * half];
+                            s[mt][4 * q] = kd.x == doc ? s[mt][4 * q] : -kInf;
+                            s[mt][4 * q + 1] = kd.y == doc ? s[mt][4 * q + 1] : -kInf;
+                            s[mt][4 * q + 2] = kd.z == doc ? s[mt][4 * q + 2] : -kInf;
+                            s[mt][4 * q + 3] = kd.w == doc ? s[mt][4 * q + 3] : -kInf;
+                        }
+                }
             }
             float top = -kInf;
 #pragma unroll
@@ -534,7 +565,9 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) T::second(vt, mt * 32, s[mt], acc);
         }
+        if (tn < t1) put_docs(docs_next, stage ^ 1);
         t = tn;
+        same = same_next;
         stage ^= 1;
     }
 
@@ -642,64 +675,67 @@ __device__ __forceinline__ void load_chunk(const char* at, float (&v)[Tr::VE]) {
 template <class Tr>
 __global__ __launch_bounds__(256) void attention_delta_kernel(AttnParams p, float* delta, unsigned* bounds, unsigned row_groups) {
     const int sub = threadIdx.x & 15;
-    float dot = 0.0f, norm = 0.0f;
-    if (blockIdx.x < row_groups) {
-        const long long n = (long long)p.batch * p.queries * p.heads;
-        const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    float most_norm = 0.0f;
+    const bool rows = blockIdx.x < row_groups;
+    const long long n = rows ? (long long)p.batch * p.queries * p.heads : (long long)p.batch * p.keys * p.kv_heads;
+    const long long step = (long long)(rows ? row_groups : gridDim.x - row_groups) * 16;
+    for (long long at = (long long)(rows ? blockIdx.x : blockIdx.x - row_groups) * 16 + (threadIdx.x >> 4);
+         at - (threadIdx.x >> 4) < n; at += step) {
         const bool live = at < n;
         const long long row = live ? at : n - 1;
-        const int head = (int)(row % p.heads);
-        const long long bi = row / p.heads;
-        const int b = (int)(bi / p.queries), i = (int)(bi % p.queries);
-        const char* o = p.out + row * p.dim * Tr::ESIZE;
-        const char* rest = p.rest ? p.rest + row * p.dim * Tr::ESIZE : nullptr;
-        const char* g = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * Tr::ESIZE;
-        if (p.dim % Tr::VE == 0) {
-            for (int c = sub; c < p.dim / Tr::VE; c += 16) {
-                float x[Tr::VE], y[Tr::VE];
-                load_chunk<Tr>(o + c * 16, x);
-                load_chunk<Tr>(g + c * 16, y);
-                if (rest) {
-                    float z[Tr::VE];
-                    load_chunk<Tr>(rest + c * 16, z);
+        float dot = 0.0f, norm = 0.0f;
+        if (rows) {
+            const int head = (int)(row % p.heads);
+            const long long bi = row / p.heads;
+            const int b = (int)(bi / p.queries), i = (int)(bi % p.queries);
+            const char* o = p.out + row * p.dim * Tr::ESIZE;
+            const char* rest = p.rest ? p.rest + row * p.dim * Tr::ESIZE : nullptr;
+            const char* g = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * Tr::ESIZE;
+            if (p.dim % Tr::VE == 0) {
+                for (int c = sub; c < p.dim / Tr::VE; c += 16) {
+                    float x[Tr::VE], y[Tr::VE];
+                    load_chunk<Tr>(o + c * 16, x);
+                    load_chunk<Tr>(g + c * 16, y);
+                    if (rest) {
+                        float z[Tr::VE];
+                        load_chunk<Tr>(rest + c * 16, z);
 #pragma unroll
-                    for (int e = 0; e < Tr::VE; ++e) x[e] += z[e];
+                        for (int e = 0; e < Tr::VE; ++e) x[e] += z[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < Tr::VE; ++e) {
+                        dot = __builtin_fmaf(x[e], y[e], dot);
+                        norm = __builtin_fmaf(y[e], y[e], norm);
+                    }
                 }
-#pragma unroll
-                for (int e = 0; e < Tr::VE; ++e) {
-                    dot = __builtin_fmaf(x[e], y[e], dot);
-                    norm = __builtin_fmaf(y[e], y[e], norm);
+            } else {
+                for (int d = sub; d < p.dim; d += 16) {
+                    const float y = load1<Tr>(g, d);
+                    dot = __builtin_fmaf(load1<Tr>(o, d) + (rest ? load1<Tr>(rest, d) : 0.0f), y, dot);
+                    norm = __builtin_fmaf(y, y, norm);
                 }
             }
+            dot = ormi_lanes_sum<16>(dot);
+            const int kvh = head / p.group;
+            if (live && sub == 0) delta[((long long)b * p.kv_heads + kvh) * p.rows + (long long)i * p.group + head % p.group] = dot;
         } else {
-            for (int d = sub; d < p.dim; d += 16) {
-                const float y = load1<Tr>(g, d);
-                dot = __builtin_fmaf(load1<Tr>(o, d) + (rest ? load1<Tr>(rest, d) : 0.0f), y, dot);
-                norm = __builtin_fmaf(y, y, norm);
-            }
-        }
-        dot = ormi_lanes_sum<16>(dot);
-        const int kvh = head / p.group;
-        if (live && sub == 0) delta[((long long)b * p.kv_heads + kvh) * p.rows + (long long)i * p.group + head % p.group] = dot;
-    } else {
-        const long long n = (long long)p.batch * p.keys * p.kv_heads;
-        const long long at = (long long)(blockIdx.x - row_groups) * 16 + (threadIdx.x >> 4);
-        const long long row = at < n ? at : n - 1;
-        const int kvh = (int)(row % p.kv_heads);
-        const long long bj = row / p.kv_heads;
-        const int b = (int)(bj / p.keys), j = (int)(bj % p.keys);
-        if (j < Span(p, b).end) {
-            const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + kvh * p.v_sh) * Tr::ESIZE;
-            for (int c = sub; c < p.chunks; c += 16) {
-                float y[Tr::VE];
-                load_chunk<Tr>(v + c * 16, y);
+            const int kvh = (int)(row % p.kv_heads);
+            const long long bj = row / p.kv_heads;
+            const int b = (int)(bj / p.keys), j = (int)(bj % p.keys);
+            if (j < Span(p, b).end) {
+                const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + kvh * p.v_sh) * Tr::ESIZE;
+                for (int c = sub; c < p.chunks; c += 16) {
+                    float y[Tr::VE];
+                    load_chunk<Tr>(v + c * 16, y);
 #pragma unroll
-                for (int e = 0; e < Tr::VE; ++e) norm = __builtin_fmaf(y[e], y[e], norm);
+                    for (int e = 0; e < Tr::VE; ++e) norm = __builtin_fmaf(y[e], y[e], norm);
+                }
             }
         }
+        if (bounds) most_norm = fmaxf(most_norm, ormi_lanes_sum<16>(norm));
     }
     if (!bounds) return;
-    norm = ormi_lanes_sum<16>(norm);
+    float norm = most_norm;
     norm = fmaxf(norm, __shfl_xor(norm, 16, 64));
     norm = fmaxf(norm, __shfl_xor(norm, 32, 64));
     __shared__ float most[4];
@@ -727,11 +763,13 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     constexpr int NW = 4, MT = BN / 32, TILEB = BN * T::ROWB;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
     __shared__ int shared_i[3 * NW];
+    __shared__ __attribute__((aligned(16))) int key_doc[2][BN];  // of a stage's keys
     lds_char* lds = (lds_char*)smem;
 
-    const int total = p.row_blocks * p.batch * p.kv_heads, item = xcd_item(total);
+    const int total = p.row_blocks * p.splits * p.batch * p.kv_heads, item = xcd_item(total);
     if (item >= total) return;
-    const int rb = p.row_blocks - 1 - item % p.row_blocks, bh = item / p.row_blocks;
+    const int split = item % p.splits, rest = item / p.splits;
+    const int rb = p.row_blocks - 1 - rest % p.row_blocks, bh = rest / p.row_blocks;
     const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
@@ -769,26 +807,12 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         docs_group.y = max(docs_group.y, shared_i[2 * NW + w]);
     }
     lim_group = __builtin_amdgcn_readfirstlane(lim_group);
-    const int t1 = (lim_group + BN - 1) / BN;
+    const int tiles = (lim_group + BN - 1) / BN;
+    const int per = (tiles + p.splits - 1) / p.splits;
+    const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
 
-    const int2* ranges = p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr;
-    constexpr int RT = kDocTile / BN;
-    unsigned long long meet = 0;
-    int meet_base = -1;
-    auto next = [&](int t) {
-        if (!p.docs) return t;
-        while (t < t1) {
-            const int rt = t / RT;
-            if (meet_base < 0 || rt >= meet_base + 64) {
-                meet_base = rt;
-                meet = tiles_meeting(ranges, rt, p.range_tiles, docs_group);
-            }
-            const unsigned long long left = meet >> (rt - meet_base);
-            if (left & 1) return t;
-            t = left ? (rt + __builtin_ctzll(left)) * RT : (meet_base + 64) * RT;
-        }
-        return t1;
-    };
+    DocTiles<BN> walk{p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr, p.range_tiles, -1, docs_group, docs_wave};
+    auto next = [&](int t) { return p.docs ? walk.next(t, t1) : t; };
     const char* kb = p.k + (b * p.k_sb + kvh * p.k_sh) * T::ES;
     const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh) * T::ES;
     using L = Loader<Tr, DP, BN, NW>;
@@ -805,21 +829,31 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
     const float unit = FORM != kPlain ? 1.0f : p.scale2;
 
-    int t = next(0), stage = 0;
-    if (t < t1) issue(t, 0);
+    auto fetch_docs = [&](int t) { return p.docs && threadIdx.x < BN ? doc_at(p, b, t * BN + (int)threadIdx.x) : -1; };
+    auto put_docs = [&](int doc, int stage) {
+        if (p.docs && threadIdx.x < BN) key_doc[stage][threadIdx.x] = doc;
+    };
+
+    int t = next(t0), stage = 0;
+    bool same = !p.docs || (t < t1 && walk.same(t));
+    if (t < t1) {
+        put_docs(fetch_docs(t), 0);
+        issue(t, 0);
+    }
     while (t < t1) {
         publish();
         const int tn = next(t + 1);
-        if (tn < t1) issue(tn, stage ^ 1);
+        bool same_next = !p.docs;
+        int docs_next = -1;
+        if (tn < t1) {
+            if (p.docs) same_next = walk.same(tn);
+            docs_next = fetch_docs(tn);
+            issue(tn, stage ^ 1);
+        }
         const int j0 = t * BN;
         if (j0 < lim_max) {
             const lds_char* kt = lds + stage * 2 * TILEB;
             const lds_char* vt = kt + TILEB;
-            bool same = true;
-            if (p.docs) {
-                const int2 kr = ranges[t / RT];
-                same = kr.x == kr.y && docs_wave.x == docs_wave.y && kr.x == docs_wave.x;
-            }
             const bool masked = j0 + BN > lim_min || !same;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -848,22 +882,40 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-                        bool seen = j < lim;
-                        if (!same) seen = seen && doc_at(p, b, j) == doc;
-                        s[e] = seen ? s[e] : 0.0f;
+                        s[e] = j < lim ? s[e] : 0.0f;
+                    }
+                    if (!same) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int4 kd = *(const int4*)&key_doc[stage][mt * 32 + 8 * q + 4 * half];
+                            s[4 * q] = kd.x == doc ? s[4 * q] : 0.0f;
+                            s[4 * q + 1] = kd.y == doc ? s[4 * q + 1] : 0.0f;
+                            s[4 * q + 2] = kd.z == doc ? s[4 * q + 2] : 0.0f;
+                            s[4 * q + 3] = kd.w == doc ? s[4 * q + 3] : 0.0f;
+                        }
                     }
                 }
                 T::second(kt, mt * 32, s, acc);
             }
         }
+        if (tn < t1) put_docs(docs_next, stage ^ 1);
         t = tn;
+        same = same_next;
         stage ^= 1;
     }
 #pragma unroll
     for (int dt = 0; dt < T::DT; ++dt) settle<Tr>(acc[dt]);
     if (r >= p.rows) return;
+    if (p.splits > 1) {
+        store_part(p.part_q + (((long long)split * p.batch * p.kv_heads + bh) * p.rows + r) * DP, acc);
+        return;
+    }
     store_row<Tr, T::DT>(p.dq + (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES, p.dim, acc, p.scale / hold);
 }
+
+// Values in LDS instead of registers: where 32 keys' k, v and both gradients
+// (16-bit rows of 128 features: 192 registers) leave too few for two waves a SIMD.
+constexpr bool values_in_lds(int dp, int es) { return dp * es >= 256 && dp * es <= 512; }
 
 // dk and dv. A wave owns 32 keys, one per lane's column: their k and v stay in
 // registers as second operands, and tiles of BM rows of q and dout pass through
@@ -875,7 +927,8 @@ template <class Tr, int DP, int FORM, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
     constexpr int NW = 4, BM = 32, TILEB = BM * T::ROWB;
-    __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
+    constexpr bool VL = DK && values_in_lds(DP, T::ES);
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB + (VL ? NW * TILEB : 0)];
     __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM], row_slope[2][BM];
     __shared__ __attribute__((aligned(16))) int row_lim[2][BM], row_pos[2][BM], row_doc[2][BM];
     lds_char* lds = (lds_char*)smem;
@@ -895,9 +948,10 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     const bool one_doc = p.docs && __all(doc == first_doc) && first_doc >= 0;
     const float hold = grad_hold<Tr>(p), shift = Shift<Tr>::bwd;
     const float hold_p = Shift<Tr>::bwd != 0.0f ? hold * __builtin_amdgcn_exp2f(-shift) : 1.0f;
-    u32x4_t kf[T::NF], vf[T::NF];
+    u32x4_t kf[T::NF], vf[VL ? 1 : T::NF];
     T::row_frags(p.k + (b * p.k_sb + (long long)keyc * p.k_sl + kvh * p.k_sh) * T::ES, p.chunks, kf);
-    if (DK) T::row_frags(p.v + (b * p.v_sb + (long long)keyc * p.v_sl + kvh * p.v_sh) * T::ES, p.chunks, vf);
+    const lds_char* vt = lds + 4 * TILEB + wave * TILEB;
+    if constexpr (DK && !VL) T::row_frags(p.v + (b * p.v_sb + (long long)keyc * p.v_sl + kvh * p.v_sh) * T::ES, p.chunks, vf);
 
     // Tiles of rows that can see the group's keys.
     const int tiles = (p.rows + BM - 1) / BM;
@@ -1002,6 +1056,19 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     if (t < t1) {
         put(fetch(t), 0);
         issue(t, 0);
+        if constexpr (VL) {
+            lds_char* vg = lds + 4 * TILEB;
+            const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh + (long long)k0 * p.v_sl) * T::ES;
+            Loader<Tr, DP, NW * 32, NW>::rows(vg, vb, (unsigned)(p.v_sl * T::ES), span.end - 1 - k0, p.chunks);
+            if (p.chunks < T::CPR) {  // both operands come from LDS: the padding of one has to be zero
+                publish();
+                const int pad = T::CPR - p.chunks;
+                for (int x = threadIdx.x; x < NW * 32 * pad; x += 64 * NW) {
+                    const int row = x / pad, c = p.chunks + x % pad;
+                    *(__attribute__((address_space(3))) u32x4_t*)(vg + row * T::ROWB + ((c ^ T::swz(row)) << 4)) = u32x4_t{0, 0, 0, 0};
+                }
+            }
+        }
     }
     while (t < t1) {
         publish();
@@ -1024,7 +1091,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 #pragma unroll
             for (int f = 0; f < T::NF; ++f) {
                 Tr::mma(T::frag(qt, 0, f), kf[f], s);
-                if (DK) Tr::mma(T::frag(gt, 0, f), vf[f], g);
+                if constexpr (VL) Tr::mma(T::frag(gt, 0, f), T::frag(vt, 0, f), g);
+                else if (DK) Tr::mma(T::frag(gt, 0, f), vf[f], g);
             }
             settle<Tr>(s);
             if (DK) settle<Tr>(g);
@@ -1092,37 +1160,45 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     if (DV && p.dv) store_row<Tr, T::DT>(p.dv + at, p.dim, acc_v, __builtin_amdgcn_exp2f(-shift));
 }
 
-// Adds the splits' partial dk and dv in split order. One wave per key.
+// Adds the splits' partial gradients in split order, one wave per row: first dq's
+// rows, then each key's dk and dv.
 template <class Tr, int DP>
-__global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttnParams p) {
-    const long long n = (long long)p.batch * p.kv_heads * p.keys;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void attention_grad_join_kernel(AttnParams p) {
+    const long long nq = p.dq && p.splits > 1 ? (long long)p.batch * p.kv_heads * p.rows : 0;
+    const long long nk = (p.dk || p.dv) && p.key_splits > 1 ? (long long)p.batch * p.kv_heads * p.keys : 0;
+    long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    if (row >= n) return;
-    const int bh = (int)(row / p.keys), j = (int)(row % p.keys), b = bh / p.kv_heads, kvh = bh % p.kv_heads;
-    const long long at = (((long long)b * p.keys + j) * p.kv_heads + kvh) * p.dim;
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        char* out = which == 0 ? p.dk : p.dv;
-        if (!out) continue;
-        const float f = which == 0 ? p.scale / grad_hold<Tr>(p) : __builtin_amdgcn_exp2f(-Shift<Tr>::bwd);
+    auto add = [&](const float* part, int splits, long long n, char* out, long long at, float f) {
 #pragma unroll
         for (int e = 0; e < DP / 64; ++e) {
             const int d = e * 64 + lane;
             float v = 0.0f;
-            for (int s = 0; s < p.key_splits; ++s) v += p.part[((which * p.key_splits + s) * n + row) * DP + d];
+            for (int s = 0; s < splits; ++s) v += part[(s * n + row) * DP + d];
             v *= f;
             if (d >= p.dim) continue;
             if constexpr (Tr::ESIZE == 4) ((float*)out)[at + d] = v;
             else ((unsigned short*)out)[at + d] = (unsigned short)pack2(Tr{}, v, v);
         }
+    };
+    const float score = p.scale / grad_hold<Tr>(p);
+    if (row < nq) {
+        const int bh = (int)(row / p.rows), r = (int)(row % p.rows), b = bh / p.kv_heads;
+        const int i = r / p.group, head = (bh % p.kv_heads) * p.group + r % p.group;
+        add(p.part_q, p.splits, nq, p.dq, (((long long)b * p.queries + i) * p.heads + head) * p.dim, score);
+        return;
     }
+    row -= nq;
+    if (row >= nk) return;
+    const int bh = (int)(row / p.keys), j = (int)(row % p.keys), b = bh / p.kv_heads, kvh = bh % p.kv_heads;
+    const long long at = (((long long)b * p.keys + j) * p.kv_heads + kvh) * p.dim;
+    if (p.dk) add(p.part, p.key_splits, nk, p.dk, at, score);
+    if (p.dv) add(p.part + p.key_splits * nk * DP, p.key_splits, nk, p.dv, at, __builtin_amdgcn_exp2f(-Shift<Tr>::bwd));
 }
 
 template <class Tr, int DP, int FORM>
 void launch_attention_grad_form(const AttnParams& p) {
     if (p.dq) {
-        const unsigned items = (unsigned)(p.row_blocks * p.batch * p.kv_heads);
+        const unsigned items = (unsigned)(p.row_blocks * p.splits * p.batch * p.kv_heads);
         attention_dq_kernel<Tr, DP, fwd_tile(DP, Tr::ESIZE, false), FORM><<<(items + 7) / 8 * 8, 256>>>(p);
     }
     if (p.dk || p.dv) {
@@ -1139,12 +1215,15 @@ void launch_attention_grad_form(const AttnParams& p) {
 template <class Tr, int DP>
 int launch_attention_grad_dp(const AttnParams& p, float* delta, unsigned* bounds) {
     const long long rows = (long long)p.batch * p.queries * p.heads, values = (long long)p.batch * p.keys * p.kv_heads;
-    const unsigned row_groups = (unsigned)((rows + 15) / 16), value_groups = bounds ? (unsigned)((values + 15) / 16) : 0;
+    // Where the work-groups meet in one word they go over several rows each.
+    const long long most = bounds ? 1024 : 1 << 30;
+    const unsigned row_groups = (unsigned)std::min((rows + 15) / 16, most), value_groups = bounds ? (unsigned)std::min((values + 15) / 16, most) : 0;
     attention_delta_kernel<Tr><<<row_groups + value_groups, 256>>>(p, delta, bounds, row_groups);
     if (p.form == kPlain) launch_attention_grad_form<Tr, DP, kPlain>(p);
     else if (p.form == kBias) launch_attention_grad_form<Tr, DP, kBias>(p);
     else launch_attention_grad_form<Tr, DP, kCap>(p);
-    if ((p.dk || p.dv) && p.key_splits > 1) attention_dkv_join_kernel<Tr, DP><<<(unsigned)((values + 3) / 4), 256>>>(p);
+    const long long join = (p.dq && p.splits > 1 ? rows : 0) + ((p.dk || p.dv) && p.key_splits > 1 ? values : 0);
+    if (join > 0) attention_grad_join_kernel<Tr, DP><<<(unsigned)((join + 3) / 4), 256>>>(p);
     return (int)hipGetLastError();
 }
 
