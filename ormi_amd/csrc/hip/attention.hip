@@ -179,7 +179,9 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
     } else {
         p.row_blocks = (p.rows + 127) / 128;
         p.key_blocks = (d->keys + 127) / 128;
-        const long long items = heads * p.key_blocks, slots = (long long)cus * 4;
+        // Rows are split so that causal work-groups of unequal length even out;
+        // with documents most of a split would see nothing, so only to fill the card.
+        const long long items = heads * p.key_blocks, slots = (long long)cus * (d->documents ? 1 : 4);
         const int tiles = (p.rows + 31) / 32;
         p.key_splits = items > 0 ? (int)std::max<long long>(1, std::min<long long>({slots / items, tiles / 8, 16})) : 1;
         if (p.key_splits > 1 && (g->dk || g->dv)) pl.part = take(pl.bytes, 2 * sizeof(float) * (size_t)p.key_splits * heads * d->keys * dp);

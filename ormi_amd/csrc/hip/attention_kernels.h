@@ -42,7 +42,10 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) float lds_float;
-typedef __attribute__((address_space(3))) int lds_int;
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) f32x4_t lds_f32x4;
+typedef __attribute__((address_space(3))) i32x4_t lds_i32x4;
 
 constexpr float kInf = __builtin_huge_valf();
 
@@ -498,6 +501,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
         if (j0 < lim_max) {
             const lds_char* kt = lds + stage * 2 * TILEB;
             const lds_char* vt = kt + TILEB;
+            const float away = (float)(pos - j0 - 4 * half);  // of the lane's first key
             f32x16_t s[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -509,9 +513,8 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
                 if constexpr (FORM != kPlain) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
                         float slope;
-                        s[mt][e] = score2<Tr, FORM>(p, s[mt][e], slope2, (float)(pos - j), slope);
+                        s[mt][e] = score2<Tr, FORM>(p, s[mt][e], slope2, away - (float)(mt * 32 + 8 * (e >> 2) + (e & 3)), slope);
                     }
                 }
             }
@@ -528,7 +531,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const int4 kd = *(const int4*)&key_doc[stage][mt * 32 + 8 * q + 4 * half];
+                            const i32x4_t kd = *(const lds_i32x4*)&key_doc[stage][mt * 32 + 8 * q + 4 * half];
                             s[mt][4 * q] = kd.x == doc ? s[mt][4 * q] : -kInf;
                             s[mt][4 * q + 1] = kd.y == doc ? s[mt][4 * q + 1] : -kInf;
                             s[mt][4 * q + 2] = kd.z == doc ? s[mt][4 * q + 2] : -kInf;
@@ -855,6 +858,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             const lds_char* kt = lds + stage * 2 * TILEB;
             const lds_char* vt = kt + TILEB;
             const bool masked = j0 + BN > lim_min || !same;
+            const float away = (float)(pos - j0 - 4 * half);  // of the lane's first key
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 f32x16_t s, g;
@@ -869,9 +873,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
                 settle<Tr>(g);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int j = j0 + mt * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
                     float slope = 1.0f, t2 = s[e];
-                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, slope2, (float)(pos - j), slope);
+                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, slope2, away - (float)(mt * 32 + 8 * (e >> 2) + (e & 3)), slope);
                     const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, -lse));
                     float ds = pr * (g[e] - delta);
                     if (FORM == kCap) ds *= slope;
@@ -887,7 +890,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
                     if (!same) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const int4 kd = *(const int4*)&key_doc[stage][mt * 32 + 8 * q + 4 * half];
+                            const i32x4_t kd = *(const lds_i32x4*)&key_doc[stage][mt * 32 + 8 * q + 4 * half];
                             s[4 * q] = kd.x == doc ? s[4 * q] : 0.0f;
                             s[4 * q + 1] = kd.y == doc ? s[4 * q + 1] : 0.0f;
                             s[4 * q + 2] = kd.z == doc ? s[4 * q + 2] : 0.0f;
@@ -929,8 +932,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     constexpr int NW = 4, BM = 32, TILEB = BM * T::ROWB;
     constexpr bool VL = DK && values_in_lds(DP, T::ES);
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB + (VL ? NW * TILEB : 0)];
-    __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM], row_slope[2][BM];
-    __shared__ __attribute__((aligned(16))) int row_lim[2][BM], row_pos[2][BM], row_doc[2][BM];
+    __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM], row_slope[2][BM], row_pos[2][BM];
+    __shared__ __attribute__((aligned(16))) int row_lim[2][BM], row_doc[2][BM];
     lds_char* lds = (lds_char*)smem;
 
     const int total = p.key_blocks * p.key_splits * p.batch * p.kv_heads, item = xcd_item(total);
@@ -946,6 +949,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     const int doc = p.docs && key < span.end ? doc_at(p, b, key) : -1;
     const int first_doc = p.docs ? __builtin_amdgcn_readfirstlane(doc) : 0;
     const bool one_doc = p.docs && __all(doc == first_doc) && first_doc >= 0;
+    const float keyf = (float)key;
     const float hold = grad_hold<Tr>(p), shift = Shift<Tr>::bwd;
     const float hold_p = Shift<Tr>::bwd != 0.0f ? hold * __builtin_amdgcn_exp2f(-shift) : 1.0f;
     u32x4_t kf[T::NF], vf[VL ? 1 : T::NF];
@@ -1039,7 +1043,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             row_lim[stage][threadIdx.x] = m.lim;
             if (FORM != kPlain) {
                 row_slope[stage][threadIdx.x] = m.slope;
-                row_pos[stage][threadIdx.x] = m.pos;
+                row_pos[stage][threadIdx.x] = (float)m.pos;
             }
             if (p.docs) row_doc[stage][threadIdx.x] = m.doc;
         }
@@ -1096,48 +1100,47 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             }
             settle<Tr>(s);
             if (DK) settle<Tr>(g);
-            f32x16_t slope;
+            // s becomes p, g the score gradient.
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
                 const int row = 8 * q4 + 4 * half;
-                const float4 ls = *(const float4*)&row_lse[stage][row];
-                const float* lsv = (const float*)&ls;
+                const f32x4_t ls = *(const lds_f32x4*)&row_lse[stage][row];
+                f32x4_t de, sl, ps;
+                if (DK) de = *(const lds_f32x4*)&row_delta[stage][row];
+                if (FORM != kPlain) {
+                    sl = *(const lds_f32x4*)&row_slope[stage][row];
+                    ps = *(const lds_f32x4*)&row_pos[stage][row];
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int x = 4 * q4 + e;
-                    float t2 = s[x], sl = 1.0f;
-                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, row_slope[stage][row + e], (float)(row_pos[stage][row + e] - key), sl);
-                    if (FORM == kCap) slope[x] = sl;
-                    s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, -lsv[e]));
+                    float t2 = s[x], slope = 1.0f;
+                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, sl[e], ps[e] - keyf, slope);
+                    s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, -ls[e]));
+                    if (!DK) continue;
+                    g[x] = s[x] * (g[x] - de[e]);
+                    if (FORM == kCap) g[x] *= slope;
+                    if (Shift<Tr>::bwd != 0.0f) g[x] *= hold_p;
                 }
             }
             if (masked) {
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const int row = 8 * (x >> 2) + 4 * half + (x & 3);
-                    bool seen = key < row_lim[stage][row];
-                    if (!same) seen = seen && row_doc[stage][row] == doc;
-                    s[x] = seen ? s[x] : 0.0f;
-                    if (DK) g[x] = seen ? g[x] : 0.0f;
-                }
-            }
-            if (DV) T::second(gt, 0, s, acc_v);
-            if (DK) {
-#pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
-                    const float4 de = *(const float4*)&row_delta[stage][8 * q4 + 4 * half];
-                    const float* dev = (const float*)&de;
+                    const int row = 8 * q4 + 4 * half;
+                    const i32x4_t li = *(const lds_i32x4*)&row_lim[stage][row];
+                    i32x4_t dc = {0, 0, 0, 0};
+                    if (!same) dc = *(const lds_i32x4*)&row_doc[stage][row];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int x = 4 * q4 + e;
-                        float ds = s[x] * (g[x] - dev[e]);
-                        if (FORM == kCap) ds *= slope[x];
-                        if (Shift<Tr>::bwd != 0.0f) ds *= hold_p;
-                        s[x] = ds;
+                        const bool seen = key < li[e] && (same || dc[e] == doc);
+                        s[x] = seen ? s[x] : 0.0f;
+                        if (DK) g[x] = seen ? g[x] : 0.0f;
                     }
                 }
-                T::second(qt, 0, s, acc_k);
             }
+            if (DV) T::second(gt, 0, s, acc_v);
+            if (DK) T::second(qt, 0, g, acc_k);
         }
         if (tn < t1) put(ahead, stage ^ 1);
         t = tn;
