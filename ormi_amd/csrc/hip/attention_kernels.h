@@ -124,15 +124,29 @@ struct Tile {
     static constexpr int NF = DP / (2 * VE);  // operand fragments along the features
     static constexpr int DT = DP / 32;        // accumulator tiles along the features
 
-    // Sixteen rows in a row meet in no bank (row reads), and neither do four
-    // rows' 64-byte pieces (transposing reads).
+    // A direct load fills 1 KB, RPS rows; such segments lie SEGB apart, and within
+    // a row chunk c stands at c ^ swz(row). Between them sixteen rows in a row meet
+    // in no bank (row reads), and neither do four rows' 64-byte pieces (transposing
+    // reads), while most steps along a row stay constant offsets of few addresses
+    // (an exchange over all 16 chunks took 16 address registers instead of 8, which
+    // the gradient kernels do not have).
+    static constexpr int RPS = 64 / CPR, SEGB = 1024 + (CPR == 32 ? 128 : 16);
     __device__ __forceinline__ static int swz(int row) {
-        return CPR == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+        return CPR == 8    ? (((row >> 1) & 1) << 2) | (((row >> 2) & 1) << 1)
+               : CPR == 16 ? (row & 3) << 2
+               : CPR == 32 ? ((row & 1) << 2) | ((row >> 2) & 3)
+                           : 0;
     }
+    __device__ __forceinline__ static constexpr int at(int row) { return row / RPS * SEGB + row % RPS * ROWB; }
+    static constexpr int bytes(int rows) { return rows / RPS * SEGB; }
     // Rows [row0, row0 + 32), fragment f: lane l holds the chunk 2 f + l / 32 of row l % 32.
     __device__ __forceinline__ static u32x4_t frag(const lds_char* t, int row0, int f) {
-        const int lane = threadIdx.x & 63, row = lane & 31, c = 2 * f + (lane >> 5);
-        return *(const __attribute__((address_space(3))) u32x4_t*)(t + row0 * ROWB + row * ROWB + ((c ^ swz(row)) << 4));
+        const int lane = threadIdx.x & 63, row = lane & 31;
+        // The bits of f that the exchange leaves alone are a constant step.
+        constexpr int kept = CPR == 8 ? 0 : CPR == 16 ? 1 : CPR == 32 ? ~3 : ~0;
+        const int fx = f & ~kept, step = (f & kept) * 32;
+        const int lane_at = at(row) + (((2 * fx + (lane >> 5)) ^ swz(row)) << 4);
+        return *(const __attribute__((address_space(3))) u32x4_t*)(t + at(row0) + step + lane_at);
     }
     // 16-bit: features [32 dt, 32 dt + 32) as rows, the depth the tile rows
     // row0 + 16 step + {4 half + 0..3, 8 + 4 half + 0..3}, accumulator order.
@@ -143,7 +157,7 @@ struct Tile {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = 8 * h + 4 * (lane >> 5) + (i >> 2);  // row % 16
-            const lds_char* p = t + (row0 + 16 * step) * ROWB + k * ROWB + (((col >> 3) ^ swz(k)) << 4) + ((col & 4) << 1);
+            const lds_char* p = t + at(row0 + 16 * step + 8 * h) + at(k - 8 * h) + (((col >> 3) ^ swz(k)) << 4) + ((col & 4) << 1);
             const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p);
             const uint2 w = __builtin_bit_cast(uint2, v);
             out[2 * h] = w.x;
@@ -155,7 +169,7 @@ struct Tile {
     __device__ __forceinline__ static float turned1(const lds_char* t, int row0, int r, int dt) {
         const int lane = threadIdx.x & 63, row = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
         const int d = dt * 32 + (lane & 31);
-        return *(const lds_float*)(t + row0 * ROWB + row * ROWB + (((d >> 2) ^ swz(row)) << 4) + (d & 3) * 4);
+        return *(const lds_float*)(t + at(row0) + at(row) + (((d >> 2) ^ swz(row)) << 4) + (d & 3) * 4);
     }
     // acc[dt] += (the tile's rows row0.. turned) x (accumulator `a` as 16- or 32-bit operand)
     __device__ __forceinline__ static void second(const lds_char* t, int row0, const f32x16_t& a, f32x16_t (&acc)[DT]) {
@@ -216,26 +230,26 @@ struct Loader {
     // written, one between a write of m0 and a load to LDS.
     __device__ __forceinline__ static void load(lds_char* dst, const char* base, const unsigned (&off)[PER]) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const unsigned d = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(dst + wave * PER * 1024));
+        const unsigned d = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(dst + wave * PER * T::SEGB));
         constexpr int N = PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1;
 #pragma unroll
         for (int s = 0; s < PER; s += N) {
             if constexpr (N == 4)
                 asm volatile(
                     "s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
-                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
-                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
-                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5" ::"s"(d + s * 1024),
-                    "v"(off[s]), "v"(off[s + 1]), "v"(off[s + 2]), "v"(off[s + 3]), "s"(base)
+                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
+                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
+                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5" ::"s"(d + s * T::SEGB),
+                    "v"(off[s]), "v"(off[s + 1]), "v"(off[s + 2]), "v"(off[s + 3]), "s"(base), "i"(T::SEGB)
                     : "memory", "m0", "scc");
             else if constexpr (N == 2)
                 asm volatile(
                     "s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
-                    "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(d + s * 1024),
-                    "v"(off[s]), "v"(off[s + 1]), "s"(base)
+                    "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(d + s * T::SEGB),
+                    "v"(off[s]), "v"(off[s + 1]), "s"(base), "i"(T::SEGB)
                     : "memory", "m0", "scc");
             else
-                asm volatile("s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(d + s * 1024),
+                asm volatile("s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(d + s * T::SEGB),
                              "v"(off[s]), "s"(base)
                              : "memory", "m0");
         }
@@ -251,6 +265,12 @@ struct Loader {
         load(dst, uniform_ptr(base), off);
     }
 };
+
+// One 4-byte value per lane into 256 bytes of LDS, from an address of its own.
+__device__ __forceinline__ void load_words(const void* dst, const void* from) {
+    const unsigned d = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char*)dst);
+    asm volatile("s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(d), "v"(from) : "memory", "m0");
+}
 
 // Waits for this wave's direct loads and LDS reads, then for the other waves.
 __device__ __forceinline__ void publish() {
@@ -396,10 +416,10 @@ __device__ __forceinline__ void store_part(float* row, const f32x16_t (&acc)[DT]
 template <class Tr, int DP, int NW, int BN, int FORM>
 __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
-    constexpr int MT = BN / 32, TILEB = BN * T::ROWB;
+    constexpr int MT = BN / 32, TILEB = T::bytes(BN);
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
     __shared__ int shared_i[3 * NW];
-    __shared__ __attribute__((aligned(16))) int key_doc[2][BN];  // of a stage's keys
+    __shared__ __attribute__((aligned(16))) int key_doc[2][64];  // of a stage's keys
     lds_char* lds = (lds_char*)smem;
 
     const int item = xcd_item(p.row_blocks * p.splits * p.batch * p.kv_heads);
@@ -462,6 +482,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
         const int last = span.end - 1 - t * BN;
         L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks);
         L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks);
+        if (p.docs && wave == 0) load_words(key_doc[stage], p.docs + b * p.docs_sb + min(t * BN + lane, p.keys - 1));
     };
 
     f32x16_t acc[T::DT];
@@ -474,29 +495,14 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
     float m = -kInf, l = 0.0f;
     const float unit = FORM != kPlain ? 1.0f : p.scale2;
 
-    // The documents of a tile's keys, one per thread: fetched before the tile's own
-    // loads, written behind the previous tile's work.
-    auto fetch_docs = [&](int t) { return p.docs && threadIdx.x < BN ? doc_at(p, b, t * BN + (int)threadIdx.x) : -1; };
-    auto put_docs = [&](int doc, int stage) {
-        if (p.docs && threadIdx.x < BN) key_doc[stage][threadIdx.x] = doc;
-    };
-
     int t = next(t0), stage = 0;
     bool same = !p.docs || (t < t1 && walk.same(t));
-    if (t < t1) {
-        put_docs(fetch_docs(t), 0);
-        issue(t, 0);
-    }
+    if (t < t1) issue(t, 0);
     while (t < t1) {
         publish();
         const int tn = next(t + 1);
-        bool same_next = !p.docs;
-        int docs_next = -1;
-        if (tn < t1) {
-            if (p.docs) same_next = walk.same(tn);
-            docs_next = fetch_docs(tn);
-            issue(tn, stage ^ 1);
-        }
+        const bool same_next = !p.docs || (tn < t1 && walk.same(tn));
+        if (tn < t1) issue(tn, stage ^ 1);
         const int j0 = t * BN;
         if (j0 < lim_max) {
             const lds_char* kt = lds + stage * 2 * TILEB;
@@ -568,7 +574,6 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) T::second(vt, mt * 32, s[mt], acc);
         }
-        if (tn < t1) put_docs(docs_next, stage ^ 1);
         t = tn;
         same = same_next;
         stage ^= 1;
@@ -763,10 +768,10 @@ __device__ __forceinline__ float grad_hold(const AttnParams& p) {
 template <class Tr, int DP, int BN, int FORM>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
-    constexpr int NW = 4, MT = BN / 32, TILEB = BN * T::ROWB;
+    constexpr int NW = 4, MT = BN / 32, TILEB = T::bytes(BN);
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
     __shared__ int shared_i[3 * NW];
-    __shared__ __attribute__((aligned(16))) int key_doc[2][BN];  // of a stage's keys
+    __shared__ __attribute__((aligned(16))) int key_doc[2][64];  // of a stage's keys
     lds_char* lds = (lds_char*)smem;
 
     const int total = p.row_blocks * p.splits * p.batch * p.kv_heads, item = xcd_item(total);
@@ -823,6 +828,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         const int last = span.end - 1 - t * BN;
         L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks);
         L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks);
+        if (p.docs && wave == 0) load_words(key_doc[stage], p.docs + b * p.docs_sb + min(t * BN + lane, p.keys - 1));
     };
 
     f32x16_t acc[T::DT];
@@ -832,27 +838,14 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
     const float unit = FORM != kPlain ? 1.0f : p.scale2;
 
-    auto fetch_docs = [&](int t) { return p.docs && threadIdx.x < BN ? doc_at(p, b, t * BN + (int)threadIdx.x) : -1; };
-    auto put_docs = [&](int doc, int stage) {
-        if (p.docs && threadIdx.x < BN) key_doc[stage][threadIdx.x] = doc;
-    };
-
     int t = next(t0), stage = 0;
     bool same = !p.docs || (t < t1 && walk.same(t));
-    if (t < t1) {
-        put_docs(fetch_docs(t), 0);
-        issue(t, 0);
-    }
+    if (t < t1) issue(t, 0);
     while (t < t1) {
         publish();
         const int tn = next(t + 1);
-        bool same_next = !p.docs;
-        int docs_next = -1;
-        if (tn < t1) {
-            if (p.docs) same_next = walk.same(tn);
-            docs_next = fetch_docs(tn);
-            issue(tn, stage ^ 1);
-        }
+        const bool same_next = !p.docs || (tn < t1 && walk.same(tn));
+        if (tn < t1) issue(tn, stage ^ 1);
         const int j0 = t * BN;
         if (j0 < lim_max) {
             const lds_char* kt = lds + stage * 2 * TILEB;
@@ -901,7 +894,6 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
                 T::second(kt, mt * 32, s, acc);
             }
         }
-        if (tn < t1) put_docs(docs_next, stage ^ 1);
         t = tn;
         same = same_next;
         stage ^= 1;
@@ -929,11 +921,12 @@ constexpr bool values_in_lds(int dp, int es) { return dp * es >= 256 && dp * es 
 template <class Tr, int DP, int FORM, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
-    constexpr int NW = 4, BM = 32, TILEB = BM * T::ROWB;
+    constexpr int NW = 4, BM = 32, TILEB = T::bytes(BM);
     constexpr bool VL = DK && values_in_lds(DP, T::ES);
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB + (VL ? NW * TILEB : 0)];
-    __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM], row_slope[2][BM], row_pos[2][BM];
-    __shared__ __attribute__((aligned(16))) int row_lim[2][BM], row_doc[2][BM];
+    // Of a stage's rows: sums and deltas, slopes and documents, positions, limits.
+    __shared__ __attribute__((aligned(16))) float row_sums[2][2 * BM], row_pos[2][BM];
+    __shared__ __attribute__((aligned(16))) int row_rule[2][2 * BM], row_lim[2][BM];
     lds_char* lds = (lds_char*)smem;
 
     const int total = p.key_blocks * p.key_splits * p.batch * p.kv_heads, item = xcd_item(total);
@@ -950,6 +943,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     const int first_doc = p.docs ? __builtin_amdgcn_readfirstlane(doc) : 0;
     const bool one_doc = p.docs && __all(doc == first_doc) && first_doc >= 0;
     const float keyf = (float)key;
+    const bool sloped = FORM != kPlain && p.slopes;
+    const int key_live = p.docs && doc < 0 ? 0x7fffffff : key;  // a key without a document is seen by no row
     const float hold = grad_hold<Tr>(p), shift = Shift<Tr>::bwd;
     const float hold_p = Shift<Tr>::bwd != 0.0f ? hold * __builtin_amdgcn_exp2f(-shift) : 1.0f;
     u32x4_t kf[T::NF], vf[VL ? 1 : T::NF];
@@ -1015,40 +1010,22 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         }
         L::load(lds + stage * 2 * TILEB, qt, qo);
         L::load(lds + stage * 2 * TILEB + TILEB, gt, go);
-    };
-    // What belongs to the rows of a tile, one row per lane of the first wave:
-    // fetched before the tile's own loads, written behind the previous tile's work.
-    struct Row { float lse, delta, slope; int lim, pos, doc; };
-    auto fetch = [&](int t) {
-        Row m = {kInf, 0.0f, 0.0f, 0, 0, -1};
-        const int rr = t * BM + (int)threadIdx.x;
-        if (threadIdx.x < BM && rr < p.rows) {
-            const int i = (int)ormi_fdiv((unsigned)rr, p.group_m, p.group_s);
-            m.lse = p.lse[(long long)bh * p.rows + rr] - shift;
-            m.delta = p.delta[(long long)bh * p.rows + rr];
-            m.pos = i + span.off;
-            m.lim = span.limit(p, m.pos);
-            if (p.docs) {
-                m.doc = doc_at(p, b, m.pos);
-                if (m.doc < 0) m.lim = 0;
+        // What belongs to the rows, one per lane of the first wave's halves; a row
+        // past the last has the limit 0, as has one without a document of its own.
+        if (wave == 0) {
+            const int rr = min(r0 + (lane & 31), p.rows - 1);
+            const int i = (int)ormi_fdiv((unsigned)rr, p.group_m, p.group_s), pos = i + span.off;
+            load_words(row_sums[stage], (half == 0 ? p.lse : p.delta) + (long long)bh * p.rows + rr);
+            if (p.docs || sloped)
+                load_words(row_rule[stage], half == 0 && sloped ? (const int*)p.slopes + kvh * p.group + rr - i * p.group
+                                            : p.docs ? p.docs + b * p.docs_sb + min(max(pos, 0), p.keys - 1)
+                                                     : (const int*)p.slopes);
+            if (half == 0) {
+                row_lim[stage][lane] = r0 + lane >= p.rows || (p.docs && pos < 0) ? 0 : span.limit(p, pos);
+                if (FORM != kPlain) row_pos[stage][lane] = (float)pos;
             }
-            if (FORM != kPlain && p.slopes) m.slope = p.slopes[kvh * p.group + rr - i * p.group] * 1.44269504f;
-        }
-        return m;
-    };
-    auto put = [&](const Row& m, int stage) {
-        if (threadIdx.x < BM) {
-            row_lse[stage][threadIdx.x] = m.lse;
-            row_delta[stage][threadIdx.x] = m.delta;
-            row_lim[stage][threadIdx.x] = m.lim;
-            if (FORM != kPlain) {
-                row_slope[stage][threadIdx.x] = m.slope;
-                row_pos[stage][threadIdx.x] = (float)m.pos;
-            }
-            if (p.docs) row_doc[stage][threadIdx.x] = m.doc;
         }
     };
-
     f32x16_t acc_k[T::DT], acc_v[T::DT];
 #pragma unroll
     for (int dt = 0; dt < T::DT; ++dt)
@@ -1058,7 +1035,6 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 
     int t = next(t0), stage = 0;
     if (t < t1) {
-        put(fetch(t), 0);
         issue(t, 0);
         if constexpr (VL) {
             lds_char* vg = lds + 4 * TILEB;
@@ -1069,7 +1045,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
                 const int pad = T::CPR - p.chunks;
                 for (int x = threadIdx.x; x < NW * 32 * pad; x += 64 * NW) {
                     const int row = x / pad, c = p.chunks + x % pad;
-                    *(__attribute__((address_space(3))) u32x4_t*)(vg + row * T::ROWB + ((c ^ T::swz(row)) << 4)) = u32x4_t{0, 0, 0, 0};
+                    *(__attribute__((address_space(3))) u32x4_t*)(vg + T::at(row) + ((c ^ T::swz(row)) << 4)) = u32x4_t{0, 0, 0, 0};
                 }
             }
         }
@@ -1077,17 +1053,13 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     while (t < t1) {
         publish();
         const int tn = next(t + 1);
-        Row ahead;
-        if (tn < t1) {
-            ahead = fetch(tn);
-            issue(tn, stage ^ 1);
-        }
+        if (tn < t1) issue(tn, stage ^ 1);
         const int lim_lane = row_lim[stage][lane & 31];
         if (__any(lim_lane > kw)) {
             const lds_char* qt = lds + stage * 2 * TILEB;
             const lds_char* gt = qt + TILEB;
             bool same = true;
-            if (p.docs) same = one_doc && __all(row_doc[stage][lane & 31] == first_doc);
+            if (p.docs) same = one_doc && __all(row_rule[stage][BM + (lane & 31)] == first_doc);
             const bool masked = !__all(lim_lane >= kw + 32) || !same;
             f32x16_t s, g;
 #pragma unroll
@@ -1104,19 +1076,19 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
                 const int row = 8 * q4 + 4 * half;
-                const f32x4_t ls = *(const lds_f32x4*)&row_lse[stage][row];
+                const f32x4_t ls = *(const lds_f32x4*)&row_sums[stage][row];
                 f32x4_t de, sl, ps;
-                if (DK) de = *(const lds_f32x4*)&row_delta[stage][row];
+                if (DK) de = *(const lds_f32x4*)&row_sums[stage][BM + row];
                 if (FORM != kPlain) {
-                    sl = *(const lds_f32x4*)&row_slope[stage][row];
+                    sl = *(const lds_f32x4*)&row_rule[stage][row];
                     ps = *(const lds_f32x4*)&row_pos[stage][row];
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int x = 4 * q4 + e;
                     float t2 = s[x], slope = 1.0f;
-                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, sl[e], ps[e] - keyf, slope);
-                    s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, -ls[e]));
+                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, sloped ? sl[e] * 1.44269504f : 0.0f, ps[e] - keyf, slope);
+                    s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, shift - ls[e]));
                     if (!DK) continue;
                     g[x] = s[x] * (g[x] - de[e]);
                     if (FORM == kCap) g[x] *= slope;
@@ -1129,11 +1101,11 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
                     const int row = 8 * q4 + 4 * half;
                     const i32x4_t li = *(const lds_i32x4*)&row_lim[stage][row];
                     i32x4_t dc = {0, 0, 0, 0};
-                    if (!same) dc = *(const lds_i32x4*)&row_doc[stage][row];
+                    if (!same) dc = *(const lds_i32x4*)&row_rule[stage][BM + row];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int x = 4 * q4 + e;
-                        const bool seen = key < li[e] && (same || dc[e] == doc);
+                        const bool seen = key_live < li[e] && (same || dc[e] == doc);
                         s[x] = seen ? s[x] : 0.0f;
                         if (DK) g[x] = seen ? g[x] : 0.0f;
                     }
@@ -1142,7 +1114,6 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             if (DV) T::second(gt, 0, s, acc_v);
             if (DK) T::second(qt, 0, g, acc_k);
         }
-        if (tn < t1) put(ahead, stage ^ 1);
         t = tn;
         stage ^= 1;
     }
