@@ -36,6 +36,7 @@ struct AttnParams {
     // Work split.
     int wide;  // 4 waves per work-group (128 rows), else one
     int row_blocks, splits;
+    int spread;  // runs of blocks per head (Work)
     float* part;    // of out, or of dk and dv
     float* part_q;  // of dq
     float2* part_ml;

@@ -159,8 +159,9 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
     p.range_tiles = (d->keys + kDocTile - 1) / kDocTile;
     if (d->documents) pl.ranges = take(pl.bytes, sizeof(int2) * (size_t)d->batch * std::max(p.range_tiles, 1));
 
-    const int dp = d->dim <= 64 ? 64 : d->dim <= 128 ? 128 : 256, cus = compute_units();
+    const int dp = d->dim <= 64 ? 64 : d->dim <= 96 ? 96 : d->dim <= 128 ? 128 : 256, cus = compute_units();
     const long long heads = (long long)d->batch * d->kv_heads;
+    p.spread = heads % 8 == 0 ? 1 : heads % 4 == 0 ? 2 : heads % 2 == 0 ? 4 : 8;
     if (!g) {
         // Few rows (single tokens): one wave per work-group. Where the rows of
         // all heads leave compute units idle the keys are split over work-groups,
@@ -168,7 +169,7 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
         p.wide = p.rows > 32;
         p.row_blocks = p.wide ? (p.rows + 127) / 128 : 1;
         const int bn = fwd_tile(dp, es, !p.wide);
-        const long long items = heads * p.row_blocks, slots = (long long)cus * (p.wide ? 2 : 4);
+        const long long items = heads * p.row_blocks, slots = (long long)cus * (p.wide ? (es == 4 ? 3 : 2) : 4);
         const int tiles = (d->keys + bn - 1) / bn;
         p.splits = items > 0 && items * 2 <= slots ? (int)std::max<long long>(1, std::min<long long>({slots / items, tiles / 2, 64})) : 1;
         if (p.splits > 1) {
@@ -187,7 +188,8 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
         if (p.key_splits > 1 && (g->dk || g->dv)) pl.part = take(pl.bytes, 2 * sizeof(float) * (size_t)p.key_splits * heads * d->keys * dp);
         const long long row_items = heads * p.row_blocks;
         const int key_tiles = (d->keys + 31) / 32;
-        p.splits = row_items > 0 && row_items * 2 <= cus * 2 ? (int)std::max<long long>(1, std::min<long long>({cus * 2 / row_items, key_tiles / 4, 16})) : 1;
+        const long long row_slots = (long long)cus * (es == 4 ? 3 : 2);
+        p.splits = row_items > 0 && row_items * 2 <= row_slots ? (int)std::max<long long>(1, std::min<long long>({row_slots / row_items, key_tiles / 4, 16})) : 1;
         if (p.splits > 1 && g->dq) pl.part_q = take(pl.bytes, sizeof(float) * (size_t)p.splits * heads * p.rows * dp);
         if (items * p.key_splits >= (1ll << 30) || heads * p.row_blocks >= (1ll << 30)) return bad("too many work-groups");
         pl.delta = take(pl.bytes, sizeof(float) * (size_t)heads * p.rows);

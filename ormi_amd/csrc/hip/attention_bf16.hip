@@ -5,12 +5,14 @@ namespace ormi_hip {
 
 int launch_attention_fwd_bf16(const AttnParams& p) {
     return p.dim <= 64    ? launch_attention_fwd_dp<TrBF16, 64>(p)
+           : p.dim <= 96  ? launch_attention_fwd_dp<TrBF16, 96>(p)
            : p.dim <= 128 ? launch_attention_fwd_dp<TrBF16, 128>(p)
                           : launch_attention_fwd_dp<TrBF16, 256>(p);
 }
 
 int launch_attention_grad_bf16(const AttnParams& p, float* delta, unsigned* bounds) {
     return p.dim <= 64    ? launch_attention_grad_dp<TrBF16, 64>(p, delta, bounds)
+           : p.dim <= 96  ? launch_attention_grad_dp<TrBF16, 96>(p, delta, bounds)
            : p.dim <= 128 ? launch_attention_grad_dp<TrBF16, 128>(p, delta, bounds)
                           : launch_attention_grad_dp<TrBF16, 256>(p, delta, bounds);
 }

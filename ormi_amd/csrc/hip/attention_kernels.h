@@ -130,20 +130,25 @@ struct Tile {
     // reads), while most steps along a row stay constant offsets of few addresses
     // (an exchange over all 16 chunks took 16 address registers instead of 8, which
     // the gradient kernels do not have).
-    static constexpr int RPS = 64 / CPR, SEGB = 1024 + (CPR == 32 ? 128 : 16);
+    // Rows of 96 features (12 or 24 chunks) do not divide a segment and lie without
+    // gaps: their stride itself takes rows to different banks.
+    static constexpr bool EVEN = 64 % CPR == 0;
+    static constexpr int RPS = EVEN ? 64 / CPR : 1, SEGB = 1024 + (EVEN ? CPR == 32 ? 128 : 16 : 0);
     __device__ __forceinline__ static int swz(int row) {
         return CPR == 8    ? (((row >> 1) & 1) << 2) | (((row >> 2) & 1) << 1)
+               : CPR == 12 ? (row >> 2) & 3
                : CPR == 16 ? (row & 3) << 2
+               : CPR == 24 ? (row >> 1) & 7
                : CPR == 32 ? ((row & 1) << 2) | ((row >> 2) & 3)
                            : 0;
     }
-    __device__ __forceinline__ static constexpr int at(int row) { return row / RPS * SEGB + row % RPS * ROWB; }
-    static constexpr int bytes(int rows) { return rows / RPS * SEGB; }
+    __device__ __forceinline__ static constexpr int at(int row) { return EVEN ? row / RPS * SEGB + row % RPS * ROWB : row * ROWB; }
+    static constexpr int bytes(int rows) { return EVEN ? rows / RPS * SEGB : rows * ROWB; }
     // Rows [row0, row0 + 32), fragment f: lane l holds the chunk 2 f + l / 32 of row l % 32.
     __device__ __forceinline__ static u32x4_t frag(const lds_char* t, int row0, int f) {
         const int lane = threadIdx.x & 63, row = lane & 31;
         // The bits of f that the exchange leaves alone are a constant step.
-        constexpr int kept = CPR == 8 ? 0 : CPR == 16 ? 1 : CPR == 32 ? ~3 : ~0;
+        constexpr int kept = CPR == 8 ? 0 : CPR == 12 ? ~1 : CPR == 16 ? 1 : CPR == 64 ? ~0 : ~3;
         const int fx = f & ~kept, step = (f & kept) * 32;
         const int lane_at = at(row) + (((2 * fx + (lane >> 5)) ^ swz(row)) << 4);
         return *(const __attribute__((address_space(3))) u32x4_t*)(t + at(row0) + step + lane_at);
@@ -211,16 +216,16 @@ struct Tile {
 template <class Tr, int DP, int ROWS, int NW>
 struct Loader {
     using T = Tile<Tr, DP>;
-    static constexpr int SEGS = ROWS * T::CPR / 64, PER = SEGS / NW;
-    static_assert(SEGS % NW == 0 && T::CPR <= 64, "whole segments per wave");
+    static constexpr int SEGS = ROWS * T::CPR / 64, PER = (SEGS + NW - 1) / NW;
+    static_assert(ROWS * T::CPR % 64 == 0 && T::CPR <= 64, "whole segments");
 
-    __device__ __forceinline__ static int seg_row(int s) {  // this lane's tile row in segment s
+    __device__ __forceinline__ static int seg_lane(int s) {  // this lane's chunk of the tile in segment s
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        return (wave * PER + s) * (64 / T::CPR) + lane / T::CPR;
+        return min((wave * PER + s) * 64 + lane, ROWS * T::CPR - 1);
     }
-    __device__ __forceinline__ static unsigned seg_chunk(int row, int chunks) {  // bytes within the row
-        const int lane = threadIdx.x & 63;
-        const int c = (lane % T::CPR) ^ T::swz(row);
+    __device__ __forceinline__ static int seg_row(int s) { return seg_lane(s) / T::CPR; }
+    __device__ __forceinline__ static unsigned seg_chunk(int s, int row, int chunks) {  // bytes within the row
+        const int c = (T::EVEN ? (int)(threadIdx.x & 63) % T::CPR : seg_lane(s) % T::CPR) ^ T::swz(row);
         return c < chunks ? (unsigned)c * 16u : 0u;
     }
     // All of the wave's segments from base + off[s], up to four per asm block. The
@@ -231,9 +236,10 @@ struct Loader {
     __device__ __forceinline__ static void load(lds_char* dst, const char* base, const unsigned (&off)[PER]) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const unsigned d = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(dst + wave * PER * T::SEGB));
-        constexpr int N = PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1;
+        constexpr int N = SEGS % NW != 0 ? 1 : PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1;
 #pragma unroll
         for (int s = 0; s < PER; s += N) {
+            if (SEGS % NW != 0 && wave * PER + s >= SEGS) break;  // the last wave's share is shorter
             if constexpr (N == 4)
                 asm volatile(
                     "s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
@@ -260,7 +266,7 @@ struct Loader {
 #pragma unroll
         for (int s = 0; s < PER; ++s) {
             const int row = seg_row(s);
-            off[s] = (unsigned)min(row, last) * row_bytes + seg_chunk(row, chunks);
+            off[s] = (unsigned)min(row, last) * row_bytes + seg_chunk(s, row, chunks);
         }
         load(dst, uniform_ptr(base), off);
     }
@@ -278,13 +284,27 @@ __device__ __forceinline__ void publish() {
     lds_barrier();
 }
 
-// Work item of a work-group. Consecutive work-groups go to different XCDs, each
-// with an L2 of its own; every XCD takes one run of items, so work-groups that
-// share keys and values share an L2.
-__device__ __forceinline__ int xcd_item(int total) {
-    const int per = (total + 7) / 8;
-    return (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-}
+// Work item of a work-group: a block of rows (or keys) of one key head, and its
+// split. Consecutive work-groups go to different XCDs, each with an L2 of its
+// own, so the heads (or, where their number is not a multiple of 8, each head's
+// blocks dealt out to `spread` runs) are the fastest index: a run always meets
+// the same XCD. Blocks are the slowest and go from long to short under a causal
+// mask, over all heads at once: run by run, the last head's longest block
+// started when the others were nearly done (float32, 32 heads of 32 blocks: 69%
+// of the compute units' time in use).
+struct Work {
+    int bh, block, split;
+    __device__ __forceinline__ Work(const AttnParams& p, int splits) {
+        const int runs = p.batch * p.kv_heads * p.spread, id = (int)blockIdx.x;
+        const int run = id % runs, q = id / runs;
+        split = q % splits;
+        block = q / splits * p.spread + run % p.spread;
+        bh = run / p.spread;
+    }
+    static unsigned grid(const AttnParams& p, int blocks, int splits) {
+        return (unsigned)(p.batch * p.kv_heads * p.spread * splits * ((blocks + p.spread - 1) / p.spread));
+    }
+};
 
 // ------------------------------------------------------------------ masks --
 // Per batch: keys that exist, position of query 0, prefix.
@@ -414,7 +434,7 @@ __device__ __forceinline__ void store_part(float* row, const f32x16_t (&acc)[DT]
 // ---------------------------------------------------------------- forward --
 // NW waves of 32 rows; BN keys per tile.
 template <class Tr, int DP, int NW, int BN, int FORM>
-__global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
+__global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
     constexpr int MT = BN / 32, TILEB = T::bytes(BN);
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
@@ -422,10 +442,9 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 256 ? 1 : 2) void attenti
     __shared__ __attribute__((aligned(16))) int key_doc[2][64];  // of a stage's keys
     lds_char* lds = (lds_char*)smem;
 
-    const int item = xcd_item(p.row_blocks * p.splits * p.batch * p.kv_heads);
-    if (item >= p.row_blocks * p.splits * p.batch * p.kv_heads) return;
-    const int split = item % p.splits, rest = item / p.splits;
-    const int rb = p.row_blocks - 1 - rest % p.row_blocks, bh = rest / p.row_blocks;  // the longest causal rows first
+    const Work work(p, p.splits);
+    if (work.block >= p.row_blocks) return;
+    const int split = work.split, bh = work.bh, rb = p.row_blocks - 1 - work.block;
     const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
@@ -604,23 +623,24 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
     if (row >= total) return;
     float top = -kInf;
     for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[s * total + row].x);
-    float l = 0.0f, o[DP / 64];
+    constexpr int NE = (DP + 63) / 64;
+    float l = 0.0f, o[NE];
 #pragma unroll
-    for (int e = 0; e < DP / 64; ++e) o[e] = 0.0f;
+    for (int e = 0; e < NE; ++e) o[e] = 0.0f;
     for (int s = 0; s < p.splits; ++s) {
         const float2 ml = p.part_ml[s * total + row];
         const float a = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
         if (ml.y == 0.0f) continue;  // saw no key; its values are zero
         l += a * ml.y;
 #pragma unroll
-        for (int e = 0; e < DP / 64; ++e) o[e] += a * p.part[(s * total + row) * DP + e * 64 + lane];
+        for (int e = 0; e < NE; ++e) o[e] += a * p.part[(s * total + row) * DP + min(e * 64 + lane, DP - 1)];
     }
     const int bh = (int)(row / p.rows), r = (int)(row % p.rows), b = bh / p.kv_heads;
     const int i = r / p.group, head = (bh % p.kv_heads) * p.group + r % p.group;
     const long long at = (((long long)b * p.queries + i) * p.heads + head) * p.dim;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < DP / 64; ++e) {
+    for (int e = 0; e < NE; ++e) {
         const int d = e * 64 + lane;
         if (d < p.dim) {
             const float v = o[e] * inv;
@@ -640,8 +660,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
 
 template <class Tr, int DP, int FORM>
 void launch_attention_fwd_form(const AttnParams& p) {
-    const int items = p.row_blocks * p.splits * p.batch * p.kv_heads;
-    const unsigned grid = (unsigned)((items + 7) / 8 * 8);
+    const unsigned grid = Work::grid(p, p.row_blocks, p.splits);
     if (p.wide) attention_fwd_kernel<Tr, DP, 4, fwd_tile(DP, Tr::ESIZE, false), FORM><<<grid, 256>>>(p);
     else attention_fwd_kernel<Tr, DP, 1, fwd_tile(DP, Tr::ESIZE, true), FORM><<<grid, 64>>>(p);
 }
@@ -766,7 +785,7 @@ __device__ __forceinline__ float grad_hold(const AttnParams& p) {
 // tile's keys and values against the row's q and dout; the score gradients then
 // meet the keys again, turned.
 template <class Tr, int DP, int BN, int FORM>
-__global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
     constexpr int NW = 4, MT = BN / 32, TILEB = T::bytes(BN);
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
@@ -774,10 +793,9 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     __shared__ __attribute__((aligned(16))) int key_doc[2][64];  // of a stage's keys
     lds_char* lds = (lds_char*)smem;
 
-    const int total = p.row_blocks * p.splits * p.batch * p.kv_heads, item = xcd_item(total);
-    if (item >= total) return;
-    const int split = item % p.splits, rest = item / p.splits;
-    const int rb = p.row_blocks - 1 - rest % p.row_blocks, bh = rest / p.row_blocks;
+    const Work work(p, p.splits);
+    if (work.block >= p.row_blocks) return;
+    const int split = work.split, bh = work.bh, rb = p.row_blocks - 1 - work.block;
     const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
@@ -917,7 +935,8 @@ constexpr bool values_in_lds(int dp, int es) { return dp * es >= 256 && dp * es 
 // LDS. Here the accumulators of the first products hold rows in their registers
 // and a key per lane, so what belongs to a row (its sum, delta, limit, position)
 // comes from LDS, four rows at a time. DV, DK: which gradients this launch makes
-// (32-bit rows of 256 features hold the registers of one at a time).
+// (rows of 256 features leave the registers for one at a time; both at once
+// spilled 208 of them and took 1.9 ms where two launches take PLACE).
 template <class Tr, int DP, int FORM, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
@@ -929,10 +948,9 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     __shared__ __attribute__((aligned(16))) int row_rule[2][2 * BM], row_lim[2][BM];
     lds_char* lds = (lds_char*)smem;
 
-    const int total = p.key_blocks * p.key_splits * p.batch * p.kv_heads, item = xcd_item(total);
-    if (item >= total) return;
-    const int split = item % p.key_splits, rest = item / p.key_splits;
-    const int kblock = rest % p.key_blocks, bh = rest / p.key_blocks;  // the first keys have the most causal rows
+    const Work work(p, p.key_splits);
+    if (work.block >= p.key_blocks) return;
+    const int split = work.split, bh = work.bh, kblock = work.block;
     const int b = bh / p.kv_heads, kvh = bh % p.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
@@ -1004,7 +1022,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         for (int s = 0; s < L::PER; ++s) {
             const int row = L::seg_row(s), rr = min(r0 + row, p.rows - 1);
             const int i = (int)ormi_fdiv((unsigned)rr, p.group_m, p.group_s), g = rr - i * p.group;
-            const unsigned c = L::seg_chunk(row, p.chunks);
+            const unsigned c = L::seg_chunk(s, row, p.chunks);
             qo[s] = ((unsigned)(i - i0) * (unsigned)p.q_sl + (unsigned)g * (unsigned)p.q_sh) * T::ES + c;
             go[s] = ((unsigned)(i - i0) * (unsigned)p.do_sl + (unsigned)g * (unsigned)p.do_sh) * T::ES + c;
         }
@@ -1144,12 +1162,12 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttnParams p) 
     const int lane = threadIdx.x & 63;
     auto add = [&](const float* part, int splits, long long n, char* out, long long at, float f) {
 #pragma unroll
-        for (int e = 0; e < DP / 64; ++e) {
+        for (int e = 0; e < (DP + 63) / 64; ++e) {
             const int d = e * 64 + lane;
+            if (d >= p.dim) continue;
             float v = 0.0f;
             for (int s = 0; s < splits; ++s) v += part[(s * n + row) * DP + d];
             v *= f;
-            if (d >= p.dim) continue;
             if constexpr (Tr::ESIZE == 4) ((float*)out)[at + d] = v;
             else ((unsigned short*)out)[at + d] = (unsigned short)pack2(Tr{}, v, v);
         }
@@ -1171,13 +1189,10 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttnParams p) 
 
 template <class Tr, int DP, int FORM>
 void launch_attention_grad_form(const AttnParams& p) {
-    if (p.dq) {
-        const unsigned items = (unsigned)(p.row_blocks * p.splits * p.batch * p.kv_heads);
-        attention_dq_kernel<Tr, DP, fwd_tile(DP, Tr::ESIZE, false), FORM><<<(items + 7) / 8 * 8, 256>>>(p);
-    }
+    if (p.dq) attention_dq_kernel<Tr, DP, fwd_tile(DP, Tr::ESIZE, false), FORM><<<Work::grid(p, p.row_blocks, p.splits), 256>>>(p);
     if (p.dk || p.dv) {
-        const unsigned items = (unsigned)(p.key_blocks * p.key_splits * p.batch * p.kv_heads), grid = (items + 7) / 8 * 8;
-        if constexpr (DP * Tr::ESIZE > 512) {
+        const unsigned grid = Work::grid(p, p.key_blocks, p.key_splits);
+        if constexpr (DP > 128) {
             if (p.dk) attention_dkv_kernel<Tr, DP, FORM, true, false><<<grid, 256>>>(p);
             if (p.dv) attention_dkv_kernel<Tr, DP, FORM, false, true><<<grid, 256>>>(p);
         } else {
