@@ -4,9 +4,7 @@
 
 namespace ormi_hip {
 
-// What a score is beside a positive multiple of q.k: kPlain (the maximum is then
-// taken of the unscaled products), kBias (slopes, or a scale of zero or less),
-// kCap (a tanh, and perhaps slopes).
+// What a score is beside a multiple of q.k: nothing, slopes, or a tanh and perhaps slopes.
 constexpr int kPlain = 0, kBias = 1, kCap = 2;
 
 constexpr int kDocTile = 64;  // tokens per document range

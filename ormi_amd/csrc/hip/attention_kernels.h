@@ -176,8 +176,10 @@ struct Tile {
         const int d = dt * 32 + (lane & 31);
         return *(const lds_float*)(t + at(row0) + at(row) + (((d >> 2) ^ swz(row)) << 4) + (d & 3) * 4);
     }
-    // acc[dt] += (the tile's rows row0.. turned) x (accumulator `a` as 16- or 32-bit operand)
-    __device__ __forceinline__ static void second(const lds_char* t, int row0, const f32x16_t& a, f32x16_t (&acc)[DT]) {
+    // acc[dt] += (the tile's rows row0.. turned) x (accumulator `a` as 16- or 32-bit
+    // operand); SUM: sum += its columns' sums, by a product with ones.
+    template <bool SUM = false>
+    __device__ __forceinline__ static void second(const lds_char* t, int row0, const f32x16_t& a, f32x16_t (&acc)[DT], f32x16_t* sum = nullptr) {
         if constexpr (ES == 2) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -186,6 +188,10 @@ struct Tile {
                 for (int e = 0; e < 4; ++e) b[e] = pack2(Tr{}, a[8 * s + 2 * e], a[8 * s + 2 * e + 1]);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) Tr::mma(turned(t, row0, s, dt), b, acc[dt]);
+                if constexpr (SUM) {
+                    constexpr unsigned one = IsF16<Tr>::value ? 0x3C003C00u : 0x3F803F80u;
+                    Tr::mma(u32x4_t{one, one, one, one}, b, *sum);
+                }
             }
         } else {
 #pragma unroll
@@ -360,18 +366,17 @@ struct DocTiles {
     __device__ __forceinline__ bool same(int t) const { return one >> (t / RT - base) & 1; }
 };
 
-// A score in powers of two; its derivative with respect to scale q.k in slope (kCap).
+// A score in powers of two, plus base; its derivative with respect to scale q.k
+// in slope (kCap).
 template <class Tr, int FORM>
-__device__ __forceinline__ float score2(const AttnParams& p, float s, float slope2, float away, float& slope) {
-    float t;
+__device__ __forceinline__ float score2(const AttnParams& p, float s, float slope2, float away, float base, float& slope) {
+    if constexpr (FORM != kPlain) base = __builtin_fmaf(-slope2, __builtin_fabsf(away), base);
     if constexpr (FORM == kCap) {
         const float u = tanh_score(Tr{}, s * p.scale_over_cap);
-        t = u * p.cap2;
         slope = __builtin_fmaf(-u, u, 1.0f);
-    } else {
-        t = s * p.scale2;
+        return __builtin_fmaf(u, p.cap2, base);
     }
-    return __builtin_fmaf(-slope2, __builtin_fabsf(away), t);
+    return __builtin_fmaf(s, p.scale2, base);
 }
 
 // ---------------------------------------------------------------- outputs --
@@ -493,7 +498,14 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
     const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
 
     DocTiles<BN> walk{p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr, p.range_tiles, -1, docs_group, docs_wave};
-    auto next = [&](int t) { return p.docs ? walk.next(t, t1) : t; };
+    // With slopes the tiles nearest to the rows come first: the maximum then seldom
+    // moves, and tiles too far off for any weight cost their scores alone.
+    const int near = FORM != kPlain && p.slopes && !p.docs ? min(max((rb * NW * 32 / p.group + span.off) / BN, t0), max(t1 - 1, t0)) : t0;
+    auto after = [&](int t) {
+        if (p.docs) return walk.next(t + 1, t1);
+        if (t >= near) return t + 1 < t1 ? t + 1 : near > t0 ? near - 1 : t1;
+        return t > t0 ? t - 1 : t1;
+    };
     const char* kb = p.k + (b * p.k_sb + kvh * p.k_sh) * T::ES;
     const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh) * T::ES;
     using L = Loader<Tr, DP, BN, NW>;
@@ -509,17 +521,23 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
     for (int dt = 0; dt < T::DT; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
-    // m: the row's maximum in powers of two (of the unscaled products' sizes when
-    // kPlain), which may lag by up to 2^8 (the sums then grow by as much).
-    float m = -kInf, l = 0.0f;
-    const float unit = FORM != kPlain ? 1.0f : p.scale2;
+    // m: the row's maximum, in powers of two; it may lag by up to 2^8 (the sums then
+    // grow by as much). base: what turns a score into the exponent of what is held.
+    float m = -kInf, l = 0.0f, base = Shift<Tr>::fwd;
+    // At 64 features the exponentials bound the kernel and the matrix pipes have
+    // time to add up their sums (bfloat16 8191 x 12 heads: PLACE).
+    constexpr bool SUM = T::ES == 2 && DP == 64;
+    f32x16_t sum;
+    if constexpr (SUM)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
 
-    int t = next(t0), stage = 0;
+    int t = p.docs ? walk.next(t0, t1) : near, stage = 0;
     bool same = !p.docs || (t < t1 && walk.same(t));
     if (t < t1) issue(t, 0);
     while (t < t1) {
         publish();
-        const int tn = next(t + 1);
+        const int tn = after(t);
         const bool same_next = !p.docs || (tn < t1 && walk.same(tn));
         if (tn < t1) issue(tn, stage ^ 1);
         const int j0 = t * BN;
@@ -535,12 +553,10 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
 #pragma unroll
                 for (int f = 0; f < T::NF; ++f) Tr::mma(T::frag(kt, mt * 32, f), qf[f], s[mt]);
                 settle<Tr>(s[mt]);
-                if constexpr (FORM != kPlain) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float slope;
-                        s[mt][e] = score2<Tr, FORM>(p, s[mt][e], slope2, away - (float)(mt * 32 + 8 * (e >> 2) + (e & 3)), slope);
-                    }
+                for (int e = 0; e < 16; ++e) {
+                    float slope;
+                    s[mt][e] = score2<Tr, FORM>(p, s[mt][e], slope2, away - (float)(mt * 32 + 8 * (e >> 2) + (e & 3)), base, slope);
                 }
             }
             if (j0 + BN > lim_min || !same) {
@@ -570,28 +586,39 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) top = max3(top, s[mt][e], s[mt][e + 1]);
             top = halves_max(top);
-            if (__any((top - m) * unit > 8.0f)) {
-                const float mn = fmaxf(m, top);
-                const float a = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * unit);
-                l *= a;
+            if (__any(m == -kInf ? top > -kInf : top > 8.0f + Shift<Tr>::fwd)) {
+                const float mn = fmaxf(m, top - base);
+                const float a = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                const float to = mn == -kInf ? base : Shift<Tr>::fwd - mn, by = to - base;
+                if constexpr (SUM) sum[0] *= a;
+                else l *= a;
 #pragma unroll
                 for (int dt = 0; dt < T::DT; ++dt)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) acc[dt][e] *= a;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[mt][e] += by;
+                top += by;
                 m = mn;
+                base = to;
             }
-            const float base = m == -kInf ? 0.0f : Shift<Tr>::fwd - m * unit;
-            float part[2] = {0.0f, 0.0f};
+            // Exponents below float32's least make every weight zero (keys far off
+            // under a steep slope, rows whose mask leaves nothing of the tile).
+            if (__any(!(top < -152.0f))) {
+                float part[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[mt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][e], unit, base));
-                    part[e & 1] += s[mt][e];
-                }
-            l += part[0] + part[1];
+                    for (int e = 0; e < 16; ++e) {
+                        s[mt][e] = __builtin_amdgcn_exp2f(s[mt][e]);
+                        if constexpr (!SUM) part[e & 1] += s[mt][e];
+                    }
+                if constexpr (!SUM) l += part[0] + part[1];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) T::second(vt, mt * 32, s[mt], acc);
+                for (int mt = 0; mt < MT; ++mt) T::template second<SUM>(vt, mt * 32, s[mt], acc, &sum);
+            }
         }
         t = tn;
         same = same_next;
@@ -600,17 +627,22 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
 
 #pragma unroll
     for (int dt = 0; dt < T::DT; ++dt) settle<Tr>(acc[dt]);
-    l = halves_sum(l);
+    if constexpr (SUM) {
+        settle<Tr>(sum);
+        l = sum[0];
+    } else {
+        l = halves_sum(l);
+    }
     if (r >= p.rows) return;
     if (p.splits > 1) {
         const long long at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows + r;
         store_part(p.part + at * DP, acc);
-        if (half == 0) p.part_ml[at] = make_float2(m == -kInf ? -kInf : m * unit - Shift<Tr>::fwd, l);
+        if (half == 0) p.part_ml[at] = make_float2(m == -kInf ? -kInf : m - Shift<Tr>::fwd, l);
         return;
     }
     const long long to = (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES;
     store_row<Tr, T::DT>(p.out + to, p.dim, acc, l == 0.0f ? 0.0f : 1.0f / l, p.rest ? p.rest + to : nullptr);
-    if (p.lse && half == 0) p.lse[(long long)bh * p.rows + r] = l == 0.0f ? kInf : m * unit - Shift<Tr>::fwd + __builtin_log2f(l);
+    if (p.lse && half == 0) p.lse[(long long)bh * p.rows + r] = l == 0.0f ? kInf : m - Shift<Tr>::fwd + __builtin_log2f(l);
 }
 
 // Joins the splits of a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
@@ -854,7 +886,6 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
     for (int dt = 0; dt < T::DT; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
-    const float unit = FORM != kPlain ? 1.0f : p.scale2;
 
     int t = next(t0), stage = 0;
     bool same = !p.docs || (t < t1 && walk.same(t));
@@ -884,9 +915,9 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
                 settle<Tr>(g);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float slope = 1.0f, t2 = s[e];
-                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, slope2, away - (float)(mt * 32 + 8 * (e >> 2) + (e & 3)), slope);
-                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, -lse));
+                    float slope = 1.0f;
+                    const float pr = __builtin_amdgcn_exp2f(
+                        score2<Tr, FORM>(p, s[e], slope2, away - (float)(mt * 32 + 8 * (e >> 2) + (e & 3)), -lse, slope));
                     float ds = pr * (g[e] - delta);
                     if (FORM == kCap) ds *= slope;
                     if (Shift<Tr>::bwd != 0.0f) ds *= hold;
@@ -1049,7 +1080,6 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     for (int dt = 0; dt < T::DT; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc_k[dt][e] = acc_v[dt][e] = 0.0f;
-    const float unit = FORM != kPlain ? 1.0f : p.scale2;
 
     int t = next(t0), stage = 0;
     if (t < t1) {
@@ -1104,9 +1134,9 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int x = 4 * q4 + e;
-                    float t2 = s[x], slope = 1.0f;
-                    if constexpr (FORM != kPlain) t2 = score2<Tr, FORM>(p, t2, sloped ? sl[e] * 1.44269504f : 0.0f, ps[e] - keyf, slope);
-                    s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(t2, unit, shift - ls[e]));
+                    float slope = 1.0f;
+                    s[x] = __builtin_amdgcn_exp2f(
+                        score2<Tr, FORM>(p, s[x], sloped ? sl[e] * 1.44269504f : 0.0f, ps[e] - keyf, shift - ls[e], slope));
                     if (!DK) continue;
                     g[x] = s[x] * (g[x] - de[e]);
                     if (FORM == kCap) g[x] *= slope;
