@@ -52,7 +52,44 @@ struct alignas(N * sizeof(typename Elem<DT>::type) >= 16 ? 16 : N * sizeof(typen
 
 constexpr int HEADS = 4;
 
-template <int IN, int OUT, int V, bool INTERLEAVED>
+// Every element is read once and written once, so where each access covers whole
+// 128-byte lines (runs of that many bytes) it goes past the caches, which stay
+// with the tables: 4 x 4096 x 16 x 128 float32 to bfloat16 45 -> 33 us, 6.0 TB/s.
+// Shorter runs share lines between accesses and would fetch them again (float16
+// runs of 48 bytes: 15.8 -> 31 us).
+template <bool PAST, class P>
+__device__ __forceinline__ P stream_in(const void* at) {
+    if constexpr (PAST && sizeof(P) % 16 == 0) {
+        P r;
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(P) / 16; ++i) {
+            const ormi_f4 w = __builtin_nontemporal_load((const ormi_f4*)at + i);
+            __builtin_memcpy((char*)&r + 16 * i, &w, 16);
+        }
+        return r;
+    } else {
+        return *(const P*)at;
+    }
+}
+template <bool PAST, class P>
+__device__ __forceinline__ void stream_out(void* at, const P& v) {
+    if constexpr (PAST && sizeof(P) % 16 == 0) {
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(P) / 16; ++i) {
+            ormi_f4 w;
+            __builtin_memcpy(&w, (const char*)&v + 16 * i, 16);
+            __builtin_nontemporal_store(w, (ormi_f4*)at + i);
+        }
+    } else if constexpr (PAST && sizeof(P) == 8) {
+        unsigned long long w;
+        __builtin_memcpy(&w, &v, 8);
+        __builtin_nontemporal_store(w, (unsigned long long*)at);
+    } else {
+        *(P*)at = v;
+    }
+}
+
+template <int IN, int OUT, int V, bool INTERLEAVED, bool PAST>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     using TI = typename Elem<IN>::type;
     using TO = typename Elem<OUT>::type;
@@ -65,28 +102,38 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     const int h0 = (int)hg * HEADS, hn = min(HEADS, p.heads - h0);
     const TI* x = (const TI*)p.x + (b * p.sb + l * p.sl + (long long)h0 * p.sh);
     TO* out = (TO*)p.out + ((long long)tok * p.heads + h0) * p.dim;
-    // The unit's 2 V elements: two runs of V, the second `apart` after the first.
+    // The unit's 2 V elements: a run of V in each half of the turned features (or
+    // of the others), so that the lanes of one access are neighbours, with
+    // interleaved pairs too.
+    constexpr bool SINGLE = INTERLEAVED && V == 1;  // a pair of neighbours
     const bool turn = u < p.turned;
     int d, apart;
     if (turn) {
-        d = INTERLEAVED ? (int)u * 2 * V : (int)u * V;
-        apart = INTERLEAVED ? V : p.part / 2;
+        d = SINGLE ? (int)u * 2 : (int)u * V;
+        apart = SINGLE ? 1 : p.part / 2;
     } else {
-        d = p.part + (int)(u - p.turned) * 2 * V;
-        apart = V;
+        d = p.part + (int)(u - p.turned) * (V > 1 ? V : 2);
+        apart = V > 1 ? (p.dim - p.part) / 2 : 1;
     }
     const bool second = turn || V > 1 || d + 1 < p.dim;  // one feature may be left over at V = 1
+    // Cosine and sine of the pairs: V of the two runs' elements, or with
+    // interleaved pairs V / 2 of each run.
     float c[V], s[V];
     if (turn) {
         const long long at = p.positions ? p.positions[b * p.pos_sb + l * p.pos_sl] : (long long)p.offset + l;
         const bool inside = at >= 0 && at < p.rows;
-        const long long row = (inside ? at : 0) * (p.part / 2) + (long long)u * V;
-        const Pack<ORMI_DTYPE_F32, V> cv = *(const Pack<ORMI_DTYPE_F32, V>*)(p.cos + row);
-        const Pack<ORMI_DTYPE_F32, V> sv = *(const Pack<ORMI_DTYPE_F32, V>*)(p.sin + row);
+        const long long row = (inside ? at : 0) * (p.part / 2);
+        constexpr int H = INTERLEAVED && V > 1 ? V / 2 : V;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            c[e] = inside ? cv.v[e] : __builtin_nanf("");
-            s[e] = inside ? sv.v[e] * p.sign : __builtin_nanf("");
+        for (int k = 0; k < V / H; ++k) {
+            const long long from = row + (long long)u * H + k * (p.part / 4);
+            const Pack<ORMI_DTYPE_F32, H> cv = *(const Pack<ORMI_DTYPE_F32, H>*)(p.cos + from);
+            const Pack<ORMI_DTYPE_F32, H> sv = *(const Pack<ORMI_DTYPE_F32, H>*)(p.sin + from);
+#pragma unroll
+            for (int e = 0; e < H; ++e) {
+                c[k * H + e] = inside ? cv.v[e] : __builtin_nanf("");
+                s[k * H + e] = inside ? sv.v[e] * p.sign : __builtin_nanf("");
+            }
         }
     }
     Pack<IN, V> r0[HEADS], r1[HEADS];
@@ -95,8 +142,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
         if (h >= hn) continue;
         const TI* at = x + h * p.sh;
         if (V > 1) {
-            r0[h] = *(const Pack<IN, V>*)(at + d);
-            r1[h] = *(const Pack<IN, V>*)(at + d + apart);
+            r0[h] = stream_in<PAST, Pack<IN, V>>(at + d);
+            r1[h] = stream_in<PAST, Pack<IN, V>>(at + d + apart);
         } else {
             r0[h].v[0] = at[d * p.sd];
             if (second) r1[h].v[0] = at[(d + apart) * p.sd];
@@ -115,14 +162,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
         } else if (INTERLEAVED && V > 1) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int i = 2 * e, j = 2 * e + 1;
-                const float a = to_f32<IN>(i < V ? r0[h].v[i % V] : r1[h].v[i % V]);
-                const float q = to_f32<IN>(j < V ? r0[h].v[j % V] : r1[h].v[j % V]);
-                const TO na = from_f32<OUT>(a * c[e] - q * s[e]), nb = from_f32<OUT>(q * c[e] + a * s[e]);
-                if (i < V) o0.v[i % V] = na;
-                else o1.v[i % V] = na;
-                if (j < V) o0.v[j % V] = nb;
-                else o1.v[j % V] = nb;
+                const Pack<IN, V>& r = e < V / 2 ? r0[h] : r1[h];
+                Pack<OUT, V>& o = e < V / 2 ? o0 : o1;
+                const int i = 2 * e % V;
+                const float a = to_f32<IN>(r.v[i]), q = to_f32<IN>(r.v[i + 1]);
+                o.v[i] = from_f32<OUT>(a * c[e] - q * s[e]);
+                o.v[i + 1] = from_f32<OUT>(q * c[e] + a * s[e]);
             }
         } else {
 #pragma unroll
@@ -133,29 +178,30 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
             }
         }
         TO* at = out + (long long)h * p.dim;
-        *(Pack<OUT, V>*)(at + d) = o0;
-        if (second) *(Pack<OUT, V>*)(at + d + apart) = o1;
+        stream_out<PAST>(at + d, o0);
+        if (second) stream_out<PAST>(at + d + apart, o1);
     }
 }
 
-template <int IN, int OUT, int V>
+template <int IN, int OUT, int V, bool PAST>
 void launch_v(const RotaryParams& p, bool interleaved) {
     const unsigned grid = (p.total + 255) / 256;
-    if (interleaved) rotary_kernel<IN, OUT, V, true><<<grid, 256>>>(p);
-    else rotary_kernel<IN, OUT, V, false><<<grid, 256>>>(p);
+    if (interleaved) rotary_kernel<IN, OUT, V, true, PAST><<<grid, 256>>>(p);
+    else rotary_kernel<IN, OUT, V, false, PAST><<<grid, 256>>>(p);
 }
 template <int IN, int OUT>
-void launch_types(const RotaryParams& p, int v, bool interleaved) {
-    if (v == 8) launch_v<IN, OUT, 8>(p, interleaved);
-    else if (v == 4) launch_v<IN, OUT, 4>(p, interleaved);
-    else launch_v<IN, OUT, 1>(p, interleaved);
+void launch_types(const RotaryParams& p, int v, bool interleaved, bool past) {
+    if constexpr (IN != ORMI_DTYPE_F32 && OUT != ORMI_DTYPE_F32)
+        if (v == 8) return past ? launch_v<IN, OUT, 8, true>(p, interleaved) : launch_v<IN, OUT, 8, false>(p, interleaved);
+    if (v == 4) past ? launch_v<IN, OUT, 4, true>(p, interleaved) : launch_v<IN, OUT, 4, false>(p, interleaved);
+    else launch_v<IN, OUT, 1, false>(p, interleaved);
 }
 template <int IN>
-void launch_in(const RotaryParams& p, int out, int v, bool interleaved) {
+void launch_in(const RotaryParams& p, int out, int v, bool interleaved, bool past) {
     switch (out) {
-        case ORMI_DTYPE_F32: launch_types<IN, ORMI_DTYPE_F32>(p, v, interleaved); break;
-        case ORMI_DTYPE_BF16: launch_types<IN, ORMI_DTYPE_BF16>(p, v, interleaved); break;
-        default: launch_types<IN, ORMI_DTYPE_F16>(p, v, interleaved);
+        case ORMI_DTYPE_F32: launch_types<IN, ORMI_DTYPE_F32>(p, v, interleaved, past); break;
+        case ORMI_DTYPE_BF16: launch_types<IN, ORMI_DTYPE_BF16>(p, v, interleaved, past); break;
+        default: launch_types<IN, ORMI_DTYPE_F16>(p, v, interleaved, past);
     }
 }
 
@@ -216,7 +262,10 @@ extern "C" int ormi_hip_rotary(const ormi_rotary_desc* d) {
                (uintptr_t)d->cos % 16 == 0 && (uintptr_t)d->sin % 16 == 0 && whole(p.sb, d->batch) && whole(p.sl, d->length) &&
                whole(p.sh, d->heads);
     };
-    const int v = fits(8) ? 8 : fits(4) ? 4 : 1;
+    const bool wide = es_in == 4 || es_out == 4;  // 4 fp32 elements are a whole access
+    const int v = !wide && fits(8) ? 8 : fits(4) ? 4 : 1;
+    const int run = d->part / 2, rest = (d->dim - d->part) / 2;
+    const bool past = run * std::min(es_in, es_out) % 128 == 0 && rest * std::min(es_in, es_out) % 128 == 0;
     p.turned = (unsigned)(d->part / 2 / v);
     p.units = p.turned + (unsigned)((d->dim - d->part + 2 * v - 1) / (2 * v));
     p.groups = (unsigned)((d->heads + HEADS - 1) / HEADS);
@@ -229,9 +278,9 @@ extern "C" int ormi_hip_rotary(const ormi_rotary_desc* d) {
         p.first = (unsigned)at;
         p.total = (unsigned)(std::min(most, tokens - at) * per_token);
         switch (d->dtype) {
-            case ORMI_DTYPE_F32: launch_in<ORMI_DTYPE_F32>(p, d->out_dtype, v, d->interleaved != 0); break;
-            case ORMI_DTYPE_BF16: launch_in<ORMI_DTYPE_BF16>(p, d->out_dtype, v, d->interleaved != 0); break;
-            default: launch_in<ORMI_DTYPE_F16>(p, d->out_dtype, v, d->interleaved != 0);
+            case ORMI_DTYPE_F32: launch_in<ORMI_DTYPE_F32>(p, d->out_dtype, v, d->interleaved != 0, past); break;
+            case ORMI_DTYPE_BF16: launch_in<ORMI_DTYPE_BF16>(p, d->out_dtype, v, d->interleaved != 0, past); break;
+            default: launch_in<ORMI_DTYPE_F16>(p, d->out_dtype, v, d->interleaved != 0, past);
         }
     }
     const hipError_t e = hipGetLastError();
