@@ -34,6 +34,7 @@ struct AttnParams {
     // Work split.
     int wide;  // 4 waves per work-group (128 rows), else one
     int row_blocks, splits;
+    int split_tiles;  // tiles per split, or 0: an equal share of the row's tiles
     int spread;  // runs of blocks per head (Work)
     float* part;    // of out, or of dk and dv
     float* part_q;  // of dq

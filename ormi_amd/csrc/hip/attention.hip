@@ -164,14 +164,22 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
     p.spread = heads % 8 == 0 ? 1 : heads % 4 == 0 ? 2 : heads % 2 == 0 ? 4 : 8;
     if (!g) {
         // Few rows (single tokens): one wave per work-group. Where the rows of
-        // all heads leave compute units idle the keys are split over work-groups,
-        // at least two tiles each, and joined.
+        // all heads leave compute units idle the keys are split over work-groups
+        // and joined.
         p.wide = p.rows > 32;
         p.row_blocks = p.wide ? (p.rows + 127) / 128 : 1;
         const int bn = fwd_tile(dp, es, !p.wide);
         const long long items = heads * p.row_blocks, slots = (long long)cus * (p.wide ? (es == 4 ? 3 : 2) : 4);
         const int tiles = (d->keys + bn - 1) / bn;
-        p.splits = items > 0 && items * 2 <= slots ? (int)std::max<long long>(1, std::min<long long>({slots / items, tiles / 2, 64})) : 1;
+        p.splits = 1;
+        if (items > 0 && items * 2 <= slots) {
+            // Single tokens over unequal lengths: splits of one size, twice as many as
+            // fit, so that short sequences leave room instead of finishing early.
+            const bool even = !p.wide && d->lengths;
+            const long long want = std::min<long long>({(even ? 2 * slots : slots) / items, p.wide ? tiles / 2 : tiles, 64});
+            p.splits = (int)std::max<long long>(1, want);
+            if (even) p.split_tiles = (tiles + p.splits - 1) / p.splits;
+        }
         if (p.splits > 1) {
             pl.part = take(pl.bytes, sizeof(float) * (size_t)p.splits * heads * p.rows * dp);
             pl.part_ml = take(pl.bytes, sizeof(float2) * (size_t)p.splits * heads * p.rows);

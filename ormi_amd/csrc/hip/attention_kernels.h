@@ -494,7 +494,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
         }
     }
     const int tiles = (lim_group + BN - 1) / BN;
-    const int per = (tiles + p.splits - 1) / p.splits;
+    const int per = p.split_tiles ? p.split_tiles : (tiles + p.splits - 1) / p.splits;
     const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
 
     DocTiles<BN> walk{p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr, p.range_tiles, -1, docs_group, docs_wave};
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
     if (r >= p.rows) return;
     if (p.splits > 1) {
         const long long at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows + r;
-        store_part(p.part + at * DP, acc);
+        if (!(l == 0.0f)) store_part(p.part + at * DP, acc);
         if (half == 0) p.part_ml[at] = make_float2(m == -kInf ? -kInf : m - Shift<Tr>::fwd, l);
         return;
     }
@@ -646,24 +646,29 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
 }
 
 // Joins the splits of a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
-// in split order. One wave per row, lanes along the features.
+// in split order. One wave per row: lane s holds split s's maximum and sum (at
+// most 64 splits), then the lanes go along the features; a split that saw no key
+// has stored no values.
 template <class Tr, int DP>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
     const long long total = (long long)p.batch * p.kv_heads * p.rows;
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= total) return;
-    float top = -kInf;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[s * total + row].x);
     constexpr int NE = (DP + 63) / 64;
-    float l = 0.0f, o[NE];
+    const float2 ml = lane < p.splits ? p.part_ml[lane * total + row] : make_float2(-kInf, 0.0f);
+    const bool some = !(ml.y == 0.0f);
+    const float top = ormi_lanes_max<64>(some ? ml.x : -kInf);
+    const float weight = some ? __builtin_amdgcn_exp2f(ml.x - top) : 0.0f;
+    const float l = ormi_lanes_sum<64>(some ? weight * ml.y : 0.0f);
+    const unsigned long long live = __ballot(some);
+    float o[NE];
 #pragma unroll
     for (int e = 0; e < NE; ++e) o[e] = 0.0f;
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
-        const float2 ml = p.part_ml[s * total + row];
-        const float a = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
-        if (ml.y == 0.0f) continue;  // saw no key; its values are zero
-        l += a * ml.y;
+        if (!(live >> s & 1)) continue;
+        const float a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), s));
 #pragma unroll
         for (int e = 0; e < NE; ++e) o[e] += a * p.part[(s * total + row) * DP + min(e * 64 + lane, DP - 1)];
     }
@@ -1196,6 +1201,7 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttnParams p) 
             const int d = e * 64 + lane;
             if (d >= p.dim) continue;
             float v = 0.0f;
+#pragma unroll 4
             for (int s = 0; s < splits; ++s) v += part[(s * n + row) * DP + d];
             v *= f;
             if constexpr (Tr::ESIZE == 4) ((float*)out)[at + d] = v;
