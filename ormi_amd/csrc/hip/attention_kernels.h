@@ -604,9 +604,9 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
                 m = mn;
                 base = to;
             }
-            // Exponents below float32's least make every weight zero (keys far off
-            // under a steep slope, rows whose mask leaves nothing of the tile).
-            if (__any(!(top < -152.0f))) {
+            // Under a steep slope exponents below float32's least make every weight of
+            // a tile far off zero.
+            if (FORM != kBias || __any(!(top < -152.0f))) {
                 float part[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
