@@ -436,6 +436,88 @@ __device__ __forceinline__ void store_part(float* row, const f32x16_t (&acc)[DT]
                 make_float4(acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]);
 }
 
+// ----------------------------------------------------------------- repair --
+// A masked position has the weight zero, and zero times an infinity or a NaN that
+// stands there is a NaN in the matrix products. Rows (and keys) that end up not
+// finite though their own sums are finite are therefore added up again, in plain
+// order and over what they see alone; nothing else pays for it but one look at
+// the accumulators. One row at a time, the wave's lanes along the features.
+template <class Tr>
+__device__ __forceinline__ float load1(const char* row, int d) {
+    if constexpr (Tr::ESIZE == 4) return ((const float*)row)[d];
+    else return unpack<Tr>(((const unsigned short*)row)[d]);
+}
+
+template <class Tr>
+__device__ __forceinline__ float row_dot(const char* a, const char* b, int dim) {
+    float v = 0.0f;
+    for (int d = threadIdx.x & 63; d < dim; d += 64) v = __builtin_fmaf(load1<Tr>(a, d), load1<Tr>(b, d), v);
+    return ormi_wave_sum(v);
+}
+// sum += w times a row's features lane, lane + 64, ...
+template <class Tr>
+__device__ __forceinline__ void add_row(const char* row, int dim, float w, float (&sum)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int d = e * 64 + (int)(threadIdx.x & 63);
+        if (d < dim) sum[e] = __builtin_fmaf(w, load1<Tr>(row, d), sum[e]);
+    }
+}
+template <class Tr>
+__device__ __forceinline__ void put_row(char* row, int dim, const float (&sum)[4], float f, char* rest) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int d = e * 64 + (int)(threadIdx.x & 63);
+        if (d >= dim) continue;
+        const float v = sum[e] * f;
+        if constexpr (Tr::ESIZE == 4) ((float*)row)[d] = v;
+        else {
+            const unsigned w = pack2(Tr{}, v, v);
+            ((unsigned short*)row)[d] = (unsigned short)w;
+            if (rest) {
+                const float left = v - unpack<Tr>(w);
+                ((unsigned short*)rest)[d] = (unsigned short)pack2(Tr{}, left, left);
+            }
+        }
+    }
+}
+// Whether any of the lane's row's accumulators, in either half, is not finite.
+template <int DT>
+__device__ __forceinline__ bool not_finite(const f32x16_t (&acc)[DT]) {
+    float z = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z = __builtin_fmaf(acc[dt][e], 0.0f, z);
+    return !(halves_sum(z) == 0.0f);
+}
+template <int DT>
+__device__ __forceinline__ void clear_if(bool yes, f32x16_t (&acc)[DT]) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] = yes ? 0.0f : acc[dt][e];
+}
+__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+
+// What a row needs to find its weights again.
+struct RepairRow {
+    int pos, lim, doc;
+    float slope2, base;
+};
+// f(j, key's weight's exponent base included) for the keys in [j0, j1) that the row sees.
+template <class Tr, int FORM, class F>
+__device__ __forceinline__ void each_seen(const AttnParams& p, int b, int kvh, const RepairRow& row, const char* q, int j0, int j1, F&& f) {
+    for (int j = j0; j < min(j1, row.lim); ++j) {
+        if (p.docs && doc_at(p, b, j) != row.doc) continue;
+        const char* k = p.k + (b * p.k_sb + (long long)j * p.k_sl + kvh * p.k_sh) * Tr::ESIZE;
+        const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + kvh * p.v_sh) * Tr::ESIZE;
+        float slope = 1.0f;
+        const float t = score2<Tr, FORM>(p, row_dot<Tr>(q, k, p.dim), row.slope2, (float)(row.pos - j), row.base, slope);
+        f(k, v, __builtin_amdgcn_exp2f(t), slope);
+    }
+}
+
 // ---------------------------------------------------------------- forward --
 // NW waves of 32 rows; BN keys per tile.
 template <class Tr, int DP, int NW, int BN, int FORM>
@@ -633,15 +715,38 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
     } else {
         l = halves_sum(l);
     }
+    const long long part_at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows;  // + row
+    clear_if(l == 0.0f, acc);
+    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && l < kInf && not_finite(acc));
+    const bool repaired = todo >> (lane & 31) & 1;
+    while (todo) {
+        const int from = __builtin_ctz(todo), rr = __builtin_amdgcn_readlane(r, from);
+        todo &= todo - 1;
+        const int hh = __builtin_amdgcn_readlane(head, from), ii = __builtin_amdgcn_readlane(i, from);
+        const RepairRow row = {__builtin_amdgcn_readlane(pos, from), __builtin_amdgcn_readlane(lim, from), __builtin_amdgcn_readlane(doc, from),
+                               lane_of(slope2, from), lane_of(base, from)};
+        const long long at = ((long long)b * p.queries + ii) * p.heads + hh;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        each_seen<Tr, FORM>(p, b, kvh, row, p.q + (b * p.q_sb + (long long)ii * p.q_sl + hh * p.q_sh) * T::ES, t0 * BN, t1 * BN,
+                            [&](const char*, const char* v, float w, float) { add_row<Tr>(v, p.dim, w, o); });
+        if (p.splits > 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e * 64 + lane < DP) p.part[(part_at + rr) * DP + e * 64 + lane] = o[e];
+        } else {
+            put_row<Tr>(p.out + at * p.dim * T::ES, p.dim, o, 1.0f / lane_of(l, from), p.rest ? p.rest + at * p.dim * T::ES : nullptr);
+        }
+    }
     if (r >= p.rows) return;
     if (p.splits > 1) {
-        const long long at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows + r;
-        if (!(l == 0.0f)) store_part(p.part + at * DP, acc);
+        const long long at = part_at + r;
+        if (!(l == 0.0f) && !repaired) store_part(p.part + at * DP, acc);
         if (half == 0) p.part_ml[at] = make_float2(m == -kInf ? -kInf : m - Shift<Tr>::fwd, l);
         return;
     }
     const long long to = (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES;
-    store_row<Tr, T::DT>(p.out + to, p.dim, acc, l == 0.0f ? 0.0f : 1.0f / l, p.rest ? p.rest + to : nullptr);
+    if (!repaired)
+        store_row<Tr, T::DT>(p.out + to, p.dim, acc, l == 0.0f ? 0.0f : 1.0f / l, p.rest ? p.rest + to : nullptr);
     if (p.lse && half == 0) p.lse[(long long)bh * p.rows + r] = l == 0.0f ? kInf : m - Shift<Tr>::fwd + __builtin_log2f(l);
 }
 
@@ -722,11 +827,6 @@ int launch_attention_fwd_dp(const AttnParams& p) {
 // <= p (|dp| + |delta|) <= 2 |dout| |v|, and held times the power of two that
 // takes that bound to 2^15 the score gradients keep to float16's normal range
 // whatever the scale of the loss. A maximum does not depend on its order.
-template <class Tr>
-__device__ __forceinline__ float load1(const char* row, int d) {
-    if constexpr (Tr::ESIZE == 4) return ((const float*)row)[d];
-    else return unpack<Tr>(((const unsigned short*)row)[d]);
-}
 template <class Tr>
 __device__ __forceinline__ void load_chunk(const char* at, float (&v)[Tr::VE]) {
     const u32x4_t w = *(const u32x4_t*)at;
@@ -954,9 +1054,34 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
     }
 #pragma unroll
     for (int dt = 0; dt < T::DT; ++dt) settle<Tr>(acc[dt]);
-    if (r >= p.rows) return;
+    const long long part_at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows;  // + row
+    clear_if(lse == kInf, acc);
+    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && __builtin_fabsf(lse) < kInf && __builtin_fabsf(delta) < kInf && not_finite(acc));
+    const bool repaired = todo >> (lane & 31) & 1;
+    while (todo) {
+        const int from = __builtin_ctz(todo), rr = __builtin_amdgcn_readlane(r, from);
+        todo &= todo - 1;
+        const int hh = __builtin_amdgcn_readlane(head, from), ii = __builtin_amdgcn_readlane(i, from);
+        const RepairRow row = {__builtin_amdgcn_readlane(pos, from), __builtin_amdgcn_readlane(lim, from), __builtin_amdgcn_readlane(doc, from),
+                               lane_of(slope2, from), -lane_of(lse, from)};
+        const float del = lane_of(delta, from);
+        const char* go = p.dout + (b * p.do_sb + (long long)ii * p.do_sl + hh * p.do_sh) * T::ES;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        each_seen<Tr, FORM>(p, b, kvh, row, p.q + (b * p.q_sb + (long long)ii * p.q_sl + hh * p.q_sh) * T::ES, t0 * BN, t1 * BN,
+                            [&](const char* k, const char* v, float w, float slope) {
+                                add_row<Tr>(k, p.dim, w * (row_dot<Tr>(go, v, p.dim) - del) * slope, o);
+                            });
+        if (p.splits > 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e * 64 + lane < DP) p.part_q[(part_at + rr) * DP + e * 64 + lane] = o[e] * hold;
+        } else {
+            put_row<Tr>(p.dq + (((long long)b * p.queries + ii) * p.heads + hh) * p.dim * T::ES, p.dim, o, p.scale, nullptr);
+        }
+    }
+    if (r >= p.rows || repaired) return;
     if (p.splits > 1) {
-        store_part(p.part_q + (((long long)split * p.batch * p.kv_heads + bh) * p.rows + r) * DP, acc);
+        store_part(p.part_q + (part_at + r) * DP, acc);
         return;
     }
     store_row<Tr, T::DT>(p.dq + (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES, p.dim, acc, p.scale / hold);
@@ -1175,9 +1300,46 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         if (DK) settle<Tr>(acc_k[dt]);
         if (DV) settle<Tr>(acc_v[dt]);
     }
-    if (key >= p.keys) return;
+    const long long n = (long long)p.batch * p.kv_heads * p.keys;
+    bool bad = false;
+    if (DK) bad = not_finite(acc_k);
+    if (DV) bad = bad | not_finite(acc_v);
+    unsigned todo = (unsigned)__ballot(half == 0 && key < p.keys && bad);
+    const bool repaired = todo >> (lane & 31) & 1;
+    while (todo) {
+        const int from = __builtin_ctz(todo), kk = kw + from, kd = __builtin_amdgcn_readlane(doc, from);
+        todo &= todo - 1;
+        const char* k = p.k + (b * p.k_sb + (long long)kk * p.k_sl + kvh * p.k_sh) * T::ES;
+        const char* v = p.v + (b * p.v_sb + (long long)kk * p.v_sl + kvh * p.v_sh) * T::ES;
+        float ok[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ov[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int rr = t0 * BM; rr < min(t1 * BM, p.rows); ++rr) {
+            const int i = rr / p.group, head = kvh * p.group + rr - i * p.group, pos = i + span.off;
+            if (kk >= span.limit(p, pos) || (p.docs && (kd < 0 || doc_at(p, b, pos) != kd))) continue;
+            const char* q = p.q + (b * p.q_sb + (long long)i * p.q_sl + head * p.q_sh) * T::ES;
+            const char* go = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * T::ES;
+            float slope = 1.0f;
+            const float w = __builtin_amdgcn_exp2f(score2<Tr, FORM>(p, row_dot<Tr>(q, k, p.dim), sloped ? p.slopes[head] * 1.44269504f : 0.0f,
+                                                                    (float)(pos - kk), -p.lse[(long long)bh * p.rows + rr], slope));
+            if (DV) add_row<Tr>(go, p.dim, w, ov);
+            if (DK) add_row<Tr>(q, p.dim, w * (row_dot<Tr>(go, v, p.dim) - p.delta[(long long)bh * p.rows + rr]) * slope, ok);
+        }
+        const long long at = (((long long)b * p.keys + kk) * p.kv_heads + kvh) * p.dim * T::ES;
+        if (p.key_splits > 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = e * 64 + lane;
+                if (d >= DP) continue;
+                if (DK) p.part[(split * n + (long long)bh * p.keys + kk) * DP + d] = ok[e] * hold;
+                if (DV) p.part[((p.key_splits + split) * n + (long long)bh * p.keys + kk) * DP + d] = ov[e] * __builtin_amdgcn_exp2f(shift);
+            }
+        } else {
+            if (DK && p.dk) put_row<Tr>(p.dk + at, p.dim, ok, p.scale, nullptr);
+            if (DV && p.dv) put_row<Tr>(p.dv + at, p.dim, ov, 1.0f, nullptr);
+        }
+    }
+    if (key >= p.keys || repaired) return;
     if (p.key_splits > 1) {
-        const long long n = (long long)p.batch * p.kv_heads * p.keys, at = (long long)bh * p.keys + key;
+        const long long at = (long long)bh * p.keys + key;
         if (DK) store_part(p.part + (split * n + at) * DP, acc_k);
         if (DV) store_part(p.part + ((p.key_splits + split) * n + at) * DP, acc_v);
         return;

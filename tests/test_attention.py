@@ -161,6 +161,65 @@ def test_keys_past_the_length_are_not_read(hip, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("form", ["plain", "slopes", "cap"])
+def test_masked_tokens_may_hold_anything(hip, dtype, dim, form):
+    """Padding tokens (no document) whose q, k, v and dout are NaN or infinite: the others' results are those
+    with zeros there, and theirs are zeros."""
+    docs = packed(2, 140, 3, 13)
+    docs[1, 50:55] = -2
+    c = make(2, 140, 140, 4, 2, dim, seed=dim, causal=True, documents=docs)
+    if form == "slopes":
+        c["slopes"] = np.float32([0.5, 0.3, 0.2, 0.0])
+    if form == "cap":
+        c["cap"] = 4.0
+    pad = docs < 0
+    for n in "qkv":
+        c[n][pad] = 0
+    w = rounded(np.random.default_rng(3).standard_normal(c["q"].shape, dtype=np.float32), dtype)
+    w[pad] = 0
+    data = {n: rounded(c[n], dtype) for n in "qkv"}
+    rules = {n: c[n] for n in ("causal", "documents", "slopes", "cap") if n in c}
+    want = ref(data["q"], data["k"], data["v"], w, dtype=dtype, **rules)
+    for n in "qkv":
+        data[n][pad] = np.nan if n != "v" else np.inf
+    w[pad] = np.nan
+    from ormi_amd import Tensor, attention, realize_all
+
+    leaves = {n: Tensor(x, "hip", requires_grad=True, dtype=dtype) for n, x in data.items()}
+    given = {n: Tensor(v, "hip", dtype=str(v.dtype)) if isinstance(v, np.ndarray) else v for n, v in rules.items()}
+    out = attention(leaves["q"], leaves["k"], leaves["v"], **given)
+    (out * Tensor(w, "hip", dtype=dtype)).sum().backward()
+    grads = [leaves[n].grad for n in "qkv"]
+    realize_all(out, *grads)
+    for n, t in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        got = t.numpy()
+        assert not got[pad].any(), n
+        assert_within(got, want[n], f"{n} ({dtype})")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,keys,heads", [(90, 90, 2), (5, 700, 8)])
+def test_later_tokens_reach_no_earlier_row(hip, dtype, rows, keys, heads):
+    """A causal token that is NaN or infinite in v or k: rows before it are those without it (with few rows the
+    keys are split over work-groups), rows from it on are not finite."""
+    c = make(1, rows, keys, heads, 1, 64, seed=30, causal=True)
+    at = keys - 3
+    want = run(c, dtype, grad=False)[0]["out"]
+    for n, bad in (("v", np.inf), ("v", np.nan), ("k", np.nan)):
+        hurt = {**c, n: c[n].copy()}
+        hurt[n][0, at] = bad
+        got = run(hurt, dtype, grad=False)[0]["out"]
+        data = {n: rounded(c[n], dtype) for n in "qkv"}
+        exact, bound = ref(data["q"], data["k"], data["v"], dtype=dtype, causal=True)["out"]
+        assert_within(got[:, :-3], (exact[:, :-3], bound[:, :-3]), n)
+        assert not np.isfinite(got[:, -3:]).any()
+    assert np.isfinite(want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size,scale", [(30.0, 1.0), (1.0, -0.4), (1.0, 0.0), (0.01, None)])
 def test_scores_large_reversed_and_flat(hip, dtype, size, scale):
     check(make(1, 100, 140, 2, 1, 64, seed=8, size=size, causal=True, scale=scale), dtype)
