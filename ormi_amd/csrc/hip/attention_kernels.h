@@ -500,22 +500,68 @@ __device__ __forceinline__ void clear_if(bool yes, f32x16_t (&acc)[DT]) {
 }
 __device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 
-// What a row needs to find its weights again.
-struct RepairRow {
-    int pos, lim, doc;
-    float slope2, base;
-};
-// f(j, key's weight's exponent base included) for the keys in [j0, j1) that the row sees.
-template <class Tr, int FORM, class F>
-__device__ __forceinline__ void each_seen(const AttnParams& p, int b, int kvh, const RepairRow& row, const char* q, int j0, int j1, F&& f) {
-    for (int j = j0; j < min(j1, row.lim); ++j) {
-        if (p.docs && doc_at(p, b, j) != row.doc) continue;
-        const char* k = p.k + (b * p.k_sb + (long long)j * p.k_sl + kvh * p.k_sh) * Tr::ESIZE;
-        const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + kvh * p.v_sh) * Tr::ESIZE;
-        float slope = 1.0f;
-        const float t = score2<Tr, FORM>(p, row_dot<Tr>(q, k, p.dim), row.slope2, (float)(row.pos - j), row.base, slope);
-        f(k, v, __builtin_amdgcn_exp2f(t), slope);
+// The launch's arguments read once more, and what follows from them: a repair takes
+// nothing but its row or key from the loop before it, which would have to keep it in
+// registers (it did: dk and dv of 4096 x 16 heads of 128 took 407 us instead of 370).
+__device__ __forceinline__ const AttnParams& arguments_again() {
+    auto at = (const __attribute__((address_space(4))) AttnParams*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const AttnParams*)at;
+}
+struct Repair {
+    const AttnParams& p;
+    const Work work;
+    const int b, kvh;
+    const Span span;
+    __device__ __forceinline__ Repair(const AttnParams& p, int splits)
+        : p(p), work(p, splits), b(work.bh / p.kv_heads), kvh(work.bh % p.kv_heads), span(p, b) {}
+    __device__ __forceinline__ long long row_at(int rr) const { return (long long)work.bh * p.rows + rr; }
+    __device__ __forceinline__ long long part_at(int rr) const {
+        return ((long long)work.split * p.batch * p.kv_heads + work.bh) * p.rows + rr;
     }
+};
+// A row of a repair, and where its values begin.
+template <class Tr, int FORM>
+struct RepairRow {
+    int i, head, pos;
+    float slope2;
+    __device__ __forceinline__ RepairRow(const Repair& w, int rr) {
+        i = rr / w.p.group, head = w.kvh * w.p.group + rr - i * w.p.group, pos = i + w.span.off;
+        slope2 = FORM != kPlain && w.p.slopes ? w.p.slopes[head] * 1.44269504f : 0.0f;
+    }
+    __device__ __forceinline__ bool sees(const Repair& w, int j) const {
+        if (j >= w.span.limit(w.p, pos)) return false;
+        const int doc = w.p.docs ? doc_at(w.p, w.b, pos) : 0;
+        return doc >= 0 && (!w.p.docs || doc_at(w.p, w.b, j) == doc);
+    }
+    __device__ __forceinline__ const char* q(const Repair& w) const {
+        return w.p.q + (w.b * w.p.q_sb + (long long)i * w.p.q_sl + head * w.p.q_sh) * Tr::ESIZE;
+    }
+    __device__ __forceinline__ const char* dout(const Repair& w) const {
+        return w.p.dout + (w.b * w.p.do_sb + (long long)i * w.p.do_sl + head * w.p.do_sh) * Tr::ESIZE;
+    }
+    // Where the row begins in out, in its rest and in dq.
+    __device__ __forceinline__ long long at(const Repair& w) const {
+        return (((long long)w.b * w.p.queries + i) * w.p.heads + head) * w.p.dim * Tr::ESIZE;
+    }
+    __device__ __forceinline__ float weight(const Repair& w, const char* k, int j, float base, float& slope) const {
+        return __builtin_amdgcn_exp2f(score2<Tr, FORM>(w.p, row_dot<Tr>(q(w), k, w.p.dim), slope2, (float)(pos - j), base, slope));
+    }
+};
+template <class Tr>
+__device__ __forceinline__ const char* key_row(const Repair& w, int j) {
+    return w.p.k + (w.b * w.p.k_sb + (long long)j * w.p.k_sl + w.kvh * w.p.k_sh) * Tr::ESIZE;
+}
+template <class Tr>
+__device__ __forceinline__ const char* value_row(const Repair& w, int j) {
+    return w.p.v + (w.b * w.p.v_sb + (long long)j * w.p.v_sl + w.kvh * w.p.v_sh) * Tr::ESIZE;
+}
+// A row of a split's partial sums.
+template <int DP>
+__device__ __forceinline__ void put_part(float* row, const float (&sum)[4], float f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (const int d = e * 64 + (int)(threadIdx.x & 63); d < DP) row[d] = sum[e] * f;
 }
 
 // ---------------------------------------------------------------- forward --
@@ -715,31 +761,24 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
     } else {
         l = halves_sum(l);
     }
-    const long long part_at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows;  // + row
     clear_if(l == 0.0f, acc);
     unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && l < kInf && not_finite(acc));
     const bool repaired = todo >> (lane & 31) & 1;
-    while (todo) {
-        const int from = __builtin_ctz(todo), rr = __builtin_amdgcn_readlane(r, from);
-        todo &= todo - 1;
-        const int hh = __builtin_amdgcn_readlane(head, from), ii = __builtin_amdgcn_readlane(i, from);
-        const RepairRow row = {__builtin_amdgcn_readlane(pos, from), __builtin_amdgcn_readlane(lim, from), __builtin_amdgcn_readlane(doc, from),
-                               lane_of(slope2, from), lane_of(base, from)};
-        const long long at = ((long long)b * p.queries + ii) * p.heads + hh;
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        each_seen<Tr, FORM>(p, b, kvh, row, p.q + (b * p.q_sb + (long long)ii * p.q_sl + hh * p.q_sh) * T::ES, t0 * BN, t1 * BN,
-                            [&](const char*, const char* v, float w, float) { add_row<Tr>(v, p.dim, w, o); });
-        if (p.splits > 1) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e * 64 + lane < DP) p.part[(part_at + rr) * DP + e * 64 + lane] = o[e];
-        } else {
-            put_row<Tr>(p.out + at * p.dim * T::ES, p.dim, o, 1.0f / lane_of(l, from), p.rest ? p.rest + at * p.dim * T::ES : nullptr);
+    if (__builtin_expect(todo != 0, 0)) {
+        const Repair w(arguments_again(), arguments_again().splits);
+        for (; todo; todo &= todo - 1) {
+            const int from = __builtin_ctz(todo), rr = __builtin_amdgcn_readlane(r, from);
+            const RepairRow<Tr, FORM> row(w, rr);
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, slope = 1.0f;
+            for (int j = t0 * BN; j < t1 * BN; ++j)
+                if (row.sees(w, j)) add_row<Tr>(value_row<Tr>(w, j), w.p.dim, row.weight(w, key_row<Tr>(w, j), j, lane_of(base, from), slope), o);
+            if (w.p.splits > 1) put_part<DP>(w.p.part + w.part_at(rr) * DP, o, 1.0f);
+            else put_row<Tr>(w.p.out + row.at(w), w.p.dim, o, 1.0f / lane_of(l, from), w.p.rest ? w.p.rest + row.at(w) : nullptr);
         }
     }
     if (r >= p.rows) return;
     if (p.splits > 1) {
-        const long long at = part_at + r;
+        const long long at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows + r;
         if (!(l == 0.0f) && !repaired) store_part(p.part + at * DP, acc);
         if (half == 0) p.part_ml[at] = make_float2(m == -kInf ? -kInf : m - Shift<Tr>::fwd, l);
         return;
@@ -1054,37 +1093,44 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
     }
 #pragma unroll
     for (int dt = 0; dt < T::DT; ++dt) settle<Tr>(acc[dt]);
-    const long long part_at = ((long long)split * p.batch * p.kv_heads + bh) * p.rows;  // + row
     clear_if(lse == kInf, acc);
-    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && __builtin_fabsf(lse) < kInf && __builtin_fabsf(delta) < kInf && not_finite(acc));
+    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && __builtin_fabsf(lse) < kInf && __builtin_fabsf(delta) < kInf &&
+                                       not_finite(acc));
     const bool repaired = todo >> (lane & 31) & 1;
-    while (todo) {
-        const int from = __builtin_ctz(todo), rr = __builtin_amdgcn_readlane(r, from);
-        todo &= todo - 1;
-        const int hh = __builtin_amdgcn_readlane(head, from), ii = __builtin_amdgcn_readlane(i, from);
-        const RepairRow row = {__builtin_amdgcn_readlane(pos, from), __builtin_amdgcn_readlane(lim, from), __builtin_amdgcn_readlane(doc, from),
-                               lane_of(slope2, from), -lane_of(lse, from)};
-        const float del = lane_of(delta, from);
-        const char* go = p.dout + (b * p.do_sb + (long long)ii * p.do_sl + hh * p.do_sh) * T::ES;
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        each_seen<Tr, FORM>(p, b, kvh, row, p.q + (b * p.q_sb + (long long)ii * p.q_sl + hh * p.q_sh) * T::ES, t0 * BN, t1 * BN,
-                            [&](const char* k, const char* v, float w, float slope) {
-                                add_row<Tr>(k, p.dim, w * (row_dot<Tr>(go, v, p.dim) - del) * slope, o);
-                            });
-        if (p.splits > 1) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e * 64 + lane < DP) p.part_q[(part_at + rr) * DP + e * 64 + lane] = o[e] * hold;
-        } else {
-            put_row<Tr>(p.dq + (((long long)b * p.queries + ii) * p.heads + hh) * p.dim * T::ES, p.dim, o, p.scale, nullptr);
+    if (__builtin_expect(todo != 0, 0)) {
+        const Repair w(arguments_again(), arguments_again().splits);
+        for (; todo; todo &= todo - 1) {
+            const int rr = __builtin_amdgcn_readlane(r, __builtin_ctz(todo));
+            const RepairRow<Tr, FORM> row(w, rr);
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, slope = 1.0f;
+            for (int j = t0 * BN; j < t1 * BN; ++j) {
+                if (!row.sees(w, j)) continue;
+                const float e = row.weight(w, key_row<Tr>(w, j), j, -w.p.lse[w.row_at(rr)], slope);
+                const float ds = e * (row_dot<Tr>(row.dout(w), value_row<Tr>(w, j), w.p.dim) - w.p.delta[w.row_at(rr)]) * slope;
+                add_row<Tr>(key_row<Tr>(w, j), w.p.dim, ds, o);
+            }
+            if (w.p.splits > 1) put_part<DP>(w.p.part_q + w.part_at(rr) * DP, o, grad_hold<Tr>(w.p));
+            else put_row<Tr>(w.p.dq + row.at(w), w.p.dim, o, w.p.scale, nullptr);
         }
     }
     if (r >= p.rows || repaired) return;
     if (p.splits > 1) {
-        store_part(p.part_q + (part_at + r) * DP, acc);
+        store_part(p.part_q + (((long long)split * p.batch * p.kv_heads + bh) * p.rows + r) * DP, acc);
         return;
     }
     store_row<Tr, T::DT>(p.dq + (((long long)b * p.queries + i) * p.heads + head) * p.dim * T::ES, p.dim, acc, p.scale / hold);
+}
+
+// The tiles of BM rows that a split goes over for the keys from k0 on: of those that
+// can see them, its share.
+template <int BM>
+__device__ __forceinline__ int2 row_tiles(const AttnParams& p, const Span& span, int k0, int split) {
+    const int tiles = (p.rows + BM - 1) / BM;
+    int lo = 0, hi = tiles;
+    if (k0 >= span.end) hi = 0;
+    else if (p.causal && span.prefix <= k0) lo = min(tiles, (int)((long long)max(0, k0 - span.off) * p.group / BM));
+    const int per = (max(hi - lo, 0) + p.key_splits - 1) / p.key_splits, t0 = min(lo + split * per, hi);
+    return make_int2(t0, min(t0 + per, hi));
 }
 
 // Values in LDS instead of registers: where 32 keys' k, v and both gradients
@@ -1132,12 +1178,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     if constexpr (DK && !VL) T::row_frags(p.v + (b * p.v_sb + (long long)keyc * p.v_sl + kvh * p.v_sh) * T::ES, p.chunks, vf);
 
     // Tiles of rows that can see the group's keys.
-    const int tiles = (p.rows + BM - 1) / BM;
-    int lo = 0, hi = tiles;
-    if (k0 >= span.end) hi = 0;
-    else if (p.causal && span.prefix <= k0) lo = min(tiles, (int)((long long)max(0, k0 - span.off) * p.group / BM));
-    const int per = (max(hi - lo, 0) + p.key_splits - 1) / p.key_splits;
-    const int t0 = min(lo + split * per, hi), t1 = min(t0 + per, hi);
+    const int2 part = row_tiles<BM>(p, span, k0, split);
+    const int t0 = part.x, t1 = part.y;
 
     // With documents, tiles whose positions share none with the group's keys are passed over.
     const int2* ranges = p.docs ? p.ranges + (long long)b * p.range_tiles : nullptr;
@@ -1300,46 +1342,43 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         if (DK) settle<Tr>(acc_k[dt]);
         if (DV) settle<Tr>(acc_v[dt]);
     }
-    const long long n = (long long)p.batch * p.kv_heads * p.keys;
     bool bad = false;
     if (DK) bad = not_finite(acc_k);
     if (DV) bad = bad | not_finite(acc_v);
     unsigned todo = (unsigned)__ballot(half == 0 && key < p.keys && bad);
     const bool repaired = todo >> (lane & 31) & 1;
-    while (todo) {
-        const int from = __builtin_ctz(todo), kk = kw + from, kd = __builtin_amdgcn_readlane(doc, from);
-        todo &= todo - 1;
-        const char* k = p.k + (b * p.k_sb + (long long)kk * p.k_sl + kvh * p.k_sh) * T::ES;
-        const char* v = p.v + (b * p.v_sb + (long long)kk * p.v_sl + kvh * p.v_sh) * T::ES;
-        float ok[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ov[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int rr = t0 * BM; rr < min(t1 * BM, p.rows); ++rr) {
-            const int i = rr / p.group, head = kvh * p.group + rr - i * p.group, pos = i + span.off;
-            if (kk >= span.limit(p, pos) || (p.docs && (kd < 0 || doc_at(p, b, pos) != kd))) continue;
-            const char* q = p.q + (b * p.q_sb + (long long)i * p.q_sl + head * p.q_sh) * T::ES;
-            const char* go = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * T::ES;
-            float slope = 1.0f;
-            const float w = __builtin_amdgcn_exp2f(score2<Tr, FORM>(p, row_dot<Tr>(q, k, p.dim), sloped ? p.slopes[head] * 1.44269504f : 0.0f,
-                                                                    (float)(pos - kk), -p.lse[(long long)bh * p.rows + rr], slope));
-            if (DV) add_row<Tr>(go, p.dim, w, ov);
-            if (DK) add_row<Tr>(q, p.dim, w * (row_dot<Tr>(go, v, p.dim) - p.delta[(long long)bh * p.rows + rr]) * slope, ok);
-        }
-        const long long at = (((long long)b * p.keys + kk) * p.kv_heads + kvh) * p.dim * T::ES;
-        if (p.key_splits > 1) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = e * 64 + lane;
-                if (d >= DP) continue;
-                if (DK) p.part[(split * n + (long long)bh * p.keys + kk) * DP + d] = ok[e] * hold;
-                if (DV) p.part[((p.key_splits + split) * n + (long long)bh * p.keys + kk) * DP + d] = ov[e] * __builtin_amdgcn_exp2f(shift);
+    if (__builtin_expect(todo != 0, 0)) {
+        for (; todo; todo &= todo - 1) {
+            const AttnParams& a = arguments_again();
+            const Work at(a, a.key_splits);
+            const int at_k0 = at.block * NW * 32, j = at_k0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32 + __builtin_ctz(todo);
+            const int2 tiles = row_tiles<BM>(a, Span(a, at.bh / a.kv_heads), at_k0, at.split);
+            float ok[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ov[4] = {0.0f, 0.0f, 0.0f, 0.0f}, slope = 1.0f;
+            for (int rr = tiles.x * BM; rr < min(tiles.y * BM, arguments_again().rows); ++rr) {
+                const Repair w(arguments_again(), arguments_again().key_splits);
+                const RepairRow<Tr, FORM> row(w, rr);
+                if (!row.sees(w, j)) continue;
+                const float e = row.weight(w, key_row<Tr>(w, j), j, -w.p.lse[w.row_at(rr)], slope);
+                if (DV) add_row<Tr>(row.dout(w), w.p.dim, e, ov);
+                if (DK)
+                    add_row<Tr>(row.q(w), w.p.dim,
+                                e * (row_dot<Tr>(row.dout(w), value_row<Tr>(w, j), w.p.dim) - w.p.delta[w.row_at(rr)]) * slope, ok);
             }
-        } else {
-            if (DK && p.dk) put_row<Tr>(p.dk + at, p.dim, ok, p.scale, nullptr);
-            if (DV && p.dv) put_row<Tr>(p.dv + at, p.dim, ov, 1.0f, nullptr);
+            const Repair w(arguments_again(), arguments_again().key_splits);
+            const long long n = (long long)w.p.batch * w.p.kv_heads * w.p.keys, row = (long long)w.work.bh * w.p.keys + j;
+            const long long to = (((long long)w.b * w.p.keys + j) * w.p.kv_heads + w.kvh) * w.p.dim * T::ES;
+            if (w.p.key_splits > 1) {
+                if (DK) put_part<DP>(w.p.part + (w.work.split * n + row) * DP, ok, grad_hold<Tr>(w.p));
+                if (DV) put_part<DP>(w.p.part + ((w.p.key_splits + w.work.split) * n + row) * DP, ov, __builtin_amdgcn_exp2f(Shift<Tr>::bwd));
+            } else {
+                if (DK && w.p.dk) put_row<Tr>(w.p.dk + to, w.p.dim, ok, w.p.scale, nullptr);
+                if (DV && w.p.dv) put_row<Tr>(w.p.dv + to, w.p.dim, ov, 1.0f, nullptr);
+            }
         }
     }
     if (key >= p.keys || repaired) return;
     if (p.key_splits > 1) {
-        const long long at = (long long)bh * p.keys + key;
+        const long long n = (long long)p.batch * p.kv_heads * p.keys, at = (long long)bh * p.keys + key;
         if (DK) store_part(p.part + (split * n + at) * DP, acc_k);
         if (DV) store_part(p.part + ((p.key_splits + split) * n + at) * DP, acc_v);
         return;
