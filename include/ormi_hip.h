@@ -429,8 +429,10 @@ int ormi_hip_rotary(const ormi_rotary_desc* desc);
  *     and j <= pos or j < prefix[b]                when causal (prefix may be NULL)
  *     and documents[pos] == documents[j] >= 0      when documents is not NULL
  *   out = sum_j p_ij v_j, p the softmax of t over the keys i sees.
- * A query that sees no key gives zeros, and so do its gradients. Keys at or
- * past the length are never read, and neither k nor v need hold numbers there.
+ * A query that sees no key gives zeros, and so do its gradients. Neither k nor
+ * v need hold numbers where no query sees them: an infinity or a NaN there
+ * reaches no result. Nor does one at a key that some queries see reach the
+ * others' rows, nor one in a query's row the gradients of keys it does not see.
  * q, k, v are strided views; out is contiguous. dtype is F32, BF16 or F16;
  * scores, sums and the softmax are fp32, out is rounded once. 16-bit
  * probabilities are rounded to 16 bits for their product with v.

@@ -108,7 +108,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, scale: f
       prefix     int32 (batch,): and, causal, every key before the prefix's end
       documents  int32 (batch, keys): tokens see their own document's; a
                  negative one sees nothing and is seen by nothing
-      lengths    int32 (batch,): keys that exist (keys); the others are not read
+      lengths    int32 (batch,): keys that exist (keys); the others do not count, whatever they hold
     A query that sees no key gives zeros. The result and the gradients have q's
     type (float32, bfloat16 or float16); gradients of shared key heads add up.
     """
