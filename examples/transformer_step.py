@@ -51,7 +51,7 @@ class AttentionBlock:
     def attend(self, q: Tensor, k: Tensor, v: Tensor, lengths: Tensor | None = None) -> Tensor:
         batch, length = q.shape[:2]
         y = attention(q, k, v, causal=True, lengths=lengths).astype("float32")
-        return (y.reshape((batch * length, self.heads * self.features)) @ self.wo).reshape((batch, length, -1))
+        return (y.reshape((batch * length, self.heads * self.features)) @ self.wo).reshape((batch, length, self.heads * self.features))
 
     def __call__(self, x: Tensor) -> Tensor:
         return self.attend(self.queries(x), *self.keys_values(x))
@@ -78,7 +78,7 @@ def token_by_token(block: AttentionBlock, x: np.ndarray) -> np.ndarray:
     k.realize(), v.realize()
     rows = []
     for at in range(length):
-        lengths = Tensor(np.full(batch, at + 1, np.int32), "hip")  # what stands after the token does not count
+        lengths = Tensor(np.full(batch, at + 1, np.int32), "hip", dtype="int32")  # what stands after the token does not count
         rows.append(block.attend(block.queries(Tensor(x[:, at:at + 1].copy(), "hip"), offset=at), k, v, lengths).numpy())
     return np.concatenate(rows, axis=1)
 
