@@ -201,6 +201,17 @@ struct Tile {
                     acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(turned1(t, row0, r, dt), a[r], acc[dt], 0, 0, 0);
         }
     }
+    // What second() rounded off its 16-bit operand.
+    __device__ __forceinline__ static void leave_rest(f32x16_t& a) {
+        if constexpr (ES == 2) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const unsigned w = pack2(Tr{}, a[e], a[e + 1]);
+                a[e] -= unpack<Tr>(w);
+                a[e + 1] -= unpack<Tr>(w >> 16);
+            }
+        }
+    }
     // A row's fragments from memory: lane l holds row `row`'s chunks 2 f + l / 32 (zero past the row's end).
     __device__ __forceinline__ static void row_frags(const char* row, int chunks, u32x4_t (&out)[NF]) {
         const int half = (threadIdx.x & 63) >> 5;
@@ -565,9 +576,11 @@ __device__ __forceinline__ void put_part(float* row, const float (&sum)[4], floa
 }
 
 // ---------------------------------------------------------------- forward --
-// NW waves of 32 rows; BN keys per tile.
+// NW waves of 32 rows; BN keys per tile. Up to 96 features three groups of waves share
+// a CU, whatever that spills outside the loop (4096 x 16 heads: 94 us, with two 99; the
+// compiler alone takes two).
 template <class Tr, int DP, int NW, int BN, int FORM>
-__global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
+__global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW == 4 && DP * Tr::ESIZE <= 192 ? 3 : 2) void attention_fwd_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
     constexpr int MT = BN / 32, TILEB = T::bytes(BN);
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];
@@ -661,6 +674,14 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
         for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
 
     int t = p.docs ? walk.next(t0, t1) : near, stage = 0;
+    // The weights are rounded to 16 bits for their product with the values. In the tile
+    // that a row begins with, what that leaves is multiplied too: it holds all keys of a
+    // row that sees few, where single weights count (and the gradient's delta, a sum over
+    // the row, would carry their rounding into every score's: dq 1.5 times as far off as
+    // rounding the result alone, now 1.05), and with slopes the heaviest. With many keys
+    // the roundings average out, and the matrix pipes bound the kernel. Rows by the
+    // wave (NW 1) wait for memory: there it is every tile, in the same time.
+    const int whole = t;
     bool same = !p.docs || (t < t1 && walk.same(t));
     if (t < t1) issue(t, 0);
     while (t < t1) {
@@ -746,6 +767,13 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : 2) 
                 if constexpr (!SUM) l += part[0] + part[1];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) T::template second<SUM>(vt, mt * 32, s[mt], acc, &sum);
+                if (T::ES == 2 && (NW == 1 || t == whole)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        T::leave_rest(s[mt]);
+                        T::template second<SUM>(vt, mt * 32, s[mt], acc, &sum);
+                    }
+                }
             }
         }
         t = tn;
@@ -1032,6 +1060,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
 
     int t = next(t0), stage = 0;
+    // As in the forward pass, one tile's score gradients go in with what rounding left of them.
+    const int whole = FORM != kPlain && p.slopes && !p.docs ? min(max((rb * NW * 32 / p.group + span.off) / BN, t0), max(t1 - 1, t0)) : t;
     bool same = !p.docs || (t < t1 && walk.same(t));
     if (t < t1) issue(t, 0);
     while (t < t1) {
@@ -1085,6 +1115,10 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
                     }
                 }
                 T::second(kt, mt * 32, s, acc);
+                if (T::ES == 2 && t == whole) {
+                    T::leave_rest(s);
+                    T::second(kt, mt * 32, s, acc);
+                }
             }
         }
         t = tn;
@@ -1254,6 +1288,9 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         for (int e = 0; e < 16; ++e) acc_k[dt][e] = acc_v[dt][e] = 0.0f;
 
     int t = next(t0), stage = 0;
+    // One tile's weights and score gradients go in with what rounding left of them: the
+    // only tile of keys that few rows see.
+    const int whole = sloped && !p.docs ? min(max((int)((long long)max(0, k0 - span.off) * p.group / BM), t0), max(t1 - 1, t0)) : t;
     if (t < t1) {
         issue(t, 0);
         if constexpr (VL) {
@@ -1333,6 +1370,16 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             }
             if (DV) T::second(gt, 0, s, acc_v);
             if (DK) T::second(qt, 0, g, acc_k);
+            if (T::ES == 2 && t == whole) {
+                if (DV) {
+                    T::leave_rest(s);
+                    T::second(gt, 0, s, acc_v);
+                }
+                if (DK) {
+                    T::leave_rest(g);
+                    T::second(qt, 0, g, acc_k);
+                }
+            }
         }
         t = tn;
         stage ^= 1;

@@ -134,6 +134,24 @@ def test_rows_that_see_nothing(hip, dtype, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("form", [{}, {"cap": 3.0}, {"slopes": np.float32([0.5, 0.25])}])
+@pytest.mark.parametrize("dim", [24, 64, 96, 128, 256])
+def test_few_keys_leave_one_rounding(hip, dtype, form, dim):
+    """Rows that see few keys keep what rounding leaves of their weights and score gradients: every value is one
+    rounding to its type (h of it; half a step below its normal range) beside float32's sums and second-order terms,
+    h of what all roundings to the type would allow, twice for weight and score gradient."""
+    case = make(2, 16, 20, 2, 1, dim, seed=31, causal=True, **form)
+    got, data, host, options, w = run(case, dtype)
+    coarse = ref(data["q"], data["k"], data["v"], w, dtype=dtype, **options, **host)
+    fine = ref(data["q"], data["k"], data["v"], w, dtype="float32", **options, **host)
+    h = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}[dtype]
+    least = {"bfloat16": 2.0 ** -134, "float16": 2.0 ** -25}[dtype]
+    for n, (exact, bound) in fine.items():
+        assert_within(got[n], (exact, bound + h * np.abs(exact) + 2 * h * coarse[n][1] + least), f"{n} ({dtype})")
+
+
+@pytest.mark.gpu
 def test_no_keys_and_no_queries(hip):
     from ormi_amd import Tensor, attention
 
