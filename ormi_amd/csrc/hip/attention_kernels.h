@@ -576,8 +576,14 @@ __device__ __forceinline__ void put_part(float* row, const float (&sum)[4], floa
 }
 
 // ---------------------------------------------------------------- forward --
-// NW waves of 32 rows; BN keys per tile. Up to 96 features three groups of waves share
-// a CU, whatever that spills outside the loop (4096 x 16 heads: 94 us, with two 99; the
+// NW waves of 32 rows; BN keys per tile. Many rows: four waves share the tiles in LDS,
+// bound by the matrix pipes with the exponentials beside them (causal, bf16, 2 x 4096
+// tokens x 16 heads of 128 on 4 key heads: 187 us, 735 TF; 12 heads of 64 over 8191
+// keys with slopes: 266 us, 770 TF, the exponentials nearly as long as the products).
+// Up to 32 rows: one wave, keys split over the chip, bound by reading them (16 single
+// tokens over up to 8192 keys x 8 heads of 128: 62 us, 5.4 TB/s of those that exist).
+// Up to 96 features three groups of waves share
+// a CU, whatever that spills (8191 x 12 heads of 64 with slopes: 266 us, with two 372; the
 // compiler alone takes two).
 template <class Tr, int DP, int NW, int BN, int FORM>
 __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW == 4 && DP * Tr::ESIZE <= 192 ? 3 : 2) void attention_fwd_kernel(AttnParams p) {
@@ -820,7 +826,8 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW 
 // Joins the splits of a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
 // in split order. One wave per row: lane s holds split s's maximum and sum (at
 // most 64 splits), then the lanes go along the features; a split that saw no key
-// has stored no values.
+// has stored no values. Bound by the wait for three loads in turn (5.9-7 us for one
+// to 512 rows).
 template <class Tr, int DP>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
     const long long total = (long long)p.batch * p.kv_heads * p.rows;
@@ -987,7 +994,8 @@ __device__ __forceinline__ float grad_hold(const AttnParams& p) {
 
 // dq. Rows, tiles and masks as in the forward kernel, with both products of a
 // tile's keys and values against the row's q and dout; the score gradients then
-// meet the keys again, turned.
+// meet the keys again, turned. Bound by the matrix pipes (2 x 4096 tokens x 16 heads
+// of 128, causal: 232 us, 890 TF; the same without a mask, longer: 1050 TF).
 template <class Tr, int DP, int BN, int FORM>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
@@ -1178,6 +1186,10 @@ constexpr bool values_in_lds(int dp, int es) { return dp * es >= 256 && dp * es 
 // comes from LDS, four rows at a time. DV, DK: which gradients this launch makes
 // (rows of 256 features leave the registers for one at a time; both at once
 // spilled 208 of them and took 1911 us where two launches take 807, 4096 x 16 heads).
+// Bound by the matrix pipes and, with both operands of three products in LDS, by its
+// reads: 2 x 4096 tokens x 16 heads of 128, causal, 375 us, 735 TF (no mask, longer:
+// 860 TF). 8192 tokens in 24 documents with capped scores, 8 heads: 190 us; its 512
+// work-groups all run at once and end when those of the longest documents do.
 template <class Tr, int DP, int FORM, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
@@ -1436,7 +1448,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 }
 
 // Adds the splits' partial gradients in split order, one wave per row: first dq's
-// rows, then each key's dk and dv.
+// rows, then each key's dk and dv. Bound by memory and its waits (84 MB in 26 us).
 template <class Tr, int DP>
 __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttnParams p) {
     const long long nq = p.dq && p.splits > 1 ? (long long)p.batch * p.kv_heads * p.rows : 0;
