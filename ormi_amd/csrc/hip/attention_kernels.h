@@ -567,6 +567,33 @@ template <class Tr>
 __device__ __forceinline__ const char* value_row(const Repair& w, int j) {
     return w.p.v + (w.b * w.p.v_sb + (long long)j * w.p.v_sl + w.kvh * w.p.v_sh) * Tr::ESIZE;
 }
+// Whether a row holds a value that is not finite.
+template <class Tr>
+__device__ __forceinline__ bool row_bad(const char* row, int dim) {
+    bool bad = false;
+    for (int d = threadIdx.x & 63; d < dim; d += 64) bad = bad | !(__builtin_fabsf(load1<Tr>(row, d)) < kInf);
+    return __any(bad);
+}
+// Whether one of the keys in [j0, j1) that a row of the wave (rows from r0 on) does not
+// see is such; with documents any of them. In the keys [w0, w1) also one that is seen:
+// what rounding left of a weight has either sign, and an infinity times that is not the
+// infinity it has to be. Without any the sums are right as they are: an infinity that
+// all rows see elsewhere costs this look, not a repair.
+template <class Tr, class F>
+__device__ __forceinline__ bool repair_needed(const Repair& w, int r0, int j0, int j1, int w0, int w1, F&& row_of) {
+    const int lim = min(w.p.docs ? 0 : w.span.limit(w.p, r0 / w.p.group + w.span.off), max(w.span.end - 1, 0));
+    for (int j = j0; j < min(j1, w.span.end); ++j)  // keys past the end read the last one
+        if ((j >= lim || (Tr::ESIZE == 2 && j >= w0 && j < w1)) && row_bad<Tr>(row_of(j), w.p.dim)) return true;
+    return false;
+}
+// Nothing brings a sum back from NaN.
+__device__ __forceinline__ bool all_nan(const float (&sum)[4], int dim) {
+    bool yes = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e * 64 + (int)(threadIdx.x & 63) < dim) yes = yes & (sum[e] != sum[e]);
+    return __all(yes);
+}
 // A row of a split's partial sums.
 template <int DP>
 __device__ __forceinline__ void put_part(float* row, const float (&sum)[4], float f) {
@@ -796,7 +823,14 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW 
         l = halves_sum(l);
     }
     clear_if(l == 0.0f, acc);
-    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && l < kInf && not_finite(acc));
+    const bool bad = not_finite(acc);  // by all lanes: it adds up the wave's halves
+    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && l < kInf && bad);
+    if (__builtin_expect(todo != 0, 0)) {
+        const Repair w(arguments_again(), arguments_again().splits);
+        if (!repair_needed<Tr>(w, __builtin_amdgcn_readfirstlane(r), t0 * BN, t1 * BN, NW == 1 ? 0 : whole * BN, NW == 1 ? t1 * BN : whole * BN + BN,
+                               [&](int j) { return value_row<Tr>(w, j); }))
+            todo = 0;
+    }
     const bool repaired = todo >> (lane & 31) & 1;
     if (__builtin_expect(todo != 0, 0)) {
         const Repair w(arguments_again(), arguments_again().splits);
@@ -804,7 +838,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW 
             const int from = __builtin_ctz(todo), rr = __builtin_amdgcn_readlane(r, from);
             const RepairRow<Tr, FORM> row(w, rr);
             float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, slope = 1.0f;
-            for (int j = t0 * BN; j < t1 * BN; ++j)
+            for (int j = t0 * BN; j < t1 * BN && !all_nan(o, w.p.dim); ++j)
                 if (row.sees(w, j)) add_row<Tr>(value_row<Tr>(w, j), w.p.dim, row.weight(w, key_row<Tr>(w, j), j, lane_of(base, from), slope), o);
             if (w.p.splits > 1) put_part<DP>(w.p.part + w.part_at(rr) * DP, o, 1.0f);
             else put_row<Tr>(w.p.out + row.at(w), w.p.dim, o, 1.0f / lane_of(l, from), w.p.rest ? w.p.rest + row.at(w) : nullptr);
@@ -1136,8 +1170,14 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
 #pragma unroll
     for (int dt = 0; dt < T::DT; ++dt) settle<Tr>(acc[dt]);
     clear_if(lse == kInf, acc);
-    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && __builtin_fabsf(lse) < kInf && __builtin_fabsf(delta) < kInf &&
-                                       not_finite(acc));
+    const bool bad = not_finite(acc);
+    unsigned todo = (unsigned)__ballot(half == 0 && r < p.rows && __builtin_fabsf(lse) < kInf && __builtin_fabsf(delta) < kInf && bad);
+    if (__builtin_expect(todo != 0, 0)) {
+        const Repair w(arguments_again(), arguments_again().splits);
+        if (!repair_needed<Tr>(w, __builtin_amdgcn_readfirstlane(r), t0 * BN, t1 * BN, whole * BN, whole * BN + BN,
+                               [&](int j) { return key_row<Tr>(w, j); }))
+            todo = 0;
+    }
     const bool repaired = todo >> (lane & 31) & 1;
     if (__builtin_expect(todo != 0, 0)) {
         const Repair w(arguments_again(), arguments_again().splits);
@@ -1145,7 +1185,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
             const int rr = __builtin_amdgcn_readlane(r, __builtin_ctz(todo));
             const RepairRow<Tr, FORM> row(w, rr);
             float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, slope = 1.0f;
-            for (int j = t0 * BN; j < t1 * BN; ++j) {
+            for (int j = t0 * BN; j < t1 * BN && !all_nan(o, w.p.dim); ++j) {
                 if (!row.sees(w, j)) continue;
                 const float e = row.weight(w, key_row<Tr>(w, j), j, -w.p.lse[w.row_at(rr)], slope);
                 const float ds = e * (row_dot<Tr>(row.dout(w), value_row<Tr>(w, j), w.p.dim) - w.p.delta[w.row_at(rr)]) * slope;
@@ -1405,6 +1445,18 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     if (DK) bad = not_finite(acc_k);
     if (DV) bad = bad | not_finite(acc_v);
     unsigned todo = (unsigned)__ballot(half == 0 && key < p.keys && bad);
+    if (__builtin_expect(todo != 0, 0)) {  // is a row not finite that does not see all of the wave's keys, or is in the tile `whole`?
+        const Repair w(arguments_again(), arguments_again().key_splits);
+        const int first = w.work.block * NW * 32, past = first + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32 + 32;
+        const int2 tiles = row_tiles<BM>(w.p, w.span, first, w.work.split);
+        bool hidden = false;
+        for (int rr = tiles.x * BM; rr < min(tiles.y * BM, w.p.rows) && !hidden; ++rr) {
+            const RepairRow<Tr, FORM> row(w, rr);  // rows past the last read it again
+            if (w.p.docs || rr == w.p.rows - 1 || w.span.limit(w.p, row.pos) < past || (T::ES == 2 && rr / BM == whole))
+                hidden = row_bad<Tr>(row.q(w), w.p.dim) || row_bad<Tr>(row.dout(w), w.p.dim);
+        }
+        if (!hidden) todo = 0;
+    }
     const bool repaired = todo >> (lane & 31) & 1;
     if (__builtin_expect(todo != 0, 0)) {
         for (; todo; todo &= todo - 1) {
@@ -1414,6 +1466,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             const int2 tiles = row_tiles<BM>(a, Span(a, at.bh / a.kv_heads), at_k0, at.split);
             float ok[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ov[4] = {0.0f, 0.0f, 0.0f, 0.0f}, slope = 1.0f;
             for (int rr = tiles.x * BM; rr < min(tiles.y * BM, arguments_again().rows); ++rr) {
+                if ((!DK || all_nan(ok, arguments_again().dim)) && (!DV || all_nan(ov, arguments_again().dim))) break;
                 const Repair w(arguments_again(), arguments_again().key_splits);
                 const RepairRow<Tr, FORM> row(w, rr);
                 if (!row.sees(w, j)) continue;

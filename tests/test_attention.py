@@ -238,6 +238,21 @@ def test_later_tokens_reach_no_earlier_row(hip, dtype, rows, keys, heads):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_what_is_seen_is_not_hidden(hip, dtype, causal):
+    """An infinity that a row sees stands in its feature and in no other; NaN everywhere stays NaN everywhere."""
+    case = make(1, 300, 300, 2, 1, 64, seed=41, causal=causal)
+    case["v"][0, 0, 0, 5] = np.inf
+    got = run(case, dtype, grad=False)[0]["out"]
+    assert (got[..., 5] == np.inf).all() and np.isfinite(np.delete(got, 5, axis=-1)).all()
+    for name in "qkv":
+        case[name] = np.full_like(case[name], np.nan)
+    got = run(case, dtype)[0]
+    assert all(np.isnan(np.asarray(g, np.float32)).all() for g in got.values())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size,scale", [(30.0, 1.0), (1.0, -0.4), (1.0, 0.0), (0.01, None)])
 def test_scores_large_reversed_and_flat(hip, dtype, size, scale):
     check(make(1, 100, 140, 2, 1, 64, seed=8, size=size, causal=True, scale=scale), dtype)
