@@ -93,6 +93,12 @@ int ormi_hip_synchronize(void);
  * int32 range saturating. */
 int ormi_hip_convert(void* dst, int dst_dtype, const void* src, int src_dtype, size_t count);
 
+/* dst, contiguous, = the elements of a strided view at src, in order and bit
+ * for bit: elem_bytes is 1, 2, 4 or 8, ndim 0 to 8, strides are in elements.
+ * The way to make integer views contiguous; maps compute in fp32, which holds
+ * integers up to 2^24. */
+int ormi_hip_copy_view(void* dst, const void* src, size_t elem_bytes, int ndim, const int* shape, const int64_t* strides);
+
 /* ------------------------------------------------------------- hipRTC JIT --
  * Replaces compile_ptx + cuModuleLoadDataEx + cuModuleGetFunction + the
  * per-call cuModuleUnload (reference csrc/backend/cuda/utils.cu:6-27,

@@ -27,10 +27,20 @@ namespace ormi::hip {
         for (int i = 0; i < 4; ++i) out[i] = n.view.strides[i];
     }
 
-    // n's values in a contiguous buffer (n's own, or a copy by the map kernel).
+    static bool is_integer(DType d) { return d == DType::Int32 || d == DType::Int64 || d == DType::Bool; }
+
+    // n's values in a contiguous buffer: n's own, or a copy, by the map kernel where
+    // its float32 holds them and bit for bit where they are integers.
     static NodePtr contiguous(const NodePtr& n) {
         realize(n);
-        if (n->view.strides == calc_contiguous_strides(n->view.shape) && (long long)n->data->numel() == shape_numel(n->view.shape)) return n;
+        const auto& shape = n->view.shape;
+        if (n->view.strides == calc_contiguous_strides(shape) && (long long)n->data->numel() == shape_numel(shape)) return n;
+        if (is_integer(n->dtype)) {
+            auto c = std::make_shared<Node>(empty(shape, DeviceEnum::HIP, n->dtype), false, n->device);
+            const std::vector<int64_t> strides(n->view.strides.begin(), n->view.strides.end());
+            ORMI_HIP_CHECK(ormi_hip_copy_view(c->data->ptr, n->data->ptr, dtype_size(n->dtype), (int)shape.size(), shape.data(), strides.data()));
+            return c;
+        }
         auto c = std::make_shared<Node>(OpEnum::CAST, std::vector<NodePtr>{n}, n->device, CastAttrs{n->dtype});
         realize(c);
         return c;

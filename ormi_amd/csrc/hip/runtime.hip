@@ -63,6 +63,27 @@ __global__ void fill_kernel(T* __restrict__ dst, T value, size_t count) {
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += stride) dst[i] = value;
 }
 
+// A strided view's elements in order, as bits: T is an unsigned integer.
+struct ViewShape {
+    int ndim;
+    int shape[ORMI_MAP_MAX_DIMS];
+    int64_t strides[ORMI_MAP_MAX_DIMS];
+};
+template <typename T>
+__global__ void copy_view_kernel(T* __restrict__ dst, const T* __restrict__ src, ViewShape v, size_t count) {
+    const size_t stride = (size_t)gridDim.x * blockDim.x;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += stride) {
+        size_t rest = i;
+        int64_t at = 0;
+        for (int d = v.ndim - 1; d >= 0; --d) {
+            const size_t q = rest / (unsigned)v.shape[d];
+            at += (int64_t)(rest - q * (unsigned)v.shape[d]) * v.strides[d];
+            rest = q;
+        }
+        dst[i] = src[at];
+    }
+}
+
 __device__ __forceinline__ float load_as_f32(const void* p, int dt, size_t i) {
     switch (dt) {
         case ORMI_DTYPE_F32: return ((const float*)p)[i];
@@ -577,6 +598,34 @@ int ormi_hip_convert(void* dst, int dst_dtype, const void* src, int src_dtype, s
     ORMI_HIP_DRAIN();
     const unsigned block = 256, grid = grid_for(count, block);
     convert_kernel<<<grid, block>>>(dst, dst_dtype, src, src_dtype, count);
+    ORMI_HIP_TRY(hipGetLastError());
+    return ORMI_HIP_OK;
+}
+
+int ormi_hip_copy_view(void* dst, const void* src, size_t elem_bytes, int ndim, const int* shape, const int64_t* strides) {
+    auto bad = [](const char* what) { return fail(ORMI_HIP_ERR_INVALID, std::string("ormi_hip_copy_view: ") + what); };
+    if (ndim < 0 || ndim > ORMI_MAP_MAX_DIMS) return bad("0 to 8 dimensions");
+    if (ndim > 0 && (!shape || !strides)) return bad("null shape or strides");
+    if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4 && elem_bytes != 8) return bad("element size must be 1, 2, 4 or 8");
+    ViewShape v{ndim, {}, {}};
+    size_t count = 1;
+    for (int d = 0; d < ndim; ++d) {
+        if (shape[d] < 0) return bad("negative extent");
+        v.shape[d] = shape[d];
+        v.strides[d] = strides[d];
+        count *= (size_t)shape[d];
+    }
+    if (count == 0) return ORMI_HIP_OK;
+    if (!dst || !src) return bad("null pointer");
+    ORMI_ENSURE_INIT();
+    ORMI_HIP_DRAIN();
+    const unsigned block = 256, grid = grid_for(count, block);
+    switch (elem_bytes) {
+        case 1: copy_view_kernel<<<grid, block>>>((unsigned char*)dst, (const unsigned char*)src, v, count); break;
+        case 2: copy_view_kernel<<<grid, block>>>((unsigned short*)dst, (const unsigned short*)src, v, count); break;
+        case 4: copy_view_kernel<<<grid, block>>>((unsigned*)dst, (const unsigned*)src, v, count); break;
+        default: copy_view_kernel<<<grid, block>>>((unsigned long long*)dst, (const unsigned long long*)src, v, count);
+    }
     ORMI_HIP_TRY(hipGetLastError());
     return ORMI_HIP_OK;
 }
