@@ -934,7 +934,11 @@ int launch_attention_fwd_dp(const AttnParams& p) {
 // the largest squared norms of a dout row and of a value row: |score gradient|
 // <= p (|dp| + |delta|) <= 2 |dout| |v|, and held times the power of two that
 // takes that bound to 2^15 the score gradients keep to float16's normal range
-// whatever the scale of the loss. A maximum does not depend on its order.
+// whatever the scale of the loss. A maximum does not depend on its order. What
+// stands at masked positions has no part in it: rows that see nothing (their
+// score gradients are zero whatever dout holds) and values past the length or
+// without a document; nor have rows that are not finite, whose own score
+// gradients are not finite at any scale.
 template <class Tr>
 __device__ __forceinline__ void load_chunk(const char* at, float (&v)[Tr::VE]) {
     const u32x4_t w = *(const u32x4_t*)at;
@@ -988,13 +992,14 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(AttnParams p, floa
                 }
             }
             dot = ormi_lanes_sum<16>(dot);
-            const int kvh = head / p.group;
-            if (live && sub == 0) delta[((long long)b * p.kv_heads + kvh) * p.rows + (long long)i * p.group + head % p.group] = dot;
+            const long long to = ((long long)b * p.kv_heads + head / p.group) * p.rows + (long long)i * p.group + head % p.group;
+            if (live && sub == 0) delta[to] = dot;
+            if (bounds && p.lse[to] == kInf) norm = 0.0f;
         } else {
             const int kvh = (int)(row % p.kv_heads);
             const long long bj = row / p.kv_heads;
             const int b = (int)(bj / p.keys), j = (int)(bj % p.keys);
-            if (j < Span(p, b).end) {
+            if (j < Span(p, b).end && !(p.docs && p.docs[b * p.docs_sb + j] < 0)) {
                 const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + kvh * p.v_sh) * Tr::ESIZE;
                 for (int c = sub; c < p.chunks; c += 16) {
                     float y[Tr::VE];
@@ -1004,7 +1009,10 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(AttnParams p, floa
                 }
             }
         }
-        if (bounds) most_norm = fmaxf(most_norm, ormi_lanes_sum<16>(norm));
+        if (bounds) {
+            norm = ormi_lanes_sum<16>(norm);
+            if (norm < kInf) most_norm = fmaxf(most_norm, norm);
+        }
     }
     if (!bounds) return;
     float norm = most_norm;
