@@ -480,9 +480,9 @@ int ormi_hip_attention(const ormi_attention_desc* desc);
  * and dv are contiguous, laid out like q, k and v's extents, of the same dtype
  * (NULL: not wanted). Shared key heads' gradients add up over their query
  * heads. float16 score gradients are held times a power of two taken from the
- * largest finite rows of dout and v, so that a small loss does not lose them;
- * rows that see no key, and keys past the length or of a negative document,
- * do not count. */
+ * largest finite rows of a batch's key head in dout and v, so that a small loss
+ * does not lose them; rows that see no key, and keys past the length or of a
+ * negative document, do not count. */
 typedef struct ormi_attention_grad_desc {
     ormi_attention_desc forward;
     const void*         dout;

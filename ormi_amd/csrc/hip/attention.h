@@ -43,7 +43,7 @@ struct AttnParams {
     const char* dout;
     long long do_sb, do_sl, do_sh;
     const float* delta;      // sum of out * dout of a row, laid out like lse
-    const float* grad_scale; // float16: what the score gradients are held times (attention_delta_kernel)
+    const float* grad_scale; // float16: two squared norms per batch and key head (attention_delta_kernel)
     char *dq, *dk, *dv;
     int key_blocks, key_splits;
     unsigned group_m, group_s;  // division by group (ormi_fdiv)
@@ -52,7 +52,7 @@ struct AttnParams {
 int launch_attention_fwd_bf16(const AttnParams& p);
 int launch_attention_fwd_f16(const AttnParams& p);
 int launch_attention_fwd_f32(const AttnParams& p);
-// bounds: two zeroed words where the score gradients are held scaled (float16), else null.
+// bounds: two zeroed words per batch and key head where the score gradients are held scaled (float16), else null.
 int launch_attention_grad_bf16(const AttnParams& p, float* delta, unsigned* bounds);
 int launch_attention_grad_f16(const AttnParams& p, float* delta, unsigned* bounds);
 int launch_attention_grad_f32(const AttnParams& p, float* delta, unsigned* bounds);

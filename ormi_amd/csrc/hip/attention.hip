@@ -48,8 +48,8 @@ __global__ __launch_bounds__(64) void attention_ranges_kernel(int2* ranges, cons
     if (threadIdx.x == 0) ranges[blockIdx.x] = make_int2(lo, hi);
 }
 
-__global__ void attention_clear_kernel(unsigned* at, int n) {
-    if ((int)threadIdx.x < n) at[threadIdx.x] = 0;
+__global__ __launch_bounds__(256) void attention_clear_kernel(unsigned* at, int n) {
+    for (int i = (int)(blockIdx.x * 256 + threadIdx.x); i < n; i += (int)gridDim.x * 256) at[i] = 0;
 }
 
 // An operand as the kernels read it.
@@ -202,7 +202,7 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
         if (items * p.key_splits >= (1ll << 30) || heads * p.row_blocks >= (1ll << 30)) return bad("too many work-groups");
         pl.delta = take(pl.bytes, sizeof(float) * (size_t)heads * p.rows);
         pl.hold = d->dtype == ORMI_DTYPE_F16;
-        if (pl.hold) pl.bounds = take(pl.bytes, 2 * sizeof(unsigned));
+        if (pl.hold) pl.bounds = take(pl.bytes, 2 * sizeof(unsigned) * (size_t)heads);
         p.dq = (char*)g->dq;
         p.dk = (char*)g->dk;
         p.dv = (char*)g->dv;
@@ -320,7 +320,10 @@ int ormi_hip_attention_grad(const ormi_attention_grad_desc* desc) {
     settle(pl, ws, d, desc);
     float* delta = (float*)(ws + pl.delta);
     unsigned* bounds = pl.hold ? (unsigned*)(ws + pl.bounds) : nullptr;
-    if (bounds) attention_clear_kernel<<<1, 64>>>(bounds, 2);
+    if (bounds) {
+        const int n = 2 * d->batch * d->kv_heads;
+        attention_clear_kernel<<<(unsigned)std::min((n + 255) / 256, 256), 256>>>(bounds, n);
+    }
     pl.p.delta = delta;
     pl.p.grad_scale = (const float*)bounds;
     switch (d->dtype) {

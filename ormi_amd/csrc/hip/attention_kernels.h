@@ -934,7 +934,9 @@ int launch_attention_fwd_dp(const AttnParams& p) {
 // the largest squared norms of a dout row and of a value row: |score gradient|
 // <= p (|dp| + |delta|) <= 2 |dout| |v|, and held times the power of two that
 // takes that bound to 2^15 the score gradients keep to float16's normal range
-// whatever the scale of the loss. A maximum does not depend on its order. What
+// whatever the scale of the loss, each batch's key head by its own two norms (a
+// sequence or a head of a far larger loss takes nothing from the others). A
+// maximum does not depend on its order. What
 // stands at masked positions has no part in it: rows that see nothing (their
 // score gradients are zero whatever dout holds) and values past the length or
 // without a document; nor have rows that are not finite, whose own score
@@ -951,85 +953,96 @@ __device__ __forceinline__ void load_chunk(const char* at, float (&v)[Tr::VE]) {
 template <class Tr>
 __global__ __launch_bounds__(256) void attention_delta_kernel(AttnParams p, float* delta, unsigned* bounds, unsigned row_groups) {
     const int sub = threadIdx.x & 15;
-    float most_norm = 0.0f;
     const bool rows = blockIdx.x < row_groups;
-    const long long n = rows ? (long long)p.batch * p.queries * p.heads : (long long)p.batch * p.keys * p.kv_heads;
-    const long long step = (long long)(rows ? row_groups : gridDim.x - row_groups) * 16;
-    for (long long at = (long long)(rows ? blockIdx.x : blockIdx.x - row_groups) * 16 + (threadIdx.x >> 4);
-         at - (threadIdx.x >> 4) < n; at += step) {
-        const bool live = at < n;
-        const long long row = live ? at : n - 1;
-        float dot = 0.0f, norm = 0.0f;
-        if (rows) {
-            const int head = (int)(row % p.heads);
-            const long long bi = row / p.heads;
-            const int b = (int)(bi / p.queries), i = (int)(bi % p.queries);
-            const char* o = p.out + row * p.dim * Tr::ESIZE;
-            const char* rest = p.rest ? p.rest + row * p.dim * Tr::ESIZE : nullptr;
-            const char* g = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * Tr::ESIZE;
-            if (p.dim % Tr::VE == 0) {
-                for (int c = sub; c < p.dim / Tr::VE; c += 16) {
-                    float x[Tr::VE], y[Tr::VE];
-                    load_chunk<Tr>(o + c * 16, x);
-                    load_chunk<Tr>(g + c * 16, y);
-                    if (rest) {
-                        float z[Tr::VE];
-                        load_chunk<Tr>(rest + c * 16, z);
+    const int group = (int)(rows ? blockIdx.x : blockIdx.x - row_groups), groups = (int)(rows ? row_groups : gridDim.x - row_groups);
+    // Without bounds the rows in out's order; with them each key head's own, some
+    // (or one) of the work-groups' runs of rows for each, heads the fastest.
+    const int all_heads = p.batch * p.kv_heads, heads = bounds ? min(all_heads, groups) : 1, slices = groups / heads;
+    const long long n = bounds ? (rows ? p.rows : p.keys) : (long long)p.batch * p.queries * p.heads;
+    for (int bh = group % heads; bh < (bounds ? all_heads : 1); bh += heads) {
+        float most_norm = 0.0f;
+        for (long long at = (long long)(group / heads) * 16 + (threadIdx.x >> 4); at - (threadIdx.x >> 4) < n; at += (long long)slices * 16) {
+            const bool live = at < n;
+            const long long row = live ? at : n - 1;
+            float dot = 0.0f, norm = 0.0f;
+            if (rows) {
+                int b, i, head;
+                if (bounds) {
+                    b = bh / p.kv_heads;
+                    i = (int)row / p.group;
+                    head = bh % p.kv_heads * p.group + (int)row % p.group;
+                } else {
+                    head = (int)(row % p.heads);
+                    const long long bi = row / p.heads;
+                    b = (int)(bi / p.queries);
+                    i = (int)(bi % p.queries);
+                }
+                const long long from = (((long long)b * p.queries + i) * p.heads + head) * p.dim * Tr::ESIZE;
+                const char* o = p.out + from;
+                const char* rest = p.rest ? p.rest + from : nullptr;
+                const char* g = p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * Tr::ESIZE;
+                if (p.dim % Tr::VE == 0) {
+                    for (int c = sub; c < p.dim / Tr::VE; c += 16) {
+                        float x[Tr::VE], y[Tr::VE];
+                        load_chunk<Tr>(o + c * 16, x);
+                        load_chunk<Tr>(g + c * 16, y);
+                        if (rest) {
+                            float z[Tr::VE];
+                            load_chunk<Tr>(rest + c * 16, z);
 #pragma unroll
-                        for (int e = 0; e < Tr::VE; ++e) x[e] += z[e];
+                            for (int e = 0; e < Tr::VE; ++e) x[e] += z[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < Tr::VE; ++e) {
+                            dot = __builtin_fmaf(x[e], y[e], dot);
+                            norm = __builtin_fmaf(y[e], y[e], norm);
+                        }
                     }
-#pragma unroll
-                    for (int e = 0; e < Tr::VE; ++e) {
-                        dot = __builtin_fmaf(x[e], y[e], dot);
-                        norm = __builtin_fmaf(y[e], y[e], norm);
+                } else {
+                    for (int d = sub; d < p.dim; d += 16) {
+                        const float y = load1<Tr>(g, d);
+                        dot = __builtin_fmaf(load1<Tr>(o, d) + (rest ? load1<Tr>(rest, d) : 0.0f), y, dot);
+                        norm = __builtin_fmaf(y, y, norm);
                     }
                 }
+                dot = ormi_lanes_sum<16>(dot);
+                const long long to = ((long long)b * p.kv_heads + head / p.group) * p.rows + (long long)i * p.group + head % p.group;
+                if (live && sub == 0) delta[to] = dot;
+                if (bounds && p.lse[to] == kInf) norm = 0.0f;
             } else {
-                for (int d = sub; d < p.dim; d += 16) {
-                    const float y = load1<Tr>(g, d);
-                    dot = __builtin_fmaf(load1<Tr>(o, d) + (rest ? load1<Tr>(rest, d) : 0.0f), y, dot);
-                    norm = __builtin_fmaf(y, y, norm);
-                }
-            }
-            dot = ormi_lanes_sum<16>(dot);
-            const long long to = ((long long)b * p.kv_heads + head / p.group) * p.rows + (long long)i * p.group + head % p.group;
-            if (live && sub == 0) delta[to] = dot;
-            if (bounds && p.lse[to] == kInf) norm = 0.0f;
-        } else {
-            const int kvh = (int)(row % p.kv_heads);
-            const long long bj = row / p.kv_heads;
-            const int b = (int)(bj / p.keys), j = (int)(bj % p.keys);
-            if (j < Span(p, b).end && !(p.docs && p.docs[b * p.docs_sb + j] < 0)) {
-                const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + kvh * p.v_sh) * Tr::ESIZE;
-                for (int c = sub; c < p.chunks; c += 16) {
-                    float y[Tr::VE];
-                    load_chunk<Tr>(v + c * 16, y);
+                const int b = bh / p.kv_heads, j = (int)row;
+                if (j < Span(p, b).end && !(p.docs && p.docs[b * p.docs_sb + j] < 0)) {
+                    const char* v = p.v + (b * p.v_sb + (long long)j * p.v_sl + bh % p.kv_heads * p.v_sh) * Tr::ESIZE;
+                    for (int c = sub; c < p.chunks; c += 16) {
+                        float y[Tr::VE];
+                        load_chunk<Tr>(v + c * 16, y);
 #pragma unroll
-                    for (int e = 0; e < Tr::VE; ++e) norm = __builtin_fmaf(y[e], y[e], norm);
+                        for (int e = 0; e < Tr::VE; ++e) norm = __builtin_fmaf(y[e], y[e], norm);
+                    }
                 }
             }
+            if (bounds) {
+                norm = ormi_lanes_sum<16>(norm);
+                if (norm < kInf) most_norm = fmaxf(most_norm, norm);
+            }
         }
-        if (bounds) {
-            norm = ormi_lanes_sum<16>(norm);
-            if (norm < kInf) most_norm = fmaxf(most_norm, norm);
-        }
+        if (!bounds) return;
+        float norm = most_norm;
+        norm = fmaxf(norm, __shfl_xor(norm, 16, 64));
+        norm = fmaxf(norm, __shfl_xor(norm, 32, 64));
+        __shared__ float most[4];
+        __syncthreads();  // the last head's have been read
+        if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = norm;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            atomicMax(bounds + 2 * bh + (rows ? 0 : 1), __float_as_uint(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))));
     }
-    if (!bounds) return;
-    float norm = most_norm;
-    norm = fmaxf(norm, __shfl_xor(norm, 16, 64));
-    norm = fmaxf(norm, __shfl_xor(norm, 32, 64));
-    __shared__ float most[4];
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = norm;
-    __syncthreads();
-    if (threadIdx.x == 0)
-        atomicMax(bounds + (blockIdx.x < row_groups ? 0 : 1),
-                  __float_as_uint(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))));
 }
-// The power of two that the score gradients are held times.
+// The power of two that the score gradients of a batch's key head are held times.
 template <class Tr>
-__device__ __forceinline__ float grad_hold(const AttnParams& p) {
+__device__ __forceinline__ float grad_hold(const AttnParams& p, int bh) {
     if (Shift<Tr>::bwd == 0.0f) return 1.0f;
-    const float bound = 2.0f * __builtin_sqrtf(p.grad_scale[0] * p.grad_scale[1]);
+    const float bound = 2.0f * __builtin_sqrtf(p.grad_scale[2 * bh] * p.grad_scale[2 * bh + 1]);
     if (!(bound > 0.0f && bound < 1e30f)) return 1.0f;
     return __builtin_amdgcn_ldexpf(1.0f, min(100, max(-100, 15 - __builtin_amdgcn_frexp_expf(bound))));
 }
@@ -1064,7 +1077,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
     }
     const float slope2 = FORM != kPlain && p.slopes ? p.slopes[head] * 1.44269504f : 0.0f;
     const float lse = p.lse[(long long)bh * p.rows + rc], delta = p.delta[(long long)bh * p.rows + rc];
-    const float hold = grad_hold<Tr>(p);
+    const float hold = grad_hold<Tr>(p, bh);
     u32x4_t qf[T::NF], gf[T::NF];
     T::row_frags(p.q + (b * p.q_sb + (long long)i * p.q_sl + head * p.q_sh) * T::ES, p.chunks, qf);
     T::row_frags(p.dout + (b * p.do_sb + (long long)i * p.do_sl + head * p.do_sh) * T::ES, p.chunks, gf);
@@ -1199,7 +1212,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
                 const float ds = e * (row_dot<Tr>(row.dout(w), value_row<Tr>(w, j), w.p.dim) - w.p.delta[w.row_at(rr)]) * slope;
                 add_row<Tr>(key_row<Tr>(w, j), w.p.dim, ds, o);
             }
-            if (w.p.splits > 1) put_part<DP>(w.p.part_q + w.part_at(rr) * DP, o, grad_hold<Tr>(w.p));
+            if (w.p.splits > 1) put_part<DP>(w.p.part_q + w.part_at(rr) * DP, o, grad_hold<Tr>(w.p, w.work.bh));
             else put_row<Tr>(w.p.dq + row.at(w), w.p.dim, o, w.p.scale, nullptr);
         }
     }
@@ -1264,7 +1277,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     const float keyf = (float)key;
     const bool sloped = FORM != kPlain && p.slopes;
     const int key_live = p.docs && doc < 0 ? 0x7fffffff : key;  // a key without a document is seen by no row
-    const float hold = grad_hold<Tr>(p), shift = Shift<Tr>::bwd;
+    const float hold = grad_hold<Tr>(p, bh), shift = Shift<Tr>::bwd;
     const float hold_p = Shift<Tr>::bwd != 0.0f ? hold * __builtin_amdgcn_exp2f(-shift) : 1.0f;
     u32x4_t kf[T::NF], vf[VL ? 1 : T::NF];
     T::row_frags(p.k + (b * p.k_sb + (long long)keyc * p.k_sl + kvh * p.k_sh) * T::ES, p.chunks, kf);
@@ -1488,7 +1501,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             const long long n = (long long)w.p.batch * w.p.kv_heads * w.p.keys, row = (long long)w.work.bh * w.p.keys + j;
             const long long to = (((long long)w.b * w.p.keys + j) * w.p.kv_heads + w.kvh) * w.p.dim * T::ES;
             if (w.p.key_splits > 1) {
-                if (DK) put_part<DP>(w.p.part + (w.work.split * n + row) * DP, ok, grad_hold<Tr>(w.p));
+                if (DK) put_part<DP>(w.p.part + (w.work.split * n + row) * DP, ok, grad_hold<Tr>(w.p, w.work.bh));
                 if (DV) put_part<DP>(w.p.part + ((w.p.key_splits + w.work.split) * n + row) * DP, ov, __builtin_amdgcn_exp2f(Shift<Tr>::bwd));
             } else {
                 if (DK && w.p.dk) put_row<Tr>(w.p.dk + to, w.p.dim, ok, w.p.scale, nullptr);
@@ -1529,18 +1542,17 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttnParams p) 
             else ((unsigned short*)out)[at + d] = (unsigned short)pack2(Tr{}, v, v);
         }
     };
-    const float score = p.scale / grad_hold<Tr>(p);
     if (row < nq) {
         const int bh = (int)(row / p.rows), r = (int)(row % p.rows), b = bh / p.kv_heads;
         const int i = r / p.group, head = (bh % p.kv_heads) * p.group + r % p.group;
-        add(p.part_q, p.splits, nq, p.dq, (((long long)b * p.queries + i) * p.heads + head) * p.dim, score);
+        add(p.part_q, p.splits, nq, p.dq, (((long long)b * p.queries + i) * p.heads + head) * p.dim, p.scale / grad_hold<Tr>(p, bh));
         return;
     }
     row -= nq;
     if (row >= nk) return;
     const int bh = (int)(row / p.keys), j = (int)(row % p.keys), b = bh / p.kv_heads, kvh = bh % p.kv_heads;
     const long long at = (((long long)b * p.keys + j) * p.kv_heads + kvh) * p.dim;
-    if (p.dk) add(p.part, p.key_splits, nk, p.dk, at, score);
+    if (p.dk) add(p.part, p.key_splits, nk, p.dk, at, p.scale / grad_hold<Tr>(p, bh));
     if (p.dv) add(p.part + p.key_splits * nk * DP, p.key_splits, nk, p.dv, at, __builtin_amdgcn_exp2f(-Shift<Tr>::bwd));
 }
 
@@ -1558,12 +1570,20 @@ void launch_attention_grad_form(const AttnParams& p) {
     }
 }
 
+// Work-groups over the rows of dout, and over those of v, where both also give their
+// largest norms: the words of all heads lie in a few lines, in which the maxima of all
+// work-groups meet (8192 tokens, 8 heads of 128: 1024 work-groups 33 us, 4096 98 us).
+constexpr int kDeltaGroups = 1024;
+
 template <class Tr, int DP>
 int launch_attention_grad_dp(const AttnParams& p, float* delta, unsigned* bounds) {
     const long long rows = (long long)p.batch * p.queries * p.heads, values = (long long)p.batch * p.keys * p.kv_heads;
-    // Where the work-groups meet in one word they go over several rows each.
-    const long long most = bounds ? 1024 : 1 << 30;
-    const unsigned row_groups = (unsigned)std::min((rows + 15) / 16, most), value_groups = bounds ? (unsigned)std::min((values + 15) / 16, most) : 0;
+    unsigned row_groups = (unsigned)((rows + 15) / 16), value_groups = 0;
+    if (bounds) {
+        const int heads = std::min(p.batch * p.kv_heads, 1 << 16), slices = std::max(1, kDeltaGroups / heads);
+        row_groups = (unsigned)(heads * std::min((p.rows + 15) / 16, slices));
+        value_groups = (unsigned)(heads * std::min((p.keys + 15) / 16, slices));
+    }
     attention_delta_kernel<Tr><<<row_groups + value_groups, 256>>>(p, delta, bounds, row_groups);
     if (p.form == kPlain) launch_attention_grad_form<Tr, DP, kPlain>(p);
     else if (p.form == kBias) launch_attention_grad_form<Tr, DP, kBias>(p);

@@ -1,6 +1,6 @@
 """float16 score gradients are held times a power of two taken from dout and v.
-What stands at positions that reach no result does not move it: gradients of
-losses of 2^-20 against the formula in 64 bits.
+What stands at positions that reach no result does not move it, nor does another
+sequence or key head: gradients of losses of 2^-20 against the formula in 64 bits.
 
 q and k are 2^6 times unequal, so that the gradient of the one with the small
 values is far above float16's least numbers while the score gradients are not."""
@@ -60,4 +60,17 @@ def test_rows_that_see_nothing_do_not_move_the_hold(hip, large, bad):
     w[0, :15] = bad
     data["v"][0, 25:] = bad
     for n, g in gradients(data, w, causal=True, lengths=lengths).items():
+        assert_within(g, want[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("large", ["q", "k"])
+@pytest.mark.parametrize("apart", ["batch", "head"])
+def test_other_sequences_and_heads_do_not_move_the_hold(hip, large, apart):
+    """One sequence's (or key head's) loss is 2^22 times the others'."""
+    data, w = case(3, 150, 150, 4, 2, 64, large, 17)
+    grown = w[1] if apart == "batch" else w[:, :, 2:]
+    grown *= np.float32(2.0 ** 22)
+    want = ref(data["q"], data["k"], data["v"], w, dtype="float16", causal=True)
+    for n, g in gradients(data, w, causal=True).items():
         assert_within(g, want[n], n)
