@@ -4,8 +4,11 @@
 
 namespace ormi_hip {
 
-// What a score is beside a multiple of q.k: nothing, slopes, or a tanh and perhaps slopes.
-constexpr int kPlain = 0, kBias = 1, kCap = 2;
+// What a score is beside a multiple of q.k: nothing, slopes, or a tanh and perhaps
+// slopes. A cap multiplies what the tanh is off by: above kWideCap 16-bit scores
+// take the tanh that is exact relative to itself, too (tanh_score).
+constexpr int kPlain = 0, kBias = 1, kCap = 2, kCapWide = 3;
+constexpr float kWideCap = 256.0f;
 
 constexpr int kDocTile = 64;  // tokens per document range
 

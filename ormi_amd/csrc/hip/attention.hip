@@ -135,7 +135,7 @@ int plan_attention(const ormi_attention_desc* d, const ormi_attention_grad_desc*
     p.out = (char*)d->out;
     p.lse = d->lse;
     p.rest = d->dtype == ORMI_DTYPE_F32 ? nullptr : (char*)d->rest;
-    p.form = d->cap > 0.0f ? kCap : d->slopes ? kBias : kPlain;
+    p.form = d->cap > kWideCap ? kCapWide : d->cap > 0.0f ? kCap : d->slopes ? kBias : kPlain;
     const int es = pl.es = d->dtype == ORMI_DTYPE_F32 ? 4 : 2, ve = 16 / es;
     pl.padded = (d->dim + ve - 1) / ve * ve;
     p.chunks = pl.padded / ve;
