@@ -214,6 +214,18 @@ struct Tile {
             }
         }
     }
+    // Zeros for the chunks that rows of fewer features do not fill, in `rows` rows of
+    // tiles that lie one after the other, by all `threads` of the work-group; before
+    // any load into them.
+    __device__ __forceinline__ static void clear_padding(lds_char* t, int rows, int chunks, int threads) {
+        if (chunks == CPR) return;
+        const int pad = CPR - chunks;
+        for (int x = threadIdx.x; x < rows * pad; x += threads) {
+            const int row = x / pad, c = chunks + x % pad;
+            *(__attribute__((address_space(3))) u32x4_t*)(t + at(row) + ((c ^ swz(row)) << 4)) = u32x4_t{0, 0, 0, 0};
+        }
+        __syncthreads();
+    }
     // A row's fragments from memory: lane l holds row `row`'s chunks 2 f + l / 32 (zero past the row's end).
     __device__ __forceinline__ static void row_frags(const char* row, int chunks, u32x4_t (&out)[NF]) {
         const int half = (threadIdx.x & 63) >> 5;
@@ -230,8 +242,10 @@ struct Tile {
 // source side. Inline assembly, as in the GEMMs: the compiler would make every
 // LDS read of the current stage wait for the next stage's loads. The kernels
 // wait themselves before the barrier that publishes a stage.
-// Chunks past the row's end re-read chunk 0: what meets them is zero in the
-// first product and is not stored in the second.
+// Chunks past the row's end are not loaded but cleared once (clear_padding): zero has
+// to meet zero there, not an infinity that stands elsewhere in the row. Each load runs
+// with the lanes whose chunks exist; a branch for whole rows instead parted the loop's
+// instructions (dk and dv of 2 x 1025 tokens, 6 heads of 80, float32: 111 us, so 106).
 template <class Tr, int DP, int ROWS, int NW>
 struct Loader {
     using T = Tile<Tr, DP>;
@@ -243,51 +257,67 @@ struct Loader {
         return min((wave * PER + s) * 64 + lane, ROWS * T::CPR - 1);
     }
     __device__ __forceinline__ static int seg_row(int s) { return seg_lane(s) / T::CPR; }
+    __device__ __forceinline__ static int seg_at(int s, int row) {  // chunk within the row
+        return (T::EVEN ? (int)(threadIdx.x & 63) % T::CPR : seg_lane(s) % T::CPR) ^ T::swz(row);
+    }
     __device__ __forceinline__ static unsigned seg_chunk(int s, int row, int chunks) {  // bytes within the row
-        const int c = (T::EVEN ? (int)(threadIdx.x & 63) % T::CPR : seg_lane(s) % T::CPR) ^ T::swz(row);
+        const int c = seg_at(s, row);
         return c < chunks ? (unsigned)c * 16u : 0u;
     }
+    // The lanes whose chunks exist, of each of the segments after which the lanes'
+    // chunks come again (pairs of them are alike with 32 chunks a row).
+    static constexpr int ALIKE = T::CPR == 32 ? 2 : 1, KINDS = T::CPR == 32 ? 4 : T::CPR == 12 ? 3 : T::CPR == 24 ? 6 : 1;
+    struct Live {
+        unsigned long long m[KINDS < PER ? KINDS : PER];
+        __device__ __forceinline__ explicit Live(int chunks) {
+#pragma unroll
+            for (int k = 0; k < KINDS && k * ALIKE < PER; ++k) m[k] = __ballot(seg_at(k * ALIKE, seg_row(k * ALIKE)) < chunks);
+        }
+        __device__ __forceinline__ unsigned long long of(int s) const { return m[s / ALIKE % KINDS]; }
+    };
     // All of the wave's segments from base + off[s], up to four per asm block. The
     // assembler's text is not checked for hazards, so the waits are written out:
     // five cycles before a memory instruction reads a scalar register that a
     // vector instruction (a lane read that restores a spilled one, say) may have
-    // written, one between a write of m0 and a load to LDS.
-    __device__ __forceinline__ static void load(lds_char* dst, const char* base, const unsigned (&off)[PER]) {
+    // written, one between a write of m0 and a load to LDS. All lanes of the wave are
+    // active here, and are again after it.
+    __device__ __forceinline__ static void load(lds_char* dst, const char* base, const unsigned (&off)[PER], const Live& live) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const unsigned d = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(dst + wave * PER * T::SEGB));
-        constexpr int N = SEGS % NW != 0 ? 1 : PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1;
+        constexpr int N = SEGS % NW != 0 || !T::EVEN ? 1 : PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1;
 #pragma unroll
         for (int s = 0; s < PER; s += N) {
             if (SEGS % NW != 0 && wave * PER + s >= SEGS) break;  // the last wave's share is shorter
             if constexpr (N == 4)
                 asm volatile(
-                    "s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+                    "s_nop 3\n\ts_mov_b64 exec, %7\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
                     "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
-                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
-                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5" ::"s"(d + s * T::SEGB),
-                    "v"(off[s]), "v"(off[s + 1]), "v"(off[s + 2]), "v"(off[s + 3]), "s"(base), "i"(T::SEGB)
+                    "s_mov_b64 exec, %8\n\ts_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
+                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\ts_mov_b64 exec, -1" ::"s"(d + s * T::SEGB),
+                    "v"(off[s]), "v"(off[s + 1]), "v"(off[s + 2]), "v"(off[s + 3]), "s"(base), "i"(T::SEGB), "s"(live.of(s)), "s"(live.of(s + 2))
                     : "memory", "m0", "scc");
             else if constexpr (N == 2)
                 asm volatile(
-                    "s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
-                    "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(d + s * T::SEGB),
-                    "v"(off[s]), "v"(off[s + 1]), "s"(base), "i"(T::SEGB)
+                    "s_nop 3\n\ts_mov_b64 exec, %5\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+                    "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, -1" ::"s"(d + s * T::SEGB),
+                    "v"(off[s]), "v"(off[s + 1]), "s"(base), "i"(T::SEGB), "s"(live.of(s))
                     : "memory", "m0", "scc");
             else
-                asm volatile("s_nop 3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(d + s * T::SEGB),
-                             "v"(off[s]), "s"(base)
+                asm volatile("s_nop 3\n\ts_mov_b64 exec, %3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1" ::"s"(
+                                 d + s * T::SEGB),
+                             "v"(off[s]), "s"(base), "s"(live.of(s))
                              : "memory", "m0");
         }
     }
     // Rows base + row * row_bytes, rows past `last` re-reading it.
-    __device__ __forceinline__ static void rows(lds_char* dst, const char* base, unsigned row_bytes, int last, int chunks) {
+    __device__ __forceinline__ static void rows(lds_char* dst, const char* base, unsigned row_bytes, int last, int chunks, const Live& live) {
         unsigned off[PER];
 #pragma unroll
         for (int s = 0; s < PER; ++s) {
             const int row = seg_row(s);
             off[s] = (unsigned)min(row, last) * row_bytes + seg_chunk(s, row, chunks);
         }
-        load(dst, uniform_ptr(base), off);
+        load(dst, uniform_ptr(base), off, live);
     }
 };
 
@@ -685,10 +715,11 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW 
     const char* kb = p.k + (b * p.k_sb + kvh * p.k_sh) * T::ES;
     const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh) * T::ES;
     using L = Loader<Tr, DP, BN, NW>;
+    const typename L::Live live(p.chunks);
     auto issue = [&](int t, int stage) {
         const int last = span.end - 1 - t * BN;
-        L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks);
-        L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks);
+        L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks, live);
+        L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks, live);
         if (p.docs && wave == 0) load_words(key_doc[stage], p.docs + b * p.docs_sb + min(t * BN + lane, p.keys - 1));
     };
 
@@ -708,6 +739,7 @@ __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW 
 #pragma unroll
         for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
 
+    T::clear_padding(lds, 4 * BN, p.chunks, 64 * NW);
     int t = p.docs ? walk.next(t0, t1) : near, stage = 0;
     // The weights are rounded to 16 bits for their product with the values. In the tile
     // that a row begins with, what that leaves is multiplied too: it holds all keys of a
@@ -1112,10 +1144,11 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
     const char* kb = p.k + (b * p.k_sb + kvh * p.k_sh) * T::ES;
     const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh) * T::ES;
     using L = Loader<Tr, DP, BN, NW>;
+    const typename L::Live live(p.chunks);
     auto issue = [&](int t, int stage) {
         const int last = span.end - 1 - t * BN;
-        L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks);
-        L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks);
+        L::rows(lds + stage * 2 * TILEB, kb + (long long)t * BN * p.k_sl * T::ES, (unsigned)(p.k_sl * T::ES), last, p.chunks, live);
+        L::rows(lds + stage * 2 * TILEB + TILEB, vb + (long long)t * BN * p.v_sl * T::ES, (unsigned)(p.v_sl * T::ES), last, p.chunks, live);
         if (p.docs && wave == 0) load_words(key_doc[stage], p.docs + b * p.docs_sb + min(t * BN + lane, p.keys - 1));
     };
 
@@ -1125,6 +1158,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.0f;
 
+    T::clear_padding(lds, 4 * BN, p.chunks, 64 * NW);
     int t = next(t0), stage = 0;
     // As in the forward pass, one tile's score gradients go in with what rounding left of them.
     const int whole = FORM != kPlain && p.slopes && !p.docs ? min(max((rb * NW * 32 / p.group + span.off) / BN, t0), max(t1 - 1, t0)) : t;
@@ -1326,6 +1360,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     const char* qb = p.q + (b * p.q_sb + (long long)kvh * p.group * p.q_sh) * T::ES;
     const char* gb = p.dout + (b * p.do_sb + (long long)kvh * p.group * p.do_sh) * T::ES;
     using L = Loader<Tr, DP, BM, NW>;
+    const typename L::Live live(p.chunks);
     auto issue = [&](int t, int stage) {
         const int r0 = t * BM, i0 = r0 / p.group;
         const char* qt = uniform_ptr(qb + (long long)i0 * p.q_sl * T::ES);
@@ -1339,8 +1374,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
             qo[s] = ((unsigned)(i - i0) * (unsigned)p.q_sl + (unsigned)g * (unsigned)p.q_sh) * T::ES + c;
             go[s] = ((unsigned)(i - i0) * (unsigned)p.do_sl + (unsigned)g * (unsigned)p.do_sh) * T::ES + c;
         }
-        L::load(lds + stage * 2 * TILEB, qt, qo);
-        L::load(lds + stage * 2 * TILEB + TILEB, gt, go);
+        L::load(lds + stage * 2 * TILEB, qt, qo, live);
+        L::load(lds + stage * 2 * TILEB + TILEB, gt, go, live);
         // What belongs to the rows, one per lane of the first wave's halves; a row
         // past the last has the limit 0, as has one without a document of its own.
         if (wave == 0) {
@@ -1363,6 +1398,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc_k[dt][e] = acc_v[dt][e] = 0.0f;
 
+    T::clear_padding(lds, (VL ? 4 + NW : 4) * BM, p.chunks, 64 * NW);
     int t = next(t0), stage = 0;
     // One tile's weights and score gradients go in with what rounding left of them: the
     // only tile of keys that few rows see.
@@ -1372,15 +1408,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
         if constexpr (VL) {
             lds_char* vg = lds + 4 * TILEB;
             const char* vb = p.v + (b * p.v_sb + kvh * p.v_sh + (long long)k0 * p.v_sl) * T::ES;
-            Loader<Tr, DP, NW * 32, NW>::rows(vg, vb, (unsigned)(p.v_sl * T::ES), span.end - 1 - k0, p.chunks);
-            if (p.chunks < T::CPR) {  // both operands come from LDS: the padding of one has to be zero
-                publish();
-                const int pad = T::CPR - p.chunks;
-                for (int x = threadIdx.x; x < NW * 32 * pad; x += 64 * NW) {
-                    const int row = x / pad, c = p.chunks + x % pad;
-                    *(__attribute__((address_space(3))) u32x4_t*)(vg + T::at(row) + ((c ^ T::swz(row)) << 4)) = u32x4_t{0, 0, 0, 0};
-                }
-            }
+            using V = Loader<Tr, DP, NW * 32, NW>;
+            V::rows(vg, vb, (unsigned)(p.v_sl * T::ES), span.end - 1 - k0, p.chunks, typename V::Live(p.chunks));
         }
     }
     while (t < t1) {
