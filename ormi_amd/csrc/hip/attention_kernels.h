@@ -103,13 +103,15 @@ __device__ __forceinline__ float tanh_score(float y) {
 }
 
 // The wait states between a matrix instruction and a vector instruction that
-// reads its result (its passes and two more), spelled out: across the branches
-// that masks bring, the compiler (ROCm 7.2) has left too few of them, and rows
-// came out wrong now and then. tests/test_mfma_waits.py checks the assembly.
+// reads its result, spelled out: 12 after a 32x32x16 product (its 8 passes and
+// four more), 18 after a 32x32x2 one (16 and two), which is what the compiler
+// puts there itself in straight-line code. Across the branches that masks bring,
+// it (ROCm 7.2) has left too few of them, and rows came out wrong now and then.
+// tests/test_mfma_wait_states.py checks the counts and the assembly.
 template <class Tr>
 __device__ __forceinline__ void settle(f32x16_t& a) {
     if constexpr (Tr::ESIZE == 4) asm("s_nop 15\n\ts_nop 1" : "+v"(a));
-    else asm("s_nop 9" : "+v"(a));
+    else asm("s_nop 11" : "+v"(a));
 }
 
 // 16-bit probabilities are held 2^kShift above their value (of at most 1, or
