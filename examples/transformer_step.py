@@ -66,8 +66,8 @@ def train(block: AttentionBlock, x: np.ndarray, target: np.ndarray, steps: int, 
         loss = (error * error).mean()
         loss.backward()
         optimizer.step()
-        optimizer.zero_grad()
         losses.append(float(loss.numpy()))
+        loss.zero_grad_graph()  # gradients point back at the nodes they came from: without it each step's graph stays
     return losses
 
 

@@ -4,7 +4,7 @@ masked softmax attention, and the AdamW step over a list of tensors.
     table = RotaryTable(head_dim, positions)
     q = rotary(x.reshape((batch, length, heads, head_dim)), table, dtype="bfloat16")
     y = attention(q, k, v, causal=True)          # differentiable, lazy like every op
-    optimizer = AdamW(parameters, lr=3e-4)       # then loss.backward(); optimizer.step()
+    optimizer = AdamW(parameters, lr=3e-4)       # loss.backward(); optimizer.step(); loss.zero_grad_graph()
 
 Additive to the reference's Python surface (ormi-core/src/ormi_core/tensor.py:10-190),
 which has none of them.
@@ -223,9 +223,16 @@ def adamw(params, grads, states, *, step: int, lr: float = 1e-3, betas=(0.9, 0.9
 class AdamW:
     """Keeps the moments of a list of parameters and steps them by their gradients.
 
+        loss.backward()
+        optimizer.step()
+        loss.zero_grad_graph()
+
     step() gives each parameter with a gradient a new value: the Tensor object
-    stays, its node is a new leaf, so a graph that read the old one keeps its
-    values. state_bits: 32, or 8 for moments of a quarter of the size.
+    stays, its node is a new leaf without a gradient, so a graph that read the
+    old one keeps its values. The old leaf's gradient is let go of; those of the
+    nodes between point back at what they were computed from, and a loop that
+    does not release them with zero_grad_graph keeps every step's graph in
+    memory. state_bits: 32, or 8 for moments of a quarter of the size.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
@@ -248,6 +255,7 @@ class AdamW:
                                 [self.states[i] for i in members], step=step, lr=self.lr, betas=self.betas, eps=self.eps,
                                 weight_decay=self.weight_decay)
             for i, p, s in zip(members, new, states):
+                self.params[i].zero_grad()  # of the leaf that was: the graph may still hold it
                 self.params[i]._node = p._node
                 self.states[i] = s
                 self.steps[i] = step
