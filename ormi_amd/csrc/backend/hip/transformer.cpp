@@ -46,8 +46,10 @@ namespace ormi::hip {
         return c;
     }
 
+    // In rows of 256 bytes, what the entries' sizes are multiples of: packed operands
+    // alone can pass the 2^31 elements of one extent.
     static std::shared_ptr<Buffer> workspace(size_t bytes) {
-        return bytes ? empty({(int)((bytes + 3) / 4)}, DeviceEnum::HIP) : nullptr;
+        return bytes ? empty({checked_extent((long long)((bytes + 255) / 256), "attention: workspace"), 64}, DeviceEnum::HIP) : nullptr;
     }
 
     // ----------------------------------------------------------- gradients --
