@@ -424,6 +424,18 @@ __device__ __forceinline__ float score2(const AttnParams& p, float s, float slop
     return __builtin_fmaf(s, p.scale2, base);
 }
 
+// 2^x for the gradients' weights. The hardware's is zero below 2^-126; a key far down
+// a slope has no other weights, and its float32 gradient, in the normal range once they
+// are times dout and q, would miss them (a tenth of a dk of 1.2e-36). The square of a
+// root reaches 2^-149 (2 x 1025 tokens, 6 heads of 80: dq 76.7 us instead of 76.2, the
+// library's own 2^x 82). 16-bit weights below 2^-126 count as zero.
+template <class Tr>
+__device__ __forceinline__ float weight2(float x) {
+    if constexpr (Tr::ESIZE == 2) return __builtin_amdgcn_exp2f(x);
+    const float root = __builtin_amdgcn_exp2f(0.5f * x);
+    return root * root;
+}
+
 // ---------------------------------------------------------------- outputs --
 // Accumulators acc[dt][r], feature 32 dt + 8 (r / 4) + 4 half + r % 4 of the
 // lane's row, times f, rounded once to the output's type; what that left goes to
@@ -590,7 +602,7 @@ struct RepairRow {
         return (((long long)w.b * w.p.queries + i) * w.p.heads + head) * w.p.dim * Tr::ESIZE;
     }
     __device__ __forceinline__ float weight(const Repair& w, const char* k, int j, float base, float& slope) const {
-        return __builtin_amdgcn_exp2f(score2<Tr, FORM>(w.p, row_dot<Tr>(q(w), k, w.p.dim), slope2, (float)(pos - j), base, slope));
+        return weight2<Tr>(score2<Tr, FORM>(w.p, row_dot<Tr>(q(w), k, w.p.dim), slope2, (float)(pos - j), base, slope));
     }
 };
 template <class Tr>
@@ -1192,7 +1204,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_d
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     float slope = 1.0f;
-                    const float pr = __builtin_amdgcn_exp2f(
+                    const float pr = weight2<Tr>(
                         score2<Tr, FORM>(p, s[e], slope2, away - (float)(mt * 32 + 8 * (e >> 2) + (e & 3)), -lse, slope));
                     float ds = pr * (g[e] - delta);
                     if (FORM >= kCap) ds *= slope;
@@ -1451,7 +1463,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
                 for (int e = 0; e < 4; ++e) {
                     const int x = 4 * q4 + e;
                     float slope = 1.0f;
-                    s[x] = __builtin_amdgcn_exp2f(
+                    s[x] = weight2<Tr>(
                         score2<Tr, FORM>(p, s[x], sloped ? sl[e] * 1.44269504f : 0.0f, ps[e] - keyf, shift - ls[e], slope));
                     if (!DK) continue;
                     g[x] = s[x] * (g[x] - de[e]);
