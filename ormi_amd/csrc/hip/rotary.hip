@@ -51,6 +51,7 @@ struct alignas(N * sizeof(typename Elem<DT>::type) >= 16 ? 16 : N * sizeof(typen
 };
 
 constexpr int HEADS = 4;
+constexpr long long kMostThreads = (1ll << 31) - 512;  // of a launch: they are counted in 31 bits
 
 // Every element is read once and written once, so where each access covers whole
 // 128-byte lines (runs of that many bytes) it goes past the caches, which stay
@@ -230,6 +231,8 @@ extern "C" int ormi_hip_rotary(const ormi_rotary_desc* d) {
     if (d->part > 0 && (!d->cos || !d->sin || d->table_rows == 0)) return bad("no tables");
     const long long tokens = (long long)d->batch * d->length;
     if (tokens >= (1ll << 31)) return bad("2^31 tokens or more");
+    // Threads of one token, at most a launch's (below): a pair of features of four heads each.
+    if (((long long)d->dim + 1) / 2 * (((long long)d->heads + HEADS - 1) / HEADS) > kMostThreads) return bad("heads * dim too large");
     int rc = ensure_init();
     if (rc != ORMI_HIP_OK || (rc = drain_queue()) != ORMI_HIP_OK) return rc;
 
@@ -272,8 +275,8 @@ extern "C" int ormi_hip_rotary(const ormi_rotary_desc* d) {
     divider(p.units, &p.units_m, &p.units_s);
     divider(p.groups, &p.groups_m, &p.groups_s);
     divider((unsigned)p.length, &p.length_m, &p.length_s);
-    // Threads are counted in 31 bits: a longer tensor goes in several launches.
-    const long long per_token = (long long)p.units * p.groups, most = std::max<long long>(1, ((1ll << 31) - 512) / per_token);
+    // A longer tensor goes in several launches.
+    const long long per_token = (long long)p.units * p.groups, most = kMostThreads / per_token;
     for (long long at = 0; at < tokens; at += most) {
         p.first = (unsigned)at;
         p.total = (unsigned)(std::min(most, tokens - at) * per_token);
