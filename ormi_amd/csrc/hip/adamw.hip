@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kMost = 32;      // tensors per launch: their entries and the scalars fit 4 KB of arguments
 constexpr int kPerGroup = 2048;  // elements per work-group: two groups of four per thread
+constexpr unsigned long long kMostGroups = (1ull << 24) - 1;  // of 256 threads: a launch holds fewer than 2^32
 
 struct AdamEntry {
     const void *p, *g, *m, *v;
@@ -271,7 +272,7 @@ int ormi_hip_adamw(const ormi_adamw_desc* d) {
     const bool small = d->state_bits == 8;
     for (int k = 0; k < d->num_tensors; ++k) {
         const ormi_adamw_tensor& t = d->tensors[k];
-        if (t.count < 0 || t.count >= (1ll << 40)) return bad("element count out of range");
+        if (t.count < 0 || t.count > (long long)kMostGroups * kPerGroup) return bad("element count out of range");
         if (!is_float(t.p_dtype) || !is_float(t.g_dtype)) return bad("p and g must be float32, bfloat16 or float16");
         if (t.count == 0) continue;
         if (!t.p || !t.g || !t.out || !t.m || !t.v || !t.m_out || !t.v_out) return bad("null tensor");
@@ -309,7 +310,7 @@ int ormi_hip_adamw(const ormi_adamw_desc* d) {
         const ormi_adamw_tensor& t = d->tensors[k];
         if (t.count == 0) continue;
         const unsigned long long need = (unsigned long long)(t.count + kPerGroup - 1) / kPerGroup;
-        if (a.n == kMost || groups + need >= (1ull << 31)) flush();
+        if (a.n == kMost || groups + need > kMostGroups) flush();
         AdamEntry& e = a.t[a.n++];
         e.p = t.p;
         e.g = t.g;
@@ -343,8 +344,11 @@ int ormi_hip_adamw_values(float* m, float* v, const void* m_codes, const float* 
     if (!m || !v || !m_codes || !m_scale || !v_codes || !v_scale) return fail(ORMI_HIP_ERR_INVALID, "ormi_hip_adamw_values: null pointer");
     int rc = ensure_init();
     if (rc != ORMI_HIP_OK || (rc = drain_queue()) != ORMI_HIP_OK) return rc;
-    adamw_values_kernel<<<(unsigned)((count + 1023) / 1024), 256>>>(m, v, (const unsigned*)m_codes, m_scale, (const unsigned*)v_codes,
-                                                                    v_scale, count);
+    for (int64_t at = 0, most = (int64_t)(kMostGroups / 4 * 4) * 1024; at < count; at += most) {  // whole blocks of codes
+        const int64_t n = std::min(most, count - at);
+        adamw_values_kernel<<<(unsigned)((n + 1023) / 1024), 256>>>(m + at, v + at, (const unsigned*)m_codes + at / 4, m_scale + at / ORMI_ADAMW_BLOCK,
+                                                                    (const unsigned*)v_codes + at / 4, v_scale + at / ORMI_ADAMW_BLOCK, n);
+    }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? ORMI_HIP_OK : fail(ORMI_HIP_ERR_RUNTIME, std::string("ormi_hip_adamw_values: ") + hipGetErrorString(e));
 }

@@ -12,7 +12,24 @@ class Rotary(ctypes.Structure):
 
 def test_rotary_refuses_tokens_of_more_threads_than_a_launch(cabi):
     """2^20 heads of 2^20 features: 2^37 threads for one token. The pointers are not touched."""
-    cabi.ormi_hip_rotary.argtypes = [ctypes.POINTER(Rotary)]
     for heads, dim in [(1 << 20, 1 << 20), ((1 << 31) - 1, (1 << 31) - 1), (1 << 16, 1 << 18)]:
         d = Rotary(0, 0, 1, 1, heads, dim, 0, 0, 0, 64, (ctypes.c_int64 * 4)(0, 0, dim, 1), 64, None, None, 0, None, (ctypes.c_int64 * 2)(), 0)
         assert cabi.ormi_hip_rotary(ctypes.byref(d)) == 3 and b"heads * dim" in cabi.ormi_hip_last_error()
+
+
+class AdamTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("p", "g", "out", "m", "v", "m_out", "v_out", "m_scale", "v_scale", "m_scale_out", "v_scale_out")] + [
+        ("count", ctypes.c_int64), ("p_dtype", ctypes.c_int), ("g_dtype", ctypes.c_int)]
+
+
+class Adam(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("tensors", ctypes.POINTER(AdamTensor)), ("bits", ctypes.c_int), ("step", ctypes.c_int64), ("lr", ctypes.c_double),
+                ("b1", ctypes.c_double), ("b2", ctypes.c_double), ("eps", ctypes.c_double), ("decay", ctypes.c_double)]
+
+
+def test_adamw_refuses_a_tensor_of_more_work_groups_than_a_launch(cabi):
+    """2^24 work-groups of 256 threads and 2048 elements are 2^32 threads. The pointers are not touched."""
+    for count in (((1 << 24) - 1) * 2048 + 1, 1 << 35, -1):
+        t = AdamTensor(*[64] * 11, count, 0, 0)
+        d = Adam(1, ctypes.pointer(t), 32, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0)
+        assert cabi.ormi_hip_adamw(ctypes.byref(d)) == 3 and b"count" in cabi.ormi_hip_last_error()
