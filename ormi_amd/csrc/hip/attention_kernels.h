@@ -1624,7 +1624,7 @@ constexpr int kDeltaGroups = 1024;
 template <class Tr, int DP>
 int launch_attention_grad_dp(const AttnParams& p, float* delta, unsigned* bounds) {
     const long long rows = (long long)p.batch * p.queries * p.heads, values = (long long)p.batch * p.keys * p.kv_heads;
-    unsigned row_groups = (unsigned)((rows + 15) / 16), value_groups = 0;
+    unsigned row_groups = (unsigned)std::min<long long>((rows + 15) / 16, 1 << 22), value_groups = 0;  // a launch holds fewer than 2^24 of 256 threads
     if (bounds) {
         const int heads = std::min(p.batch * p.kv_heads, 1 << 16), slices = std::max(1, kDeltaGroups / heads);
         row_groups = (unsigned)(heads * std::min((p.rows + 15) / 16, slices));

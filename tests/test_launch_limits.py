@@ -2,6 +2,9 @@
 launches that do, or refused before anything is read; none is cut short."""
 import ctypes
 
+import numpy as np
+import pytest
+
 
 class Rotary(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("batch", ctypes.c_int), ("length", ctypes.c_int), ("heads", ctypes.c_int),
@@ -33,3 +36,22 @@ def test_adamw_refuses_a_tensor_of_more_work_groups_than_a_launch(cabi):
         t = AdamTensor(*[64] * 11, count, 0, 0)
         d = Adam(1, ctypes.pointer(t), 32, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0)
         assert cabi.ormi_hip_adamw(ctypes.byref(d)) == 3 and b"count" in cabi.ormi_hip_last_error()
+
+
+@pytest.mark.gpu
+def test_the_gradient_of_more_rows_than_a_launch_takes(hip, ob):
+    """2^28 queries and more of one feature over one key: 16 rows to a work-group would be 2^32 threads. The key's
+    weight is 1, so dv is the number of rows and dq and dk are zero, all exactly."""
+    from ormi_amd import Tensor, attention, realize_all
+
+    rows = (1 << 28) + 64
+    one = lambda x, **more: Tensor(np.full((1, 1, 1, 1), x, np.float32), "hip", dtype="bfloat16", **more)  # noqa: E731
+    q, k, v = one(0.25, requires_grad=True), one(1.0, requires_grad=True), one(0.5, requires_grad=True)
+    many = q.expand((1, rows, 1, 1))
+    out = attention(many, k, v)
+    (out * one(1.0).expand((1, rows, 1, 1))).sum().backward()
+    size = (many.grad * many.grad).sum()
+    realize_all(size, k.grad, v.grad)
+    assert float(v.grad.numpy()[0, 0, 0, 0]) == 2.0 ** 28 and float(k.grad.numpy()[0, 0, 0, 0]) == 0.0 and float(size.numpy()) == 0.0
+    del many, out, size, q, k, v
+    ob.empty_cache()
