@@ -6,7 +6,7 @@ Training: products -> rotary positions (stored as bfloat16) -> causal attention
 with shared key heads -> product -> mean square error, its gradients through all
 of them, and an AdamW step over the four weights. Then the same weights answer
 one token at a time: each token's query is turned by its own position and attends
-the keys that stand before it, which gives the rows that the whole sequence gives.
+the keys up to it, which gives the rows that the whole sequence gives.
 """
 from __future__ import annotations
 
@@ -72,7 +72,11 @@ def train(block: AttentionBlock, x: np.ndarray, target: np.ndarray, steps: int, 
 
 
 def token_by_token(block: AttentionBlock, x: np.ndarray) -> np.ndarray:
-    """The block's rows, one query at a time over the tokens' keys and values."""
+    """The block's rows, one query at a time over the tokens' keys and values.
+
+    Tensors are not written after they are made and the graph has no op that extends
+    one, so all keys and values are made first; lengths hides those after the token.
+    """
     batch, length, _ = x.shape
     k, v = block.keys_values(Tensor(x, "hip"))
     k.realize(), v.realize()

@@ -441,7 +441,17 @@ int ormi_hip_rotary(const ormi_rotary_desc* desc);
  * others' rows, nor one in a query's row the gradients of keys it does not see.
  * q, k, v are strided views; out is contiguous. dtype is F32, BF16 or F16;
  * scores, sums and the softmax are fp32, out is rounded once. 16-bit
- * probabilities are rounded to 16 bits for their product with v.
+ * probabilities are rounded to 16 bits for their product with v (that of dout
+ * in the gradient), and score gradients for theirs with k and q: the matrix
+ * instructions' operands. What that leaves is added for one tile of keys of a
+ * row (of rows of a key), all there is of short ones, and forward always for up
+ * to 32 rows of a key head; over long rows it averages out, at up to 1.4 times
+ * the error of rounding the results alone. F32 has no such roundings. Weights below 2^-126
+ * of their row's sum count as zero, but for the F32 gradient. A query whose
+ * every score is minus infinity counts as one that sees no key.
+ * Rows that end up not finite because of what others see, or of an infinity
+ * among values that they see, are added up again one key at a time: right, but
+ * hundreds of times slower than the rest, as is a gradient's key.
  * rest (or NULL; not read or written for F32) receives what out's rounding to
  * 16 bits left, itself rounded to them: the gradient is more exact with it.
  * lse (or NULL) receives log2 of each row's sum of exponentials, (batch,

@@ -181,7 +181,10 @@ struct Tile {
         return *(const lds_float*)(t + at(row0) + at(row) + (((d >> 2) ^ swz(row)) << 4) + (d & 3) * 4);
     }
     // acc[dt] += (the tile's rows row0.. turned) x (accumulator `a` as 16- or 32-bit
-    // operand); SUM: sum += its columns' sums, by a product with ones.
+    // operand); SUM: sum += its columns' sums, by a product with ones. The matrix
+    // instruction takes 16-bit operands, so weights and score gradients are rounded here;
+    // a second product with what that leaves (leave_rest) would cost as much again, and is
+    // made where it counts: one tile of a row or key, and all of them where memory bounds.
     template <bool SUM = false>
     __device__ __forceinline__ static void second(const lds_char* t, int row0, const f32x16_t& a, f32x16_t (&acc)[DT], f32x16_t* sum = nullptr) {
         if constexpr (ES == 2) {
@@ -651,13 +654,12 @@ __device__ __forceinline__ void put_part(float* row, const float (&sum)[4], floa
 // ---------------------------------------------------------------- forward --
 // NW waves of 32 rows; BN keys per tile. Many rows: four waves share the tiles in LDS,
 // bound by the matrix pipes with the exponentials beside them (causal, bf16, 2 x 4096
-// tokens x 16 heads of 128 on 4 key heads: 187 us, 735 TF; 12 heads of 64 over 8191
-// keys with slopes: 266 us, 770 TF, the exponentials nearly as long as the products).
+// tokens x 16 heads of 128 on 4 key heads: 161 us, 854 TF; 12 heads of 64 over 8191
+// keys with slopes: 254 us, 814 TF, the exponentials nearly as long as the products).
 // Up to 32 rows: one wave, keys split over the chip, bound by reading them (16 single
 // tokens over up to 8192 keys x 8 heads of 128: 62 us, 5.4 TB/s of those that exist).
-// Up to 96 features three groups of waves share
-// a CU, whatever that spills (8191 x 12 heads of 64 with slopes: 266 us, with two 372; the
-// compiler alone takes two).
+// Up to 96 features three groups of waves share a CU, whatever that spills (with two, as
+// the compiler alone would have it, those 12 heads of 64 take 1.4 times as long).
 template <class Tr, int DP, int NW, int BN, int FORM>
 __global__ __launch_bounds__(64 * NW, DP * Tr::ESIZE > 512 || DP > 128 ? 1 : NW == 4 && DP * Tr::ESIZE <= 192 ? 3 : 2) void attention_fwd_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
@@ -1099,7 +1101,7 @@ __device__ __forceinline__ float grad_hold(const AttnParams& p, int bh) {
 // dq. Rows, tiles and masks as in the forward kernel, with both products of a
 // tile's keys and values against the row's q and dout; the score gradients then
 // meet the keys again, turned. Bound by the matrix pipes (2 x 4096 tokens x 16 heads
-// of 128, causal: 232 us, 890 TF; the same without a mask, longer: 1050 TF).
+// of 128, causal: 207 us, 996 TF; 8192 tokens without a mask: 1158 TF).
 template <class Tr, int DP, int BN, int FORM>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 384 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
     using T = Tile<Tr, DP>;
@@ -1299,8 +1301,8 @@ constexpr bool values_in_lds(int dp, int es) { return dp * es >= 256 && dp * es 
 // (rows of 256 features leave the registers for one at a time; both at once
 // spilled 208 of them and took 1911 us where two launches take 807, 4096 x 16 heads).
 // Bound by the matrix pipes and, with both operands of three products in LDS, by its
-// reads: 2 x 4096 tokens x 16 heads of 128, causal, 375 us, 735 TF (no mask, longer:
-// 860 TF). 8192 tokens in 24 documents with capped scores, 8 heads: 190 us; its 512
+// reads: 2 x 4096 tokens x 16 heads of 128, causal, 305 us, 901 TF (8192 tokens without a
+// mask: 1035 TF). 8192 tokens in 24 documents with capped scores, 8 heads: 186 us; its 512
 // work-groups all run at once and end when those of the longest documents do.
 template <class Tr, int DP, int FORM, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
@@ -1568,7 +1570,8 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
 }
 
 // Adds the splits' partial gradients in split order, one wave per row: first dq's
-// rows, then each key's dk and dv. Bound by memory and its waits (84 MB in 26 us).
+// rows, then each key's dk and dv. Bound by memory (four splits of
+// 8 x 4096 keys of 128 features: 134 MB read and 17 written in 25 us).
 template <class Tr, int DP>
 __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttnParams p) {
     const long long nq = p.dq && p.splits > 1 ? (long long)p.batch * p.kv_heads * p.rows : 0;

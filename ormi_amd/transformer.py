@@ -111,6 +111,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, scale: f
       lengths    int32 (batch,): keys that exist (keys); the others do not count, whatever they hold
     A query that sees no key gives zeros. The result and the gradients have q's
     type (float32, bfloat16 or float16); gradients of shared key heads add up.
+    Scores and sums are float32. In the 16-bit types the gradient that comes in is
+    rounded to the type, and so are weights and score gradients for their products.
     """
     for t, what in ((k, "k"), (v, "v")):
         _node(t, q, what)
