@@ -1327,7 +1327,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
     const int doc = p.docs && key < span.end ? doc_at(p, b, key) : -1;
     const int first_doc = p.docs ? __builtin_amdgcn_readfirstlane(doc) : 0;
     const bool one_doc = p.docs && __all(doc == first_doc) && first_doc >= 0;
-    const float keyf = (float)key;
+    const float keyf = (float)(key - k0);  // with row_pos: positions from k0 on, so that near ones are exact past 2^24
     const bool sloped = FORM != kPlain && p.slopes;
     const int key_live = p.docs && doc < 0 ? 0x7fffffff : key;  // a key without a document is seen by no row
     const float hold = grad_hold<Tr>(p, bh), shift = Shift<Tr>::bwd;
@@ -1404,7 +1404,7 @@ __global__ __launch_bounds__(256, DP * Tr::ESIZE > 256 ? 1 : 2) void attention_d
                                                      : (const int*)p.slopes);
             if (half == 0) {
                 row_lim[stage][lane] = r0 + lane >= p.rows || (p.docs && pos < 0) ? 0 : span.limit(p, pos);
-                if (FORM != kPlain) row_pos[stage][lane] = (float)pos;
+                if (FORM != kPlain) row_pos[stage][lane] = (float)(pos - k0);
             }
         }
     };

@@ -4,7 +4,8 @@ and with key lengths, slopes steep enough for tiles without any weight."""
 import numpy as np
 import pytest
 
-from test_attention import DTYPES, check, make, packed
+from attention_ref import assert_within, attention as ref
+from test_attention import DTYPES, check, make, packed, rounded
 
 
 def few_long(b, keys, cuts, tail=0):
@@ -73,3 +74,33 @@ def test_steep_slopes(hip, dtype, causal, queries, keys, heads, lengths):
 def test_steep_slopes_and_documents(hip, dtype):
     docs = few_long(1, 1300, [[500, 505]], tail=20)
     check(make(1, 700, 1300, 2, 2, 96, seed=8, causal=True, documents=docs, slopes=np.float32([3.0, 0.5])), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_slopes_past_two_to_the_24(hip, dtype):
+    """Positions that float32 does not hold: distances are exact all the same. The weights reach back some 300
+    keys; of the keys before the last 1024 the gradients are zero."""
+    from ormi_amd import Tensor, attention, realize_all
+
+    keys, near = (1 << 24) + 1041, 1024
+    slopes = np.float32([0.5, 1.0])
+    c = make(1, 5, near, 2, 1, 8, seed=3)
+    data = {n: rounded(c[n], dtype) for n in "qkv"}
+    w = rounded(np.random.default_rng(4).standard_normal(c["q"].shape, dtype=np.float32), dtype)
+    want = ref(data["q"], data["k"], data["v"], w, dtype=dtype, causal=True, slopes=slopes)
+    t = {}
+    for n in "kv":
+        whole = np.zeros((1, keys, 1, 8), np.float32)
+        whole[:, keys - near:] = data[n]
+        t[n] = Tensor(whole, "hip", requires_grad=True, dtype=dtype)
+    q = Tensor(data["q"], "hip", requires_grad=True, dtype=dtype)
+    out = attention(q, t["k"], t["v"], causal=True, slopes=Tensor(slopes, "hip"))
+    (out * Tensor(w, "hip", dtype=dtype)).sum().backward()
+    realize_all(out, q.grad, t["k"].grad, t["v"].grad)
+    assert_within(out.numpy(), want["out"], "out")
+    assert_within(q.grad.numpy(), want["dq"], "dq")
+    for n in "kv":
+        g = t[n].grad.numpy()
+        assert_within(g[:, keys - near:], want["d" + n], "d" + n)
+        assert not g[:, : keys - near].any(), n
