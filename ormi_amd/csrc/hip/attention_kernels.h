@@ -501,7 +501,10 @@ __device__ __forceinline__ void store_part(float* row, const f32x16_t (&acc)[DT]
 // stands there is a NaN in the matrix products. Rows (and keys) that end up not
 // finite though their own sums are finite are therefore added up again, in plain
 // order and over what they see alone; nothing else pays for it but one look at
-// the accumulators. One row at a time, the wave's lanes along the features.
+// the accumulators. One row at a time, the wave's lanes along the features, about
+// 1 us for each key: an infinite value in the tile that all rows of 2 x 4096 causal
+// tokens, 16 heads of 128, begin with takes 128 ms instead of 0.2, one in a row of
+// dout 116 ms instead of 0.7.
 template <class Tr>
 __device__ __forceinline__ float load1(const char* row, int d) {
     if constexpr (Tr::ESIZE == 4) return ((const float*)row)[d];
