@@ -549,6 +549,147 @@ int ormi_hip_adamw(const ormi_adamw_desc* desc);
 int ormi_hip_adamw_values(float* m, float* v, const void* m_codes, const float* m_scale, const void* v_codes,
                           const float* v_scale, int64_t count);
 
+/* ---------------------------------------------------------- recurrence --
+ * Gated linear recurrence over the tokens of each batch and channel (no
+ * counterpart in the reference, whose graphs would take a node per token):
+ *   h_t = a_t h_{t-1} + b_t,  out_t = h_t,  h_{-1} = initial (0 when NULL)
+ *   logits 0: a = g, b = x;   logits 1: a = 1 / (1 + e^-g), b = (1 - a) x
+ * g is gates, (batch, length, channels) like x and out. gates and x are views
+ * whose channels are neighbours (strides over batch and tokens); out is
+ * contiguous. dtype: F32, BF16 or F16, of x and out; gates have it or are F32.
+ * The state starts from nothing at a token whose documents entry differs from
+ * the token's before it; tokens of a negative document give zeros and leave a
+ * state of zeros. Tokens from lengths[b] on (clamped to [0, length]) give zeros and leave the
+ * state as it is. What stands at such tokens is not read, and nothing from
+ * before a restart, infinity or NaN, reaches what is after it.
+ * last (or NULL) receives the state after the last token, (batch, channels).
+ * States, gates and products of gates are fp32, results are rounded once.
+ * Spans of tokens are joined by the products of their gates, so gates whose
+ * product over some span passes 2^128 (none up to magnitude 1 does) give
+ * results that are not finite; an infinite state may become NaN.
+ * states (or NULL) receives the state before every ORMI_RECURRENCE_TILE-th
+ * token, (batch, ceil(length / tile), channels) fp32: the gradient needs it.
+ * workspace: device memory of *_workspace_size() bytes, 256-byte aligned (NULL
+ * where that is 0), for this call and for the gradient's. Lengths go up to 2^30.
+ * Sums have a fixed order: the same call gives the same bits. */
+#define ORMI_RECURRENCE_TILE 128
+typedef struct ormi_recurrence_desc {
+    int            dtype, gate_dtype;
+    int            batch, length, channels;
+    int            logits;
+    const void*    gates;
+    int64_t        gate_strides[2];                 /* batch, token; elements */
+    const void*    x;
+    int64_t        x_strides[2];
+    const float*   initial;                         /* (batch, channels), or NULL */
+    const int32_t* documents;                       /* (batch, length), or NULL */
+    int64_t        documents_batch_stride;          /* elements; the tokens are contiguous */
+    const int32_t* lengths;                         /* (batch), or NULL */
+    void*          out;
+    float*         last;
+    float*         states;
+    void*          workspace;
+    size_t         workspace_bytes;
+} ormi_recurrence_desc;
+int ormi_hip_recurrence_workspace_size(const ormi_recurrence_desc* desc, size_t* bytes);
+int ormi_hip_recurrence(const ormi_recurrence_desc* desc);
+
+/* The gradient of ormi_hip_recurrence with respect to gates, x and initial.
+ * forward describes the call that was made, with its states (out and last are
+ * not read). dout (or NULL: zeros) is a view like x, of x's type or F32, dlast (or NULL) the
+ * gradient of last. dgates and dx are contiguous, of the types of gates and x;
+ * dinitial is fp32 (NULL: not wanted). */
+typedef struct ormi_recurrence_grad_desc {
+    ormi_recurrence_desc forward;
+    int                  dout_dtype;
+    const void*          dout;
+    int64_t              dout_strides[2];
+    const float*         dlast;                     /* (batch, channels), or NULL */
+    void*                dgates;
+    void*                dx;
+    float*               dinitial;
+} ormi_recurrence_grad_desc;
+int ormi_hip_recurrence_grad(const ormi_recurrence_grad_desc* desc);
+
+/* --------------------------------------------------- causal convolution --
+ * A short convolution of each channel over the tokens of its batch (no
+ * counterpart in the reference):
+ *   z_t = bias + sum_j weight[j] x_{t - width + 1 + j},  j = 0 .. width - 1
+ *   out_t = z_t, or with silu z_t / (1 + e^-z_t)
+ * x and out are (batch, length, channels), x a view whose channels are
+ * neighbours, out contiguous; weight (channels, width) and bias (channels) are
+ * fp32. initial holds the inputs x_{1 - width} .. x_{-1} (zeros when NULL),
+ * (batch, width - 1, channels), contiguous, of x's type. width: 1 to
+ * ORMI_CONV_MAX_WIDTH. dtype: F32, BF16 or F16.
+ * A token reads its own document's inputs: none from before the last token
+ * where the documents entry changed (initial belongs to the first token's);
+ * tokens of a negative document give zeros. Tokens from lengths[b] on (clamped
+ * to [0, length]) give zeros. What stands at such tokens is not read, and none
+ * of it, infinity or NaN, reaches other documents' results.
+ * last (or NULL) receives the inputs that a token after the last one that
+ * counts would read if it went on with its document, laid out like initial
+ * (zeros after a token of a negative document).
+ * Sums are fp32 in a fixed order, results are rounded once. */
+#define ORMI_CONV_MAX_WIDTH 8
+typedef struct ormi_conv_desc {
+    int            dtype;
+    int            batch, length, channels, width;
+    int            silu;
+    const void*    x;
+    int64_t        x_strides[2];                    /* batch, token; elements */
+    const float*   weight;
+    const float*   bias;                            /* or NULL */
+    const void*    initial;                         /* or NULL */
+    const int32_t* documents;                       /* (batch, length), or NULL */
+    int64_t        documents_batch_stride;
+    const int32_t* lengths;                         /* (batch), or NULL */
+    void*          out;
+    void*          last;
+} ormi_conv_desc;
+int ormi_hip_conv(const ormi_conv_desc* desc);
+
+/* The gradient of ormi_hip_conv. forward describes the call that was made (out
+ * and last are not read). dout (or NULL: zeros) is a view like x, of x's type
+ * or F32; dlast (or NULL) is fp32, laid out like last. dx and dinitial have x's
+ * type, dweight and dbias are fp32; all contiguous, NULL: not wanted.
+ * workspace as above, of ormi_hip_conv_grad_workspace_size() bytes. */
+typedef struct ormi_conv_grad_desc {
+    ormi_conv_desc forward;
+    int            dout_dtype;
+    const void*    dout;
+    int64_t        dout_strides[2];
+    const float*   dlast;
+    void*          dx;
+    float*         dweight;
+    float*         dbias;
+    void*          dinitial;
+    void*          workspace;
+    size_t         workspace_bytes;
+} ormi_conv_grad_desc;
+int ormi_hip_conv_grad_workspace_size(const ormi_conv_grad_desc* desc, size_t* bytes);
+int ormi_hip_conv_grad(const ormi_conv_grad_desc* desc);
+
+/* ------------------------------------------------------ gradient clipping --
+ * The norm over a list of tensors, and their values times a factor (no
+ * counterpart in the reference). Tensors are contiguous, F32, BF16 or F16, and
+ * any number of them.
+ *   norm = sqrt(sum of all squares), factor = min(1, max_norm / norm)
+ * in 64 bits, in a fixed order, each rounded to fp32 once (either may be NULL). A norm that is
+ * NaN makes the factor NaN, an infinite one makes it 0. workspace as above. */
+typedef struct ormi_tensor_ref {
+    const void* data;
+    void*       out;                                /* ormi_hip_scale: of data's type; may be data */
+    int64_t     count;
+    int         dtype;
+} ormi_tensor_ref;
+int ormi_hip_norm_workspace_size(const ormi_tensor_ref* tensors, int num_tensors, size_t* bytes);
+int ormi_hip_norm(const ormi_tensor_ref* tensors, int num_tensors, double max_norm, float* norm, float* factor,
+                  void* workspace, size_t workspace_bytes);
+/* out = data * factor[0] in fp32, rounded once. */
+int ormi_hip_scale(const ormi_tensor_ref* tensors, int num_tensors, const float* factor);
+/* ormi_hip_adamw with every gradient times factor[0] (fp32, on the device). */
+int ormi_hip_adamw_scaled(const ormi_adamw_desc* desc, const float* factor);
+
 /* ---------------------------------------------------------------- timing --
  * HIP events on the library's stream, for measuring kernel time from
  * outside (benchmarks). */

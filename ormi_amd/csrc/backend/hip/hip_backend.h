@@ -95,9 +95,15 @@ namespace ormi::hip {
         long long step = 1;
         double lr = 1e-3, beta1 = 0.9, beta2 = 0.999, eps = 1e-8, weight_decay = 0.01;
         int bits = 32;
+        NodePtr factor;  // of every gradient, a float32 scalar; null: none
     };
     void adamw(const std::vector<NodePtr>& params, const std::vector<NodePtr>& grads, const std::vector<std::vector<NodePtr>>& states,
                const AdamWOptions& options, std::vector<NodePtr>* new_params, std::vector<std::vector<NodePtr>>* new_states);
+    // The norm over all gradients' elements and min(1, max_norm / norm), float32
+    // scalars on the device.
+    std::pair<NodePtr, NodePtr> grad_norm(const std::vector<NodePtr>& grads, double max_norm);
+    // Each gradient times the factor, new buffers of its type.
+    std::vector<NodePtr> scale_grads(const std::vector<NodePtr>& grads, const NodePtr& factor);
     // The float32 moments that 8-bit states stand for, of the given shape.
     std::pair<NodePtr, NodePtr> adamw_values(const std::vector<NodePtr>& state, const std::vector<int>& shape);
 

@@ -5,8 +5,7 @@
 #include <string>
 #include <vector>
 
-#include "backend/hip/hip_backend.h"
-#include "core/memory.h"
+#include "backend/hip/operands.h"
 #include "core/shape.h"
 #include "ormi_hip.h"
 #include "runtime/graph_breakers.h"
@@ -14,7 +13,7 @@
 namespace ormi::hip {
     using ops::OpEnum;
 
-    static int abi_dtype(DType d) {
+    int abi_dtype(DType d) {
         switch (d) {
             case DType::Float32: return ORMI_DTYPE_F32;
             case DType::BFloat16: return ORMI_DTYPE_BF16;
@@ -29,9 +28,7 @@ namespace ormi::hip {
 
     static bool is_integer(DType d) { return d == DType::Int32 || d == DType::Int64 || d == DType::Bool; }
 
-    // n's values in a contiguous buffer: n's own, or a copy, by the map kernel where
-    // its float32 holds them and bit for bit where they are integers.
-    static NodePtr contiguous(const NodePtr& n) {
+    NodePtr contiguous(const NodePtr& n) {
         realize(n);
         const auto& shape = n->view.shape;
         if (n->view.strides == calc_contiguous_strides(shape) && (long long)n->data->numel() == shape_numel(shape)) return n;
@@ -48,19 +45,20 @@ namespace ormi::hip {
 
     // In rows of 256 bytes, what the entries' sizes are multiples of: packed operands
     // alone can pass the 2^31 elements of one extent.
-    static std::shared_ptr<Buffer> workspace(size_t bytes) {
-        return bytes ? empty({checked_extent((long long)((bytes + 255) / 256), "attention: workspace"), 64}, DeviceEnum::HIP) : nullptr;
+    std::shared_ptr<Buffer> workspace(size_t bytes) {
+        return bytes ? empty({checked_extent((long long)((bytes + 255) / 256), "workspace"), 64}, DeviceEnum::HIP) : nullptr;
     }
 
     // ----------------------------------------------------------- gradients --
     int gradient_parent(const Node& n) {
         if (n.op == OpEnum::ATTENTION_GRAD) return 1;
+        if (n.op == OpEnum::RECURRENCE_GRAD || n.op == OpEnum::CONV_GRAD) return std::get<SequenceAttrs>(n.attrs).dout ? 1 : -1;
         return n.op == OpEnum::ROTARY && std::get<RotaryAttrs>(n.attrs).inverse ? 0 : -1;
     }
     DType gradient_dtype(const Node& n) {
         // A rotation back reads the gradient as it comes; where that is a product
         // with the seed, as what the product holds.
-        return n.op == OpEnum::ATTENTION_GRAD ? n.parents[0]->dtype : std::get<RotaryAttrs>(n.attrs).upstream;
+        return n.op != OpEnum::ROTARY ? n.parents[0]->dtype : std::get<RotaryAttrs>(n.attrs).upstream;
     }
 
     // -------------------------------------------------------------- rotary --
@@ -220,6 +218,8 @@ namespace ormi::hip {
                const AdamWOptions& o, std::vector<NodePtr>* new_params, std::vector<std::vector<NodePtr>>* new_states) {
         require(params.size() == grads.size() && params.size() == states.size(), "as many gradients and states as parameters, please.");
         require(o.bits == 32 || o.bits == 8, "states have 32 or 8 bits.");
+        require(!o.factor || (o.factor->device.type == DeviceEnum::HIP && o.factor->dtype == DType::Float32 && shape_numel(o.factor->view.shape) == 1),
+                "the gradients' factor is a float32 scalar on the hip device.");
         for (size_t i = 0; i < params.size(); ++i) {
             const NodePtr &p = params[i], &g = grads[i];
             require(p && g, "a null tensor.");
@@ -275,7 +275,57 @@ namespace ormi::hip {
         d.beta2 = o.beta2;
         d.eps = o.eps;
         d.weight_decay = o.weight_decay;
-        ORMI_HIP_CHECK(ormi_hip_adamw(&d));
+        if (o.factor) ORMI_HIP_CHECK(ormi_hip_adamw_scaled(&d, (const float*)in(o.factor)));
+        else ORMI_HIP_CHECK(ormi_hip_adamw(&d));
+    }
+
+    // ------------------------------------------------------------ clipping --
+    // The gradients, realized together, as the entries take them.
+    static std::vector<ormi_tensor_ref> tensor_refs(const std::vector<NodePtr>& grads, std::vector<NodePtr>& hold) {
+        for (const auto& g : grads) {
+            if (!g) throw std::runtime_error("clipping: a null tensor.");
+            if (g->device.type != DeviceEnum::HIP) throw std::runtime_error("clipping: gradients live on the hip device.");
+            abi_dtype(g->dtype);
+        }
+        realize_group(grads);
+        std::vector<ormi_tensor_ref> list;
+        list.reserve(grads.size());
+        for (const auto& g : grads) {
+            hold.push_back(contiguous(g));
+            ormi_tensor_ref t{};
+            t.data = hold.back()->data->ptr;
+            t.count = shape_numel(g->view.shape);
+            t.dtype = abi_dtype(hold.back()->data->dtype);
+            list.push_back(t);
+        }
+        return list;
+    }
+
+    std::pair<NodePtr, NodePtr> grad_norm(const std::vector<NodePtr>& grads, double max_norm) {
+        std::vector<NodePtr> hold;
+        const auto list = tensor_refs(grads, hold);
+        const Device dev = grads.empty() ? Device(DeviceEnum::HIP) : grads[0]->device;
+        auto norm = state_leaf({}, DType::Float32, dev), factor = state_leaf({}, DType::Float32, dev);
+        size_t bytes = 0;
+        ORMI_HIP_CHECK(ormi_hip_norm_workspace_size(list.data(), (int)list.size(), &bytes));
+        const auto ws = workspace(bytes);
+        ORMI_HIP_CHECK(ormi_hip_norm(list.data(), (int)list.size(), max_norm, (float*)norm->data->ptr, (float*)factor->data->ptr, ws ? ws->ptr : nullptr,
+                                     ws ? ws->bytes : 0));
+        return {norm, factor};
+    }
+
+    std::vector<NodePtr> scale_grads(const std::vector<NodePtr>& grads, const NodePtr& factor) {
+        if (!factor || factor->device.type != DeviceEnum::HIP || factor->dtype != DType::Float32 || shape_numel(factor->view.shape) != 1)
+            throw std::runtime_error("clipping: the factor is a float32 scalar on the hip device.");
+        std::vector<NodePtr> hold, out;
+        auto list = tensor_refs(grads, hold);
+        realize(factor);
+        for (size_t i = 0; i < list.size(); ++i) {
+            out.push_back(state_leaf(grads[i]->view.shape, hold[i]->data->dtype, grads[i]->device));
+            list[i].out = out.back()->data->ptr;
+        }
+        ORMI_HIP_CHECK(ormi_hip_scale(list.data(), (int)list.size(), (const float*)factor->data->ptr));
+        return out;
     }
 
     std::pair<NodePtr, NodePtr> adamw_values(const std::vector<NodePtr>& state, const std::vector<int>& shape) {

@@ -270,7 +270,7 @@ PYBIND11_MODULE(ormi_backend, m) {
 
     {
         auto e = py::enum_<ops::OpEnum>(m, "OpEnum");
-        for (int i = (int)ops::OpEnum::LEAF; i <= (int)ops::OpEnum::ATTENTION_GRAD; ++i) {
+        for (int i = (int)ops::OpEnum::LEAF; i <= (int)ops::OpEnum::LAST_STATE_GRAD; ++i) {
             auto op = (ops::OpEnum)i;
             e.value(ops::op_name(op), op);
         }
@@ -365,9 +365,20 @@ PYBIND11_MODULE(ormi_backend, m) {
     }, py::arg("x"), py::arg("cos"), py::arg("sin"), py::arg("positions").none(true), py::arg("offset"), py::arg("interleaved"), py::arg("dtype"));
     m.def("attention", &ops::attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("cap"), py::arg("causal"),
           py::arg("slopes").none(true), py::arg("documents").none(true), py::arg("prefix").none(true), py::arg("lengths").none(true));
+    m.def("recurrence", [](std::shared_ptr<Node> gates, std::shared_ptr<Node> x, std::shared_ptr<Node> initial, std::shared_ptr<Node> documents,
+                           std::shared_ptr<Node> lengths, bool logits) {
+        const auto n = ops::recurrence(gates, x, initial, documents, lengths, logits);
+        return py::make_tuple(ops::sequence_out(n), ops::last_state(n));
+    }, py::arg("gates"), py::arg("x"), py::arg("initial").none(true), py::arg("documents").none(true), py::arg("lengths").none(true), py::arg("logits"));
+    m.def("conv", [](std::shared_ptr<Node> x, std::shared_ptr<Node> weight, std::shared_ptr<Node> bias, std::shared_ptr<Node> initial,
+                     std::shared_ptr<Node> documents, std::shared_ptr<Node> lengths, bool silu) {
+        const auto n = ops::conv(x, weight, bias, initial, documents, lengths, silu);
+        return py::make_tuple(ops::sequence_out(n), ops::last_state(n));
+    }, py::arg("x"), py::arg("weight"), py::arg("bias").none(true), py::arg("initial").none(true), py::arg("documents").none(true),
+       py::arg("lengths").none(true), py::arg("silu"));
     m.def("adamw", [](const std::vector<std::shared_ptr<Node>>& params, const std::vector<std::shared_ptr<Node>>& grads,
                       const std::vector<std::vector<std::shared_ptr<Node>>>& states, int bits, long long step, double lr, double beta1,
-                      double beta2, double eps, double weight_decay) {
+                      double beta2, double eps, double weight_decay, std::shared_ptr<Node> factor) {
         hip::AdamWOptions o;
         o.bits = bits;
         o.step = step;
@@ -376,12 +387,18 @@ PYBIND11_MODULE(ormi_backend, m) {
         o.beta2 = beta2;
         o.eps = eps;
         o.weight_decay = weight_decay;
+        o.factor = factor;
         std::vector<std::shared_ptr<Node>> p;
         std::vector<std::vector<std::shared_ptr<Node>>> s;
         hip::adamw(params, grads, states, o, &p, &s);
         return py::make_tuple(p, s);
     }, py::arg("params"), py::arg("grads"), py::arg("states"), py::arg("bits"), py::arg("step"), py::arg("lr"), py::arg("beta1"),
-       py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"));
+       py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("factor").none(true) = py::none());
+    m.def("grad_norm", [](const std::vector<std::shared_ptr<Node>>& grads, double max_norm) {
+        const auto r = hip::grad_norm(grads, max_norm);
+        return py::make_tuple(r.first, r.second);
+    }, py::arg("grads"), py::arg("max_norm"));
+    m.def("scale_grads", &hip::scale_grads, py::arg("grads"), py::arg("factor"));
     m.def("adamw_values", &hip::adamw_values);
 
     m.def("execute_graph", &execute_graph);

@@ -51,5 +51,34 @@ namespace ormi {
         int which = 0;             // ATTENTION_GRAD: 0 q, 1 k, 2 v
     };
 
-    using OpAttributes = std::variant<NoAttrs, ReduceAttrs, PermuteAttrs, ReshapeAttrs, ExpandAttrs, CastAttrs, RotaryAttrs, AttentionAttrs>;
+    // RECURRENCE: parents gates, x, then those of initial, documents and lengths
+    // that are set. CONV: parents x, weight, then those of bias, initial, documents
+    // and lengths that are set. A graph reads either through SEQUENCE_OUT, a view of
+    // its result, and LAST_STATE, the state it leaves, so that each has a gradient of
+    // its own; LAST_STATE_GRAD is the latter's, of the result's shape only to be
+    // added to the former's. The gradients: the node,
+    // its result's gradient and its last state's (those that are set), and the
+    // node's parents.
+    struct SequenceAttrs {
+        int width = 0;             // of a convolution; 0: a recurrence
+        bool logits = false;       // recurrence: gates are logits
+        bool silu = false;         // convolution
+        bool bias = false, initial = false, documents = false, lengths = false;
+        std::vector<int> shape;    // of the result
+        // What realizing the node leaves: the state after the last token, and for a
+        // recurrence's gradient those before its tiles.
+        struct Saved { std::shared_ptr<Buffer> last, states; };
+        std::shared_ptr<Saved> saved;
+        // As of an attention's gradients.
+        struct Grads {
+            bool want[4] = {false, false, false, false};
+            std::shared_ptr<Buffer> made[4];
+        };
+        std::shared_ptr<Grads> grads;
+        int which = 0;             // gradients: the node's parent that it belongs to
+        bool dout = false, dlast = false;
+        int first() const { return 1 + dout + dlast; }  // where a gradient's parents hold the node's
+    };
+
+    using OpAttributes = std::variant<NoAttrs, ReduceAttrs, PermuteAttrs, ReshapeAttrs, ExpandAttrs, CastAttrs, RotaryAttrs, AttentionAttrs, SequenceAttrs>;
 }

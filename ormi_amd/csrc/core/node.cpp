@@ -15,12 +15,20 @@ namespace ormi {
 
     static DType result_dtype(ops::OpEnum op, const std::vector<std::shared_ptr<Node>>& parents, const OpAttributes& attrs) {
         switch (op) {
-            case ops::OpEnum::TRANSPOSE: case ops::OpEnum::RESHAPE: case ops::OpEnum::EXPAND:
+            case ops::OpEnum::TRANSPOSE: case ops::OpEnum::RESHAPE: case ops::OpEnum::EXPAND: case ops::OpEnum::SEQUENCE_OUT:
                 return parents.empty() ? DType::Float32 : parents[0]->dtype;
             case ops::OpEnum::CAST: return std::get<CastAttrs>(attrs).dtype;
             case ops::OpEnum::ROTARY: return std::get<RotaryAttrs>(attrs).dtype;
             case ops::OpEnum::ATTENTION: return parents[0]->dtype;
             case ops::OpEnum::ATTENTION_GRAD: return parents[2 + std::get<AttentionAttrs>(attrs).which]->dtype;
+            case ops::OpEnum::RECURRENCE: return parents[1]->dtype;
+            case ops::OpEnum::CONV: return parents[0]->dtype;
+            case ops::OpEnum::RECURRENCE_GRAD: case ops::OpEnum::CONV_GRAD: {
+                const auto& a = std::get<SequenceAttrs>(attrs);
+                return parents[a.first() + a.which]->dtype;
+            }
+            // The states of a recurrence are float32, those of a convolution its inputs.
+            case ops::OpEnum::LAST_STATE: return std::get<SequenceAttrs>(attrs).width ? parents[0]->dtype : DType::Float32;
             case ops::OpEnum::ARGMAX: return DType::Int64;
             default: return DType::Float32;
         }

@@ -19,6 +19,10 @@ namespace ormi::ops {
             case OpEnum::EQ: return "EQ"; case OpEnum::CAST: return "CAST";
             case OpEnum::ROTARY: return "ROTARY"; case OpEnum::ATTENTION: return "ATTENTION";
             case OpEnum::ATTENTION_GRAD: return "ATTENTION_GRAD";
+            case OpEnum::RECURRENCE: return "RECURRENCE"; case OpEnum::RECURRENCE_GRAD: return "RECURRENCE_GRAD";
+            case OpEnum::CONV: return "CONV"; case OpEnum::CONV_GRAD: return "CONV_GRAD";
+            case OpEnum::SEQUENCE_OUT: return "SEQUENCE_OUT";
+            case OpEnum::LAST_STATE: return "LAST_STATE"; case OpEnum::LAST_STATE_GRAD: return "LAST_STATE_GRAD";
         }
         return "?";
     }

@@ -6,7 +6,8 @@ namespace ormi::ops {
     // need and the reference lacks: activations with their derivative ops
     // (adjoints build these instead of allocating constants), MAX/ARGMAX
     // reductions, an equality mask for the MAX adjoint, a dtype CAST, and a
-    // transformer block's rotary positions and attention with its gradient.
+    // transformer block's rotary positions and attention with its gradient, and a
+    // recurrent block's recurrence, convolution and the states they leave.
     enum class OpEnum {
         LEAF, CONST,
         NEG, EXP, LOG, SIN, COS,
@@ -15,7 +16,8 @@ namespace ormi::ops {
         FRAC_DERIV,
         RELU, STEP, TANH, TANH_GRAD, SIGMOID, SIGMOID_GRAD, GELU, GELU_GRAD,
         MAX, ARGMAX, EQ, CAST,
-        ROTARY, ATTENTION, ATTENTION_GRAD
+        ROTARY, ATTENTION, ATTENTION_GRAD,
+        RECURRENCE, RECURRENCE_GRAD, CONV, CONV_GRAD, SEQUENCE_OUT, LAST_STATE, LAST_STATE_GRAD
     };
 
     const char* op_name(OpEnum op);

@@ -50,4 +50,17 @@ namespace ormi::ops {
     // lengths (batch) int32. The queries are the last of their sequence.
     NodePtr attention(NodePtr q, NodePtr k, NodePtr v, float scale, float cap, bool causal, NodePtr slopes, NodePtr documents,
                       NodePtr prefix, NodePtr lengths);
+
+    // Gated linear recurrence over the tokens of x (batch, length, channels); gates
+    // of its shape (logits: before their sigmoid). initial (batch, channels) float32,
+    // documents (batch, length) and lengths (batch) int32 may be null.
+    NodePtr recurrence(NodePtr gates, NodePtr x, NodePtr initial, NodePtr documents, NodePtr lengths, bool logits);
+    // Convolution of each channel with its own weights (channels, width) over the
+    // token and those before it; bias (channels) float32, initial (batch, width - 1,
+    // channels) of x's type, documents and lengths may be null.
+    NodePtr conv(NodePtr x, NodePtr weight, NodePtr bias, NodePtr initial, NodePtr documents, NodePtr lengths, bool silu);
+    // What a RECURRENCE or CONV node gives: its result, and the state that the last
+    // token leaves.
+    NodePtr sequence_out(NodePtr sequence);
+    NodePtr last_state(NodePtr sequence);
 }

@@ -113,7 +113,10 @@ __device__ __forceinline__ void update(const AdamParams& a, float g, float& p, f
     p = p - a.lr * (rate + a.decay * p);
 }
 
-__global__ __launch_bounds__(256) void adamw_kernel(AdamParams a) {
+// SCALED: every gradient times *factor.
+template <bool SCALED>
+__global__ __launch_bounds__(256) void adamw_kernel(AdamParams a, const float* factor) {
+    const float scale = SCALED ? *factor : 1.0f;
     const AdamEntry& t = a.t[find_tensor(a)];
     const long long base = (long long)(blockIdx.x - t.first) * kPerGroup;
     f32x4 p[2], g[2], m[2], v[2];
@@ -131,7 +134,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamParams a) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) update(a, g[k].v[e], p[k].v[e], m[k].v[e], v[k].v[e]);
+        for (int e = 0; e < 4; ++e) update(a, SCALED ? g[k].v[e] * scale : g[k].v[e], p[k].v[e], m[k].v[e], v[k].v[e]);
         store4(t.out, t.p_dtype, i[k], n[k], t.vec, p[k]);
         store4(t.m_out, ORMI_DTYPE_F32, i[k], n[k], t.vec, m[k]);
         store4(t.v_out, ORMI_DTYPE_F32, i[k], n[k], t.vec, v[k]);
@@ -178,7 +181,9 @@ __device__ __forceinline__ float scale_inverse(float scale) {
 }
 
 // A wave per block of 256 elements, four per lane (their codes one word).
-__global__ __launch_bounds__(256) void adamw8_kernel(AdamParams a) {
+template <bool SCALED>
+__global__ __launch_bounds__(256) void adamw8_kernel(AdamParams a, const float* factor) {
+    const float scale = SCALED ? *factor : 1.0f;
     const AdamEntry& t = a.t[find_tensor(a)];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const long long blocks = (t.count + ORMI_ADAMW_BLOCK - 1) / ORMI_ADAMW_BLOCK;
@@ -209,7 +214,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamParams a) {
         for (int e = 0; e < 4; ++e) {
             m.v[e] = decode_m((int)(signed char)(mc[k] >> (8 * e)), ms[k]);
             v.v[e] = decode_v((int)(unsigned char)(vc[k] >> (8 * e)), vs[k]);
-            update(a, g[k].v[e], p[k].v[e], m.v[e], v.v[e]);
+            update(a, SCALED ? g[k].v[e] * scale : g[k].v[e], p[k].v[e], m.v[e], v.v[e]);
             if (e >= n[k]) m.v[e] = v.v[e] = 0.0f;  // padding past the tensor's end
             mt = ormi_maximum(mt, __builtin_fabsf(m.v[e]));
             vt = ormi_maximum(vt, __builtin_fabsf(v.v[e]));
@@ -259,9 +264,7 @@ int size_of(int dt) { return dt == ORMI_DTYPE_F32 ? 4 : 2; }
 
 using namespace ormi_hip;
 
-extern "C" {
-
-int ormi_hip_adamw(const ormi_adamw_desc* d) {
+static int adamw_step(const ormi_adamw_desc* d, const float* factor) {
     auto bad = [](const char* what) { return fail(ORMI_HIP_ERR_INVALID, std::string("ormi_hip_adamw: ") + what); };
     if (!d) return bad("null descriptor");
     if (d->num_tensors < 0 || (d->num_tensors > 0 && !d->tensors)) return bad("bad tensor list");
@@ -301,8 +304,8 @@ int ormi_hip_adamw(const ormi_adamw_desc* d) {
     unsigned long long groups = 0;
     auto flush = [&] {
         if (a.n == 0) return;
-        if (small) adamw8_kernel<<<(unsigned)groups, 256>>>(a);
-        else adamw_kernel<<<(unsigned)groups, 256>>>(a);
+        if (small) factor ? adamw8_kernel<true><<<(unsigned)groups, 256>>>(a, factor) : adamw8_kernel<false><<<(unsigned)groups, 256>>>(a, factor);
+        else factor ? adamw_kernel<true><<<(unsigned)groups, 256>>>(a, factor) : adamw_kernel<false><<<(unsigned)groups, 256>>>(a, factor);
         a.n = 0;
         groups = 0;
     };
@@ -335,6 +338,15 @@ int ormi_hip_adamw(const ormi_adamw_desc* d) {
     flush();
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? ORMI_HIP_OK : fail(ORMI_HIP_ERR_RUNTIME, std::string("ormi_hip_adamw: ") + hipGetErrorString(e));
+}
+
+extern "C" {
+
+int ormi_hip_adamw(const ormi_adamw_desc* d) { return adamw_step(d, nullptr); }
+
+int ormi_hip_adamw_scaled(const ormi_adamw_desc* d, const float* factor) {
+    if (!factor) return fail(ORMI_HIP_ERR_INVALID, "ormi_hip_adamw_scaled: null factor");
+    return adamw_step(d, factor);
 }
 
 int ormi_hip_adamw_values(float* m, float* v, const void* m_codes, const float* m_scale, const void* v_codes, const float* v_scale,

@@ -17,7 +17,7 @@ import numpy as np
 
 from ._ext import ormi_backend
 from .exceptions import raise_device_mismatch
-from .tensor import Tensor
+from .tensor import Tensor, _parse_device
 
 _BLOCK = 256  # elements that share a scale in 8-bit moments
 
@@ -199,12 +199,14 @@ class AdamState8:
 
 
 def adamw(params, grads, states, *, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-          weight_decay: float = 0.01):
+          weight_decay: float = 0.01, max_norm: float | None = None):
     """One AdamW step over lists of tensors: (new parameters, new states).
 
     Runs at once (the gradients are realized together), as few launches for
     however many tensors. states: AdamState or AdamState8, one kind per call.
-    step counts from 1. What was passed in keeps its values.
+    step counts from 1. What was passed in keeps its values. With max_norm the
+    gradients count times min(1, max_norm / grad_norm(grads)), as clip_grads would
+    give them but for its rounding of 16-bit ones.
       m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
       p = p - lr ((m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps) + weight_decay p)
     in float32; a 16-bit parameter is rounded to its type once.
@@ -212,14 +214,57 @@ def adamw(params, grads, states, *, step: int, lr: float = 1e-3, betas=(0.9, 0.9
     params, grads, states = list(params), list(grads), list(states)
     if any(not isinstance(t, Tensor) for t in params + grads):
         raise TypeError("params and grads must be Tensors.")
+    factor = None if max_norm is None else _norm_and_factor(grads, max_norm)[1]
+    return _adamw(params, grads, states, step, lr, betas, eps, weight_decay, factor)
+
+
+def _adamw(params, grads, states, step, lr, betas, eps, weight_decay, factor):
     kinds = {type(s) for s in states}
     if not kinds <= {AdamState, AdamState8} or len(kinds) > 1:
         raise TypeError("states must be all AdamState or all AdamState8.")
     kind = kinds.pop() if kinds else AdamState
     p, s = ormi_backend.adamw([t._node for t in params], [t._node for t in grads], [t._nodes() for t in states], kind.bits, step, lr,
-                              betas[0], betas[1], eps, weight_decay)
+                              betas[0], betas[1], eps, weight_decay, factor)
     return ([Tensor._wrap(n, t.device) for n, t in zip(p, params)],
             [kind._from(n, t.shape, t.device) for n, t in zip(s, params)])
+
+
+def _norm_and_factor(grads, max_norm: float):
+    """The nodes of the norm and of min(1, max_norm / norm)."""
+    if not max_norm >= 0:
+        raise ValueError("max_norm must not be negative.")
+    return ormi_backend.grad_norm([t._node for t in grads], max_norm)
+
+
+def _grads(grads):
+    grads = list(grads)
+    if any(not isinstance(t, Tensor) for t in grads):
+        raise TypeError("grads must be Tensors.")
+    return grads
+
+
+def grad_norm(grads) -> Tensor:
+    """The square root of the sum of all elements' squares, a float32 scalar on the device.
+
+    Runs at once (the gradients are realized together). Squares are added in 64
+    bits, in a fixed order. No gradients: 0.
+    """
+    grads = _grads(grads)
+    node = ormi_backend.grad_norm([t._node for t in grads], math.inf)[0]
+    return Tensor._wrap(node, grads[0].device if grads else _parse_device("hip"))
+
+
+def clip_grads(grads, max_norm: float):
+    """(the gradients times min(1, max_norm / norm), norm), norm that of grad_norm.
+
+    Nothing waits for the device: the factor stays there. Each product is rounded
+    once to its gradient's type. A norm that is NaN makes every element NaN, an
+    infinite one makes finite elements 0 and the others NaN.
+    """
+    grads = _grads(grads)
+    norm, factor = _norm_and_factor(grads, max_norm)
+    device = grads[0].device if grads else _parse_device("hip")
+    return [Tensor._wrap(n, t.device) for n, t in zip(ormi_backend.scale_grads([t._node for t in grads], factor), grads)], Tensor._wrap(norm, device)
 
 
 class AdamW:
@@ -234,15 +279,20 @@ class AdamW:
     old one keeps its values. The old leaf's gradient is let go of; those of the
     nodes between point back at what they were computed from, and a loop that
     does not release them with zero_grad_graph keeps every step's graph in
-    memory. state_bits: 32, or 8 for moments of a quarter of the size.
+    memory. state_bits: 32, or 8 for moments of a quarter of the size. max_norm:
+    the gradients of a step count times min(1, max_norm / norm), norm being theirs
+    taken together; self.norm then holds the last step's, on the device.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
-                 state_bits: int = 32):
+                 state_bits: int = 32, max_norm: float | None = None):
         if state_bits not in (32, 8):
             raise ValueError("state_bits must be 32 or 8.")
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError("max_norm must not be negative.")
         self.params = list(params)
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.max_norm, self.norm = max_norm, None
         kind = AdamState if state_bits == 32 else AdamState8
         self.states = [kind.zeros(p.shape, p.device) for p in self.params]
         self.steps = [0] * len(self.params)
@@ -252,19 +302,28 @@ class AdamW:
         for i, p in enumerate(self.params):
             if p.grad is not None:
                 by_step.setdefault(self.steps[i] + 1, []).append(i)
+        factor = None
+        if self.max_norm is not None and by_step:
+            norm, factor = _norm_and_factor([self.params[i].grad for members in by_step.values() for i in members], self.max_norm)
+            self.norm = Tensor._wrap(norm, self.params[0].device)
         for step, members in by_step.items():
-            new, states = adamw([self.params[i] for i in members], [self.params[i].grad for i in members],
-                                [self.states[i] for i in members], step=step, lr=self.lr, betas=self.betas, eps=self.eps,
-                                weight_decay=self.weight_decay)
+            new, states = self._step([self.params[i] for i in members], [self.states[i] for i in members], step, factor)
             for i, p, s in zip(members, new, states):
                 self.params[i].zero_grad()  # of the leaf that was: the graph may still hold it
                 self.params[i]._node = p._node
                 self.states[i] = s
                 self.steps[i] = step
 
+    def _step(self, params, states, step: int, factor):
+        grads = [p.grad for p in params]
+        options = dict(lr=self.lr, betas=self.betas, eps=self.eps, weight_decay=self.weight_decay)
+        if factor is None:
+            return adamw(params, grads, states, step=step, **options)
+        return _adamw(params, grads, states, step, factor=factor, **options)
+
     def zero_grad(self) -> None:
         for p in self.params:
             p.zero_grad()
 
 
-__all__ = ["RotaryTable", "rotary", "attention", "AdamState", "AdamState8", "adamw", "AdamW"]
+__all__ = ["RotaryTable", "rotary", "attention", "AdamState", "AdamState8", "adamw", "AdamW", "grad_norm", "clip_grads"]
