@@ -6,18 +6,19 @@
 
 namespace ormi_hip {
 
-constexpr int kRecSegments = 32;                      // of a tile, one after the other in time
-constexpr int kRecTokens = 4;                         // of a segment: a thread's
-constexpr int kRecTile = kRecSegments * kRecTokens;   // tokens between the states kept for the gradient
+constexpr int kRecLanes = 16;                         // threads side by side over the channels
+constexpr int kRecRun = 4;                            // channels of a thread
+constexpr int kRecChannels = kRecLanes * kRecRun;     // of a work-group
+constexpr int kRecTokens = 8;                         // of a segment: a thread's
+constexpr int kRecTile = 256 / kRecLanes * kRecTokens;  // tokens between the states kept for the gradient
+constexpr int kRecWindow = 4;                         // tiles before a chained one that it looks at together
 static_assert(kRecTile == ORMI_RECURRENCE_TILE, "the header's tile");
-constexpr int kRecLanes = 8;                          // threads side by side over the channels
-constexpr int kRecMostSplits = 64;
 
 struct RecParams {
     const char *gates, *x, *dout;
     long long g_sb, g_sl, x_sb, x_sl, do_sb, do_sl;  // strides in elements; channels are neighbours
     int batch, length, channels;
-    int channel_blocks, splits, split_tiles, tiles;
+    int channel_blocks, chains, tiles, chained;  // chains: channel blocks of all batches
     const float* initial;
     const int *docs, *lengths;
     long long docs_sb;
@@ -27,10 +28,11 @@ struct RecParams {
     const float* dlast;
     char *dgates, *dx;
     float* dinitial;
-    // Of each split, batch and channel: the product of its gates and what it leaves
-    // of nothing, then (one per batch and split) whether its tokens forget.
-    float2* part;
-    int* part_cut;
+    // Chained tiles: the spans and states that are there, by tile, chain and channel, and
+    // how many tiles were begun.
+    unsigned long long* chain_spans;
+    unsigned* chain_states;
+    unsigned* ticket;
 };
 
 // xt: the type of x and the result; gates and dout have it or are float32 (their flags).

@@ -23,32 +23,27 @@ const char* check(const ormi_recurrence_desc* d) {
     if (d->gate_dtype != d->dtype && d->gate_dtype != ORMI_DTYPE_F32) return "gates must have x's type or float32";
     if (d->batch < 0 || d->length < 0 || d->channels < 0) return "negative extent";
     if (d->length > kMostTokens) return "more than 2^30 tokens";
-    if ((long long)d->batch * ((d->channels + 31ll) / 32) > kMostGroups) return "batch * channels too large";
+    if ((long long)d->batch * ((d->channels + kRecChannels - 1ll) / kRecChannels) > kMostGroups) return "batch * channels too large";
     return nullptr;
 }
 
 bool nothing(const ormi_recurrence_desc* d) { return d->batch == 0 || d->channels == 0; }
 
-// The tiles and how they are split. A work-group goes through its split's tiles;
-// with fewer than two to a compute unit the card's memory is not kept busy.
+// The tiles, and whether they are chained: with fewer than two work-groups to a
+// compute unit the others do not keep the card's memory busy.
 void plan(const ormi_recurrence_desc* d, RecParams* p) {
-    const int wide = d->dtype == ORMI_DTYPE_F32 ? 4 : 8;
     p->batch = d->batch;
     p->length = d->length;
     p->channels = d->channels;
     p->tiles = (d->length + kRecTile - 1) / kRecTile;
-    p->channel_blocks = (int)((d->channels + (long long)kRecLanes * wide - 1) / (kRecLanes * wide));
-    const long long groups = (long long)p->channel_blocks * d->batch, want = 2ll * compute_units();
-    p->splits = (int)std::max(1ll, std::min({(want + groups - 1) / groups, (long long)kRecMostSplits, (long long)p->tiles / 2}));
-    p->split_tiles = std::max(1, (p->tiles + p->splits - 1) / p->splits);
-    p->splits = std::max(1, (p->tiles + p->split_tiles - 1) / p->split_tiles);
+    p->channel_blocks = (int)((d->channels + kRecChannels - 1ll) / kRecChannels);
+    p->chains = p->channel_blocks * d->batch;
+    p->chained = p->tiles > 1 && p->chains < 2 * compute_units();
 }
 
-size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-size_t part_bytes(const RecParams& p) { return padded((size_t)p.batch * p.splits * p.channels * sizeof(float2)); }
-size_t workspace_bytes(const RecParams& p) {
-    return p.splits <= 1 ? 0 : part_bytes(p) + padded((size_t)p.batch * p.splits * sizeof(int));
-}
+size_t span_bytes(const RecParams& p) { return (size_t)p.tiles * p.chains * kRecChannels * sizeof(unsigned long long); }
+// Spans, states, then the ticket.
+size_t workspace_bytes(const RecParams& p) { return p.chained ? span_bytes(p) / 2 * 3 + 256 : 0; }
 
 void fill(const ormi_recurrence_desc* d, RecParams* p) {
     p->gates = (const char*)d->gates;
@@ -64,8 +59,12 @@ void fill(const ormi_recurrence_desc* d, RecParams* p) {
     p->out = (char*)d->out;
     p->last = d->last;
     p->states = d->states;
-    p->part = (float2*)d->workspace;
-    p->part_cut = p->splits > 1 ? (int*)((char*)d->workspace + part_bytes(*p)) : nullptr;
+    if (p->chained) {
+        char* ws = (char*)d->workspace;
+        p->chain_spans = (unsigned long long*)ws;
+        p->chain_states = (unsigned*)(ws + span_bytes(*p));
+        p->ticket = (unsigned*)(ws + span_bytes(*p) / 2 * 3);
+    }
 }
 
 int launch(const ormi_recurrence_desc* d, const RecParams& p, const RecCall& c, const char* name) {
@@ -106,7 +105,7 @@ int ormi_hip_recurrence(const ormi_recurrence_desc* d) {
     plan(d, &p);
     if (workspace_bytes(p) > 0 && (!d->workspace || d->workspace_bytes < workspace_bytes(p))) return bad("workspace too small");
     fill(d, &p);
-    if ((long long)p.channel_blocks * p.splits * p.batch > kMostGroups) return bad("batch * channels too large");
+    if (p.chained && (long long)p.chains * p.tiles > kMostGroups) return bad("batch * length * channels too large");
     return launch(d, p, RecCall{d->gate_dtype == ORMI_DTYPE_F32, false, d->logits != 0, false}, "ormi_hip_recurrence");
 }
 
@@ -131,7 +130,7 @@ int ormi_hip_recurrence_grad(const ormi_recurrence_grad_desc* g) {
     p.dgates = (char*)g->dgates;
     p.dx = (char*)g->dx;
     p.dinitial = g->dinitial;
-    if ((long long)p.channel_blocks * p.splits * p.batch > kMostGroups) return bad("batch * channels too large");
+    if (p.chained && (long long)p.chains * p.tiles > kMostGroups) return bad("batch * length * channels too large");
     return launch(d, p, RecCall{d->gate_dtype == ORMI_DTYPE_F32, g->dout && g->dout_dtype == ORMI_DTYPE_F32, d->logits != 0, true},
                   "ormi_hip_recurrence_grad");
 }

@@ -7,13 +7,17 @@
 //
 // A span of tokens takes the state before it to A h + B, A the product of its
 // gates and B what it makes of nothing, and spans join by (A1 A2, A2 B1 + B2). A
-// tile is 32 segments of 4 tokens by 8 threads' channels (128 bytes of a row, a
-// cache line). A thread takes its own segment's span, segments join by lane
-// exchanges in a wave and through LDS across the four waves, and each thread then
-// walks its tokens again from the state before them. One work-group goes through
-// the tiles of its channels with the state in registers; where batch and channels
-// give too few of them, the length is split: a first launch takes each split's
-// span, the second starts from the joined ones.
+// tile is 16 segments of 8 tokens by 16 threads of 4 channels. A thread takes its
+// own segment's span, segments join by lane exchanges in a wave and through LDS
+// across the four waves, and each thread then walks its tokens again from the
+// state before them.
+//
+// Where batch and channels give enough work-groups, one goes through all tiles of
+// its channels, the state in registers, the next tile's loads in flight. Otherwise
+// (CHAINED) a work-group has one tile, and the state before it comes from the
+// tiles before: each publishes its span, and the state past it as soon as it knows
+// the one before it; a tile composes the spans back to the nearest state that is
+// there. Inputs are read once either way.
 //
 // Where a token forgets (a document's first one, or one of none) the state before
 // it must not matter at all, NaN included, so spans carry a flag: a product that
@@ -90,8 +94,8 @@ __device__ __forceinline__ float after(float a, float b, bool cut, float h) {
     return MASKED && cut ? b : r;
 }
 
-// s joined with the spans of the lanes before it (those `up` lanes lower) or, with
-// DOWN, after it: inclusive over the eight segments of a wave, then exclusive.
+// s joined with the spans of the lanes before it (of higher lanes with DOWN):
+// inclusive over a wave's segments, then exclusive; `whole` is the wave's.
 template <int V, bool MASKED, bool DOWN>
 __device__ __forceinline__ void scan_wave(Span<V>& s, Span<V>& whole) {
     const int lane = threadIdx.x & 63;
@@ -110,15 +114,12 @@ __device__ __forceinline__ void scan_wave(Span<V>& s, Span<V>& whole) {
         }
         if (MASKED && has) s.cut = s.cut || ocut;
     }
-    // The wave's whole span stands in its last (first) segment.
-    const int full = (DOWN ? 0 : 56) + (lane & 7), from = DOWN ? lane + kRecLanes : lane - kRecLanes;
-    const bool has = DOWN ? lane < 56 : lane >= kRecLanes;
-    const bool wcut = MASKED ? __shfl((int)s.cut, full, 64) != 0 : false, ecut = MASKED ? __shfl((int)s.cut, from & 63, 64) != 0 : false;
-    whole.cut = wcut;
+    whole = s;  // in the last (first) segment's lanes
+    const int from = DOWN ? lane + kRecLanes : lane - kRecLanes;
+    const bool has = DOWN ? lane < 64 - kRecLanes : lane >= kRecLanes;
+    const bool ecut = MASKED ? __shfl((int)s.cut, from & 63, 64) != 0 : false;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        whole.a[e] = __shfl(s.a[e], full, 64);
-        whole.b[e] = __shfl(s.b[e], full, 64);
         const float oa = __shfl(s.a[e], from & 63, 64), ob = __shfl(s.b[e], from & 63, 64);
         s.a[e] = has ? oa : 1.0f;
         s.b[e] = has ? ob : 0.0f;
@@ -133,20 +134,20 @@ struct WaveSpans {
     float2 s[2][4][kRecLanes][V];
     int cut[2][4];
 };
-template <int V>
+template <int V, bool DOWN>
 __device__ __forceinline__ void put_wave(WaveSpans<V>& l, int at, const Span<V>& whole) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane < kRecLanes) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = DOWN ? lane : lane - (64 - kRecLanes);
+    if (k >= 0 && k < kRecLanes) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) l.s[at][wave][lane][e] = make_float2(whole.a[e], whole.b[e]);
-        if (lane == 0) l.cut[at][wave] = whole.cut;
+        for (int e = 0; e < V; ++e) l.s[at][wave][k][e] = make_float2(whole.a[e], whole.b[e]);
+        if (k == 0) l.cut[at][wave] = whole.cut;
     }
 }
 // The state before this wave's first segment (after its last with DOWN) in h, and
 // the one past the tile in `carry`, which holds the one before it.
 template <int V, bool MASKED, bool DOWN>
 __device__ __forceinline__ void cross_waves(const WaveSpans<V>& l, int at, float (&carry)[V], float (&h)[V]) {
-    const int lane = threadIdx.x & 7, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x % kRecLanes, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int w = DOWN ? 3 - k : k;
@@ -163,84 +164,190 @@ __device__ __forceinline__ void cross_waves(const WaveSpans<V>& l, int at, float
     }
 }
 
-// What a work-group has: its channels, batch and tiles.
+// What a thread has: its channels, batch and tokens that exist.
 struct Place {
-    int b, c, n, split, first, tiles, end;
+    int b, c, n, end;
 };
-template <int V>
-__device__ __forceinline__ Place place_of(const RecParams& p) {
+__device__ __forceinline__ Place place_of(const RecParams& p, int chain) {
     Place w;
-    const int blocks = p.channel_blocks, id = blockIdx.x;
-    const int cb = id % blocks, rest = id / blocks;
-    w.split = rest % p.splits;
-    w.b = rest / p.splits;
-    w.c = (cb * kRecLanes + (threadIdx.x & 7)) * V;
-    w.n = max(0, min(V, p.channels - w.c));
-    w.first = w.split * p.split_tiles;
-    w.tiles = max(0, min(p.split_tiles, p.tiles - w.first));
+    const int cb = chain % p.channel_blocks;
+    w.b = chain / p.channel_blocks;
+    w.c = cb * kRecChannels + (int)(threadIdx.x % kRecLanes) * kRecRun;
+    w.n = max(0, min(kRecRun, p.channels - w.c));
     w.end = p.length;
     if (p.lengths) w.end = max(0, min(p.length, p.lengths[w.b]));
     return w;
 }
-// The carry that a split starts from: `start` and the splits before it (after it).
-template <int V, bool MASKED, bool DOWN>
-__device__ __forceinline__ void join_splits(const RecParams& p, const Place& w, const float* start, float (&carry)[V]) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) carry[e] = start && e < w.n ? start[(long long)w.b * p.channels + w.c + e] : 0.0f;
-    const int others = DOWN ? p.splits - 1 - w.split : w.split;
-    for (int k = 0; k < others; ++k) {
-        const long long row = (long long)w.b * p.splits + (DOWN ? p.splits - 1 - k : k);
-        const bool cut = MASKED && p.part_cut[row] != 0;
-        const float2* at = p.part + row * p.channels + w.c;
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e < w.n) carry[e] = after<MASKED>(at[e].x, at[e].y, cut, carry[e]);
-    }
+
+// ------------------------------------------------------------ chained tiles --
+// A tile's span (gates' product and rest in one word, so that no order between
+// words matters) and the state past it, per channel. All bits set: not there yet.
+// Published NaN have other bits, and a span that forgets has them in the product's
+// place.
+constexpr unsigned kNone = 0xffffffffu;
+constexpr unsigned long long kNoSpan = ~0ull;
+// Looks at a tile before it that is not there yet, seconds' worth: the
+// tiles that a tile waits for were begun before it and wait for none after them, so
+// this ends a wait only where a work-group was lost; the states are NaN then.
+constexpr int kMostLooks = 1 << 21;
+
+__device__ __forceinline__ unsigned published(float v) { return v == v ? __float_as_uint(v) : 0x7fc00000u; }
+__device__ __forceinline__ unsigned look_state(const RecParams& p, long long at) {
+    return __hip_atomic_load(p.chain_states + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <int V>
-__device__ __forceinline__ void put_split(const RecParams& p, const Place& w, const Span<V>& s) {
-    if (threadIdx.x >= kRecLanes) return;
-    const long long row = (long long)w.b * p.splits + w.split;
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-        if (e < w.n) p.part[row * p.channels + w.c + e] = make_float2(s.a[e], s.b[e]);
-    if (w.c == 0) p.part_cut[row] = s.cut;
+__device__ __forceinline__ unsigned long long look_span(const RecParams& p, long long at) {
+    return __hip_atomic_load(p.chain_spans + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Forward; SPANS: only the splits' spans.
-template <int GT, int XT, bool LOGIT, bool MASKED, bool SPANS>
+// Of one channel: the state before tile `pos` of a chain (counted in the order that
+// the tiles go), whose span is (a, b, cut); publishes what others need.
+__device__ __forceinline__ float chained_state(const RecParams& p, int chain, int pos, int channel, float start, float a, float b, bool cut) {
+    const long long stride = (long long)p.chains * kRecChannels, at = pos * stride + (long long)chain * kRecChannels + channel;
+    float h = start;
+    if (pos > 0) {
+        unsigned first = look_state(p, at - stride);
+        if (first == kNone) {
+            const unsigned long long word = (unsigned long long)(cut ? kNone : published(a)) << 32 | published(b);
+            __hip_atomic_store(p.chain_spans + at, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            // The spans from tile pos - back to pos - 1 so far, and the states and spans
+            // of the next kRecWindow tiles before them, looked at together.
+            float sa = 1.0f, sb = 0.0f;
+            int back = 1, looks = 0;
+            bool done = false;
+            while (!done) {
+                unsigned state[kRecWindow];
+                unsigned long long span[kRecWindow];
+#pragma unroll
+                for (int k = 0; k < kRecWindow; ++k) {
+                    const long long from = at - (long long)min(back + k, pos) * stride;
+                    state[k] = look_state(p, from);
+                    span[k] = look_span(p, from);
+                }
+                bool ready = true;
+#pragma unroll
+                for (int k = 0; k < kRecWindow; ++k) {
+                    if (done || !ready) continue;
+                    if (state[k] != kNone) {
+                        h = __builtin_fmaf(sa, __uint_as_float(state[k]), sb);
+                        done = true;
+                    } else if (span[k] != kNoSpan) {
+                        const unsigned ka = (unsigned)(span[k] >> 32);
+                        const float kb = __uint_as_float((unsigned)span[k]);
+                        sb = __builtin_fmaf(sa, kb, sb);
+                        sa *= __uint_as_float(ka);
+                        ++back;
+                        if (ka == kNone) {
+                            h = sb;
+                            done = true;
+                        }
+                    } else {
+                        ready = false;
+                    }
+                }
+                if (!done && !ready) {
+                    if (++looks > kMostLooks) {
+                        h = __builtin_nanf("");
+                        done = true;
+                    }
+                    __builtin_amdgcn_s_sleep(1);
+                }
+            }
+        } else {
+            h = __uint_as_float(first);
+        }
+    }
+    const float past = cut ? b : __builtin_fmaf(a, h, b);
+    __hip_atomic_store(p.chain_states + at, published(past), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return h;
+}
+// A tile's whole span of one channel, from its waves'.
+template <int V, bool MASKED, bool DOWN>
+__device__ __forceinline__ void tile_span(const WaveSpans<V>& l, int at, int channel, float& a, float& b, bool& cut) {
+    a = 1.0f;
+    b = 0.0f;
+    cut = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int w = DOWN ? 3 - k : k;
+        const float2 s = l.s[at][w][channel / V][channel % V];
+        const bool c = MASKED && l.cut[at][w] != 0;
+        b = after<MASKED>(s.x, s.y, c, b);
+        a *= s.x;
+        cut = cut || c;
+    }
+}
+
+// The work-group's tile and chain: the next in order, chains side by side.
+__device__ __forceinline__ unsigned next_tile(const RecParams& p, unsigned* lds) {
+    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)*lds);
+}
+
+__global__ __launch_bounds__(256) void recurrence_clear_kernel(unsigned* at, long long count, unsigned* ticket) {
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i == 0) *ticket = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (i + k < count) at[i + k] = kNone;
+}
+
+template <int V>
+__device__ __forceinline__ void start_from(const float* start, const RecParams& p, const Place& w, float (&carry)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) carry[e] = start && e < w.n ? start[(long long)w.b * p.channels + w.c + e] : 0.0f;
+}
+template <int V>
+__device__ __forceinline__ void put_state(float* to, const Place& w, const float (&h)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (e < w.n) to[e] = h[e];
+}
+
+template <int GT, int XT, bool LOGIT, bool MASKED, bool CHAINED>
 __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
-    constexpr int V = XT == ORMI_DTYPE_F32 ? 4 : 8, S = kRecTokens;
+    constexpr int V = kRecRun, S = kRecTokens;
     using TG = typename ElemOf<GT>::type;
     using TX = typename ElemOf<XT>::type;
     __shared__ WaveSpans<V> lds;
-    const Place w = place_of<V>(p);
-    if (SPANS && w.split == p.splits - 1) return;  // nothing starts from it
-    const int seg = threadIdx.x >> 3;
+    __shared__ float chain_carry[CHAINED ? kRecChannels : 1];
+    __shared__ unsigned ticket;
+    int chain = (int)blockIdx.x, first = 0, tiles = p.tiles;
+    if (CHAINED) {
+        const unsigned item = next_tile(p, &ticket);
+        if (item >= gridDim.x) return;  // one tile to each work-group
+        first = (int)(item / (unsigned)p.chains);
+        chain = (int)(item % (unsigned)p.chains);
+        tiles = 1;
+    }
+    const Place w = place_of(p, chain);
+    const int seg = threadIdx.x / kRecLanes;
     const TG* gates = (const TG*)p.gates + w.b * p.g_sb + w.c;
     const TX* x = (const TX*)p.x + w.b * p.x_sb + w.c;
     TX* out = (TX*)p.out + (long long)w.b * p.length * p.channels + w.c;
     float carry[V];
-    Span<V> total;
-    total.cut = false;
-#pragma unroll
-    for (int e = 0; e < V; ++e) total.a[e] = 1.0f, total.b[e] = 0.0f;
-    if (!SPANS) join_splits<V, MASKED, false>(p, w, p.initial, carry);
-    for (int k = 0; k < w.tiles; ++k) {
-        const int tile = w.first + k, t0 = tile * kRecTile + seg * S;
-        const Rules rule = token_rules<MASKED>(p, w.b, w.end, t0);
-        Run<GT, V> rg[S];
-        Run<XT, V> rx[S];
+    if (!CHAINED) start_from<V>(p.initial, p, w, carry);
+    Run<GT, V> rg[S];
+    Run<XT, V> rx[S];
+    Rules rule;
+    auto fetch = [&](int tile) {
+        const int t0 = tile * kRecTile + seg * S;
+        rule = token_rules<MASKED>(p, w.b, w.end, t0);
         load_rows<GT, V>(rg, gates + t0 * p.g_sl, p.g_sl, rule.on, w.n, LOGIT ? kPassLogit : 1.0f);
         load_rows<XT, V>(rx, x + t0 * p.x_sl, p.x_sl, rule.on, w.n, 0.0f);
+    };
+    if (tiles > 0) fetch(first);
+    for (int k = 0; k < tiles; ++k) {
+        const int tile = first + k, t0 = tile * kRecTile + seg * S;
+        const Rules now = rule;
         float a[S][V], b[S][V];
         Span<V> s;
-        s.cut = MASKED && rule.cut != 0;
+        s.cut = MASKED && now.cut != 0;
 #pragma unroll
         for (int e = 0; e < V; ++e) s.a[e] = 1.0f, s.b[e] = 0.0f;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const bool cut = MASKED && (rule.cut >> i & 1);
+            const bool cut = MASKED && (now.cut >> i & 1);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 if (LOGIT) {
@@ -255,37 +362,34 @@ __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
                 s.a[e] *= a[i][e];
             }
         }
+        if (!CHAINED && k + 1 < tiles) fetch(tile + 1);
         Span<V> whole;
         scan_wave<V, MASKED, false>(s, whole);
-        put_wave<V>(lds, k & 1, whole);
+        put_wave<V, false>(lds, k & 1, whole);
         __syncthreads();
-        float h[V];
-        if (SPANS) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const bool cut = MASKED && lds.cut[k & 1][q] != 0;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float2 o = lds.s[k & 1][q][threadIdx.x & 7][e];
-                    total.b[e] = after<MASKED>(o.x, o.y, cut, total.b[e]);
-                    total.a[e] *= o.x;
+        if (CHAINED) {
+            if (threadIdx.x < kRecChannels) {
+                const int c = w.c - (int)(threadIdx.x % kRecLanes) * kRecRun + (int)threadIdx.x;  // this lane's one channel
+                float sa, sb, h = 0.0f;
+                bool cut;
+                tile_span<V, MASKED, false>(lds, k & 1, threadIdx.x, sa, sb, cut);
+                if (c < p.channels) {
+                    h = chained_state(p, chain, tile, threadIdx.x, p.initial ? p.initial[(long long)w.b * p.channels + c] : 0.0f, sa, sb, cut);
                 }
-                total.cut = total.cut || cut;
+                chain_carry[threadIdx.x] = h;
             }
-            continue;
-        }
-        if (p.states && seg == 0) {
-            float* at = p.states + ((long long)w.b * p.tiles + tile) * p.channels + w.c;
+            __syncthreads();
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (e < w.n) at[e] = carry[e];
+            for (int e = 0; e < V; ++e) carry[e] = chain_carry[threadIdx.x % kRecLanes * V + e];
         }
+        if (p.states && seg == 0) put_state<V>(p.states + ((long long)w.b * p.tiles + tile) * p.channels + w.c, w, carry);
+        float h[V];
         cross_waves<V, MASKED, false>(lds, k & 1, carry, h);
 #pragma unroll
         for (int e = 0; e < V; ++e) h[e] = after<MASKED>(s.a[e], s.b[e], s.cut, h[e]);
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const bool cut = MASKED && (rule.cut >> i & 1), on = rule.on >> i & 1;
+            const bool cut = MASKED && (now.cut >> i & 1), on = now.on >> i & 1;
             Run<XT, V> o;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -295,100 +399,104 @@ __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
             if (t0 + i < p.length) o.store(out + (long long)(t0 + i) * p.channels, w.n);
         }
     }
-    if (SPANS) put_split<V>(p, w, total);
-    else if (p.last && w.split == p.splits - 1 && threadIdx.x < kRecLanes) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e < w.n) p.last[(long long)w.b * p.channels + w.c + e] = carry[e];
-    }
+    if (p.last && seg == 0 && first + tiles == p.tiles) put_state<V>(p.last + (long long)w.b * p.channels + w.c, w, carry);
 }
 
 // Gradient, tiles from the last to the first. m is the gradient of the state before
 // a token but for that state's own output: m_t = a_t (dh_t + m_{t+1}), a recurrence
 // of the same gates the other way. The states before a tile's tokens are made again
 // from the one that the forward pass kept, in full precision.
-template <int GT, int XT, int DT, bool LOGIT, bool MASKED, bool SPANS>
+template <int GT, int XT, int DT, bool LOGIT, bool MASKED, bool CHAINED>
 __global__ __launch_bounds__(256) void recurrence_grad_kernel(RecParams p) {
-    constexpr int V = XT == ORMI_DTYPE_F32 ? 4 : 8, S = kRecTokens;
+    constexpr int V = kRecRun, S = kRecTokens;
     using TG = typename ElemOf<GT>::type;
     using TX = typename ElemOf<XT>::type;
     using TD = typename ElemOf<DT>::type;
     __shared__ WaveSpans<V> back, forth;
-    const Place w = place_of<V>(p);
-    if (SPANS && w.split == 0) return;
-    const int seg = threadIdx.x >> 3;
+    __shared__ float chain_carry[CHAINED ? kRecChannels : 1];
+    __shared__ unsigned ticket;
+    int chain = (int)blockIdx.x, first = p.tiles - 1, tiles = p.tiles;
+    if (CHAINED) {
+        const unsigned item = next_tile(p, &ticket);
+        if (item >= gridDim.x) return;  // one tile to each work-group
+        first = p.tiles - 1 - (int)(item / (unsigned)p.chains);
+        chain = (int)(item % (unsigned)p.chains);
+        tiles = 1;
+    }
+    const Place w = place_of(p, chain);
+    const int seg = threadIdx.x / kRecLanes;
     const TG* gates = (const TG*)p.gates + w.b * p.g_sb + w.c;
     const TX* x = (const TX*)p.x + w.b * p.x_sb + w.c;
     const TD* dout = (const TD*)p.dout + w.b * p.do_sb + w.c;
     const long long base = (long long)w.b * p.length * p.channels + w.c;
     float carry[V];
-    Span<V> total;
-    total.cut = false;
-#pragma unroll
-    for (int e = 0; e < V; ++e) total.a[e] = 1.0f, total.b[e] = 0.0f;
-    if (!SPANS) join_splits<V, MASKED, true>(p, w, p.dlast, carry);
-    for (int k = w.tiles - 1; k >= 0; --k) {
-        const int tile = w.first + k, t0 = tile * kRecTile + seg * S;
-        const Rules rule = token_rules<MASKED>(p, w.b, w.end, t0);
-        Run<GT, V> rg[S];
-        Run<XT, V> rx[S];
-        Run<DT, V> rd[S];
+    if (!CHAINED) start_from<V>(p.dlast, p, w, carry);
+    Run<GT, V> rg[S];
+    Run<XT, V> rx[S];
+    Run<DT, V> rd[S];
+    float kept[V];
+    Rules rule;
+    auto fetch = [&](int tile) {
+        const int t0 = tile * kRecTile + seg * S;
+        rule = token_rules<MASKED>(p, w.b, w.end, t0);
         load_rows<GT, V>(rg, gates + t0 * p.g_sl, p.g_sl, rule.on, w.n, LOGIT ? kPassLogit : 1.0f);
+        load_rows<XT, V>(rx, x + t0 * p.x_sl, p.x_sl, rule.on, w.n, 0.0f);
         load_rows<DT, V>(rd, dout + t0 * p.do_sl, p.do_sl, p.dout ? rule.on : 0u, w.n, 0.0f);
-        if (!SPANS) load_rows<XT, V>(rx, x + t0 * p.x_sl, p.x_sl, rule.on, w.n, 0.0f);
-        float a[S][V], take[S][V], before[V];
-        if (!SPANS) {
-            const float* at = p.states + ((long long)w.b * p.tiles + tile) * p.channels + w.c;
+        start_from<V>(p.states + (long long)w.b * p.tiles * p.channels - (long long)w.b * p.channels + (long long)tile * p.channels, p, w, kept);
+    };
+    if (tiles > 0) fetch(first);
+    for (int k = 0; k < tiles; ++k) {
+        const int tile = first - k, t0 = tile * kRecTile + seg * S;
+        const Rules now = rule;
+        float a[S][V], take[S][V], v[S][V], d[S][V], before[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) before[e] = e < w.n ? at[e] : 0.0f;
-        }
+        for (int e = 0; e < V; ++e) before[e] = kept[e];
         Span<V> f, r;
-        f.cut = r.cut = MASKED && rule.cut != 0;
+        f.cut = r.cut = MASKED && now.cut != 0;
 #pragma unroll
         for (int e = 0; e < V; ++e) f.a[e] = 1.0f, f.b[e] = r.b[e] = 0.0f;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const bool cut = MASKED && (rule.cut >> i & 1);
+            const bool cut = MASKED && (now.cut >> i & 1);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 if (LOGIT) gate_of(rg[i].get(e), a[i][e], take[i][e]);
                 else a[i][e] = rg[i].get(e);
+                v[i][e] = rx[i].get(e);
+                d[i][e] = rd[i].get(e);
                 f.a[e] *= a[i][e];
-                if (!SPANS) {
-                    const float v = rx[i].get(e);
-                    f.b[e] = after<MASKED>(a[i][e], LOGIT ? take[i][e] * v : v, cut, f.b[e]);
-                }
+                f.b[e] = after<MASKED>(a[i][e], LOGIT ? take[i][e] * v[i][e] : v[i][e], cut, f.b[e]);
             }
         }
 #pragma unroll
         for (int i = S - 1; i >= 0; --i) {
-            const bool cut = MASKED && (rule.cut >> i & 1);
+            const bool cut = MASKED && (now.cut >> i & 1);
 #pragma unroll
-            for (int e = 0; e < V; ++e) r.b[e] = MASKED && cut ? 0.0f : a[i][e] * (rd[i].get(e) + r.b[e]);
+            for (int e = 0; e < V; ++e) r.b[e] = MASKED && cut ? 0.0f : a[i][e] * (d[i][e] + r.b[e]);
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) r.a[e] = f.a[e];
+        if (!CHAINED && k + 1 < tiles) fetch(tile - 1);
         Span<V> whole;
         scan_wave<V, MASKED, true>(r, whole);
-        put_wave<V>(back, k & 1, whole);
-        if (!SPANS) {
-            scan_wave<V, MASKED, false>(f, whole);
-            put_wave<V>(forth, k & 1, whole);
-        }
+        put_wave<V, true>(back, k & 1, whole);
+        scan_wave<V, MASKED, false>(f, whole);
+        put_wave<V, false>(forth, k & 1, whole);
         __syncthreads();
-        if (SPANS) {
-#pragma unroll
-            for (int q = 3; q >= 0; --q) {
-                const bool cut = MASKED && back.cut[k & 1][q] != 0;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float2 o = back.s[k & 1][q][threadIdx.x & 7][e];
-                    total.b[e] = after<MASKED>(o.x, o.y, cut, total.b[e]);
-                    total.a[e] *= o.x;
+        if (CHAINED) {
+            if (threadIdx.x < kRecChannels) {
+                const int c = w.c - (int)(threadIdx.x % kRecLanes) * kRecRun + (int)threadIdx.x;  // this lane's one channel
+                float sa, sb, h = 0.0f;
+                bool cut;
+                tile_span<V, MASKED, true>(back, k & 1, threadIdx.x, sa, sb, cut);
+                if (c < p.channels) {
+                    h = chained_state(p, chain, p.tiles - 1 - tile, threadIdx.x, p.dlast ? p.dlast[(long long)w.b * p.channels + c] : 0.0f, sa, sb, cut);
                 }
-                total.cut = total.cut || cut;
+                chain_carry[threadIdx.x] = h;
             }
-            continue;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < V; ++e) carry[e] = chain_carry[threadIdx.x % kRecLanes * V + e];
         }
         float m[V], h[V], prev[S][V];
         cross_waves<V, MASKED, true>(back, k & 1, carry, m);
@@ -400,26 +508,25 @@ __global__ __launch_bounds__(256) void recurrence_grad_kernel(RecParams p) {
         }
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const bool cut = MASKED && (rule.cut >> i & 1);
+            const bool cut = MASKED && (now.cut >> i & 1);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 prev[i][e] = MASKED && cut ? 0.0f : h[e];
-                const float v = rx[i].get(e);
-                h[e] = __builtin_fmaf(a[i][e], prev[i][e], LOGIT ? take[i][e] * v : v);
+                h[e] = __builtin_fmaf(a[i][e], prev[i][e], LOGIT ? take[i][e] * v[i][e] : v[i][e]);
             }
         }
 #pragma unroll
         for (int i = S - 1; i >= 0; --i) {
-            const bool cut = MASKED && (rule.cut >> i & 1), on = rule.on >> i & 1;
+            const bool cut = MASKED && (now.cut >> i & 1), on = now.on >> i & 1;
             Run<GT, V> og;
             Run<XT, V> ox;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float l = rd[i].get(e) + m[e];
+                const float l = d[i][e] + m[e];
                 float dx = l, dg = l * prev[i][e];
                 if (LOGIT) {
                     dx = l * take[i][e];
-                    dg = dx * a[i][e] * (prev[i][e] - rx[i].get(e));
+                    dg = dx * a[i][e] * (prev[i][e] - v[i][e]);
                 }
                 m[e] = MASKED && cut ? 0.0f : a[i][e] * l;
                 og.set(e, MASKED && !on ? 0.0f : dg);
@@ -432,23 +539,22 @@ __global__ __launch_bounds__(256) void recurrence_grad_kernel(RecParams p) {
             }
         }
     }
-    if (SPANS) put_split<V>(p, w, total);
-    else if (p.dinitial && w.split == 0 && threadIdx.x < kRecLanes) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e < w.n) p.dinitial[(long long)w.b * p.channels + w.c + e] = carry[e];
-    }
+    if (p.dinitial && seg == 0 && first - tiles < 0) put_state<V>(p.dinitial + (long long)w.b * p.channels + w.c, w, carry);
 }
 
 template <int GT, int XT, int DT, bool LOGIT, bool MASKED>
 void launch_masked(const RecParams& p, bool gradient) {
-    const unsigned grid = (unsigned)(p.channel_blocks * p.splits * p.batch);
+    const unsigned chains = (unsigned)p.chains, tiles = chains * (unsigned)p.tiles;
+    if (p.chained) {
+        const long long words = 3ll * tiles * kRecChannels;  // spans and states
+        recurrence_clear_kernel<<<(unsigned)((words + 1023) / 1024), 256>>>((unsigned*)p.chain_spans, words, p.ticket);
+    }
     if (gradient) {
-        if (p.splits > 1) recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, true><<<grid, 256>>>(p);
-        recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, false><<<grid, 256>>>(p);
+        if (p.chained) recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, true><<<tiles, 256>>>(p);
+        else recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, false><<<chains, 256>>>(p);
     } else if constexpr (DT == XT) {
-        if (p.splits > 1) recurrence_kernel<GT, XT, LOGIT, MASKED, true><<<grid, 256>>>(p);
-        recurrence_kernel<GT, XT, LOGIT, MASKED, false><<<grid, 256>>>(p);
+        if (p.chained) recurrence_kernel<GT, XT, LOGIT, MASKED, true><<<tiles, 256>>>(p);
+        else recurrence_kernel<GT, XT, LOGIT, MASKED, false><<<chains, 256>>>(p);
     }
 }
 template <int GT, int XT, int DT>
