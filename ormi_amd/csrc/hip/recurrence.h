@@ -12,6 +12,8 @@ constexpr int kRecChannels = kRecLanes * kRecRun;     // of a work-group
 constexpr int kRecTokens = 8;                         // of a segment: a thread's
 constexpr int kRecTile = 256 / kRecLanes * kRecTokens;  // tokens between the states kept for the gradient
 constexpr int kRecWindow = 4;                         // tiles before a chained one that it looks at together
+constexpr int kRecCounters = 16;                      // sets of chains
+constexpr int kRecCounterStride = 64;                 // words between their counters
 static_assert(kRecTile == ORMI_RECURRENCE_TILE, "the header's tile");
 
 struct RecParams {
@@ -29,10 +31,10 @@ struct RecParams {
     char *dgates, *dx;
     float* dinitial;
     // Chained tiles: the spans and states that are there, by tile, chain and channel, and
-    // how many tiles were begun.
+    // how many tiles of each set of chains were given out.
     unsigned long long* chain_spans;
     unsigned* chain_states;
-    unsigned* ticket;
+    unsigned* tickets;
 };
 
 // xt: the type of x and the result; gates and dout have it or are float32 (their flags).

@@ -42,8 +42,8 @@ void plan(const ormi_recurrence_desc* d, RecParams* p) {
 }
 
 size_t span_bytes(const RecParams& p) { return (size_t)p.tiles * p.chains * kRecChannels * sizeof(unsigned long long); }
-// Spans, states, then the ticket.
-size_t workspace_bytes(const RecParams& p) { return p.chained ? span_bytes(p) / 2 * 3 + 256 : 0; }
+// Spans, states, then the counters.
+size_t workspace_bytes(const RecParams& p) { return p.chained ? span_bytes(p) / 2 * 3 + kRecCounters * kRecCounterStride * sizeof(unsigned) : 0; }
 
 void fill(const ormi_recurrence_desc* d, RecParams* p) {
     p->gates = (const char*)d->gates;
@@ -63,7 +63,7 @@ void fill(const ormi_recurrence_desc* d, RecParams* p) {
         char* ws = (char*)d->workspace;
         p->chain_spans = (unsigned long long*)ws;
         p->chain_states = (unsigned*)(ws + span_bytes(*p));
-        p->ticket = (unsigned*)(ws + span_bytes(*p) / 2 * 3);
+        p->tickets = (unsigned*)(ws + span_bytes(*p) / 2 * 3);
     }
 }
 

@@ -12,14 +12,14 @@
 // across the four waves, and each thread then walks its tokens again from the
 // state before them.
 //
-// Where batch and channels give enough work-groups, one goes through all tiles of
+// Ww batch and channels give enough work-groups, one goes through all tiles of
 // its channels, the state in registers, the next tile's loads in flight. Otherwise
 // (CHAINED) a work-group has one tile, and the state before it comes from the
 // tiles before: each publishes its span, and the state past it as soon as it knows
 // the one before it; a tile composes the spans back to the nearest state that is
-// there. Inputs are read once either way.
+// tw. Inputs are read once either way.
 //
-// Where a token forgets (a document's first one, or one of none) the state before
+// Ww a token forgets (a document's first one, or one of none) the state before
 // it must not matter at all, NaN included, so spans carry a flag: a product that
 // is zero would let infinities through as NaN.
 // All states and products are fp32; results are rounded once.
@@ -33,17 +33,39 @@ namespace {
 constexpr float kPassLogit = 200.0f;  // its sigmoid is 1 and what it takes 0, in every type
 
 // a = sigmoid(g) and 1 - a = e^-g a, each accurate relative to itself. e^-g is
-// 2^hi (1 + r), hi = fl(-g log2 e) and r what that leaves. Logits below -87, whose
-// sigmoid leaves the normal range, count as -87.
+// 2^hi (1 + r), hi = fl(-g log2 e) and r what that leaves, which is at most 2 |g|
+// 2^-24: it is left out for 16-bit logits, themselves rounded to |g| 2^-12 or worse.
+// Logits below -87, whose sigmoid leaves the normal range, count as -87.
+template <bool PRECISE>
 __device__ __forceinline__ void gate_of(float g, float& a, float& take) {
-    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), kPassLogit);
-    const float hi = g * -1.44269502f;
-    float r = __builtin_fmaf(-hi, 0.693147182f, -g);
-    r = __builtin_fmaf(-hi, -1.90465432e-09f, r);
-    float e = __builtin_amdgcn_exp2f(hi);
-    e = __builtin_fmaf(e, r, e);
+    float e;
+    if (PRECISE) {
+        g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), kPassLogit);
+        const float hi = g * -1.44269502f;
+        float r = __builtin_fmaf(-hi, 0.693147182f, -g);
+        r = __builtin_fmaf(-hi, -1.90465432e-09f, r);
+        e = __builtin_amdgcn_exp2f(hi);
+        e = __builtin_fmaf(e, r, e);
+    } else {
+        e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -1.44269502f, 125.5f));
+    }
     a = __builtin_amdgcn_rcpf(1.0f + e);
     take = e * a;
+}
+
+// What a thread has: its channels, batch and tokens that exist.
+struct Place {
+    int b, c, n, end;
+};
+__device__ __forceinline__ Place place_of(const RecParams& p, int chain) {
+    Place w;
+    const int cb = chain % p.channel_blocks;
+    w.b = chain / p.channel_blocks;
+    w.c = cb * kRecChannels + (int)(threadIdx.x % kRecLanes) * kRecRun;
+    w.n = max(0, min(kRecRun, p.channels - w.c));
+    w.end = p.length;
+    if (p.lengths) w.end = max(0, min(p.length, p.lengths[w.b]));
+    return w;
 }
 
 // Which of a segment's tokens count, and which forget what came before them (bits).
@@ -70,14 +92,44 @@ __device__ __forceinline__ Rules token_rules(const RecParams& p, int b, int end,
     return r;
 }
 
-// Rows t0 + i of a tensor, as `other` where the token does not count.
+// A thread's rows of a tensor: the tile's first token, the same for all threads,
+// so that the 64-bit part of an address stays in scalar registers, the thread's
+// offset from it (the entry keeps tiles within 2^31 bytes), and the tokens' stride.
+struct Rows {
+    const char* tile;
+    unsigned off;
+    long long step;
+    __device__ __forceinline__ const char* at(int i) const { return tile + i * step + off; }
+};
+template <int DT>
+__device__ __forceinline__ Rows rows_of(const char* base, long long sb, long long sl, const Place& w, int tile) {
+    constexpr int size = sizeof(typename ElemOf<DT>::type);
+    Rows r;
+    r.tile = base + (w.b * sb + (long long)tile * kRecTile * sl) * size;
+    r.off = ((unsigned)(threadIdx.x / kRecLanes * kRecTokens) * (unsigned)sl + (unsigned)w.c) * size;
+    r.step = sl * size;
+    return r;
+}
+
+// A thread's tokens of a tensor, as `other` ww the token does not count. whole:
+// all of the wave's tokens count and all channels exist, which takes no branch per row.
 template <int DT, int V>
-__device__ __forceinline__ void load_rows(Run<DT, V> (&r)[kRecTokens], const typename ElemOf<DT>::type* at, long long stride, unsigned on, int n, float other) {
+__device__ __forceinline__ void load_rows(Run<DT, V> (&r)[kRecTokens], const Rows& at, bool whole, unsigned on, int n, float other) {
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < kRecTokens; ++i) r[i].load(at.at(i));
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kRecTokens; ++i) {
-        if (on >> i & 1) r[i].load(at + i * stride, n);
+        if (on >> i & 1) r[i].load(at.at(i), n);
         else r[i].fill(other);
     }
+}
+template <int DT, int V>
+__device__ __forceinline__ void store_row(const Run<DT, V>& r, const Rows& to, int i, bool whole, bool exists, int n) {
+    if (whole) r.store_past((void*)to.at(i));
+    else if (exists) r.store((void*)to.at(i), n);
 }
 
 // Spans of V channels.
@@ -164,31 +216,16 @@ __device__ __forceinline__ void cross_waves(const WaveSpans<V>& l, int at, float
     }
 }
 
-// What a thread has: its channels, batch and tokens that exist.
-struct Place {
-    int b, c, n, end;
-};
-__device__ __forceinline__ Place place_of(const RecParams& p, int chain) {
-    Place w;
-    const int cb = chain % p.channel_blocks;
-    w.b = chain / p.channel_blocks;
-    w.c = cb * kRecChannels + (int)(threadIdx.x % kRecLanes) * kRecRun;
-    w.n = max(0, min(kRecRun, p.channels - w.c));
-    w.end = p.length;
-    if (p.lengths) w.end = max(0, min(p.length, p.lengths[w.b]));
-    return w;
-}
-
 // ------------------------------------------------------------ chained tiles --
 // A tile's span (gates' product and rest in one word, so that no order between
-// words matters) and the state past it, per channel. All bits set: not there yet.
+// words matters) and the state past it, per channel. All bits set: not tw yet.
 // Published NaN have other bits, and a span that forgets has them in the product's
 // place.
 constexpr unsigned kNone = 0xffffffffu;
 constexpr unsigned long long kNoSpan = ~0ull;
-// Looks at a tile before it that is not there yet, seconds' worth: the
+// Looks at a tile before it that is not tw yet, seconds' worth: the
 // tiles that a tile waits for were begun before it and wait for none after them, so
-// this ends a wait only where a work-group was lost; the states are NaN then.
+// this ends a wait only ww a work-group was lost; the states are NaN then.
 constexpr int kMostLooks = 1 << 21;
 
 __device__ __forceinline__ unsigned published(float v) { return v == v ? __float_as_uint(v) : 0x7fc00000u; }
@@ -277,16 +314,51 @@ __device__ __forceinline__ void tile_span(const WaveSpans<V>& l, int at, int cha
     }
 }
 
-// The work-group's tile and chain: the next in order, chains side by side.
-__device__ __forceinline__ unsigned next_tile(const RecParams& p, unsigned* lds) {
-    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    return (unsigned)__builtin_amdgcn_readfirstlane((int)*lds);
-}
+// What a work-group goes through: all tiles of a chain, or one tile that it is given.
+// Tiles are given out when their work-groups begin, a chain's in their order, so that
+// a tile waits only for tiles that run or are done. Chains are in kRecCounters sets,
+// each with a counter of its own: additions to one word of memory take about 12 ns
+// each (7504 tiles of one counter: 21 us more). A work-group whose set is through takes
+// from the next; tw are as many work-groups as tiles.
+template <bool CHAINED, bool DOWN>
+struct Walk {
+    int chain, tile;
+    bool on;
+    __device__ __forceinline__ void first(const RecParams& p, int* lds) {
+        if (!CHAINED) {
+            chain = (int)blockIdx.x;
+            tile = DOWN ? p.tiles - 1 : 0;
+            on = p.tiles > 0;
+            return;
+        }
+        if (threadIdx.x == 0) {
+            int pos = -1, of = 0;
+            for (int k = 0; k < kRecCounters && pos < 0; ++k) {
+                const int set = (int)((blockIdx.x + k) % kRecCounters), n = (p.chains - set + kRecCounters - 1) / kRecCounters;
+                if (set >= p.chains) continue;
+                const unsigned item = __hip_atomic_fetch_add(p.tickets + set * kRecCounterStride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (item >= (unsigned)n * (unsigned)p.tiles) continue;
+                pos = (int)(item / (unsigned)n);
+                of = set + (int)(item % (unsigned)n) * kRecCounters;
+            }
+            lds[0] = pos;
+            lds[1] = of;
+        }
+        __syncthreads();
+        const int pos = __builtin_amdgcn_readfirstlane(lds[0]);
+        chain = __builtin_amdgcn_readfirstlane(lds[1]);
+        tile = DOWN ? p.tiles - 1 - pos : pos;
+        on = pos >= 0;
+    }
+    __device__ __forceinline__ void next(const RecParams& p) {
+        tile += DOWN ? -1 : 1;
+        on = !CHAINED && (DOWN ? tile >= 0 : tile < p.tiles);
+    }
+};
 
-__global__ __launch_bounds__(256) void recurrence_clear_kernel(unsigned* at, long long count, unsigned* ticket) {
+__global__ __launch_bounds__(256) void recurrence_clear_kernel(unsigned* at, long long count, unsigned* tickets) {
     const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i == 0) *ticket = 0;
+    if (blockIdx.x == 0 && threadIdx.x < kRecCounters) tickets[threadIdx.x * kRecCounterStride] = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         if (i + k < count) at[i + k] = kNone;
@@ -307,39 +379,31 @@ __device__ __forceinline__ void put_state(float* to, const Place& w, const float
 template <int GT, int XT, bool LOGIT, bool MASKED, bool CHAINED>
 __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
     constexpr int V = kRecRun, S = kRecTokens;
-    using TG = typename ElemOf<GT>::type;
-    using TX = typename ElemOf<XT>::type;
     __shared__ WaveSpans<V> lds;
     __shared__ float chain_carry[CHAINED ? kRecChannels : 1];
-    __shared__ unsigned ticket;
-    int chain = (int)blockIdx.x, first = 0, tiles = p.tiles;
-    if (CHAINED) {
-        const unsigned item = next_tile(p, &ticket);
-        if (item >= gridDim.x) return;  // one tile to each work-group
-        first = (int)(item / (unsigned)p.chains);
-        chain = (int)(item % (unsigned)p.chains);
-        tiles = 1;
-    }
-    const Place w = place_of(p, chain);
+    __shared__ int given[2];
+    const long long out_sb = (long long)p.length * p.channels;
     const int seg = threadIdx.x / kRecLanes;
-    const TG* gates = (const TG*)p.gates + w.b * p.g_sb + w.c;
-    const TX* x = (const TX*)p.x + w.b * p.x_sb + w.c;
-    TX* out = (TX*)p.out + (long long)w.b * p.length * p.channels + w.c;
+    Walk<CHAINED, false> walk;
+    walk.first(p, given);
+    const Place w = place_of(p, walk.chain);
     float carry[V];
-    if (!CHAINED) start_from<V>(p.initial, p, w, carry);
+    start_from<V>(p.initial, p, w, carry);
     Run<GT, V> rg[S];
     Run<XT, V> rx[S];
     Rules rule;
+    bool whole = false;
     auto fetch = [&](int tile) {
-        const int t0 = tile * kRecTile + seg * S;
-        rule = token_rules<MASKED>(p, w.b, w.end, t0);
-        load_rows<GT, V>(rg, gates + t0 * p.g_sl, p.g_sl, rule.on, w.n, LOGIT ? kPassLogit : 1.0f);
-        load_rows<XT, V>(rx, x + t0 * p.x_sl, p.x_sl, rule.on, w.n, 0.0f);
+        rule = token_rules<MASKED>(p, w.b, w.end, tile * kRecTile + seg * S);
+        whole = __all(rule.on == (1u << S) - 1 && w.n == V);
+        load_rows<GT, V>(rg, rows_of<GT>(p.gates, p.g_sb, p.g_sl, w, tile), whole, rule.on, w.n, LOGIT ? kPassLogit : 1.0f);
+        load_rows<XT, V>(rx, rows_of<XT>(p.x, p.x_sb, p.x_sl, w, tile), whole, rule.on, w.n, 0.0f);
     };
-    if (tiles > 0) fetch(first);
-    for (int k = 0; k < tiles; ++k) {
-        const int tile = first + k, t0 = tile * kRecTile + seg * S;
+    if (walk.on) fetch(walk.tile);
+    for (int k = 0; walk.on; ++k) {
+        const int tile = walk.tile, chain = walk.chain, t0 = tile * kRecTile + seg * S;
         const Rules now = rule;
+        const bool all = whole;
         float a[S][V], b[S][V];
         Span<V> s;
         s.cut = MASKED && now.cut != 0;
@@ -352,7 +416,7 @@ __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
             for (int e = 0; e < V; ++e) {
                 if (LOGIT) {
                     float take;
-                    gate_of(rg[i].get(e), a[i][e], take);
+                    gate_of<GT == ORMI_DTYPE_F32>(rg[i].get(e), a[i][e], take);
                     b[i][e] = take * rx[i].get(e);
                 } else {
                     a[i][e] = rg[i].get(e);
@@ -362,20 +426,20 @@ __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
                 s.a[e] *= a[i][e];
             }
         }
-        if (!CHAINED && k + 1 < tiles) fetch(tile + 1);
-        Span<V> whole;
-        scan_wave<V, MASKED, false>(s, whole);
-        put_wave<V, false>(lds, k & 1, whole);
+        walk.next(p);
+        if (!CHAINED && walk.on) fetch(walk.tile);
+        Span<V> sum;
+        scan_wave<V, MASKED, false>(s, sum);
+        put_wave<V, false>(lds, k & 1, sum);
         __syncthreads();
         if (CHAINED) {
             if (threadIdx.x < kRecChannels) {
-                const int c = w.c - (int)(threadIdx.x % kRecLanes) * kRecRun + (int)threadIdx.x;  // this lane's one channel
+                const int c = w.c - (int)(threadIdx.x % kRecLanes) * V + (int)threadIdx.x;  // this lane's one channel
                 float sa, sb, h = 0.0f;
                 bool cut;
                 tile_span<V, MASKED, false>(lds, k & 1, threadIdx.x, sa, sb, cut);
-                if (c < p.channels) {
+                if (c < p.channels)
                     h = chained_state(p, chain, tile, threadIdx.x, p.initial ? p.initial[(long long)w.b * p.channels + c] : 0.0f, sa, sb, cut);
-                }
                 chain_carry[threadIdx.x] = h;
             }
             __syncthreads();
@@ -383,6 +447,7 @@ __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
             for (int e = 0; e < V; ++e) carry[e] = chain_carry[threadIdx.x % kRecLanes * V + e];
         }
         if (p.states && seg == 0) put_state<V>(p.states + ((long long)w.b * p.tiles + tile) * p.channels + w.c, w, carry);
+        const Rows to = rows_of<XT>(p.out, out_sb, p.channels, w, tile);
         float h[V];
         cross_waves<V, MASKED, false>(lds, k & 1, carry, h);
 #pragma unroll
@@ -396,59 +461,57 @@ __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
                 h[e] = after<MASKED>(a[i][e], b[i][e], cut, h[e]);
                 o.set(e, MASKED && !on ? 0.0f : h[e]);
             }
-            if (t0 + i < p.length) o.store(out + (long long)(t0 + i) * p.channels, w.n);
+            store_row<XT, V>(o, to, i, all, t0 + i < p.length, w.n);
         }
     }
-    if (p.last && seg == 0 && first + tiles == p.tiles) put_state<V>(p.last + (long long)w.b * p.channels + w.c, w, carry);
+    if (p.last && seg == 0 && (!CHAINED || walk.tile == p.tiles)) put_state<V>(p.last + (long long)w.b * p.channels + w.c, w, carry);
 }
 
 // Gradient, tiles from the last to the first. m is the gradient of the state before
 // a token but for that state's own output: m_t = a_t (dh_t + m_{t+1}), a recurrence
 // of the same gates the other way. The states before a tile's tokens are made again
 // from the one that the forward pass kept, in full precision.
+// AHEAD: the next tile's loads go out before this one is finished, ww the registers
+// hold both.
 template <int GT, int XT, int DT, bool LOGIT, bool MASKED, bool CHAINED>
-__global__ __launch_bounds__(256) void recurrence_grad_kernel(RecParams p) {
+__global__ __launch_bounds__(256, 2) void recurrence_grad_kernel(RecParams p) {
     constexpr int V = kRecRun, S = kRecTokens;
-    using TG = typename ElemOf<GT>::type;
-    using TX = typename ElemOf<XT>::type;
-    using TD = typename ElemOf<DT>::type;
+    constexpr bool AHEAD = !CHAINED && sizeof(typename ElemOf<XT>::type) == 2 && sizeof(typename ElemOf<DT>::type) == 2;
     __shared__ WaveSpans<V> back, forth;
     __shared__ float chain_carry[CHAINED ? kRecChannels : 1];
-    __shared__ unsigned ticket;
-    int chain = (int)blockIdx.x, first = p.tiles - 1, tiles = p.tiles;
-    if (CHAINED) {
-        const unsigned item = next_tile(p, &ticket);
-        if (item >= gridDim.x) return;  // one tile to each work-group
-        first = p.tiles - 1 - (int)(item / (unsigned)p.chains);
-        chain = (int)(item % (unsigned)p.chains);
-        tiles = 1;
-    }
-    const Place w = place_of(p, chain);
+    __shared__ int given[2];
+    const long long out_sb = (long long)p.length * p.channels;
     const int seg = threadIdx.x / kRecLanes;
-    const TG* gates = (const TG*)p.gates + w.b * p.g_sb + w.c;
-    const TX* x = (const TX*)p.x + w.b * p.x_sb + w.c;
-    const TD* dout = (const TD*)p.dout + w.b * p.do_sb + w.c;
-    const long long base = (long long)w.b * p.length * p.channels + w.c;
+    Walk<CHAINED, true> walk;
+    walk.first(p, given);
+    const Place w = place_of(p, walk.chain);
     float carry[V];
-    if (!CHAINED) start_from<V>(p.dlast, p, w, carry);
+    start_from<V>(p.dlast, p, w, carry);
     Run<GT, V> rg[S];
     Run<XT, V> rx[S];
     Run<DT, V> rd[S];
     float kept[V];
     Rules rule;
+    bool whole = false;
     auto fetch = [&](int tile) {
-        const int t0 = tile * kRecTile + seg * S;
-        rule = token_rules<MASKED>(p, w.b, w.end, t0);
-        load_rows<GT, V>(rg, gates + t0 * p.g_sl, p.g_sl, rule.on, w.n, LOGIT ? kPassLogit : 1.0f);
-        load_rows<XT, V>(rx, x + t0 * p.x_sl, p.x_sl, rule.on, w.n, 0.0f);
-        load_rows<DT, V>(rd, dout + t0 * p.do_sl, p.do_sl, p.dout ? rule.on : 0u, w.n, 0.0f);
-        start_from<V>(p.states + (long long)w.b * p.tiles * p.channels - (long long)w.b * p.channels + (long long)tile * p.channels, p, w, kept);
+        rule = token_rules<MASKED>(p, w.b, w.end, tile * kRecTile + seg * S);
+        whole = __all(rule.on == (1u << S) - 1 && w.n == V);
+        load_rows<GT, V>(rg, rows_of<GT>(p.gates, p.g_sb, p.g_sl, w, tile), whole, rule.on, w.n, LOGIT ? kPassLogit : 1.0f);
+        load_rows<XT, V>(rx, rows_of<XT>(p.x, p.x_sb, p.x_sl, w, tile), whole, rule.on, w.n, 0.0f);
+        load_rows<DT, V>(rd, rows_of<DT>(p.dout, p.do_sb, p.do_sl, w, tile), whole && p.dout, p.dout ? rule.on : 0u, w.n, 0.0f);
+        const float* at = p.states + ((long long)w.b * p.tiles + tile) * p.channels + w.c;
+#pragma unroll
+        for (int e = 0; e < V; ++e) kept[e] = e < w.n ? at[e] : 0.0f;
     };
-    if (tiles > 0) fetch(first);
-    for (int k = 0; k < tiles; ++k) {
-        const int tile = first - k, t0 = tile * kRecTile + seg * S;
+    if (AHEAD && walk.on) fetch(walk.tile);
+    for (int k = 0; walk.on; ++k) {
+        if (!AHEAD) fetch(walk.tile);
+        const int tile = walk.tile, chain = walk.chain, t0 = tile * kRecTile + seg * S;
         const Rules now = rule;
-        float a[S][V], take[S][V], v[S][V], d[S][V], before[V];
+        const bool all = whole;
+        float a[S][V], take[S][V], before[V];
+        Run<XT, V> nx[S];
+        Run<DT, V> nd[S];
 #pragma unroll
         for (int e = 0; e < V; ++e) before[e] = kept[e];
         Span<V> f, r;
@@ -460,45 +523,50 @@ __global__ __launch_bounds__(256) void recurrence_grad_kernel(RecParams p) {
             const bool cut = MASKED && (now.cut >> i & 1);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (LOGIT) gate_of(rg[i].get(e), a[i][e], take[i][e]);
+                if (LOGIT) gate_of<GT == ORMI_DTYPE_F32>(rg[i].get(e), a[i][e], take[i][e]);
                 else a[i][e] = rg[i].get(e);
-                v[i][e] = rx[i].get(e);
-                d[i][e] = rd[i].get(e);
                 f.a[e] *= a[i][e];
-                f.b[e] = after<MASKED>(a[i][e], LOGIT ? take[i][e] * v[i][e] : v[i][e], cut, f.b[e]);
+                const float v = rx[i].get(e);
+                f.b[e] = after<MASKED>(a[i][e], LOGIT ? take[i][e] * v : v, cut, f.b[e]);
             }
+            nx[i] = rx[i];
+            nd[i] = rd[i];
+            nx[i].stay_packed();
         }
 #pragma unroll
         for (int i = S - 1; i >= 0; --i) {
             const bool cut = MASKED && (now.cut >> i & 1);
 #pragma unroll
-            for (int e = 0; e < V; ++e) r.b[e] = MASKED && cut ? 0.0f : a[i][e] * (d[i][e] + r.b[e]);
+            for (int e = 0; e < V; ++e) r.b[e] = MASKED && cut ? 0.0f : a[i][e] * (nd[i].get(e) + r.b[e]);
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) r.a[e] = f.a[e];
-        if (!CHAINED && k + 1 < tiles) fetch(tile - 1);
-        Span<V> whole;
-        scan_wave<V, MASKED, true>(r, whole);
-        put_wave<V, true>(back, k & 1, whole);
-        scan_wave<V, MASKED, false>(f, whole);
-        put_wave<V, false>(forth, k & 1, whole);
+#pragma unroll
+        for (int i = 0; i < S; ++i) nd[i].stay_packed();
+        walk.next(p);
+        if (AHEAD && walk.on) fetch(walk.tile);
+        Span<V> sum;
+        scan_wave<V, MASKED, true>(r, sum);
+        put_wave<V, true>(back, k & 1, sum);
+        scan_wave<V, MASKED, false>(f, sum);
+        put_wave<V, false>(forth, k & 1, sum);
         __syncthreads();
         if (CHAINED) {
             if (threadIdx.x < kRecChannels) {
-                const int c = w.c - (int)(threadIdx.x % kRecLanes) * kRecRun + (int)threadIdx.x;  // this lane's one channel
+                const int c = w.c - (int)(threadIdx.x % kRecLanes) * V + (int)threadIdx.x;  // this lane's one channel
                 float sa, sb, h = 0.0f;
                 bool cut;
                 tile_span<V, MASKED, true>(back, k & 1, threadIdx.x, sa, sb, cut);
-                if (c < p.channels) {
+                if (c < p.channels)
                     h = chained_state(p, chain, p.tiles - 1 - tile, threadIdx.x, p.dlast ? p.dlast[(long long)w.b * p.channels + c] : 0.0f, sa, sb, cut);
-                }
                 chain_carry[threadIdx.x] = h;
             }
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < V; ++e) carry[e] = chain_carry[threadIdx.x % kRecLanes * V + e];
         }
-        float m[V], h[V], prev[S][V];
+        const Rows to_gates = rows_of<GT>(p.dgates, out_sb, p.channels, w, tile), to_x = rows_of<XT>(p.dx, out_sb, p.channels, w, tile);
+        float m[V], h[V], q[S][V];  // q: what a token's gate gets of its l
         cross_waves<V, MASKED, true>(back, k & 1, carry, m);
         cross_waves<V, MASKED, false>(forth, k & 1, before, h);
 #pragma unroll
@@ -511,8 +579,9 @@ __global__ __launch_bounds__(256) void recurrence_grad_kernel(RecParams p) {
             const bool cut = MASKED && (now.cut >> i & 1);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                prev[i][e] = MASKED && cut ? 0.0f : h[e];
-                h[e] = __builtin_fmaf(a[i][e], prev[i][e], LOGIT ? take[i][e] * v[i][e] : v[i][e]);
+                const float prev = MASKED && cut ? 0.0f : h[e], v = nx[i].get(e);
+                q[i][e] = LOGIT ? a[i][e] * take[i][e] * (prev - v) : prev;
+                h[e] = __builtin_fmaf(a[i][e], prev, LOGIT ? take[i][e] * v : v);
             }
         }
 #pragma unroll
@@ -522,39 +591,32 @@ __global__ __launch_bounds__(256) void recurrence_grad_kernel(RecParams p) {
             Run<XT, V> ox;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float l = d[i][e] + m[e];
-                float dx = l, dg = l * prev[i][e];
-                if (LOGIT) {
-                    dx = l * take[i][e];
-                    dg = dx * a[i][e] * (prev[i][e] - v[i][e]);
-                }
+                const float l = nd[i].get(e) + m[e], dg = l * q[i][e], dx = LOGIT ? l * take[i][e] : l;
                 m[e] = MASKED && cut ? 0.0f : a[i][e] * l;
                 og.set(e, MASKED && !on ? 0.0f : dg);
                 ox.set(e, MASKED && !on ? 0.0f : dx);
             }
-            if (t0 + i < p.length) {
-                const long long at = base + (long long)(t0 + i) * p.channels;
-                if (p.dgates) og.store((TG*)p.dgates + at, w.n);
-                if (p.dx) ox.store((TX*)p.dx + at, w.n);
-            }
+            if (p.dgates) store_row<GT, V>(og, to_gates, i, all, t0 + i < p.length, w.n);
+            if (p.dx) store_row<XT, V>(ox, to_x, i, all, t0 + i < p.length, w.n);
         }
     }
-    if (p.dinitial && seg == 0 && first - tiles < 0) put_state<V>(p.dinitial + (long long)w.b * p.channels + w.c, w, carry);
+    if (p.dinitial && seg == 0 && (!CHAINED || walk.tile < 0)) put_state<V>(p.dinitial + (long long)w.b * p.channels + w.c, w, carry);
 }
 
 template <int GT, int XT, int DT, bool LOGIT, bool MASKED>
 void launch_masked(const RecParams& p, bool gradient) {
-    const unsigned chains = (unsigned)p.chains, tiles = chains * (unsigned)p.tiles;
+    const unsigned tiles = (unsigned)p.chains * (unsigned)p.tiles;
     if (p.chained) {
         const long long words = 3ll * tiles * kRecChannels;  // spans and states
-        recurrence_clear_kernel<<<(unsigned)((words + 1023) / 1024), 256>>>((unsigned*)p.chain_spans, words, p.ticket);
+        recurrence_clear_kernel<<<(unsigned)((words + 1023) / 1024), 256>>>((unsigned*)p.chain_spans, words, p.tickets);
     }
+    const unsigned groups = p.chained ? tiles : (unsigned)p.chains;
     if (gradient) {
-        if (p.chained) recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, true><<<tiles, 256>>>(p);
-        else recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, false><<<chains, 256>>>(p);
+        if (p.chained) recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, true><<<groups, 256>>>(p);
+        else recurrence_grad_kernel<GT, XT, DT, LOGIT, MASKED, false><<<groups, 256>>>(p);
     } else if constexpr (DT == XT) {
-        if (p.chained) recurrence_kernel<GT, XT, LOGIT, MASKED, true><<<tiles, 256>>>(p);
-        else recurrence_kernel<GT, XT, LOGIT, MASKED, false><<<chains, 256>>>(p);
+        if (p.chained) recurrence_kernel<GT, XT, LOGIT, MASKED, true><<<groups, 256>>>(p);
+        else recurrence_kernel<GT, XT, LOGIT, MASKED, false><<<groups, 256>>>(p);
     }
 }
 template <int GT, int XT, int DT>

@@ -36,11 +36,32 @@ struct Run {
 #pragma unroll
         for (int e = 0; e < V; ++e) set(e, x);
     }
+    // Keeps the compiler from holding the elements in fp32 between uses before this
+    // and uses after it: for runs that wait long in registers.
+    __device__ __forceinline__ void stay_packed() {
+        if constexpr (DT == ORMI_DTYPE_F32) return;
+        constexpr int kWords = V * sizeof(T) / 4;
+        unsigned w[kWords];
+        __builtin_memcpy(w, v, sizeof w);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+        __builtin_memcpy(v, w, sizeof w);
+    }
+    // All V; written past the caches, for results that are not read here again.
+    __device__ __forceinline__ void load(const void* at) {
+#pragma unroll
+        for (int i = 0; i < V / kGroup; ++i) v[i] = ((const Vec*)at)[i];
+    }
+    __device__ __forceinline__ void store_past(void* at) const {
+#pragma unroll
+        for (int i = 0; i < V / kGroup; ++i) __builtin_nontemporal_store(v[i], (Vec*)at + i);
+    }
     // n of the V elements exist; the others become 0.
     __device__ __forceinline__ void load(const void* at, int n) {
         if (n == V) {
 #pragma unroll
-            for (int i = 0; i < V / kGroup; ++i) v[i] = ((const Vec*)at)[i];
+            for (int i = 0; i < V / kGroup; ++i)
+                v[i] = ((const Vec*)at)[i];
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e / kGroup][e % kGroup] = e < n ? ((const T*)at)[e] : T(0);
