@@ -570,7 +570,8 @@ int ormi_hip_adamw_values(float* m, float* v, const void* m_codes, const float* 
  * states (or NULL) receives the state before every ORMI_RECURRENCE_TILE-th
  * token, (batch, ceil(length / tile), channels) fp32: the gradient needs it.
  * workspace: device memory of *_workspace_size() bytes, 256-byte aligned (NULL
- * where that is 0), for this call and for the gradient's. Lengths go up to 2^30.
+ * where that is 0), for this call and for the gradient's. Lengths go up to 2^30,
+ * channels and strides over tokens (not negative) to 2^20.
  * Sums have a fixed order: the same call gives the same bits. */
 #define ORMI_RECURRENCE_TILE 128
 typedef struct ormi_recurrence_desc {
@@ -629,7 +630,8 @@ int ormi_hip_recurrence_grad(const ormi_recurrence_grad_desc* desc);
  * last (or NULL) receives the inputs that a token after the last one that
  * counts would read if it went on with its document, laid out like initial
  * (zeros after a token of a negative document).
- * Sums are fp32 in a fixed order, results are rounded once. */
+ * Sums are fp32 in a fixed order, results are rounded once. Lengths go up to
+ * 2^30, channels and strides over tokens (not negative) to 2^20. */
 #define ORMI_CONV_MAX_WIDTH 8
 typedef struct ormi_conv_desc {
     int            dtype;

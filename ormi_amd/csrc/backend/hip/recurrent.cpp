@@ -13,10 +13,12 @@ namespace ormi::hip {
     using ops::OpEnum;
 
     namespace {
-        // n (batch, length, channels) as the entries read it, neighbouring channels.
+        // n (batch, length, channels) as the entries read it: neighbouring channels, and
+        // tokens at most 2^20 elements apart.
         NodePtr rows(const NodePtr& n) {
             realize(n);
-            return n->view.shape[2] <= 1 || n->view.strides[2] == 1 ? n : contiguous(n);
+            const auto& v = n->view;
+            return (v.shape[2] <= 1 || v.strides[2] == 1) && (v.shape[1] <= 1 || v.strides[1] <= 1 << 20) ? n : contiguous(n);
         }
         void strides2(const Node& n, int64_t (&out)[2]) {
             out[0] = n.view.strides[0];

@@ -6,14 +6,12 @@
 
 namespace ormi_hip {
 
-constexpr int kConvLanes = 8;       // threads side by side over the channels
-constexpr int kConvRuns = 32;       // runs of tokens of a tile
-constexpr int kConvTokens = 8;      // of a run, forward
-constexpr int kConvGradTokens = 8;  // of a run, backward
-
-// Channels of a thread: a 16-byte access, half of one for 16-bit channels with
-// more weights than registers hold beside their sums.
-constexpr int conv_run(int dt, int width) { return dt == ORMI_DTYPE_F32 || width > 4 ? 4 : 8; }
+constexpr int kConvLanes = 16;                 // threads side by side over the channels
+constexpr int kConvRun = 4;                    // channels of a thread
+constexpr int kConvRuns = 256 / kConvLanes;    // runs of tokens of a tile
+// Widths that kernels are built for: 3 and 4, and 4 and 8 for all up to them.
+constexpr int conv_width(int width, bool masked) { return width == 3 && !masked ? 3 : width <= 4 ? 4 : 8; }
+constexpr int run_tokens(int width) { return 32 / width * width; }  // of a thread's run: whole groups of that width
 
 struct ConvParams {
     const char *x, *initial, *dout;

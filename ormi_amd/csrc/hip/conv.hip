@@ -14,7 +14,11 @@ namespace {
 constexpr long long kMostGroups = (1ll << 24) - 1;  // of 256 threads: a launch holds fewer than 2^32
 constexpr int kMostTokens = 1 << 30;                // token numbers of a last tile stay in 31 bits
 
+constexpr int kMostStride = 1 << 20;                // elements between tokens: a tile's offsets stay in 32 bits
+
 bool is_float(int dt) { return dt == ORMI_DTYPE_F32 || dt == ORMI_DTYPE_BF16 || dt == ORMI_DTYPE_F16; }
+
+bool near(int length, int64_t stride) { return length <= 1 || (stride >= 0 && stride <= kMostStride); }
 
 const char* check(const ormi_conv_desc* d) {
     if (!d) return "null descriptor";
@@ -22,27 +26,27 @@ const char* check(const ormi_conv_desc* d) {
     if (d->batch < 0 || d->length < 0 || d->channels < 0) return "negative extent";
     if (d->width < 1 || d->width > ORMI_CONV_MAX_WIDTH) return "width must be 1 to 8";
     if (d->length > kMostTokens) return "more than 2^30 tokens";
+    if (d->channels > kMostStride) return "more than 2^20 channels";
+    if (!near(d->length, d->x_strides[1])) return "tokens more than 2^20 elements apart";
     return nullptr;
 }
 
 // False: more work-groups than a launch holds.
 bool plan(const ormi_conv_desc* d, bool gradient, ConvParams* p) {
-    const int run = conv_run(d->dtype, d->width), tokens = kConvRuns * (gradient ? kConvGradTokens : kConvTokens);
+    const int tokens = kConvRuns * run_tokens(conv_width(d->width, d->documents || d->lengths));
     p->batch = d->batch;
     p->length = d->length;
     p->channels = d->channels;
     p->width = d->width;
     p->silu = d->silu;
-    p->channel_blocks = (int)((d->channels + (long long)kConvLanes * run - 1) / (kConvLanes * run));
+    p->channel_blocks = (int)((d->channels + kConvLanes * kConvRun - 1ll) / (kConvLanes * kConvRun));
     p->tiles = (d->length + tokens - 1) / tokens;
     p->parts = p->tiles;
     const long long rows = (long long)p->channel_blocks * d->batch;
     if (gradient) {
         // A work-group's sums of the weights' gradients are a row for the second
-        // launch: no more of them than keep the card busy. No token still leaves
-        // the initial inputs' gradient.
-        p->tiles = std::max(1, p->tiles);
-        p->parts = (int)std::max(1ll, std::min<long long>(p->tiles, (8ll * compute_units() + rows - 1) / std::max(1ll, rows)));
+        // launch: no more of them than keep the card busy.
+        p->parts = (int)std::min<long long>(p->tiles, (8ll * compute_units() + rows - 1) / std::max(1ll, rows));
     }
     return rows * p->parts <= kMostGroups;
 }
@@ -113,6 +117,7 @@ int ormi_hip_conv_grad(const ormi_conv_grad_desc* g) {
     const ormi_conv_desc* d = &g->forward;
     if (const char* what = check(d)) return bad(what);
     if (g->dout && g->dout_dtype != d->dtype && g->dout_dtype != ORMI_DTYPE_F32) return bad("dout must have x's type or float32");
+    if (g->dout && !near(d->length, g->dout_strides[1])) return bad("tokens more than 2^20 elements apart");
     if (d->channels == 0) return ORMI_HIP_OK;
     if (!d->weight) return bad("null weight");
     if (d->length > 0 && d->batch > 0 && !d->x) return bad("null x");

@@ -2,10 +2,12 @@
 //   z_t = bias + sum_j w_j x_{t - W + 1 + j},  y = z or z sigmoid(z)
 // and its gradient, with dz = dy, or dy (s + z s (1 - s)), s = sigmoid(z):
 //   dx_t = sum_j w_j dz_{t + W - 1 - j},  dw_j = sum_t dz_t x_{t - W + 1 + j},  db = sum_t dz_t.
-// Bound by memory: 2 W flops an element forward, 4 W more backward. A thread has the
-// channels of a 16-byte access and a run of tokens; the rows before (and, backward,
-// after) its run come out of the caches, where its neighbours' reads left them. A
-// work-group is 32 such runs by 128 bytes of a row.
+// Bound by memory: 2 W flops an element forward, 4 W more backward. A thread has four
+// channels and goes through a run of tokens, W at a time: the inputs that they read
+// and the gradients still being summed stay in registers, the next W rows are on
+// their way. A work-group is 16 such runs by 64 channels. (All of a run's rows in
+// registers at once took 256 of them, one wave to a SIMD: 229 us for the gradient of
+// 8 x 2048 x 4096 bf16.)
 // dw and db are summed by a thread over its tokens, then over a work-group, which
 // goes through several tiles; each leaves one partial row, and a second launch adds
 // those up in their order.
@@ -16,57 +18,34 @@
 namespace ormi_hip {
 namespace {
 
-// The inputs of one batch: x, and `initial` before it.
-template <int DT>
-struct Inputs {
-    using T = typename ElemOf<DT>::type;
-    const T *x, *initial;  // at the thread's channels
-    long long stride, initial_stride;
-};
-
-// The first token of token t's run of one document within width - 1 tokens before
-// it (initial inputs have negative numbers): no farther than that matters.
-__device__ __forceinline__ int run_start(const int* docs, int t, int width) {
-    int from = t;
-    const int first = t - (width - 1);
-    if (!docs) return first;
-    const int own = docs[t];
-    while (from > first) {
-        if (from > 0 && docs[from - 1] != own) break;
-        --from;
-    }
-    return from;
+// 1 / (1 + e^-z). For 16-bit results without what rounding -z log2 e leaves, at most
+// 2 |z| 2^-24 of e^-z.
+template <bool PRECISE>
+__device__ __forceinline__ float conv_sigmoid(float z) {
+    if (PRECISE) return ormi_sigmoid(z);
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269502f));
 }
-
-__device__ __forceinline__ float silu(float z) { return z * ormi_sigmoid(z); }
 // s + z s (1 - s): for large z the difference loses its own accuracy, not the sum.
+template <bool PRECISE>
 __device__ __forceinline__ float silu_grad(float z) {
-    const float s = ormi_sigmoid(z);
+    const float s = conv_sigmoid<PRECISE>(z);
     return __builtin_fmaf(z * s, 1.0f - s, s);
 }
 
 struct ConvPlace {
-    int b, c, n, part, end;
+    int b, c, n, part, end, run;
 };
-template <int V>
 __device__ __forceinline__ ConvPlace conv_place(const ConvParams& p) {
     ConvPlace w;
-    const int cb = blockIdx.x % p.channel_blocks, rest = blockIdx.x / p.channel_blocks;
+    const int cb = (int)(blockIdx.x % p.channel_blocks), rest = (int)(blockIdx.x / p.channel_blocks);
     w.part = rest % p.parts;
     w.b = rest / p.parts;
-    w.c = (cb * kConvLanes + (threadIdx.x & 7)) * V;
-    w.n = max(0, min(V, p.channels - w.c));
+    w.run = threadIdx.x / kConvLanes;
+    w.c = (cb * kConvLanes + (int)(threadIdx.x % kConvLanes)) * kConvRun;
+    w.n = max(0, min(kConvRun, p.channels - w.c));
     w.end = p.length;
     if (p.lengths) w.end = max(0, min(p.length, p.lengths[w.b]));
     return w;
-}
-
-// Input t (t < 0: an initial one), 0 where there is none.
-template <int DT, int V>
-__device__ __forceinline__ void load_input(Run<DT, V>& r, const Inputs<DT>& in, int t, int end, int back, int n) {
-    if (t >= 0 && t < end) r.load(in.x + t * in.stride, n);
-    else if (t < 0 && t >= -back && in.initial) r.load(in.initial + (t + back) * in.initial_stride, n);
-    else r.fill(0.0f);
 }
 
 // Kernels exist for widths 3 and 4; MASKED ones of W also take smaller widths, whose
@@ -75,88 +54,170 @@ template <int W, bool MASKED>
 __device__ __forceinline__ int width_of(const ConvParams& p) {
     return MASKED ? p.width : W;
 }
-
-template <int W, int V, bool MASKED>
-__device__ __forceinline__ void load_weights(const ConvParams& p, const ConvPlace& w, float (&weight)[W][V], float (&bias)[V]) {
+template <int W, bool MASKED>
+__device__ __forceinline__ void load_weights(const ConvParams& p, const ConvPlace& w, float (&weight)[W][kConvRun], float (&bias)[kConvRun]) {
     const int width = width_of<W, MASKED>(p), pad = W - width;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
+    for (int e = 0; e < kConvRun; ++e) {
 #pragma unroll
         for (int j = 0; j < W; ++j) weight[j][e] = e < w.n && j >= pad ? p.weight[(long long)(w.c + e) * width + j - pad] : 0.0f;
         bias[e] = p.bias && e < w.n ? p.bias[w.c + e] : 0.0f;
     }
 }
 
-// What a token of number t is: whether it counts, and the first input that it reads.
-struct Reach {
-    bool on;
-    int from;
+// The rows of one batch of x or dout. `initial` (or null): the `back` rows before them.
+struct Source {
+    const char* rows;
+    long long step;  // bytes between tokens
+    const char* initial;
+    long long initial_step;
+    int back, end;
 };
-template <int W, bool MASKED>
-__device__ __forceinline__ Reach reach_of(const int* docs, int t, int end, int width) {
-    Reach r;
-    r.on = t < end;
-    r.from = t - (width - 1);
-    if (MASKED && r.on && docs) {
-        r.on = docs[t] >= 0;
-        r.from = run_start(docs, t, width);
+// A thread's N rows from token `first` on, of which [0, end) and the initial ones are
+// there; others are 0. tile0: the work-group's first token, so that the 64-bit part of
+// the addresses is the same for all its threads. Inside a sequence no row needs a
+// branch; at its ends one that is not there is read where token 0 is.
+template <int DT, int N>
+__device__ __forceinline__ void load_run(Run<DT, kConvRun> (&rows)[N], const Source& x, int tile0, int ahead, int first, const ConvPlace& w) {
+    constexpr int size = sizeof(typename ElemOf<DT>::type), V = kConvRun;
+    const unsigned c = (unsigned)w.c * size;
+    if (__all(first >= 0 && first + N <= x.end && w.n == V)) {
+        const char* tile = x.rows + (long long)(tile0 + ahead) * x.step;
+        const unsigned off = (unsigned)(first - ahead - tile0) * (unsigned)x.step + c;
+#pragma unroll
+        for (int i = 0; i < N; ++i) rows[i].load(tile + i * x.step + off);
+        return;
     }
-    if (MASKED && !r.on) r.from = t + 1;
-    return r;
-}
-template <int DT, int W, int V, int N, bool MASKED>
-__device__ __forceinline__ void load_inputs(Run<DT, V> (&rows)[N], const Inputs<DT>& in, const int* docs, int t0, const ConvPlace& w, int width) {
+    if (w.n == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) rows[i].fill(0.0f);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        // Rows that no token here reads are not read either: those past the end, and
-        // those of tokens without a document.
-        const int t = t0 + i - (W - 1);
-        const bool dead = t0 >= w.end || (MASKED && docs && t >= 0 && t < w.end && docs[t] < 0);
-        load_input<DT, V>(rows[i], in, dead ? w.end : t, w.end, width - 1, w.n);
+        const int t = first + i;
+        const bool here = t >= 0 && t < x.end, before = t < 0 && t >= -x.back && x.initial;
+        rows[i].load((here ? x.rows + t * x.step : before ? x.initial + (t + x.back) * x.initial_step : x.rows) + c, w.n);
+        if (!here && !before) rows[i].fill(0.0f);
     }
 }
-// z of token t of a thread whose row `at` is its first input.
-template <int W, bool MASKED, int DT, int V, int N>
-__device__ __forceinline__ float preact(const float (&weight)[W][V], const float (&bias)[V], const Run<DT, V> (&rows)[N], int at, int t, const Reach& r, int e) {
+
+// Of a thread's N tokens from `first` on (bit i: token first + i): which count, and
+// which go on with the document of the one before. Initial inputs are the first
+// token's document's.
+struct Flow {
+    unsigned on, on_with;
+};
+template <int N, bool MASKED>
+__device__ __forceinline__ Flow flow_of(const int* docs, int length, int first, int end) {
+    Flow f = {0, ~0u};
+#pragma unroll
+    for (int i = 0; i < N; ++i) f.on |= (unsigned)(first + i >= 0 && first + i < end) << i;
+    if (!MASKED || !docs) return f;
+    int d[N + 1];
+#pragma unroll
+    for (int i = 0; i <= N; ++i) d[i] = docs[max(0, min(first + i - 1, length - 1))];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (d[i + 1] < 0) f.on &= ~(1u << i);
+        if (d[i] != d[i + 1]) f.on_with &= ~(1u << i);
+    }
+    return f;
+}
+// Whether token i reads the input q tokens before it.
+template <bool MASKED>
+__device__ __forceinline__ bool reads(const Flow& f, int i, int q, int width) {
+    if (!MASKED) return true;
+    const unsigned span = (1u << q) - 1;
+    return (f.on >> i & 1) && q < width && (f.on_with >> (i - q + 1) & span) == span;
+}
+
+// The fp32 inputs that a group of W tokens reads: W - 1 before it, then its own.
+template <int W>
+struct Window {
+    float x[2 * W - 1][kConvRun];
+    template <int DT>
+    __device__ __forceinline__ void start(const Run<DT, kConvRun> (&r)[W]) {  // rows -W .. -1: the last W - 1 are taken
+#pragma unroll
+        for (int i = 1; i < W; ++i)
+#pragma unroll
+            for (int e = 0; e < kConvRun; ++e) x[W - 1 + i][e] = r[i].get(e);
+    }
+    template <int DT>
+    __device__ __forceinline__ void next(const Run<DT, kConvRun> (&r)[W]) {
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i)
+#pragma unroll
+            for (int e = 0; e < kConvRun; ++e) x[i][e] = x[W + i][e];
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int e = 0; e < kConvRun; ++e) x[W - 1 + i][e] = r[i].get(e);
+    }
+};
+
+// z of token i of the group. f: the window's tokens.
+template <int W, bool MASKED>
+__device__ __forceinline__ float preact(const float (&weight)[W][kConvRun], const float (&bias)[kConvRun], const Window<W>& in, int i, const Flow& f, int width,
+                                        int e) {
     float z = bias[e];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-        const float v = rows[at + j].get(e);
-        z = __builtin_fmaf(weight[j][e], MASKED && t - (W - 1) + j < r.from ? 0.0f : v, z);
-    }
+    for (int j = 0; j < W; ++j) z = __builtin_fmaf(weight[j][e], reads<MASKED>(f, i + W - 1, W - 1 - j, width) ? in.x[i + j][e] : 0.0f, z);
     return z;
 }
 
-template <int DT, int W, int S, bool MASKED>
+template <int DT, int W, bool MASKED>
 __global__ __launch_bounds__(256) void conv_kernel(ConvParams p) {
-    constexpr int V = conv_run(DT, W);
-    using T = typename ElemOf<DT>::type;
-    const ConvPlace w = conv_place<V>(p);
+    constexpr int V = kConvRun, R = run_tokens(W);
+    constexpr bool PRECISE = DT == ORMI_DTYPE_F32;
+    constexpr int size = sizeof(typename ElemOf<DT>::type);
+    const ConvPlace w = conv_place(p);
     const int width = width_of<W, MASKED>(p);
-    if (w.n == 0) return;
-    const int t0 = (w.part * kConvRuns + (int)(threadIdx.x >> 3)) * S;
+    const int tile0 = w.part * kConvRuns * R, t0 = tile0 + w.run * R;
     const int* docs = p.docs ? p.docs + w.b * p.docs_sb : nullptr;
-    const Inputs<DT> in{(const T*)p.x + w.b * p.x_sb + w.c, p.initial ? (const T*)p.initial + (long long)w.b * (width - 1) * p.channels + w.c : nullptr,
-                        p.x_sl, p.channels};
+    const Source x{p.x + w.b * p.x_sb * size, p.x_sl * size, p.initial ? p.initial + (long long)w.b * (width - 1) * p.channels * size : nullptr,
+                   (long long)p.channels * size, width - 1, w.end};
     float weight[W][V], bias[V];
-    load_weights<W, V, MASKED>(p, w, weight, bias);
-    Run<DT, V> rows[S + W - 1];
-    load_inputs<DT, W, V, S + W - 1, MASKED>(rows, in, docs, t0, w, width);
-    T* out = (T*)p.out + (long long)w.b * p.length * p.channels + w.c;
+    Run<DT, V> before[W], rows[W];
+    load_run<DT, W>(before, x, tile0, -W, t0 - W, w);
+    load_run<DT, W>(rows, x, tile0, 0, t0, w);
+    load_weights<W, MASKED>(p, w, weight, bias);
+    Window<W> in;
+    in.start(before);
+    char* tile = p.out + ((long long)w.b * p.length + tile0) * p.channels * size;
+    const unsigned off = ((unsigned)(w.run * R) * (unsigned)p.channels + (unsigned)w.c) * size;
+#pragma unroll 1
+    for (int g = 0; g < R; g += W) {
+        if (!__any(t0 + g < p.length)) break;
+        in.next(rows);
+        if (g + W < R) load_run<DT, W>(rows, x, tile0, g + W, t0 + g + W, w);
+        const Flow f = flow_of<2 * W - 1, MASKED>(docs, p.length, t0 + g - (W - 1), w.end);
+        const bool whole = __all(t0 + g + W <= p.length && w.n == V);
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        const int t = t0 + i;
-        if (t >= p.length) break;
-        const Reach r = reach_of<W, MASKED>(docs, t, w.end, width);
-        Run<DT, V> o;
+        for (int i = 0; i < W; ++i) {
+            Run<DT, V> o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            float z = preact<W, MASKED, DT, V, S + W - 1>(weight, bias, rows, i, t, r, e);
-            if (p.silu) z = silu(z);
-            o.set(e, MASKED && !r.on ? 0.0f : z);
+            for (int e = 0; e < V; ++e) {
+                float z = preact<W, MASKED>(weight, bias, in, i, f, width, e);
+                if (p.silu) z *= conv_sigmoid<PRECISE>(z);
+                o.set(e, MASKED && !(f.on >> (i + W - 1) & 1) ? 0.0f : z);
+            }
+            char* to = tile + (long long)(g + i) * p.channels * size;
+            if (whole) o.store_past(to + off);
+            else if (t0 + g + i < p.length) o.store(to + off, w.n);
         }
-        o.store(out + (long long)t * p.channels, w.n);
     }
+}
+
+// The first token that a token after `end` of the last one's document reads no further
+// back than: token numbers from 1 - width (the initial inputs') on.
+__device__ __forceinline__ int last_run(const int* docs, int end, int width) {
+    const int first = end - (width - 1);
+    if (end == 0 || !docs) return first;
+    if (docs[end - 1] < 0) return end;
+    int from = end - 1;
+    while (from > first && !(from > 0 && docs[from - 1] != docs[from])) --from;
+    return from;
 }
 
 // The inputs that a next token reads. A thread per channel.
@@ -168,8 +229,7 @@ __global__ __launch_bounds__(256) void conv_last_kernel(ConvParams p) {
     if (id >= (long long)p.batch * p.channels) return;
     const int b = (int)(id / p.channels), c = (int)(id % p.channels);
     const int end = p.lengths ? max(0, min(p.length, p.lengths[b])) : p.length;
-    const int* docs = p.docs ? p.docs + b * p.docs_sb : nullptr;
-    const int from = end == 0 ? 1 - width : docs && docs[end - 1] < 0 ? end : run_start(docs, end - 1, width);
+    const int from = last_run(p.docs ? p.docs + b * p.docs_sb : nullptr, end, width);
     T* last = (T*)p.last + (long long)b * (width - 1) * p.channels + c;
     for (int j = 0; j < width - 1; ++j) {
         const int t = end - (width - 1) + j;
@@ -182,22 +242,60 @@ __global__ __launch_bounds__(256) void conv_last_kernel(ConvParams p) {
     }
 }
 
-template <int DT, int GT, int W, int S, bool MASKED>
-__global__ __launch_bounds__(256) void conv_grad_kernel(ConvParams p) {
-    constexpr int V = conv_run(DT, W), M = S + W - 1, N = M + W - 1;  // M: tokens that read the thread's inputs
+// The gradient of the initial inputs, a thread per channel: the tokens of the first
+// width - 1 that read each, and the last state's where it still holds it.
+template <int DT, int GT>
+__global__ __launch_bounds__(256) void conv_initial_grad_kernel(ConvParams p) {
     using T = typename ElemOf<DT>::type;
     using TG = typename ElemOf<GT>::type;
+    const int width = p.width;
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= (long long)p.batch * p.channels) return;
+    const int b = (int)(id / p.channels), c = (int)(id % p.channels);
+    const int end = p.lengths ? max(0, min(p.length, p.lengths[b])) : p.length;
+    const int* docs = p.docs ? p.docs + b * p.docs_sb : nullptr;
+    const T* x = (const T*)p.x + b * p.x_sb + c;
+    const T* initial = p.initial ? (const T*)p.initial + (long long)b * (width - 1) * p.channels + c : nullptr;
+    const float* weight = p.weight + (long long)c * width;
+    // Tokens that go on with what was before the first.
+    int tokens = 0;
+    while (tokens < min(end, width - 1) && !(docs && (docs[tokens] < 0 || docs[tokens] != docs[0]))) ++tokens;
+    const int from = last_run(docs, end, width);
+    for (int k = 0; k < width - 1; ++k) {  // input k - (width - 1)
+        float g = 0.0f;
+        for (int t = 0; t < min(tokens, k + 1); ++t) {
+            float dz = p.dout ? elem_to_f32<GT>(((const TG*)p.dout)[b * p.do_sb + t * p.do_sl + c]) : 0.0f;
+            if (p.silu) {
+                float z = p.bias ? p.bias[c] : 0.0f;
+                for (int j = 0; j < width; ++j) {
+                    const int at = t - (width - 1) + j;
+                    const float v = at >= 0 ? elem_to_f32<DT>(x[at * p.x_sl]) : initial ? elem_to_f32<DT>(initial[(long long)(at + width - 1) * p.channels]) : 0.0f;
+                    z = __builtin_fmaf(weight[j], v, z);
+                }
+                dz *= silu_grad<true>(z);
+            }
+            g = __builtin_fmaf(weight[k - t], dz, g);
+        }
+        const int at = k - (width - 1), j = at - (end - (width - 1));
+        if (p.dlast && j >= 0 && at >= from) g += p.dlast[((long long)b * (width - 1) + j) * p.channels + c];
+        ((T*)p.dinitial)[((long long)b * (width - 1) + k) * p.channels + c] = elem_from_f32<DT>(g);
+    }
+}
+
+template <int DT, int GT, int W, bool MASKED>
+__global__ __launch_bounds__(256) void conv_grad_kernel(ConvParams p) {
+    constexpr int V = kConvRun, R = run_tokens(W);
+    constexpr bool PRECISE = DT == ORMI_DTYPE_F32;
+    constexpr int size = sizeof(typename ElemOf<DT>::type), gsize = sizeof(typename ElemOf<GT>::type);
     __shared__ float lds[4][kConvLanes][(W + 1) * V];
-    const ConvPlace w = conv_place<V>(p);
+    const ConvPlace w = conv_place(p);
     const int width = width_of<W, MASKED>(p);
-    const int run = threadIdx.x >> 3;
     const int* docs = p.docs ? p.docs + w.b * p.docs_sb : nullptr;
-    const Inputs<DT> in{(const T*)p.x + w.b * p.x_sb + w.c, p.initial ? (const T*)p.initial + (long long)w.b * (width - 1) * p.channels + w.c : nullptr,
-                        p.x_sl, p.channels};
-    const TG* dout = p.dout ? (const TG*)p.dout + w.b * p.do_sb + w.c : nullptr;
-    T* dx = p.dx ? (T*)p.dx + (long long)w.b * p.length * p.channels + w.c : nullptr;
+    const Source x{p.x + w.b * p.x_sb * size, p.x_sl * size, p.initial ? p.initial + (long long)w.b * (width - 1) * p.channels * size : nullptr,
+                   (long long)p.channels * size, width - 1, w.end};
+    const Source dout{p.dout + w.b * p.do_sb * gsize, p.do_sl * gsize, nullptr, 0, 0, w.end};
     float weight[W][V], bias[V], dw[W][V], db[V];
-    load_weights<W, V, MASKED>(p, w, weight, bias);
+    load_weights<W, MASKED>(p, w, weight, bias);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
 #pragma unroll
@@ -206,96 +304,97 @@ __global__ __launch_bounds__(256) void conv_grad_kernel(ConvParams p) {
     }
     // The inputs that the last state holds have its gradient too.
     const float* dlast = p.dlast ? p.dlast + (long long)w.b * (width - 1) * p.channels + w.c : nullptr;
-    const int last_from = w.end == 0 ? 1 - width : docs && docs[w.end - 1] < 0 ? w.end : run_start(docs, w.end - 1, width);
-    auto add_last = [&](int t, float (&g)[V]) {
-        const int j = t - (w.end - (width - 1));
-        if (!dlast || j < 0 || t >= w.end || t < last_from) return;
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e < w.n) g[e] += dlast[(long long)j * p.channels + e];
-    };
+    const int last_from = p.dlast ? last_run(docs, w.end, width) : 0;
     for (int tile = w.part; tile < p.tiles; tile += p.parts) {
-        const int t0 = (tile * kConvRuns + run) * S;
-        Run<DT, V> rows[N];
-        Run<GT, V> rd[M];
-        load_inputs<DT, W, V, N, MASKED>(rows, in, docs, t0, w, width);
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-            const int t = t0 + i;
-            const bool on = dout && t < w.end && !(MASKED && docs && docs[t] < 0);
-            if (on) rd[i].load(dout + t * p.do_sl, w.n);
-            else rd[i].fill(0.0f);
-        }
-        float d[W][V];  // the gradients of the last W inputs that are still being summed: input t0 + k in d[k % W]
-        float dz[V];
-        auto dz_of = [&](int i, const Reach& r) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                dz[e] = rd[i].get(e);
-                if (p.silu) dz[e] *= silu_grad(preact<W, MASKED, DT, V, N>(weight, bias, rows, i, t0 + i, r, e));
-            }
+        const int tile0 = tile * kConvRuns * R, t0 = tile0 + w.run * R;
+        Run<DT, V> before[W], rows[W];
+        Run<GT, V> rd[W];
+        auto fetch = [&](int g) {
+            load_run<DT, W>(rows, x, tile0, g, t0 + g, w);
+            if (p.dout) load_run<GT, W>(rd, dout, tile0, g, t0 + g, w);
         };
+        if (!p.dout) {
 #pragma unroll
-        for (int i = 0; i < M; ++i) {
-            const int t = t0 + i;
-            const Reach r = reach_of<W, MASKED>(docs, t, w.end, width);
-            dz_of(i, r);
-            if (i < S) {
+            for (int i = 0; i < W; ++i) rd[i].fill(0.0f);
+        }
+        load_run<DT, W>(before, x, tile0, -W, t0 - W, w);
+        fetch(0);
+        Window<W> in;
+        in.start(before);
+        float d[W][V];  // of inputs whose gradients are still being summed: that of token t0 + k in d[k % W]
 #pragma unroll
-                for (int e = 0; e < V; ++e) d[i % W][e] = 0.0f, db[e] += MASKED && !r.on ? 0.0f : dz[e];
-            }
+        for (int i = 0; i < W; ++i)
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const bool skip = MASKED && t - (W - 1) + j < r.from;
-                const int to = i - (W - 1) + j;  // the input among the thread's
+            for (int e = 0; e < V; ++e) d[i][e] = 0.0f;
+        char* dx_tile = p.dx + ((long long)w.b * p.length + tile0) * p.channels * size;
+        const unsigned off = ((unsigned)(w.run * R) * (unsigned)p.channels + (unsigned)w.c) * size;
+        // One group more than the run's: its tokens read the last inputs.
+#pragma unroll 1
+        for (int g = 0; g <= R; g += W) {
+            if (!__any(t0 + g < p.length + W - 1)) break;
+            in.next(rows);
+            float dy[W][V];
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) dy[i][e] = rd[i].get(e);
+            if (g < R) fetch(g + W);
+            const Flow f = flow_of<2 * W - 1, MASKED>(docs, p.length, t0 + g - (W - 1), w.end);
+            const bool whole = __all(t0 + g + 1 <= p.length && w.n == V);  // inputs up to t0 + g are written
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                float dz[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float g = skip ? 0.0f : dz[e];
-                    if (to >= 0 && to < S) d[to % W][e] = __builtin_fmaf(weight[j][e], g, d[to % W][e]);
-                    if (i < S) dw[j][e] = __builtin_fmaf(g, skip ? 0.0f : rows[i + j].get(e), dw[j][e]);
+                    dz[e] = MASKED && !(f.on >> (i + W - 1) & 1) ? 0.0f : dy[i][e];
+                    if (p.silu) dz[e] *= silu_grad<PRECISE>(preact<W, MASKED>(weight, bias, in, i, f, width, e));
+                    d[i][e] = 0.0f;
                 }
-            }
-            const int done = i - (W - 1), td = t - (W - 1);
-            if (done >= 0 && dx && td < p.length) {
-                Run<DT, V> o;
-                add_last(td, d[done % W]);
 #pragma unroll
-                for (int e = 0; e < V; ++e) o.set(e, d[done % W][e]);
-                o.store(dx + (long long)td * p.channels, w.n);
-            }
-        }
-        if (p.dinitial && t0 == 0) {  // the inputs before the first token's
-            for (int k = 0; k < width - 1; ++k) {
-                float g[V];
+                for (int j = 0; j < W; ++j) {
+                    const int q = W - 1 - j, slot = (i - q + W) % W;
+                    const bool skip = !reads<MASKED>(f, i + W - 1, q, width);
 #pragma unroll
-                for (int e = 0; e < V; ++e) g[e] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < W - 1; ++i) {  // the tokens that read it: i <= k
-                    if (i > k || i >= M) continue;
-                    const Reach r = reach_of<W, MASKED>(docs, i, w.end, width);
-                    dz_of(i, r);
-                    if (!(k - (width - 1) < r.from))
-#pragma unroll
-                        for (int e = 0; e < V; ++e) g[e] = __builtin_fmaf(e < w.n ? p.weight[(long long)(w.c + e) * width + k - i] : 0.0f, dz[e], g[e]);
+                    for (int e = 0; e < V; ++e) d[slot][e] = __builtin_fmaf(weight[j][e], skip ? 0.0f : dz[e], d[slot][e]);
                 }
-                add_last(k - (width - 1), g);
-                Run<DT, V> o;
+                if (g < R) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) o.set(e, g[e]);
-                o.store((T*)p.dinitial + ((long long)w.b * (width - 1) + k) * p.channels + w.c, w.n);
+                    for (int j = 0; j < W; ++j) {
+                        const bool skip = !reads<MASKED>(f, i + W - 1, W - 1 - j, width);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) dw[j][e] = __builtin_fmaf(skip ? 0.0f : dz[e], skip ? 0.0f : in.x[i + j][e], dw[j][e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < V; ++e) db[e] += dz[e];
+                }
+                const int done = g + i - (W - 1), slot = (i + 1) % W;  // the input that no later token reads
+                if (done >= 0 && done < R && p.dx) {
+                    const int t = t0 + done, j = t - (w.end - (width - 1));
+                    if (dlast && j >= 0 && t < w.end && t >= last_from) {
+#pragma unroll
+                        for (int e = 0; e < V; ++e)
+                            if (e < w.n) d[slot][e] += dlast[(long long)j * p.channels + e];
+                    }
+                    Run<DT, V> o;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) o.set(e, d[slot][e]);
+                    char* to = dx_tile + (long long)done * p.channels * size;
+                    if (whole) o.store_past(to + off);
+                    else if (t < p.length) o.store(to + off, w.n);
+                }
             }
         }
     }
     if (!p.part_sums) return;
-    // Over the eight runs of a wave, then the four waves.
+    // Over the runs of a wave, then the four waves.
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int j = 0; j <= W; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             float v = j < W ? dw[j < W ? j : 0][e] : db[e];
-            v += __shfl_xor(v, 8, 64);
-            v += __shfl_xor(v, 16, 64);
+#pragma unroll
+            for (int step = kConvLanes; step < 32; step *= 2) v += __shfl_xor(v, step, 64);
             v += __shfl_xor(v, 32, 64);
             if (lane < kConvLanes) lds[wave][lane][j * V + e] = v;
         }
@@ -340,27 +439,28 @@ __global__ __launch_bounds__(256) void conv_sums_kernel(ConvParams p) {
     }
 }
 
+template <int DT, int GT, int W, bool MASKED>
+void launch_grad(const ConvParams& p) {
+    const unsigned grid = (unsigned)((long long)p.channel_blocks * p.parts * p.batch);
+    if (grid > 0) conv_grad_kernel<DT, GT, W, MASKED><<<grid, 256>>>(p);
+    const long long threads = (long long)p.batch * p.channels;
+    if (p.dinitial && p.width > 1 && threads > 0) conv_initial_grad_kernel<DT, GT><<<(unsigned)((threads + 255) / 256), 256>>>(p);
+    if (p.dweight || p.dbias) conv_sums_kernel<<<(unsigned)(((p.width + 1ll) * p.channels + 63) / 64), 256>>>(p);
+}
 template <int DT, int W, bool MASKED>
 void launch_masked(const ConvParams& p, bool gradient, bool wide_dout) {
-    const unsigned grid = (unsigned)((long long)p.channel_blocks * p.parts * p.batch);
-    if (!gradient) {
-        if (p.tiles > 0) conv_kernel<DT, W, kConvTokens, MASKED><<<grid, 256>>>(p);
-        if (p.width > 1 && p.last) conv_last_kernel<DT><<<(unsigned)(((long long)p.batch * p.channels + 255) / 256), 256>>>(p);
-        return;
-    }
-    if (grid > 0) {
-        if (wide_dout) conv_grad_kernel<DT, ORMI_DTYPE_F32, W, kConvGradTokens, MASKED><<<grid, 256>>>(p);
-        else conv_grad_kernel<DT, DT, W, kConvGradTokens, MASKED><<<grid, 256>>>(p);
-    }
-    if (p.dweight || p.dbias) conv_sums_kernel<<<(unsigned)(((p.width + 1ll) * p.channels + 63) / 64), 256>>>(p);
+    if (gradient) return wide_dout ? launch_grad<DT, ORMI_DTYPE_F32, W, MASKED>(p) : launch_grad<DT, DT, W, MASKED>(p);
+    if (p.tiles > 0) conv_kernel<DT, W, MASKED><<<(unsigned)((long long)p.channel_blocks * p.parts * p.batch), 256>>>(p);
+    if (p.width > 1 && p.last) conv_last_kernel<DT><<<(unsigned)(((long long)p.batch * p.channels + 255) / 256), 256>>>(p);
 }
 template <int DT>
 int launch_conv(const ConvParams& p, bool gradient, bool wide_dout) {
-    const bool masked = p.docs || p.lengths;
-    if (p.width == 4 && !masked) launch_masked<DT, 4, false>(p, gradient, wide_dout);
-    else if (p.width == 3 && !masked) launch_masked<DT, 3, false>(p, gradient, wide_dout);
-    else if (p.width <= 4) launch_masked<DT, 4, true>(p, gradient, wide_dout);
-    else launch_masked<DT, 8, true>(p, gradient, wide_dout);
+    const bool masked = p.docs || p.lengths || p.width < 3 || p.width > 4;
+    switch (conv_width(p.width, masked)) {
+        case 3: launch_masked<DT, 3, false>(p, gradient, wide_dout); break;
+        case 4: masked ? launch_masked<DT, 4, true>(p, gradient, wide_dout) : launch_masked<DT, 4, false>(p, gradient, wide_dout); break;
+        default: launch_masked<DT, 8, true>(p, gradient, wide_dout);
+    }
     return (int)hipGetLastError();
 }
 

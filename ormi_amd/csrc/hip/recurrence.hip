@@ -15,7 +15,11 @@ namespace {
 constexpr long long kMostGroups = (1ll << 24) - 1;  // of 256 threads: a launch holds fewer than 2^32
 constexpr int kMostTokens = 1 << 30;                // token numbers of a last tile stay in 31 bits
 
+constexpr int kMostStride = 1 << 20;                // elements between tokens: a tile's offsets stay in 32 bits
+
 bool is_float(int dt) { return dt == ORMI_DTYPE_F32 || dt == ORMI_DTYPE_BF16 || dt == ORMI_DTYPE_F16; }
+
+bool near(int length, int64_t stride) { return length <= 1 || (stride >= 0 && stride <= kMostStride); }
 
 const char* check(const ormi_recurrence_desc* d) {
     if (!d) return "null descriptor";
@@ -23,6 +27,8 @@ const char* check(const ormi_recurrence_desc* d) {
     if (d->gate_dtype != d->dtype && d->gate_dtype != ORMI_DTYPE_F32) return "gates must have x's type or float32";
     if (d->batch < 0 || d->length < 0 || d->channels < 0) return "negative extent";
     if (d->length > kMostTokens) return "more than 2^30 tokens";
+    if (d->channels > kMostStride) return "more than 2^20 channels";
+    if (!near(d->length, d->gate_strides[1]) || !near(d->length, d->x_strides[1])) return "tokens more than 2^20 elements apart";
     if ((long long)d->batch * ((d->channels + kRecChannels - 1ll) / kRecChannels) > kMostGroups) return "batch * channels too large";
     return nullptr;
 }
@@ -115,6 +121,7 @@ int ormi_hip_recurrence_grad(const ormi_recurrence_grad_desc* g) {
     const ormi_recurrence_desc* d = &g->forward;
     if (const char* what = check(d)) return bad(what);
     if (g->dout && g->dout_dtype != d->dtype && g->dout_dtype != ORMI_DTYPE_F32) return bad("dout must have x's type or float32");
+    if (g->dout && !near(d->length, g->dout_strides[1])) return bad("tokens more than 2^20 elements apart");
     if (nothing(d)) return ORMI_HIP_OK;
     if (d->length > 0 && (!d->gates || !d->x || !d->states)) return bad("null gates, x or states");
     int rc = ensure_init();

@@ -17,7 +17,7 @@
 // (CHAINED) a work-group has one tile, and the state before it comes from the
 // tiles before: each publishes its span, and the state past it as soon as it knows
 // the one before it; a tile composes the spans back to the nearest state that is
-// tw. Inputs are read once either way.
+// there. Inputs are read once either way.
 //
 // Ww a token forgets (a document's first one, or one of none) the state before
 // it must not matter at all, NaN included, so spans carry a flag: a product that
@@ -111,7 +111,7 @@ __device__ __forceinline__ Rows rows_of(const char* base, long long sb, long lon
     return r;
 }
 
-// A thread's tokens of a tensor, as `other` ww the token does not count. whole:
+// A thread's tokens of a tensor, as `other` where the token does not count. whole:
 // all of the wave's tokens count and all channels exist, which takes no branch per row.
 template <int DT, int V>
 __device__ __forceinline__ void load_rows(Run<DT, V> (&r)[kRecTokens], const Rows& at, bool whole, unsigned on, int n, float other) {
@@ -218,14 +218,14 @@ __device__ __forceinline__ void cross_waves(const WaveSpans<V>& l, int at, float
 
 // ------------------------------------------------------------ chained tiles --
 // A tile's span (gates' product and rest in one word, so that no order between
-// words matters) and the state past it, per channel. All bits set: not tw yet.
+// words matters) and the state past it, per channel. All bits set: not there yet.
 // Published NaN have other bits, and a span that forgets has them in the product's
 // place.
 constexpr unsigned kNone = 0xffffffffu;
 constexpr unsigned long long kNoSpan = ~0ull;
-// Looks at a tile before it that is not tw yet, seconds' worth: the
+// Looks at a tile before it that is not there yet, seconds' worth: the
 // tiles that a tile waits for were begun before it and wait for none after them, so
-// this ends a wait only ww a work-group was lost; the states are NaN then.
+// this ends a wait only where a work-group was lost; the states are NaN then.
 constexpr int kMostLooks = 1 << 21;
 
 __device__ __forceinline__ unsigned published(float v) { return v == v ? __float_as_uint(v) : 0x7fc00000u; }
@@ -319,7 +319,7 @@ __device__ __forceinline__ void tile_span(const WaveSpans<V>& l, int at, int cha
 // a tile waits only for tiles that run or are done. Chains are in kRecCounters sets,
 // each with a counter of its own: additions to one word of memory take about 12 ns
 // each (7504 tiles of one counter: 21 us more). A work-group whose set is through takes
-// from the next; tw are as many work-groups as tiles.
+// from the next; there are as many work-groups as tiles.
 template <bool CHAINED, bool DOWN>
 struct Walk {
     int chain, tile;
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(256) void recurrence_kernel(RecParams p) {
 // a token but for that state's own output: m_t = a_t (dh_t + m_{t+1}), a recurrence
 // of the same gates the other way. The states before a tile's tokens are made again
 // from the one that the forward pass kept, in full precision.
-// AHEAD: the next tile's loads go out before this one is finished, ww the registers
+// AHEAD: the next tile's loads go out before this one is finished, where the registers
 // hold both.
 template <int GT, int XT, int DT, bool LOGIT, bool MASKED, bool CHAINED>
 __global__ __launch_bounds__(256, 2) void recurrence_grad_kernel(RecParams p) {

@@ -33,8 +33,10 @@ def rules(length, batch, documents, lengths):
 
 
 # Roundings per token, in u: the gate (exp2 2, its correction 2, 1 + e 1, the reciprocal 2; 1 - a a product more: at
-# most 12 with the input's), the product of gates, the multiply-add. 16 a token; a value then passes at most 3 joins
-# of segments, 5 of waves and 64 of splits more, whatever its token: 80.
+# most 12 with the input's), the product of gates, the multiply-add: 16. e^-g of a 16-bit logit goes without the
+# correction: -g log2 e is off by half a spacing and by the constant's own, together under 2 |g| u of e^-g (logits
+# past 88 count as that). A value then passes at most 2 joins of segments, 4 of waves and those of the tiles before
+# it (64 for the longest here), whatever its token: 80.
 STEP, JOIN = 16, 80
 
 
@@ -50,8 +52,9 @@ def recurrence(g, x, logit, initial=None, documents=None, lengths=None, dy=None,
     h = np.zeros((batch, channels)) if initial is None else initial.astype(np.float64)
     big, err = np.abs(h), np.zeros_like(h)
     hs, bigs, errs = [h], [big], [err]
+    step = STEP + (2 * np.minimum(np.abs(g), 88.0) if logit else np.zeros_like(g))
     for t in range(length):
-        err = np.abs(keep[t]) * err + STEP * U * (np.abs(keep[t]) * big + np.abs(b[t]))
+        err = np.abs(keep[t]) * err + step[t] * U * (np.abs(keep[t]) * big + np.abs(b[t]))
         big = np.abs(keep[t]) * big + np.abs(b[t])
         h = keep[t] * h + b[t]
         hs.append(h), bigs.append(big), errs.append(err)
@@ -69,13 +72,13 @@ def recurrence(g, x, logit, initial=None, documents=None, lengths=None, dy=None,
         l, lb, le = d[t] + m, np.abs(d[t]) + mb, me + JOIN * U * mb + U * np.abs(d[t])
         prev, pb, pe = (np.where(cut[t], 0.0, s[t]) for s in (hs, bigs, errs))
         if logit:
-            dx[t], ex[t] = l * take[t], (le + STEP * U * lb) * take[t]
+            dx[t], ex[t] = l * take[t], (le + step[t] * U * lb) * take[t]
             dg[t] = l * (prev - x[t]) * a[t] * take[t]
-            eg[t] = ((le + 2 * STEP * U * lb) * (pb + np.abs(x[t])) + lb * pe) * a[t] * take[t]
+            eg[t] = ((le + 2 * step[t] * U * lb) * (pb + np.abs(x[t])) + lb * pe) * a[t] * take[t]
         else:
             dx[t], ex[t] = l, le
             dg[t], eg[t] = l * prev, (le + 4 * U * lb) * pb + lb * pe
-        me = np.abs(keep[t]) * me + STEP * U * np.abs(keep[t]) * lb
+        me = np.abs(keep[t]) * me + step[t] * U * np.abs(keep[t]) * lb
         mb = np.abs(keep[t]) * lb
         m = keep[t] * l
     values |= {"dg": np.where(on, dg, 0.0), "dx": np.where(on, dx, 0.0), "dinitial": m}
@@ -90,10 +93,11 @@ def _batch_first(d):
 def conv(x, weight, bias, silu, initial=None, documents=None, lengths=None, dy=None, dlast=None):
     """(values, bounds), dicts of y, last and with dy or dlast dx, dw, db, dinitial.
 
-    Roundings: width + 1 multiply-adds of z, 6 of the sigmoid and what is made of it;
-    silu' is at most 1.1 and its slope at most 1/2, the silu's own at most 1.1. A
-    weight's gradient adds up to 64 tokens in a row, 32 runs and the rows of the second
-    launch, in a tree of at most 8 * tiles + 40 additions a term.
+    Roundings: width + 1 multiply-adds of z, 6 of the sigmoid and what is made of it
+    (and 2 |z| u of e^-z for 16-bit results, as for the recurrence); silu' is at most
+    1.1 and its slope at most 1/2, the silu's own at most 1.1. A weight's gradient adds
+    32 tokens in a row, 16 runs pairwise, and the rows of the second launch, one for
+    each batch and 480 or 512 tokens: at most 40 additions a term and those.
     """
     batch, length, channels = x.shape
     width = weight.shape[1]
@@ -122,7 +126,7 @@ def conv(x, weight, bias, silu, initial=None, documents=None, lengths=None, dy=N
     with np.errstate(over="ignore"):
         s = 1 / (1 + np.exp(-z))
     values = {"y": z * s if silu else z}
-    bounds = {"y": 1.1 * ez + 8 * U * np.abs(z) * s if silu else ez}
+    bounds = {"y": 1.1 * ez + (8 + 2 * np.abs(z)) * U * np.abs(z) * s if silu else ez}
     values["last"] = np.stack([np.where(last_reads[b][:, None], rows[b, last_at[b]:last_at[b] + width - 1], 0.0) for b in range(batch)]) \
         if batch else np.zeros((0, width - 1, channels))
     if dy is None and dlast is None:
@@ -130,7 +134,7 @@ def conv(x, weight, bias, silu, initial=None, documents=None, lengths=None, dy=N
     d = np.zeros_like(x) if dy is None else np.where(on, dy.astype(np.float64), 0.0)
     slope = s * (1 + z * (1 - s)) if silu else np.ones_like(z)
     dz = d * slope
-    edz = np.abs(d) * (0.5 * ez + 12 * U * (s + np.abs(z) * s)) if silu else np.zeros_like(z)
+    edz = np.abs(d) * (0.5 * ez + (12 + 2 * np.abs(z)) * U * (s + np.abs(z) * s)) if silu else np.zeros_like(z)
     drows, erows = np.zeros_like(rows), np.zeros_like(rows)
     for j in range(width):
         r = reads[:, :, j:j + 1]
@@ -142,7 +146,7 @@ def conv(x, weight, bias, silu, initial=None, documents=None, lengths=None, dy=N
             drows[b, last_at[b]:last_at[b] + width - 1] += part
             erows[b, last_at[b]:last_at[b] + width - 1] += U * np.abs(part)
     erows += 2 * U * np.abs(drows)
-    adds = (8 * (-(-length // 256)) + 40 + batch) * U
+    adds = (40 + batch * -(-length // 480)) * U
     edz = edz + adds * np.abs(dz)
     values |= {"dx": drows[:, width - 1:], "dinitial": drows[:, :width - 1], "dw": (dz[..., None] * taps).sum((0, 1)), "db": dz.sum((0, 1))}
     bounds |= {"dx": erows[:, width - 1:], "dinitial": erows[:, :width - 1], "dw": (edz[..., None] * np.abs(taps)).sum((0, 1)),
