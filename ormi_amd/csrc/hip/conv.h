@@ -6,9 +6,10 @@
 
 namespace ormi_hip {
 
-constexpr int kConvLanes = 16;                 // threads side by side over the channels
+constexpr int kConvLanes = 32;                 // threads side by side over the channels: 256 bytes of a 16-bit row
 constexpr int kConvRun = 4;                    // channels of a thread
 constexpr int kConvRuns = 256 / kConvLanes;    // runs of tokens of a tile
+static_assert(kConvRuns >= ORMI_CONV_MAX_WIDTH - 1, "a run's threads for each row of the last state");
 // Widths that kernels are built for: 3 and 4, and 4 and 8 for all up to them.
 constexpr int conv_width(int width, bool masked) { return width == 3 && !masked ? 3 : width <= 4 ? 4 : 8; }
 constexpr int run_tokens(int width) { return 32 / width * width; }  // of a thread's run: whole groups of that width

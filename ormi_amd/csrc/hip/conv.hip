@@ -43,6 +43,7 @@ bool plan(const ormi_conv_desc* d, bool gradient, ConvParams* p) {
     p->tiles = (d->length + tokens - 1) / tokens;
     p->parts = p->tiles;
     const long long rows = (long long)p->channel_blocks * d->batch;
+    if (!gradient && p->tiles == 0) p->tiles = p->parts = 1;  // it leaves the initial inputs as the last state
     if (gradient) {
         // A work-group's sums of the weights' gradients are a row for the second
         // launch: no more of them than keep the card busy.

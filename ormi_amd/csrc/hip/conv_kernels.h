@@ -102,35 +102,45 @@ __device__ __forceinline__ void load_run(Run<DT, kConvRun> (&rows)[N], const Sou
     }
 }
 
-// Of a thread's N tokens from `first` on (bit i: token first + i): which count, and
-// which go on with the document of the one before. Initial inputs are the first
-// token's document's.
+// Of the tokens from t0 - W to t0 + R + W - 1 of a thread's run (bit i: token
+// t0 - W + i): which count, and which go on with the document of the one before.
+// Initial inputs are the first token's document's. A run's threads look at a token or
+// two each.
 struct Flow {
-    unsigned on, on_with;
+    unsigned long long on, on_with;
 };
-template <int N, bool MASKED>
-__device__ __forceinline__ Flow flow_of(const int* docs, int length, int first, int end) {
-    Flow f = {0, ~0u};
+template <int W, bool MASKED>
+__device__ __forceinline__ Flow flow_of(const int* docs, int length, int t0, int end) {
+    static_assert(run_tokens(W) + 2 * W <= 64, "bits");
+    Flow f = {~0ull, ~0ull};
+    if (!MASKED) return f;
+    const int first = t0 - W, lane = threadIdx.x % kConvLanes, at = (int)(threadIdx.x & 63) - lane;
+    f = {0, 0};
 #pragma unroll
-    for (int i = 0; i < N; ++i) f.on |= (unsigned)(first + i >= 0 && first + i < end) << i;
-    if (!MASKED || !docs) return f;
-    int d[N + 1];
-#pragma unroll
-    for (int i = 0; i <= N; ++i) d[i] = docs[max(0, min(first + i - 1, length - 1))];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (d[i + 1] < 0) f.on &= ~(1u << i);
-        if (d[i] != d[i + 1]) f.on_with &= ~(1u << i);
+    for (int k = 0; k < 64; k += kConvLanes) {
+        const int t = first + k + lane, here = max(0, min(t, length - 1)), before = max(0, min(t - 1, length - 1));
+        const int d = docs ? docs[here] : 0, last = docs ? docs[before] : 0;
+        const unsigned long long on = __ballot(t >= 0 && t < end && d >= 0) >> at, with = __ballot(d == last) >> at;
+        f.on |= (on & 0xffffffffull) << k;
+        f.on_with |= (with & 0xffffffffull) << k;
     }
     return f;
 }
-// Whether token i reads the input q tokens before it.
-template <bool MASKED>
-__device__ __forceinline__ bool reads(const Flow& f, int i, int q, int width) {
-    if (!MASKED) return true;
-    const unsigned span = (1u << q) - 1;
-    return (f.on >> i & 1) && q < width && (f.on_with >> (i - q + 1) & span) == span;
-}
+// The window of the group from token t0 + g on: the W - 1 tokens before it, then its own.
+template <int W, bool MASKED>
+struct GroupFlow {
+    unsigned on = 0, on_with = 0;
+    __device__ __forceinline__ GroupFlow(const Flow& f, int g) {
+        if (MASKED) on = (unsigned)(f.on >> (g + 1)), on_with = (unsigned)(f.on_with >> (g + 1));
+    }
+    __device__ __forceinline__ bool counts(int i) const { return !MASKED || (on >> (i + W - 1) & 1); }
+    // Whether token i reads the input q tokens before it.
+    __device__ __forceinline__ bool reads(int i, int q, int width) const {
+        if (!MASKED) return true;
+        const unsigned span = (1u << q) - 1;
+        return counts(i) && q < width && (on_with >> (i + W - q) & span) == span;
+    }
+};
 
 // The fp32 inputs that a group of W tokens reads: W - 1 before it, then its own.
 template <int W>
@@ -156,14 +166,36 @@ struct Window {
     }
 };
 
-// z of token i of the group. f: the window's tokens.
+// z of token i of the group.
 template <int W, bool MASKED>
-__device__ __forceinline__ float preact(const float (&weight)[W][kConvRun], const float (&bias)[kConvRun], const Window<W>& in, int i, const Flow& f, int width,
-                                        int e) {
+__device__ __forceinline__ float preact(const float (&weight)[W][kConvRun], const float (&bias)[kConvRun], const Window<W>& in, int i, const GroupFlow<W, MASKED>& f,
+                                        int width, int e) {
     float z = bias[e];
 #pragma unroll
-    for (int j = 0; j < W; ++j) z = __builtin_fmaf(weight[j][e], reads<MASKED>(f, i + W - 1, W - 1 - j, width) ? in.x[i + j][e] : 0.0f, z);
+    for (int j = 0; j < W; ++j) z = __builtin_fmaf(weight[j][e], f.reads(i, W - 1 - j, width) ? in.x[i + j][e] : 0.0f, z);
     return z;
+}
+
+// The first token that a token after `end` of the last one's document reads no further
+// back than: token numbers from 1 - width (the initial inputs') on.
+__device__ __forceinline__ int last_run(const int* docs, int end, int width) {
+    const int first = end - (width - 1);
+    if (end == 0 || !docs) return first;
+    if (docs[end - 1] < 0) return end;
+    int from = end - 1;
+    while (from > first && !(from > 0 && docs[from - 1] != docs[from])) --from;
+    return from;
+}
+// Row j of the inputs that a next token reads, a thread's channels of it.
+template <int DT>
+__device__ __forceinline__ void put_last(const ConvParams& p, const ConvPlace& w, const Source& x, const int* docs, int width, int j) {
+    constexpr int size = sizeof(typename ElemOf<DT>::type);
+    const int t = w.end - (width - 1) + j;
+    const bool here = t >= 0, before = !here && x.initial, kept = (here || before) && t >= last_run(docs, w.end, width);
+    Run<DT, kConvRun> r;
+    if (kept) r.load((here ? x.rows + t * x.step : x.initial + (t + x.back) * x.initial_step) + (long long)w.c * size, w.n);
+    else r.fill(0.0f);
+    r.store(p.last + (((long long)w.b * (width - 1) + j) * p.channels + w.c) * size, w.n);
 }
 
 template <int DT, int W, bool MASKED>
@@ -177,6 +209,10 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvParams p) {
     const int* docs = p.docs ? p.docs + w.b * p.docs_sb : nullptr;
     const Source x{p.x + w.b * p.x_sb * size, p.x_sl * size, p.initial ? p.initial + (long long)w.b * (width - 1) * p.channels * size : nullptr,
                    (long long)p.channels * size, width - 1, w.end};
+    if (p.length == 0) {  // no row is there
+        if (p.last && w.run < width - 1 && w.n > 0) put_last<DT>(p, w, x, nullptr, width, w.run);
+        return;
+    }
     float weight[W][V], bias[V];
     Run<DT, V> before[W], rows[W];
     load_run<DT, W>(before, x, tile0, -W, t0 - W, w);
@@ -184,14 +220,16 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvParams p) {
     load_weights<W, MASKED>(p, w, weight, bias);
     Window<W> in;
     in.start(before);
+    const Flow flow = flow_of<W, MASKED>(docs, p.length, t0, w.end);
     char* tile = p.out + ((long long)w.b * p.length + tile0) * p.channels * size;
     const unsigned off = ((unsigned)(w.run * R) * (unsigned)p.channels + (unsigned)w.c) * size;
+    if (p.last && w.part == p.parts - 1 && w.run < width - 1 && w.n > 0) put_last<DT>(p, w, x, docs, width, w.run);
 #pragma unroll 1
     for (int g = 0; g < R; g += W) {
         if (!__any(t0 + g < p.length)) break;
         in.next(rows);
         if (g + W < R) load_run<DT, W>(rows, x, tile0, g + W, t0 + g + W, w);
-        const Flow f = flow_of<2 * W - 1, MASKED>(docs, p.length, t0 + g - (W - 1), w.end);
+        const GroupFlow<W, MASKED> f(flow, g);
         const bool whole = __all(t0 + g + W <= p.length && w.n == V);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
@@ -200,45 +238,12 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvParams p) {
             for (int e = 0; e < V; ++e) {
                 float z = preact<W, MASKED>(weight, bias, in, i, f, width, e);
                 if (p.silu) z *= conv_sigmoid<PRECISE>(z);
-                o.set(e, MASKED && !(f.on >> (i + W - 1) & 1) ? 0.0f : z);
+                o.set(e, f.counts(i) ? z : 0.0f);
             }
             char* to = tile + (long long)(g + i) * p.channels * size;
             if (whole) o.store_past(to + off);
             else if (t0 + g + i < p.length) o.store(to + off, w.n);
         }
-    }
-}
-
-// The first token that a token after `end` of the last one's document reads no further
-// back than: token numbers from 1 - width (the initial inputs') on.
-__device__ __forceinline__ int last_run(const int* docs, int end, int width) {
-    const int first = end - (width - 1);
-    if (end == 0 || !docs) return first;
-    if (docs[end - 1] < 0) return end;
-    int from = end - 1;
-    while (from > first && !(from > 0 && docs[from - 1] != docs[from])) --from;
-    return from;
-}
-
-// The inputs that a next token reads. A thread per channel.
-template <int DT>
-__global__ __launch_bounds__(256) void conv_last_kernel(ConvParams p) {
-    using T = typename ElemOf<DT>::type;
-    const int width = p.width;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (long long)p.batch * p.channels) return;
-    const int b = (int)(id / p.channels), c = (int)(id % p.channels);
-    const int end = p.lengths ? max(0, min(p.length, p.lengths[b])) : p.length;
-    const int from = last_run(p.docs ? p.docs + b * p.docs_sb : nullptr, end, width);
-    T* last = (T*)p.last + (long long)b * (width - 1) * p.channels + c;
-    for (int j = 0; j < width - 1; ++j) {
-        const int t = end - (width - 1) + j;
-        T v = T(0);
-        if (t >= from) {
-            if (t >= 0) v = ((const T*)p.x)[b * p.x_sb + t * p.x_sl + c];
-            else if (p.initial) v = ((const T*)p.initial)[((long long)b * (width - 1) + t + width - 1) * p.channels + c];
-        }
-        last[(long long)j * p.channels] = v;
     }
 }
 
@@ -321,6 +326,7 @@ __global__ __launch_bounds__(256) void conv_grad_kernel(ConvParams p) {
         fetch(0);
         Window<W> in;
         in.start(before);
+        const Flow flow = flow_of<W, MASKED>(docs, p.length, t0, w.end);
         float d[W][V];  // of inputs whose gradients are still being summed: that of token t0 + k in d[k % W]
 #pragma unroll
         for (int i = 0; i < W; ++i)
@@ -339,28 +345,28 @@ __global__ __launch_bounds__(256) void conv_grad_kernel(ConvParams p) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) dy[i][e] = rd[i].get(e);
             if (g < R) fetch(g + W);
-            const Flow f = flow_of<2 * W - 1, MASKED>(docs, p.length, t0 + g - (W - 1), w.end);
+            const GroupFlow<W, MASKED> f(flow, g);
             const bool whole = __all(t0 + g + 1 <= p.length && w.n == V);  // inputs up to t0 + g are written
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 float dz[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    dz[e] = MASKED && !(f.on >> (i + W - 1) & 1) ? 0.0f : dy[i][e];
+                    dz[e] = f.counts(i) ? dy[i][e] : 0.0f;
                     if (p.silu) dz[e] *= silu_grad<PRECISE>(preact<W, MASKED>(weight, bias, in, i, f, width, e));
                     d[i][e] = 0.0f;
                 }
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
                     const int q = W - 1 - j, slot = (i - q + W) % W;
-                    const bool skip = !reads<MASKED>(f, i + W - 1, q, width);
+                    const bool skip = !f.reads(i, q, width);
 #pragma unroll
                     for (int e = 0; e < V; ++e) d[slot][e] = __builtin_fmaf(weight[j][e], skip ? 0.0f : dz[e], d[slot][e]);
                 }
                 if (g < R) {
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
-                        const bool skip = !reads<MASKED>(f, i + W - 1, W - 1 - j, width);
+                        const bool skip = !f.reads(i, W - 1 - j, width);
 #pragma unroll
                         for (int e = 0; e < V; ++e) dw[j][e] = __builtin_fmaf(skip ? 0.0f : dz[e], skip ? 0.0f : in.x[i + j][e], dw[j][e]);
                     }
@@ -450,8 +456,7 @@ void launch_grad(const ConvParams& p) {
 template <int DT, int W, bool MASKED>
 void launch_masked(const ConvParams& p, bool gradient, bool wide_dout) {
     if (gradient) return wide_dout ? launch_grad<DT, ORMI_DTYPE_F32, W, MASKED>(p) : launch_grad<DT, DT, W, MASKED>(p);
-    if (p.tiles > 0) conv_kernel<DT, W, MASKED><<<(unsigned)((long long)p.channel_blocks * p.parts * p.batch), 256>>>(p);
-    if (p.width > 1 && p.last) conv_last_kernel<DT><<<(unsigned)(((long long)p.batch * p.channels + 255) / 256), 256>>>(p);
+    conv_kernel<DT, W, MASKED><<<(unsigned)((long long)p.channel_blocks * p.parts * p.batch), 256>>>(p);
 }
 template <int DT>
 int launch_conv(const ConvParams& p, bool gradient, bool wide_dout) {

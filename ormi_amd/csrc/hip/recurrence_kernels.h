@@ -74,21 +74,18 @@ struct Rules {
 };
 template <bool MASKED>
 __device__ __forceinline__ Rules token_rules(const RecParams& p, int b, int end, int t0) {
-    Rules r = {0, 0};
-#pragma unroll
-    for (int i = 0; i < kRecTokens; ++i) {
-        const int t = t0 + i;
-        if (t >= end) continue;
-        bool on = true, cut = false;
-        if constexpr (MASKED)
-            if (p.docs) {
-                const int* d = p.docs + b * p.docs_sb + t;
-                on = d[0] >= 0;
-                cut = !on || (t > 0 && d[-1] != d[0]);
-            }
-        r.on |= (unsigned)on << i;
-        r.cut |= (unsigned)cut << i;
-    }
+    constexpr unsigned all = (1u << kRecTokens) - 1;
+    const int left = end - t0;
+    Rules r = {left >= kRecTokens ? all : left > 0 ? (1u << left) - 1 : 0u, 0};
+    if constexpr (MASKED)
+        if (p.docs) {  // a thread of the segment looks at a token
+            const int* docs = p.docs + b * p.docs_sb;
+            const int lane = threadIdx.x % kRecLanes, at = (int)(threadIdx.x & 63) - lane, t = t0 + lane;
+            const int d = docs[min(t, p.length - 1)], last = docs[max(0, min(t - 1, p.length - 1))];  // token 0 goes on with itself
+            const unsigned none = (unsigned)(__ballot(d < 0) >> at), other = (unsigned)(__ballot(d != last) >> at);
+            r.cut = (none | other) & r.on;
+            r.on &= ~none;
+        }
     return r;
 }
 
