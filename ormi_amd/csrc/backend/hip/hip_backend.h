@@ -102,8 +102,8 @@ namespace ormi::hip {
     // The norm over all gradients' elements and min(1, max_norm / norm), float32
     // scalars on the device.
     std::pair<NodePtr, NodePtr> grad_norm(const std::vector<NodePtr>& grads, double max_norm);
-    // Each gradient times the factor, new buffers of its type.
-    std::vector<NodePtr> scale_grads(const std::vector<NodePtr>& grads, const NodePtr& factor);
+    // Each gradient times that factor, new buffers of its type, and the norm.
+    std::pair<std::vector<NodePtr>, NodePtr> clip_grads(const std::vector<NodePtr>& grads, double max_norm);
     // The float32 moments that 8-bit states stand for, of the given shape.
     std::pair<NodePtr, NodePtr> adamw_values(const std::vector<NodePtr>& state, const std::vector<int>& shape);
 

@@ -301,10 +301,8 @@ namespace ormi::hip {
         return list;
     }
 
-    std::pair<NodePtr, NodePtr> grad_norm(const std::vector<NodePtr>& grads, double max_norm) {
-        std::vector<NodePtr> hold;
-        const auto list = tensor_refs(grads, hold);
-        const Device dev = grads.empty() ? Device(DeviceEnum::HIP) : grads[0]->device;
+    // Norm and factor of the listed gradients, new scalars.
+    static std::pair<NodePtr, NodePtr> norm_of(const std::vector<ormi_tensor_ref>& list, const Device& dev, double max_norm) {
         auto norm = state_leaf({}, DType::Float32, dev), factor = state_leaf({}, DType::Float32, dev);
         size_t bytes = 0;
         ORMI_HIP_CHECK(ormi_hip_norm_workspace_size(list.data(), (int)list.size(), &bytes));
@@ -314,18 +312,23 @@ namespace ormi::hip {
         return {norm, factor};
     }
 
-    std::vector<NodePtr> scale_grads(const std::vector<NodePtr>& grads, const NodePtr& factor) {
-        if (!factor || factor->device.type != DeviceEnum::HIP || factor->dtype != DType::Float32 || shape_numel(factor->view.shape) != 1)
-            throw std::runtime_error("clipping: the factor is a float32 scalar on the hip device.");
+    std::pair<NodePtr, NodePtr> grad_norm(const std::vector<NodePtr>& grads, double max_norm) {
+        std::vector<NodePtr> hold;
+        const auto list = tensor_refs(grads, hold);
+        return norm_of(list, grads.empty() ? Device(DeviceEnum::HIP) : grads[0]->device, max_norm);
+    }
+
+    std::pair<std::vector<NodePtr>, NodePtr> clip_grads(const std::vector<NodePtr>& grads, double max_norm) {
         std::vector<NodePtr> hold, out;
         auto list = tensor_refs(grads, hold);
-        realize(factor);
+        const auto [norm, factor] = norm_of(list, grads.empty() ? Device(DeviceEnum::HIP) : grads[0]->device, max_norm);
+        out.reserve(list.size());
         for (size_t i = 0; i < list.size(); ++i) {
             out.push_back(state_leaf(grads[i]->view.shape, hold[i]->data->dtype, grads[i]->device));
             list[i].out = out.back()->data->ptr;
         }
         ORMI_HIP_CHECK(ormi_hip_scale(list.data(), (int)list.size(), (const float*)factor->data->ptr));
-        return out;
+        return {out, norm};
     }
 
     std::pair<NodePtr, NodePtr> adamw_values(const std::vector<NodePtr>& state, const std::vector<int>& shape) {

@@ -398,7 +398,10 @@ PYBIND11_MODULE(ormi_backend, m) {
         const auto r = hip::grad_norm(grads, max_norm);
         return py::make_tuple(r.first, r.second);
     }, py::arg("grads"), py::arg("max_norm"));
-    m.def("scale_grads", &hip::scale_grads, py::arg("grads"), py::arg("factor"));
+    m.def("clip_grads", [](const std::vector<std::shared_ptr<Node>>& grads, double max_norm) {
+        const auto r = hip::clip_grads(grads, max_norm);
+        return py::make_tuple(r.first, r.second);
+    }, py::arg("grads"), py::arg("max_norm"));
     m.def("adamw_values", &hip::adamw_values);
 
     m.def("execute_graph", &execute_graph);

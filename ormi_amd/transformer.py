@@ -229,10 +229,14 @@ def _adamw(params, grads, states, step, lr, betas, eps, weight_decay, factor):
             [kind._from(n, t.shape, t.device) for n, t in zip(s, params)])
 
 
-def _norm_and_factor(grads, max_norm: float):
-    """The nodes of the norm and of min(1, max_norm / norm)."""
+def _check_max_norm(max_norm: float) -> None:
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative.")
+
+
+def _norm_and_factor(grads, max_norm: float):
+    """The nodes of the norm and of min(1, max_norm / norm)."""
+    _check_max_norm(max_norm)
     return ormi_backend.grad_norm([t._node for t in grads], max_norm)
 
 
@@ -262,9 +266,9 @@ def clip_grads(grads, max_norm: float):
     infinite one makes finite elements 0 and the others NaN.
     """
     grads = _grads(grads)
-    norm, factor = _norm_and_factor(grads, max_norm)
-    device = grads[0].device if grads else _parse_device("hip")
-    return [Tensor._wrap(n, t.device) for n, t in zip(ormi_backend.scale_grads([t._node for t in grads], factor), grads)], Tensor._wrap(norm, device)
+    _check_max_norm(max_norm)
+    nodes, norm = ormi_backend.clip_grads([t._node for t in grads], max_norm)
+    return [Tensor._wrap(n, t.device) for n, t in zip(nodes, grads)], Tensor._wrap(norm, grads[0].device if grads else _parse_device("hip"))
 
 
 class AdamW:
@@ -288,8 +292,8 @@ class AdamW:
                  state_bits: int = 32, max_norm: float | None = None):
         if state_bits not in (32, 8):
             raise ValueError("state_bits must be 32 or 8.")
-        if max_norm is not None and not max_norm >= 0:
-            raise ValueError("max_norm must not be negative.")
+        if max_norm is not None:
+            _check_max_norm(max_norm)
         self.params = list(params)
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.max_norm, self.norm = max_norm, None
