@@ -11,7 +11,8 @@ constexpr int kRecRun = 4;                            // channels of a thread
 constexpr int kRecChannels = kRecLanes * kRecRun;     // of a work-group
 constexpr int kRecTokens = 8;                         // of a segment: a thread's
 constexpr int kRecTile = 256 / kRecLanes * kRecTokens;  // tokens between the states kept for the gradient
-constexpr int kRecWindow = 4;                         // tiles before a chained one that it looks at together
+constexpr int kRecGroup = 8;                          // chained tiles that share a state
+constexpr int kRecWindow = 8;                         // groups that a tile looks at together
 constexpr int kRecCounters = 16;                      // sets of chains
 constexpr int kRecCounterStride = 64;                 // words between their counters
 static_assert(kRecTile == ORMI_RECURRENCE_TILE, "the header's tile");
@@ -30,12 +31,18 @@ struct RecParams {
     const float* dlast;
     char *dgates, *dx;
     float* dinitial;
-    // Chained tiles: the spans and states that are there, by tile, chain and channel, and
-    // how many tiles of each set of chains were given out.
-    unsigned long long* chain_spans;
-    unsigned* chain_states;
+    // Chained tiles, by tile or group, chain and channel: what is there of the tiles' and
+    // the groups' spans and of the states before groups; and how many tiles of each set
+    // of chains were given out.
+    unsigned long long *chain_spans, *group_spans;
+    unsigned* group_states;
     unsigned* tickets;
 };
+
+// Groups of a chain, the last one perhaps of fewer tiles; one more state than whole
+// groups. 32-bit words of all spans and states, one after the other.
+inline long long chain_groups(const RecParams& p) { return (p.tiles + kRecGroup - 1) / kRecGroup + 1; }
+inline long long chain_words(const RecParams& p) { return (2ll * p.tiles + 3 * chain_groups(p)) * p.chains * kRecChannels; }
 
 // xt: the type of x and the result; gates and dout have it or are float32 (their flags).
 struct RecCall {

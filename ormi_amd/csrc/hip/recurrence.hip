@@ -47,9 +47,10 @@ void plan(const ormi_recurrence_desc* d, RecParams* p) {
     p->chained = p->tiles > 1 && p->chains < 2 * compute_units();
 }
 
-size_t span_bytes(const RecParams& p) { return (size_t)p.tiles * p.chains * kRecChannels * sizeof(unsigned long long); }
 // Spans, states, then the counters.
-size_t workspace_bytes(const RecParams& p) { return p.chained ? span_bytes(p) / 2 * 3 + kRecCounters * kRecCounterStride * sizeof(unsigned) : 0; }
+size_t workspace_bytes(const RecParams& p) {
+    return p.chained ? (chain_words(p) * sizeof(unsigned) + 255) / 256 * 256 + kRecCounters * kRecCounterStride * sizeof(unsigned) : 0;
+}
 
 void fill(const ormi_recurrence_desc* d, RecParams* p) {
     p->gates = (const char*)d->gates;
@@ -66,10 +67,11 @@ void fill(const ormi_recurrence_desc* d, RecParams* p) {
     p->last = d->last;
     p->states = d->states;
     if (p->chained) {
-        char* ws = (char*)d->workspace;
-        p->chain_spans = (unsigned long long*)ws;
-        p->chain_states = (unsigned*)(ws + span_bytes(*p));
-        p->tickets = (unsigned*)(ws + span_bytes(*p) / 2 * 3);
+        const long long row = (long long)p->chains * kRecChannels;
+        p->chain_spans = (unsigned long long*)d->workspace;
+        p->group_spans = p->chain_spans + p->tiles * row;
+        p->group_states = (unsigned*)(p->group_spans + chain_groups(*p) * row);
+        p->tickets = (unsigned*)((char*)d->workspace + workspace_bytes(*p)) - kRecCounters * kRecCounterStride;
     }
 }
 

@@ -14,10 +14,8 @@
 //
 // Ww batch and channels give enough work-groups, one goes through all tiles of
 // its channels, the state in registers, the next tile's loads in flight. Otherwise
-// (CHAINED) a work-group has one tile, and the state before it comes from the
-// tiles before: each publishes its span, and the state past it as soon as it knows
-// the one before it; a tile composes the spans back to the nearest state that is
-// there. Inputs are read once either way.
+// (CHAINED) a work-group has one tile, and the state before it comes from what the
+// tiles before publish (chained_state). Inputs are read once either way.
 //
 // Ww a token forgets (a document's first one, or one of none) the state before
 // it must not matter at all, NaN included, so spans carry a flag: a product that
@@ -214,84 +212,117 @@ __device__ __forceinline__ void cross_waves(const WaveSpans<V>& l, int at, float
 }
 
 // ------------------------------------------------------------ chained tiles --
-// A tile's span (gates' product and rest in one word, so that no order between
-// words matters) and the state past it, per channel. All bits set: not there yet.
-// Published NaN have other bits, and a span that forgets has them in the product's
-// place.
+// The state before a tile is found from what other tiles publish, per channel: each
+// tile its span, and the last tile of every kRecGroup the span of the group and, once
+// it knows it, the state past it. A tile applies the spans of the groups from the
+// nearest state that is there on, one after the other, then those of its own group's
+// tiles before it. A group's state came about in the same way, so which one is there
+// in time makes no difference to any bit. Nothing waits for a state: spans depend on
+// their own tiles alone, groups' on their tiles'.
+// A span is one word (its gates' product above the rest), so that no order between
+// words matters. All bits set: not there yet. Published NaN have other bits, and a span
+// that forgets has them in the product's place.
 constexpr unsigned kNone = 0xffffffffu;
 constexpr unsigned long long kNoSpan = ~0ull;
-// Looks at a tile before it that is not there yet, seconds' worth: the
-// tiles that a tile waits for were begun before it and wait for none after them, so
-// this ends a wait only where a work-group was lost; the states are NaN then.
+// Looks at a span that is not there yet, seconds' worth: the tiles that a tile waits
+// for were begun before it and wait for none after them, so this ends a wait only
+// where a work-group was lost; the states are NaN then.
 constexpr int kMostLooks = 1 << 21;
 
 __device__ __forceinline__ unsigned published(float v) { return v == v ? __float_as_uint(v) : 0x7fc00000u; }
-__device__ __forceinline__ unsigned look_state(const RecParams& p, long long at) {
-    return __hip_atomic_load(p.chain_states + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ unsigned long long as_word(float a, float b, bool cut) {
+    return (unsigned long long)(cut ? kNone : published(a)) << 32 | published(b);
 }
-__device__ __forceinline__ unsigned long long look_span(const RecParams& p, long long at) {
-    return __hip_atomic_load(p.chain_spans + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ float apply(unsigned long long span, float h) {
+    const unsigned a = (unsigned)(span >> 32);
+    const float b = __uint_as_float((unsigned)span);
+    return a == kNone ? b : __builtin_fmaf(__uint_as_float(a), h, b);
+}
+template <class T>
+__device__ __forceinline__ T look(const T* at) {
+    return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class T>
+__device__ __forceinline__ void publish(T* at, T v) {
+    __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Of one channel: the state before tile `pos` of a chain (counted in the order that
-// the tiles go), whose span is (a, b, cut); publishes what others need.
+// the tiles go), whose span is (a, b, cut).
 __device__ __forceinline__ float chained_state(const RecParams& p, int chain, int pos, int channel, float start, float a, float b, bool cut) {
-    const long long stride = (long long)p.chains * kRecChannels, at = pos * stride + (long long)chain * kRecChannels + channel;
+    constexpr int G = kRecGroup;
+    const long long stride = (long long)p.chains * kRecChannels, column = (long long)chain * kRecChannels + channel;
+    const int group = pos / G, before = pos % G;
+    unsigned long long* const spans = p.chain_spans + (long long)group * G * stride + column;  // of the group's tiles
+    const unsigned long long* const groups = p.group_spans + column;
+    unsigned* const states = p.group_states + column;
+    const unsigned long long own = as_word(a, b, cut);
+    publish(spans + before * stride, own);
+    // The group's tiles before this one.
+    unsigned long long tile[G - 1];
+    unsigned got;
+    int looks = 0;
+    while (true) {
+        got = look(states + group * stride);
+#pragma unroll
+        for (int k = 0; k < G - 1; ++k) tile[k] = k < before ? look(spans + k * stride) : 0;
+        bool there = true;
+#pragma unroll
+        for (int k = 0; k < G - 1; ++k) there = there && tile[k] != kNoSpan;
+        if (there) break;
+        if (++looks > kMostLooks) return __builtin_nanf("");
+        __builtin_amdgcn_s_sleep(1);
+    }
+    float ga = 1.0f, gb = 0.0f;
+    bool gcut = false;
+    if (before == G - 1) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+            const unsigned long long s = k < G - 1 ? tile[k < G - 1 ? k : 0] : own;
+            gb = apply(s, gb);
+            gcut = gcut || (unsigned)(s >> 32) == kNone;
+            ga *= __uint_as_float((unsigned)(s >> 32));
+        }
+        publish(p.group_spans + group * stride + column, as_word(ga, gb, gcut));
+    }
     float h = start;
-    if (pos > 0) {
-        unsigned first = look_state(p, at - stride);
-        if (first == kNone) {
-            const unsigned long long word = (unsigned long long)(cut ? kNone : published(a)) << 32 | published(b);
-            __hip_atomic_store(p.chain_spans + at, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            // The spans from tile pos - back to pos - 1 so far, and the states and spans
-            // of the next kRecWindow tiles before them, looked at together.
-            float sa = 1.0f, sb = 0.0f;
-            int back = 1, looks = 0;
-            bool done = false;
-            while (!done) {
-                unsigned state[kRecWindow];
-                unsigned long long span[kRecWindow];
+    if (group > 0 && got != kNone) {
+        h = __uint_as_float(got);
+    } else if (group > 0) {
+        int from = 0;  // h is the state before group `from`
+        for (int back = 1; back < group && from == 0; back += kRecWindow) {
+            unsigned state[kRecWindow];
 #pragma unroll
-                for (int k = 0; k < kRecWindow; ++k) {
-                    const long long from = at - (long long)min(back + k, pos) * stride;
-                    state[k] = look_state(p, from);
-                    span[k] = look_span(p, from);
-                }
-                bool ready = true;
+            for (int k = 0; k < kRecWindow; ++k) state[k] = look(states + max(group - back - k, 1) * stride);
 #pragma unroll
-                for (int k = 0; k < kRecWindow; ++k) {
-                    if (done || !ready) continue;
-                    if (state[k] != kNone) {
-                        h = __builtin_fmaf(sa, __uint_as_float(state[k]), sb);
-                        done = true;
-                    } else if (span[k] != kNoSpan) {
-                        const unsigned ka = (unsigned)(span[k] >> 32);
-                        const float kb = __uint_as_float((unsigned)span[k]);
-                        sb = __builtin_fmaf(sa, kb, sb);
-                        sa *= __uint_as_float(ka);
-                        ++back;
-                        if (ka == kNone) {
-                            h = sb;
-                            done = true;
-                        }
-                    } else {
-                        ready = false;
-                    }
+            for (int k = 0; k < kRecWindow; ++k)
+                if (from == 0 && group - back - k > 0 && state[k] != kNone) {
+                    from = group - back - k;
+                    h = __uint_as_float(state[k]);
                 }
-                if (!done && !ready) {
-                    if (++looks > kMostLooks) {
-                        h = __builtin_nanf("");
-                        done = true;
-                    }
-                    __builtin_amdgcn_s_sleep(1);
-                }
+        }
+        while (from < group) {
+            unsigned long long span[kRecWindow];
+#pragma unroll
+            for (int k = 0; k < kRecWindow; ++k) span[k] = look(groups + min(from + k, group - 1) * stride);
+            bool there = true;
+#pragma unroll
+            for (int k = 0; k < kRecWindow; ++k) {
+                there = there && span[k] != kNoSpan;
+                if (!there || from == group) continue;
+                h = apply(span[k], h);
+                ++from;
             }
-        } else {
-            h = __uint_as_float(first);
+            if (!there) {
+                if (++looks > kMostLooks) return __builtin_nanf("");
+                __builtin_amdgcn_s_sleep(1);
+            }
         }
     }
-    const float past = cut ? b : __builtin_fmaf(a, h, b);
-    __hip_atomic_store(p.chain_states + at, published(past), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (before == G - 1) publish(states + (group + 1) * stride, published(gcut ? gb : __builtin_fmaf(ga, h, gb)));
+#pragma unroll
+    for (int k = 0; k < G - 1; ++k)
+        if (k < before) h = apply(tile[k], h);
     return h;
 }
 // A tile's whole span of one channel, from its waves'.
@@ -604,7 +635,7 @@ template <int GT, int XT, int DT, bool LOGIT, bool MASKED>
 void launch_masked(const RecParams& p, bool gradient) {
     const unsigned tiles = (unsigned)p.chains * (unsigned)p.tiles;
     if (p.chained) {
-        const long long words = 3ll * tiles * kRecChannels;  // spans and states
+        const long long words = chain_words(p);
         recurrence_clear_kernel<<<(unsigned)((words + 1023) / 1024), 256>>>((unsigned*)p.chain_spans, words, p.tickets);
     }
     const unsigned groups = p.chained ? tiles : (unsigned)p.chains;

@@ -170,6 +170,31 @@ def test_views_give_the_same_bits(hip, dtype):
 
 
 @pytest.mark.gpu
+def test_more_elements_than_2_to_the_31(hip, ob):
+    """One tap of 2 and a bias of 1: each result is the same, each input's gradient too, at every offset; the weights'
+    gradients are the number of tokens times exact values, which float32 holds."""
+    from ormi_amd import causal_conv, realize_all
+
+    tokens = 1 << 20
+    shape = (2, tokens, 1040)
+    x = tensor(np.full((1, 1, 1040), 0.75, np.float32), "bfloat16", True)
+    taps = np.zeros((1040, 4), np.float32)
+    taps[:, 2] = 2.0
+    weight, bias = (tensor(t, grad=True) for t in (taps, np.ones(1040, np.float32)))
+    many = x.expand(shape)
+    y, last = causal_conv(many, weight, bias, tensor(np.full((2, 3, 1040), 0.75, np.float32), "bfloat16"))
+    (y * tensor(np.full((1, 1, 1), 0.5, np.float32), "bfloat16").expand(shape)).sum().backward()
+    realize_all(y, last, many.grad, weight.grad, bias.grad)
+    assert (y.max(2).numpy() == 2.5).all() and ((-y).max(2).numpy() == -2.5).all() and (last.numpy() == 0.75).all()
+    dx = many.grad.max(2).numpy()
+    assert np.array_equal(dx, (-((-many.grad).max(2))).numpy())  # channels alike
+    assert (dx[:, :-1] == 1.0).all() and (dx[:, -1] == 0.0).all()  # no token reads the last one as its third tap
+    assert (weight.grad.numpy() == 2 * tokens * 0.375).all() and (bias.grad.numpy() == tokens).all()
+    del y, last, many, x
+    ob.empty_cache()
+
+
+@pytest.mark.gpu
 def test_large_activations_stay_finite(hip):
     from ormi_amd import causal_conv, realize_all
 

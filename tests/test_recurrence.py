@@ -250,6 +250,49 @@ def test_views_give_the_same_bits(hip, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 40000, 128), (3, 6000, 520), (8, 2000, 1000)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_calls_give_the_same_bits(hip, shape, masked):
+    """Tiles wait for one another in whatever order they run: no bit of any result depends on it."""
+    from ormi_amd import linear_recurrence, realize_all
+
+    rng = np.random.default_rng(21)
+    g, x = values(shape, False, rng)
+    g, x, w = tensor(np.abs(g), grad=True), tensor(x, "bfloat16", True), tensor(rng.standard_normal(shape).astype(np.float32), "bfloat16")
+    masks = {"documents": tensor(documents_of(*shape[:2], 5, rng), "int32")} if masked else {}
+    first = None
+    for _ in range(6):
+        for t in (g, x):
+            t.zero_grad()
+        y, last = linear_recurrence(g, x, **masks)
+        total = (y * w).sum()
+        total.backward()
+        realize_all(y, last, g.grad, x.grad)
+        got = [t.numpy() for t in (y, last, g.grad, x.grad)]
+        total.zero_grad_graph()
+        first = first or got
+        assert all(np.array_equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.gpu
+def test_more_elements_than_2_to_the_31(hip, ob):
+    """Gates of zero pass nothing on: each state is its input, each input's gradient the result's, at every offset."""
+    from ormi_amd import linear_recurrence, realize_all
+
+    shape = (2, (1 << 20) + 300, 1040)
+    x, g = tensor(np.full((1, 1, 1040), 0.75, np.float32), "bfloat16", True), tensor(np.zeros((1, 1, 1040), np.float32), "bfloat16")
+    many = x.expand(shape)
+    y, last = linear_recurrence(g.expand(shape), many)
+    (y * tensor(np.full((1, 1, 1), 0.5, np.float32), "bfloat16").expand(shape)).sum().backward()
+    realize_all(y, last, many.grad)
+    for t, value in ((y, 0.75), (many.grad, 0.5)):
+        assert (t.max(2).numpy() == value).all() and ((-t).max(2).numpy() == -value).all()
+    assert (last.numpy() == 0.75).all()
+    del y, last, many, x, g
+    ob.empty_cache()
+
+
+@pytest.mark.gpu
 def test_gradient_reaches_through_the_last_state_alone_and_twice(hip):
     from ormi_amd import linear_recurrence, realize_all
 
