@@ -560,8 +560,8 @@ int ormi_hip_adamw_values(float* m, float* v, const void* m_codes, const float* 
  * The state starts from nothing at a token whose documents entry differs from
  * the token's before it; tokens of a negative document give zeros and leave a
  * state of zeros. Tokens from lengths[b] on (clamped to [0, length]) give zeros and leave the
- * state as it is. What stands at such tokens is not read, and nothing from
- * before a restart, infinity or NaN, reaches what is after it.
+ * state as it is. What stands at such tokens has no part in any result, and
+ * nothing from before a restart, infinity or NaN, reaches what is after it.
  * last (or NULL) receives the state after the last token, (batch, channels).
  * States, gates and products of gates are fp32, results are rounded once.
  * Spans of tokens are joined by the products of their gates, so gates whose
@@ -625,8 +625,8 @@ int ormi_hip_recurrence_grad(const ormi_recurrence_grad_desc* desc);
  * A token reads its own document's inputs: none from before the last token
  * where the documents entry changed (initial belongs to the first token's);
  * tokens of a negative document give zeros. Tokens from lengths[b] on (clamped
- * to [0, length]) give zeros. What stands at such tokens is not read, and none
- * of it, infinity or NaN, reaches other documents' results.
+ * to [0, length]) give zeros. What stands at such tokens, infinity or NaN, has no
+ * part in any result, nor has one document's in another's.
  * last (or NULL) receives the inputs that a token after the last one that
  * counts would read if it went on with its document, laid out like initial
  * (zeros after a token of a negative document).

@@ -5,7 +5,8 @@
 // overflow nor vanish, and cost less than the memory (a conversion and a
 // multiply-add an element). Pointers travel in the kernels' arguments as
 // AdamW's do. A work-group leaves one partial sum, and a last launch of one
-// work-group adds those up: the order is fixed by the sizes.
+// work-group adds those up: the order is fixed by the sizes. 25 M float32 parameters:
+// 20 us (5.0 TB/s), 4 and 31 (the second read comes partly out of the Infinity Cache).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -36,7 +36,9 @@ const char* check(const ormi_recurrence_desc* d) {
 bool nothing(const ormi_recurrence_desc* d) { return d->batch == 0 || d->channels == 0; }
 
 // The tiles, and whether they are chained: with fewer than two work-groups to a
-// compute unit the others do not keep the card's memory busy.
+// compute unit the others do not keep the card's memory busy. Measured: 256 chains of 8
+// tiles (16 x 1000 x 1024 fp16) 31 us chained, 40 one after the other; 512 chains of 16
+// with their gradient (8 x 2048 x 4096 bf16) 254 and 232.
 void plan(const ormi_recurrence_desc* d, RecParams* p) {
     p->batch = d->batch;
     p->length = d->length;

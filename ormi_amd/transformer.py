@@ -1,5 +1,6 @@
 """What a transformer block needs beside products and maps: rotary positions,
-masked softmax attention, and the AdamW step over a list of tensors.
+masked softmax attention, and the AdamW step over a list of tensors with the
+norm over their gradients.
 
     table = RotaryTable(head_dim, positions)
     q = rotary(x.reshape((batch, length, heads, head_dim)), table, dtype="bfloat16")
