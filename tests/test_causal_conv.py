@@ -170,6 +170,32 @@ def test_views_give_the_same_bits(hip, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [1, 2, 4, 8])
+def test_gradient_through_the_kept_inputs_alone(hip, width):
+    """Of two calls in a row, and of a call whose result nothing reads; inputs without a gradient get none."""
+    from ormi_amd import causal_conv, realize_all
+
+    rng = np.random.default_rng(17)
+    run((2, 70, 20), width, "bfloat16", "silu", rng, initial=True, lengths=np.array([3, 70], np.int32), dy=False, dlast=True)
+    x, w = rng.standard_normal((2, 2, 50, 10)).astype(np.float32)
+    taps = tensor(rng.standard_normal((10, width)).astype(np.float32), grad=True)
+    parts = [tensor(x[:, s].copy(), grad=True) for s in (slice(0, 2), slice(2, 50))]
+    y0, kept = causal_conv(parts[0], taps)
+    y1, _ = causal_conv(parts[1], taps, None, kept)
+    ((y0 * tensor(w[:, :2].copy())).sum() + (y1 * tensor(w[:, 2:].copy())).sum()).backward()
+    want, bound = ref.conv(x, taps.numpy(), None, False, dy=w)
+    realize_all(taps.grad, *(p.grad for p in parts))
+    ref.close(np.concatenate([p.grad.numpy() for p in parts], 1), want["dx"], bound["dx"] + 4 * ref.U * (np.abs(want["dx"]) + 8), "float32")
+    ref.close(taps.grad.numpy(), want["dw"], bound["dw"] + 4 * ref.U * np.abs(want["dw"]), "float32")
+    only = tensor(x)
+    y, _ = causal_conv(only, taps)
+    taps.zero_grad()
+    (y * tensor(w)).sum().backward()
+    assert only.grad is None
+    ref.close(taps.grad.numpy(), want["dw"], bound["dw"], "float32")
+
+
+@pytest.mark.gpu
 def test_more_elements_than_2_to_the_31(hip, ob):
     """One tap of 2 and a bias of 1: each result is the same, each input's gradient too, at every offset; the weights'
     gradients are the number of tokens times exact values, which float32 holds."""

@@ -323,6 +323,28 @@ def test_gradient_reaches_through_the_last_state_alone_and_twice(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("logit", [False, True])
+def test_gradients_of_some_inputs_and_of_two_passes(hip, logit):
+    """Only what asks for a gradient gets one; a second backward pass over new graphs of the same leaves adds to the first's."""
+    from ormi_amd import linear_recurrence
+
+    rng = np.random.default_rng(14)
+    shape = (2, 300, 18)
+    g, x = values(shape, logit, rng)
+    w = rng.standard_normal(shape).astype(np.float32)
+    want, bound = ref.recurrence(g, x, logit, np.zeros((2, 18)), dy=w)
+    for which in range(3):
+        leaves = [tensor(t, grad=k == which) for k, t in enumerate((g, x, np.zeros((2, 18), np.float32)))]
+        for times in (1, 2):
+            y, last = linear_recurrence(*leaves, gate="logit" if logit else "value")
+            (y * tensor(w)).sum().backward()
+            got = leaves[which].grad.numpy()
+            name = ("dg", "dx", "dinitial")[which]
+            ref.close(got, times * want[name], times * bound[name] + 2 * ref.U * np.abs(want[name]), "float32", name)
+        assert all(t.grad is None for k, t in enumerate(leaves) if k != which)
+
+
+@pytest.mark.gpu
 def test_same_tensor_as_gates_and_inputs(hip):
     from ormi_amd import linear_recurrence
 
