@@ -13,12 +13,12 @@
 // across the four waves, and each thread then walks its tokens again from the
 // state before them.
 //
-// Ww batch and channels give enough work-groups, one goes through all tiles of
+// Where batch and channels give enough work-groups, one goes through all tiles of
 // its channels, the state in registers, the next tile's loads in flight. Otherwise
 // (CHAINED) a work-group has one tile, and the state before it comes from what the
 // tiles before publish (chained_state). Inputs are read once either way.
 //
-// Ww a token forgets (a document's first one, or one of none) the state before
+// Where a token forgets (a document's first one, or one of none) the state before
 // it must not matter at all, NaN included, so spans carry a flag: a product that
 // is zero would let infinities through as NaN.
 // All states and products are fp32; results are rounded once.

@@ -312,7 +312,8 @@ def test_refusals(cpu, cabi):
     assert cabi.ormi_hip_conv(None) == 3 and b"null descriptor" in cabi.ormi_hip_last_error()
     assert cabi.ormi_hip_conv_grad(None) == 3 and cabi.ormi_hip_conv_grad_workspace_size(None, None) == 3
     good = dict(dtype=0, batch=1, length=4, channels=4, width=4, x=64, weight=64, out=64)
-    for bad in [dict(dtype=1), dict(batch=-1), dict(length=-1), dict(channels=-1), dict(length=(1 << 30) + 1), dict(width=0), dict(width=9), dict(x=None),
+    for bad in [dict(dtype=1), dict(batch=-1), dict(length=-1), dict(channels=-1), dict(length=(1 << 30) + 1), dict(channels=(1 << 20) + 1), dict(x_strides=(ctypes.c_int64 * 2)(0, (1 << 20) + 1)),
+                dict(x_strides=(ctypes.c_int64 * 2)(0, -1)), dict(width=0), dict(width=9), dict(x=None),
                 dict(weight=None), dict(out=None)]:
         d = Desc(**{**good, **bad})
         assert cabi.ormi_hip_conv(ctypes.byref(d)) == 3, bad

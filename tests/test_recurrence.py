@@ -293,6 +293,31 @@ def test_more_elements_than_2_to_the_31(hip, ob):
 
 
 @pytest.mark.gpu
+def test_tokens_far_apart(hip, cabi):
+    """Tokens 2^21 elements apart: more than a tile's offsets hold, so the call reads a copy; the entry itself refuses them."""
+    from ormi_amd import causal_conv, linear_recurrence, realize_all
+
+    rng = np.random.default_rng(19)
+    held = (rng.integers(-4, 5, (3, 1 << 19, 4)) / 4).astype(np.float32)
+    near = np.ascontiguousarray(held.transpose(1, 0, 2))
+    taps = tensor(rng.standard_normal((4, 3)).astype(np.float32))
+    results = []
+    for far in (True, False):
+        leaf = tensor(held if far else near, grad=True)
+        x = leaf.transpose([1, 0, 2]) if far else leaf
+        y, last = linear_recurrence(x, x)
+        z, kept = causal_conv(x, taps)
+        ((y * x).sum() + (z * x).sum()).backward()
+        realize_all(y, last, z, kept, leaf.grad)
+        results.append([t.numpy() for t in (y, last, z, kept)] + [leaf.grad.numpy().transpose(1, 0, 2) if far else leaf.grad.numpy()])
+    assert all(np.array_equal(a, b) for a, b in zip(*results))
+    d = Desc(dtype=0, gate_dtype=0, batch=1, length=4, channels=4, gates=64, x=64, out=64)
+    for strides in ((0, (1 << 20) + 1), (0, -1)):
+        d.x_strides = (ctypes.c_int64 * 2)(*strides)
+        assert cabi.ormi_hip_recurrence(ctypes.byref(d)) == 3 and b"apart" in cabi.ormi_hip_last_error()
+
+
+@pytest.mark.gpu
 def test_gradient_reaches_through_the_last_state_alone_and_twice(hip):
     from ormi_amd import linear_recurrence, realize_all
 
@@ -436,7 +461,7 @@ def test_refusals(cpu, cabi):
     assert cabi.ormi_hip_recurrence_workspace_size(None, ctypes.byref(size)) == 3
     good = dict(dtype=0, gate_dtype=0, batch=1, length=4, channels=4, gates=64, x=64, out=64)
     for bad in [dict(dtype=1), dict(gate_dtype=3), dict(dtype=3, gate_dtype=4), dict(batch=-1), dict(length=-1), dict(channels=-1), dict(length=(1 << 30) + 1),
-                dict(gates=None), dict(x=None), dict(out=None), dict(batch=1 << 24, channels=64)]:
+                dict(channels=(1 << 20) + 1), dict(gates=None), dict(x=None), dict(out=None), dict(batch=1 << 24, channels=64)]:
         d = Desc(**{**good, **bad})
         assert cabi.ormi_hip_recurrence(ctypes.byref(d)) == 3, bad
     for bad in [dict(forward=Desc(**good)), dict(forward=Desc(**good, states=64), dout=64, dout_dtype=3)]:
