@@ -47,11 +47,13 @@ struct Run {
         for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
         __builtin_memcpy(v, w, sizeof w);
     }
-    // All V; written past the caches, for results that are not read here again.
+    // All V, without a branch.
     __device__ __forceinline__ void load(const void* at) {
 #pragma unroll
         for (int i = 0; i < V / kGroup; ++i) v[i] = ((const Vec*)at)[i];
     }
+    // The same, past the caches: for results that are not read here again (8 x 2048 x 4096
+    // bf16, recurrence and gradient: 2%).
     __device__ __forceinline__ void store_past(void* at) const {
 #pragma unroll
         for (int i = 0; i < V / kGroup; ++i) __builtin_nontemporal_store(v[i], (Vec*)at + i);
