@@ -50,6 +50,33 @@ namespace ormi {
         dtype = result_dtype(op, parents, attrs);
     }
 
+    // Nodes to let go of, while some node's destructor on this thread is at it.
+    static thread_local std::vector<std::shared_ptr<Node>>* t_releasing = nullptr;
+
+    Node::~Node() {
+        auto leave = [](std::shared_ptr<Node>& n) {
+            if (n.use_count() == 1) t_releasing->push_back(std::move(n));
+            else n.reset();  // perhaps the last of two references of its child: that one comes here with t_releasing set
+        };
+        auto leave_all = [&] {
+            for (auto& p : parents) leave(p);
+            if (grad) leave(grad);
+        };
+        if (t_releasing) {
+            leave_all();
+            return;
+        }
+        if (parents.empty() && !grad) return;
+        std::vector<std::shared_ptr<Node>> list;
+        t_releasing = &list;
+        leave_all();
+        while (!list.empty()) {
+            const auto n = std::move(list.back());
+            list.pop_back();
+        }
+        t_releasing = nullptr;
+    }
+
     bool Node::is_realized() const { return data != nullptr; }
 
     void Node::realize() {

@@ -24,6 +24,9 @@ namespace ormi {
         Node(std::shared_ptr<Buffer> mem, bool req_grad, Device dev);
         Node(ops::OpEnum operation, std::vector<std::shared_ptr<Node>> parent_nodes, Device dev,
              OpAttributes attributes = NoAttrs{});
+        // A graph may be as deep as a program's run is long: what a node alone holds
+        // is let go of one by one, not by destructors inside one another.
+        ~Node();
 
         bool is_realized() const;
         void realize();
