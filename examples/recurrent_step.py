@@ -73,8 +73,7 @@ def token_by_token(block: RecurrentBlock, x: np.ndarray) -> np.ndarray:
     for at in range(x.shape[1]):
         y, state = block(Tensor(x[:, at:at + 1].copy(), "hip"), state)
         rows.append(y.numpy())
-        for t in state:
-            t.realize()  # the next call's graph starts from it
+        state = tuple(t.detach() for t in state)  # the weights have gradients: a state as it is keeps every token's graph
     return np.concatenate(rows, axis=1)
 
 

@@ -120,10 +120,15 @@ namespace ormi::hip {
             finish(n, out);
         }
 
+        // A state that no gradient goes back through lets go of the call that left it:
+        // passed from call to call it would hold on to all of them.
         void last_state_handler(const NodePtr& n) {
-            const auto& a = std::get<SequenceAttrs>(n->attrs);
+            auto& a = std::get<SequenceAttrs>(n->attrs);
             if (!a.saved->last) throw std::runtime_error("LAST_STATE: its sequence kept none.");
             finish(n, a.saved->last);
+            if (n->requires_grad) return;
+            a.saved = nullptr;
+            n->parents.clear();
         }
 
         // The upstream gradients of node n: that of the result as it comes, of x's type

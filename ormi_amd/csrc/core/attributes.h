@@ -66,7 +66,8 @@ namespace ormi {
         bool bias = false, initial = false, documents = false, lengths = false;
         std::vector<int> shape;    // of the result
         // What realizing the node leaves: the state after the last token, and for a
-        // recurrence's gradient those before its tiles.
+        // recurrence's gradient those before its tiles. A realized LAST_STATE without a
+        // gradient has no parents and no `saved` any more.
         struct Saved { std::shared_ptr<Buffer> last, states; };
         std::shared_ptr<Saved> saved;
         // As of an attention's gradients.

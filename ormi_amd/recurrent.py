@@ -5,6 +5,10 @@ that goes before it. Both carry their state from one call to the next.
     x, conv_state = causal_conv(x, weight, bias, conv_state, activation="silu")
     y, state = linear_recurrence(logits, x, state, gate="logit")    # differentiable, lazy like every op
 
+A state without a gradient keeps nothing of its call once it is realized. One with a
+gradient (weights that learn are among what it came from) keeps its call, and through
+it every call before: pass state.detach() on where gradients are not to go back.
+
 Additive to the reference's Python surface (ormi-core/src/ormi_core/tensor.py:10-190),
 which has neither.
 """
@@ -31,8 +35,8 @@ def linear_recurrence(gates: Tensor, x: Tensor, initial: Tensor | None = None, *
                changes; a token of a negative one gives zeros and leaves zeros
     lengths    int32 (batch,): tokens that exist (all); the others give zeros,
                whatever they hold, and leave the state as it is
-    h has x's type, the state is float32 (batch, channels): pass it as the next
-    call's initial. Gradients go to gates, x and initial, from h and from the state.
+    h has x's type, the state is float32 (batch, channels): pass it, or it
+    detached, as the next call's initial. Gradients go to gates, x and initial, from h and from the state.
     States are float32, results are rounded once. Gates whose product over some run
     of tokens passes 2^128, which none of magnitude up to 1 do, give results that
     are not finite.
@@ -57,7 +61,7 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Tensor | None = None, initial: 
                 changed (initial is the first token's); one of a negative document gives zeros
     lengths     int32 (batch,): tokens that exist (all); the others give zeros, whatever they hold
     The result and the inputs kept (batch, width - 1, channels) have x's type: pass the
-    latter as the next call's initial. Gradients go to x, weight, bias and initial.
+    latter, or them detached, as the next call's initial. Gradients go to x, weight, bias and initial.
     Sums are float32, results are rounded once.
     """
     if activation not in (None, "silu"):

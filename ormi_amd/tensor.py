@@ -4,7 +4,7 @@ Same constructor, operators, views, realize/numpy/backward/zero_grad as
 ormi_core.Tensor (reference ormi-core/src/ormi_core/tensor.py:10-190). Additive:
 the "hip" device, a dtype argument for leaves, and element-wise / reduction
 methods for the ops the reference lacks (relu, tanh, sigmoid, gelu, sum, mean,
-max, argmax, astype).
+max, argmax, astype), and detach.
 """
 from __future__ import annotations
 
@@ -296,6 +296,14 @@ class Tensor:
             return self
         ormi_backend.execute_graph(self._node)
         return self
+
+    def detach(self) -> "Tensor":
+        """The same values, in the same buffer, as a leaf without a gradient: realizes them and keeps nothing of
+        the graph that they came from."""
+        self.realize()
+        node = Node(self._node.data, False, self.device)
+        node.view = self._node.view
+        return Tensor._wrap(node, self.device)
 
     def numpy(self) -> np.ndarray:
         self.realize()
