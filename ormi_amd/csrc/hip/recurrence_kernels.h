@@ -610,7 +610,9 @@ __global__ __launch_bounds__(256, 2) void recurrence_grad_kernel(RecParams p) {
             for (int e = 0; e < V; ++e) {
                 const float prev = MASKED && cut ? 0.0f : h[e], v = nx[i].get(e);
                 q[i][e] = LOGIT ? a[i][e] * take[i][e] * (prev - v) : prev;
-                h[e] = __builtin_fmaf(a[i][e], prev, LOGIT ? take[i][e] * v : v);
+                // As the forward pass joins them. Of a restart's gate nothing is left where it is a value;
+                // a logit's is finite, or its b is NaN too.
+                h[e] = after<MASKED && !LOGIT>(a[i][e], LOGIT ? take[i][e] * v : v, cut, prev);
             }
         }
 #pragma unroll
