@@ -350,29 +350,33 @@ __global__ __launch_bounds__(256) void conv_grad_kernel(ConvParams p) {
             const bool whole = __all(t0 + g + 1 <= p.length && w.n == V);  // inputs up to t0 + g are written
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                float dz[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    dz[e] = f.counts(i) ? dy[i][e] : 0.0f;
-                    if (p.silu) dz[e] *= silu_grad<PRECISE>(preact<W, MASKED>(weight, bias, in, i, f, width, e));
-                    d[i][e] = 0.0f;
-                }
+                for (int e = 0; e < V; ++e) d[i][e] = 0.0f;
+                // Past the last token stand the inputs before it with a gradient of zero, and zero times infinity is not zero.
+                if (MASKED || t0 + g + i < p.length) {
+                    float dz[V];
 #pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    const int q = W - 1 - j, slot = (i - q + W) % W;
-                    const bool skip = !f.reads(i, q, width);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) d[slot][e] = __builtin_fmaf(weight[j][e], skip ? 0.0f : dz[e], d[slot][e]);
-                }
-                if (g < R) {
-#pragma unroll
-                    for (int j = 0; j < W; ++j) {
-                        const bool skip = !f.reads(i, W - 1 - j, width);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) dw[j][e] = __builtin_fmaf(skip ? 0.0f : dz[e], skip ? 0.0f : in.x[i + j][e], dw[j][e]);
+                    for (int e = 0; e < V; ++e) {
+                        dz[e] = f.counts(i) ? dy[i][e] : 0.0f;
+                        if (p.silu) dz[e] *= silu_grad<PRECISE>(preact<W, MASKED>(weight, bias, in, i, f, width, e));
                     }
 #pragma unroll
-                    for (int e = 0; e < V; ++e) db[e] += dz[e];
+                    for (int j = 0; j < W; ++j) {
+                        const int q = W - 1 - j, slot = (i - q + W) % W;
+                        const bool skip = !f.reads(i, q, width);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) d[slot][e] = __builtin_fmaf(weight[j][e], skip ? 0.0f : dz[e], d[slot][e]);
+                    }
+                    if (g < R) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) {
+                            const bool skip = !f.reads(i, W - 1 - j, width);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) dw[j][e] = __builtin_fmaf(skip ? 0.0f : dz[e], skip ? 0.0f : in.x[i + j][e], dw[j][e]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < V; ++e) db[e] += dz[e];
+                    }
                 }
                 const int done = g + i - (W - 1), slot = (i + 1) % W;  // the input that no later token reads
                 if (done >= 0 && done < R && p.dx) {
