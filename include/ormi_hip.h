@@ -566,7 +566,9 @@ int ormi_hip_adamw_values(float* m, float* v, const void* m_codes, const float* 
  * States, gates and products of gates are fp32, results are rounded once.
  * Spans of tokens are joined by the products of their gates, so gates whose
  * product over some span passes 2^128 (none up to magnitude 1 does) give
- * results that are not finite; an infinite state may become NaN.
+ * results that are not finite, and a product below 2^-126 is held to 2^-149 of
+ * the state that it passes on; an infinite state may become NaN. (A launch of
+ * which a work-group is lost ends after seconds, with states of NaN.)
  * states (or NULL) receives the state before every ORMI_RECURRENCE_TILE-th
  * token, (batch, ceil(length / tile), channels) fp32: the gradient needs it.
  * workspace: device memory of *_workspace_size() bytes, 256-byte aligned (NULL
@@ -676,8 +678,9 @@ int ormi_hip_conv_grad(const ormi_conv_grad_desc* desc);
  * counterpart in the reference). Tensors are contiguous, F32, BF16 or F16, and
  * any number of them.
  *   norm = sqrt(sum of all squares), factor = min(1, max_norm / norm)
- * in 64 bits, in a fixed order, each rounded to fp32 once (either may be NULL). A norm that is
- * NaN makes the factor NaN, an infinite one makes it 0. workspace as above. */
+ * in 64 bits, in a fixed order, each rounded to fp32 once (either may be NULL): a factor below
+ * 2^-126 has fewer bits. A norm that is NaN makes the factor NaN, an infinite one makes it 0
+ * unless max_norm is infinite too (1). workspace as above. */
 typedef struct ormi_tensor_ref {
     const void* data;
     void*       out;                                /* ormi_hip_scale: of data's type; may be data */

@@ -7,7 +7,7 @@
 // and the gradients still being summed stay in registers, the next W rows are on
 // their way. A work-group is 8 such runs by 128 channels. (All of a run's rows in
 // registers at once took 256 of them, one wave to a SIMD: 229 us for the gradient of
-// 8 x 2048 x 4096 bf16; now 101, 4.0 TB/s, and 64 forward, 4.2. 128 bytes of a row to a
+// 8 x 2048 x 4096 bf16; now 105, 3.8 TB/s, and 64 forward, 4.2. 128 bytes of a row to a
 // work-group in place of 256: 5% more there, 14% in float32.)
 // dw and db are summed by a thread over its tokens, then over a work-group, which
 // goes through several tiles; each leaves one partial row, and a second launch adds
@@ -49,7 +49,7 @@ __device__ __forceinline__ ConvPlace conv_place(const ConvParams& p) {
     return w;
 }
 
-// Kernels exist for widths 3 and 4; MASKED ones of W also take smaller widths, whose
+// Kernels without masks are for widths 3 and 4; MASKED ones of W also take smaller widths, whose
 // first W - width taps no token reads.
 template <int W, bool MASKED>
 __device__ __forceinline__ int width_of(const ConvParams& p) {
@@ -352,7 +352,9 @@ __global__ __launch_bounds__(256) void conv_grad_kernel(ConvParams p) {
             for (int i = 0; i < W; ++i) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) d[i][e] = 0.0f;
-                // Past the last token stand the inputs before it with a gradient of zero, and zero times infinity is not zero.
+                // Past the last token stand the inputs before it with a gradient of zero, and zero
+                // times infinity is not zero. (101 us without the question; asked of a whole group,
+                // with its body twice: 190 registers for 150.)
                 if (MASKED || t0 + g + i < p.length) {
                     float dz[V];
 #pragma unroll

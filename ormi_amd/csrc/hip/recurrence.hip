@@ -36,9 +36,12 @@ const char* check(const ormi_recurrence_desc* d) {
 bool nothing(const ormi_recurrence_desc* d) { return d->batch == 0 || d->channels == 0; }
 
 // The tiles, and whether they are chained: with fewer than two work-groups to a
-// compute unit the others do not keep the card's memory busy. Measured: 256 chains of 8
-// tiles (16 x 1000 x 1024 fp16) 31 us chained, 40 one after the other; 512 chains of 16
-// with their gradient (8 x 2048 x 4096 bf16) 254 and 232.
+// compute unit the others do not keep the card's memory busy. Measured, chained and one
+// after the other: 256 chains of 8 tiles (16 x 1000 x 1024 fp16) 31 and 40 us; chains of
+// 16 tiles with their gradient (batches of 2048 x 4096 bf16), 320: 172 and 190, 384: 204
+// and 201, 448: 234 and 210, 512: 263 and 233. Past 512 work-groups, as many as are on
+// the card at once, the last ones have it to themselves: 640: 335 and 363, 832: 428 and
+// 445, 1024: 537 and 496.
 void plan(const ormi_recurrence_desc* d, RecParams* p) {
     p->batch = d->batch;
     p->length = d->length;

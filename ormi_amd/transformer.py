@@ -264,7 +264,8 @@ def clip_grads(grads, max_norm: float):
 
     Nothing waits for the device: the factor stays there. Each product is rounded
     once to its gradient's type. A norm that is NaN makes every element NaN, an
-    infinite one makes finite elements 0 and the others NaN.
+    infinite one makes finite elements 0 and the others NaN (max_norm=inf leaves
+    them as they are).
     """
     grads = _grads(grads)
     _check_max_norm(max_norm)
