@@ -13,4 +13,19 @@ namespace ormi::hip {
     NodePtr contiguous(const NodePtr& n);
     // Device memory of at least `bytes`, null for 0.
     std::shared_ptr<Buffer> workspace(size_t bytes);
+
+    // Buffers of gradients that one call fills, with the first of them that is
+    // realized. The others find theirs only once the call is made: where it is refused,
+    // or memory runs out, each tries again.
+    template <size_t N>
+    struct FilledTogether {
+        std::shared_ptr<Buffer> buffers[N];
+        void* add(size_t w, const Node& like) {
+            buffers[w] = empty(like.view.shape, DeviceEnum::HIP, like.dtype);
+            return buffers[w]->ptr;
+        }
+        void leave(std::shared_ptr<Buffer> (&made)[N]) {
+            for (size_t w = 0; w < N; ++w) made[w] = std::move(buffers[w]);
+        }
+    };
 }

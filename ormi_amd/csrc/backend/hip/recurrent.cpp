@@ -156,12 +156,9 @@ namespace ormi::hip {
             return u;
         }
 
-        // The wanted gradients' buffers, made together with the first that is realized.
-        void* made_buffer(const Node& n, const SequenceAttrs& a, int w) {
-            if (!a.grads->want[w]) return nullptr;
-            const NodePtr& x = n.parents[a.first() + w];
-            a.grads->made[w] = empty(x->view.shape, DeviceEnum::HIP, x->dtype);
-            return a.grads->made[w]->ptr;
+        // A wanted gradient's buffer, or null.
+        void* wanted(FilledTogether<4>& filled, const Node& n, const SequenceAttrs& a, int w) {
+            return a.grads->want[w] ? filled.add(w, *n.parents[a.first() + w]) : nullptr;
         }
         void take_made(const NodePtr& n, const SequenceAttrs& a) {
             finish(n, a.grads->made[a.which]);
@@ -183,14 +180,16 @@ namespace ormi::hip {
                     strides2(*u.dout, d.dout_strides);
                 }
                 if (u.dlast) d.dlast = (const float*)u.dlast->data->ptr;
-                d.dgates = made_buffer(*n, a, 0);
-                d.dx = made_buffer(*n, a, 1);
-                if (a.initial) d.dinitial = (float*)made_buffer(*n, a, 2);
+                FilledTogether<4> filled;
+                d.dgates = wanted(filled, *n, a, 0);
+                d.dx = wanted(filled, *n, a, 1);
+                if (a.initial) d.dinitial = (float*)wanted(filled, *n, a, 2);
                 size_t bytes = 0;
                 ORMI_HIP_CHECK(ormi_hip_recurrence_workspace_size(&d.forward, &bytes));
                 const auto ws = workspace(bytes);
                 if (ws) d.forward.workspace = ws->ptr, d.forward.workspace_bytes = ws->bytes;
                 ORMI_HIP_CHECK(ormi_hip_recurrence_grad(&d));
+                filled.leave(a.grads->made);
             }
             take_made(n, a);
         }
@@ -209,15 +208,17 @@ namespace ormi::hip {
                 }
                 if (u.dlast) d.dlast = (const float*)u.dlast->data->ptr;
                 int w = 2;
-                d.dx = made_buffer(*n, a, 0);
-                d.dweight = (float*)made_buffer(*n, a, 1);
-                if (a.bias) d.dbias = (float*)made_buffer(*n, a, w++);
-                if (a.initial) d.dinitial = made_buffer(*n, a, w);
+                FilledTogether<4> filled;
+                d.dx = wanted(filled, *n, a, 0);
+                d.dweight = (float*)wanted(filled, *n, a, 1);
+                if (a.bias) d.dbias = (float*)wanted(filled, *n, a, w++);
+                if (a.initial) d.dinitial = wanted(filled, *n, a, w);
                 size_t bytes = 0;
                 ORMI_HIP_CHECK(ormi_hip_conv_grad_workspace_size(&d, &bytes));
                 const auto ws = workspace(bytes);
                 if (ws) d.workspace = ws->ptr, d.workspace_bytes = ws->bytes;
                 ORMI_HIP_CHECK(ormi_hip_conv_grad(&d));
+                filled.leave(a.grads->made);
             }
             take_made(n, a);
         }

@@ -173,16 +173,15 @@ namespace ormi::hip {
             d.dout = g->data->ptr;
             strides4(*g, d.dout_strides);
             void** outs[3] = {&d.dq, &d.dk, &d.dv};
-            for (int w = 0; w < 3; ++w) {
-                if (!a.grads->want[w]) continue;
-                made[w] = empty(n->parents[2 + w]->view.shape, DeviceEnum::HIP, n->parents[2 + w]->dtype);
-                *outs[w] = made[w]->ptr;
-            }
+            FilledTogether<3> filled;
+            for (int w = 0; w < 3; ++w)
+                if (a.grads->want[w]) *outs[w] = filled.add(w, *n->parents[2 + w]);
             size_t bytes = 0;
             ORMI_HIP_CHECK(ormi_hip_attention_grad_workspace_size(&d, &bytes));
             const auto ws = workspace(bytes);
             if (ws) d.forward.workspace = ws->ptr, d.forward.workspace_bytes = ws->bytes;
             ORMI_HIP_CHECK(ormi_hip_attention_grad(&d));
+            filled.leave(made);
         }
         n->data = made[a.which];
         made[a.which] = nullptr;  // the node's own from here on
